@@ -257,6 +257,88 @@ int sage_quant_q(int dtype, int qk_int8,
                  void* q8, float* sq, float* cq, void* stream);
 
 /*
+ * Serving from a quantized, paged K/V cache. No counterpart in the reference, whose SK1 path
+ * quantizes the K and V of every call anew (`sageattention/sk1_backend/__init__.py:1150-1284`).
+ *
+ * A cache is a pool of pages of SAGE_CACHE_PAGE tokens:
+ *   k8 (num_pages, H_kv, 64, D) int8 (k_int8, fp16 only) or fp8 e4m3; v8 likewise, fp8 e4m3;
+ *   sk, sv (num_pages, H_kv, 64) fp32 row scales, by the prologue's scheme without smoothing.
+ *   block_table (B, max_pages) int32, rows t_sb elements apart: position p of sequence b lies in page
+ *   block_table[b][p / 64], row p % 64. A number outside [0, num_pages) names no page, as does a
+ *   position from max_pages * 64 on: nothing is written there, zeros are read, nobody attends to it.
+ * Codes are never NaN: a row of K or V that holds a NaN or an infinity is held as zero codes under a
+ * NaN scale (it reads back as NaN, and so come out the rows that attend to it, and only they).
+ * All tensors of a pool are 16-byte aligned. start, lens, kv_lens, q_lens: (B) int32 on the device.
+ */
+#define SAGE_CACHE_PAGE 64
+
+/*
+ * Rotary positions: o = x with each pair (a, b) of the first R columns turned to
+ * (a c - b s, b c + a s); the other columns are copied. In fp32, one rounding to `dtype`.
+ *   x, o         logical (B, H, N, D) views, D = 64 or 128; o may be x itself, and else does not overlap it
+ *   table        (table_rows, R) fp32, 16-byte aligned: R/2 cosines, then R/2 sines per position
+ *   R            a multiple of 16 in [16, D]
+ *   positions    (B, N) int32, rows p_sb elements apart (0: all sequences share a row). Where one lies
+ *                outside the table, the rotated columns become NaN.
+ *   interleaved  1: pairs (2i, 2i + 1); 0: pairs (i, i + R/2)
+ *   inverse      1: by the negative angle (the transposed rotation: the gradient of the rotation)
+ */
+int sage_rotary(int dtype, const void* x, int64_t x_sb, int64_t x_sh, int64_t x_sr, void* o,
+                int64_t o_sb, int64_t o_sh, int64_t o_sr, int64_t B, int64_t H, int64_t N,
+                int64_t D, const float* table, int64_t table_rows, int64_t R,
+                const int32_t* positions, int64_t p_sb, int interleaved, int inverse,
+                void* stream);
+
+/*
+ * Rows n < lens[b] of k and v (logical (B, H_kv, N, D) views) quantized into positions start[b] + n of
+ * sequence b's pages; lens NULL: all N. With `table`, K is rotated first (as sage_rotary does, in
+ * fp32, without the rounding to 16 bits between). The rest of the pool stays as it was. No two
+ * rows of a call may go to the same place of the pool.
+ */
+int sage_cache_write(int dtype, int k_int8, const void* k, int64_t k_sb, int64_t k_sh,
+                     int64_t k_sr, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_sr,
+                     int64_t B, int64_t H_kv, int64_t N, int64_t D, void* k8, float* sk, void* v8,
+                     float* sv, int64_t num_pages, const int32_t* block_table, int64_t t_sb,
+                     int64_t max_pages, const int32_t* start, const int32_t* lens,
+                     const float* table, int64_t table_rows, int64_t R, const int32_t* positions,
+                     int64_t p_sb, int interleaved, void* stream);
+
+/*
+ * Positions start[b] + n, n < lens[b], of sequence b read into row n of k and v (logical (B, H_kv, N,
+ * D) views of `dtype`): code * scale, rounded once. Rows from lens[b] on are zeros. start NULL: 0.
+ */
+int sage_cache_read(int dtype, int k_int8, const void* k8, const float* sk, const void* v8,
+                    const float* sv, int64_t num_pages, const int32_t* block_table, int64_t t_sb,
+                    int64_t max_pages, const int32_t* start, const int32_t* lens, void* k,
+                    int64_t k_sb, int64_t k_sh, int64_t k_sr, void* v, int64_t v_sb, int64_t v_sh,
+                    int64_t v_sr, int64_t B, int64_t H_kv, int64_t N, int64_t D, void* stream);
+
+/*
+ * Attention of each sequence's T newest tokens, whose K and V are in the cache, over all of its
+ * kv_lens[b] cached tokens, in one or two launches. New token i (of q_lens[b], NULL: T) sees the
+ * kv_lens[b] - q_lens[b] tokens before the new ones, and new token j where mask[b][i][j] is not zero;
+ * without a mask, where j <= i (T = 1: plain decoding).
+ *   q, o      logical (B, H, T, D) views; query head h reads K/V head h / (H / H_kv)
+ *   mask      (B, T, T) bytes, strides m_sb, m_sr in elements (m_sb 0: one mask for all), last stride 1
+ *   lse       optional (B, H, T) fp32: the natural logsumexp of each row's scores times sm_scale
+ *   workspace sage_cache_attn_workspace_bytes bytes, 16-byte aligned; NULL where that is 0
+ * Rows that see nothing, and rows of tokens i >= q_lens[b], are zeros with a logsumexp of -infinity.
+ * Q is not quantized: scores are exact products of 16-bit queries and 8-bit codes, summed in fp32.
+ */
+int sage_cache_attn(int dtype, int k_int8, const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sr,
+                    const void* k8, const float* sk, const void* v8, const float* sv,
+                    int64_t num_pages, const int32_t* block_table, int64_t t_sb,
+                    int64_t max_pages, const int32_t* kv_lens, const int32_t* q_lens,
+                    const void* mask, int64_t m_sb, int64_t m_sr, void* o, int64_t o_sb,
+                    int64_t o_sh, int64_t o_sr, int64_t B, int64_t H, int64_t T, int64_t H_kv,
+                    int64_t D, float sm_scale, float* lse, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace of a sage_cache_attn call of these sizes (0: none), or -SAGE_ERR_INVALID. */
+int64_t sage_cache_attn_workspace_bytes(int64_t B, int64_t H, int64_t H_kv, int64_t T,
+                                        int64_t max_pages, int64_t D);
+
+/*
  * MFMA accumulator layout probe (known-answer test of the fragment layouts the main loop relies
  * on). One wave computes C = A(32x32, int8) * B(32x32, int8) with v_mfma_i32_32x32x32_i8 and
  * D = E(32x64, fp8) * F(64x32, fp8) with v_mfma_scale_f32_32x32x64_f8f6f4, loading operands in

@@ -207,6 +207,80 @@ int kernel_for(int64_t B, int64_t H, int64_t N, int64_t D, int causal, int64_t c
                                                               : SAGE_KERNEL_PIPE;
 }
 
+// Rotary positions' arguments, given a table.
+int check_rotary(const float* table, int64_t rows, int64_t R, const int32_t* positions,
+                 int64_t p_sb, int64_t N, int64_t D) {
+  if (!table || !positions) return fail(SAGE_ERR_INVALID, "rotary: table or positions is NULL");
+  if (!aligned16(table)) return fail(SAGE_ERR_INVALID, "ptr_align: the table must be 16-byte aligned");
+  if (rows < 1) return fail(SAGE_ERR_INVALID, "rotary: the table has no rows");
+  if (R < 16 || R > D || R % 16)
+    return fail(SAGE_ERR_INVALID, "rotary: R must be a multiple of 16 in [16, D] (R=%lld D=%lld)",
+                (long long)R, (long long)D);
+  if (p_sb < N && p_sb != 0)
+    return fail(SAGE_ERR_INVALID, "rotary: rows of positions overlap (stride %lld for N=%lld)",
+                (long long)p_sb, (long long)N);
+  return SAGE_OK;
+}
+
+int check_rows(const char* what, int64_t B, int64_t H, int64_t N, int64_t D) {
+  if (B < 1 || H < 1 || N < 1)
+    return fail(SAGE_ERR_INVALID, "seq_len: B, H and N must be >= 1 (B=%lld H=%lld N=%lld)",
+                (long long)B, (long long)H, (long long)N);
+  const int rc = check_head_dim(D);
+  if (rc) return rc;
+  if (B > kInt32Max || H > kInt32Max || N > kInt32Max || B * H > kInt32Max / N)
+    return fail(SAGE_ERR_INVALID, "grid: shape too large (B=%lld H=%lld N=%lld)", (long long)B,
+                (long long)H, (long long)N);
+  return check_grid(what, (B * H * N * (D / 8) + 255) / 256, 256);
+}
+
+int check_pool(int dtype, int k_int8, const void* k8, const float* sk, const void* v8,
+               const float* sv, int64_t num_pages, const int32_t* table, int64_t t_sb,
+               int64_t max_pages, sage::CachePool* pool) {
+  if (dtype != SAGE_F16 && dtype != SAGE_BF16)
+    return fail(SAGE_ERR_INVALID, "dtype: unsupported dtype code %d", dtype);
+  if (dtype == SAGE_BF16 && k_int8)
+    return fail(SAGE_ERR_INVALID, "bf16_int8: int8 K is served for fp16 inputs only");
+  if (!k8 || !sk || !v8 || !sv || !table) return fail(SAGE_ERR_INVALID, "pool: a pointer is NULL");
+  if (!aligned16(k8) || !aligned16(sk) || !aligned16(v8) || !aligned16(sv))
+    return fail(SAGE_ERR_INVALID, "ptr_align: the pool's tensors must be 16-byte aligned");
+  if (num_pages < 1 || num_pages > kInt32Max)
+    return fail(SAGE_ERR_INVALID, "pool: num_pages out of range (%lld)", (long long)num_pages);
+  // positions and page starts are 32-bit numbers
+  if (max_pages < 1 || max_pages > (1 << 24))
+    return fail(SAGE_ERR_INVALID, "block_table: max_pages must be in [1, 2^24] (got %lld)",
+                (long long)max_pages);
+  if (t_sb < max_pages && t_sb != 0)
+    return fail(SAGE_ERR_INVALID, "block_table: rows overlap (stride %lld for %lld pages)",
+                (long long)t_sb, (long long)max_pages);
+  pool->k_int8 = k_int8 ? 1 : 0;
+  pool->k8 = const_cast<void*>(k8);
+  pool->sk = const_cast<float*>(sk);
+  pool->v8 = const_cast<void*>(v8);
+  pool->sv = const_cast<float*>(sv);
+  pool->num_pages = num_pages;
+  pool->table = table;
+  pool->t_sb = t_sb;
+  pool->max_pages = max_pages;
+  return SAGE_OK;
+}
+
+int check_cache_attn_shape(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_t max_pages,
+                           int64_t D) {
+  if (H_kv < 1 || H < 1 || H % H_kv != 0)
+    return fail(SAGE_ERR_INVALID, "heads: H (%lld) must be a multiple of H_kv (%lld)",
+                (long long)H, (long long)H_kv);
+  int rc = check_rows("the cached attention", B, H, T, D);
+  if (rc) return rc;
+  if (max_pages < 1 || max_pages > (1 << 24))
+    return fail(SAGE_ERR_INVALID, "block_table: max_pages must be in [1, 2^24] (got %lld)",
+                (long long)max_pages);
+  // the join has D/4 threads a row
+  if ((rc = check_grid("the join", (B * H * T * (D / 4) + 255) / 256, 256))) return rc;
+  return check_grid("the cached attention", sage::cache_attn_plan(B, H, H_kv, T, max_pages).blocks,
+                    256);
+}
+
 }  // namespace
 
 extern "C" {
@@ -523,6 +597,172 @@ int sage_attn_fwd(int dtype, int qk_int8, int causal, const void* q, int64_t q_s
   return sage_attn_fwd_ex(dtype, qk_int8, causal, q, q_sb, q_sh, q_sr, k8, kconst, v8t, s, o,
                           o_sb, o_sh, o_sr, B, H, N, H, N, N_pad, 128, sm_scale,
                           SAGE_KERNEL_AUTO, nullptr, nullptr, nullptr, stream);
+}
+
+int sage_rotary(int dtype, const void* x, int64_t x_sb, int64_t x_sh, int64_t x_sr, void* o,
+                int64_t o_sb, int64_t o_sh, int64_t o_sr, int64_t B, int64_t H, int64_t N,
+                int64_t D, const float* table, int64_t table_rows, int64_t R,
+                const int32_t* positions, int64_t p_sb, int interleaved, int inverse,
+                void* stream) {
+  if (dtype != SAGE_F16 && dtype != SAGE_BF16)
+    return fail(SAGE_ERR_INVALID, "dtype: unsupported dtype code %d", dtype);
+  int rc = check_rows("rotary", B, H, N, D);
+  if (rc) return rc;
+  if ((rc = check_view("x", x, x_sb, x_sh, x_sr))) return rc;
+  if ((rc = check_view("o", o, o_sb, o_sh, o_sr))) return rc;
+  if ((rc = check_rotary(table, table_rows, R, positions, p_sb, N, D))) return rc;
+  sage::RotaryArgs a;
+  a.dtype = dtype;
+  a.x = x;
+  a.x_sb = x_sb;
+  a.x_sh = x_sh;
+  a.x_sr = x_sr;
+  a.o = o;
+  a.o_sb = o_sb;
+  a.o_sh = o_sh;
+  a.o_sr = o_sr;
+  a.table = table;
+  a.rows = table_rows;
+  a.R = R;
+  a.positions = positions;
+  a.p_sb = p_sb;
+  a.B = B;
+  a.H = H;
+  a.N = N;
+  a.D = D;
+  a.interleaved = interleaved ? 1 : 0;
+  a.inverse = inverse ? 1 : 0;
+  return hip_status(sage::launch_rotary(a, (hipStream_t)stream), "sage_rotary launch");
+}
+
+int sage_cache_write(int dtype, int k_int8, const void* k, int64_t k_sb, int64_t k_sh,
+                     int64_t k_sr, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_sr,
+                     int64_t B, int64_t H_kv, int64_t N, int64_t D, void* k8, float* sk, void* v8,
+                     float* sv, int64_t num_pages, const int32_t* block_table, int64_t t_sb,
+                     int64_t max_pages, const int32_t* start, const int32_t* lens,
+                     const float* table, int64_t table_rows, int64_t R, const int32_t* positions,
+                     int64_t p_sb, int interleaved, void* stream) {
+  sage::CacheRowsArgs a = {};
+  int rc = check_pool(dtype, k_int8, k8, sk, v8, sv, num_pages, block_table, t_sb, max_pages, &a.pool);
+  if (rc) return rc;
+  if ((rc = check_rows("the cache write", B, H_kv, N, D))) return rc;
+  if ((rc = check_view("k", k, k_sb, k_sh, k_sr))) return rc;
+  if ((rc = check_view("v", v, v_sb, v_sh, v_sr))) return rc;
+  if (!start) return fail(SAGE_ERR_INVALID, "start: the sequences' lengths before the call are NULL");
+  if (table && (rc = check_rotary(table, table_rows, R, positions, p_sb, N, D))) return rc;
+  a.dtype = dtype;
+  a.k = const_cast<void*>(k);
+  a.k_sb = k_sb;
+  a.k_sh = k_sh;
+  a.k_sr = k_sr;
+  a.v = const_cast<void*>(v);
+  a.v_sb = v_sb;
+  a.v_sh = v_sh;
+  a.v_sr = v_sr;
+  a.B = B;
+  a.H = H_kv;
+  a.N = N;
+  a.D = D;
+  a.start = start;
+  a.lens = lens;
+  a.rotary.table = table;
+  a.rotary.rows = table_rows;
+  a.rotary.R = R;
+  a.rotary.positions = positions;
+  a.rotary.p_sb = p_sb;
+  a.rotary.interleaved = interleaved ? 1 : 0;
+  return hip_status(sage::launch_cache_write(a, (hipStream_t)stream), "sage_cache_write launch");
+}
+
+int sage_cache_read(int dtype, int k_int8, const void* k8, const float* sk, const void* v8,
+                    const float* sv, int64_t num_pages, const int32_t* block_table, int64_t t_sb,
+                    int64_t max_pages, const int32_t* start, const int32_t* lens, void* k,
+                    int64_t k_sb, int64_t k_sh, int64_t k_sr, void* v, int64_t v_sb, int64_t v_sh,
+                    int64_t v_sr, int64_t B, int64_t H_kv, int64_t N, int64_t D, void* stream) {
+  sage::CacheRowsArgs a = {};
+  int rc = check_pool(dtype, k_int8, k8, sk, v8, sv, num_pages, block_table, t_sb, max_pages, &a.pool);
+  if (rc) return rc;
+  if ((rc = check_rows("the cache read", B, H_kv, N, D))) return rc;
+  if ((rc = check_view("k", k, k_sb, k_sh, k_sr))) return rc;
+  if ((rc = check_view("v", v, v_sb, v_sh, v_sr))) return rc;
+  if (!lens) return fail(SAGE_ERR_INVALID, "lens: the tokens to read are NULL");
+  a.dtype = dtype;
+  a.k = k;
+  a.k_sb = k_sb;
+  a.k_sh = k_sh;
+  a.k_sr = k_sr;
+  a.v = v;
+  a.v_sb = v_sb;
+  a.v_sh = v_sh;
+  a.v_sr = v_sr;
+  a.B = B;
+  a.H = H_kv;
+  a.N = N;
+  a.D = D;
+  a.start = start;
+  a.lens = lens;
+  return hip_status(sage::launch_cache_read(a, (hipStream_t)stream), "sage_cache_read launch");
+}
+
+int64_t sage_cache_attn_workspace_bytes(int64_t B, int64_t H, int64_t H_kv, int64_t T,
+                                        int64_t max_pages, int64_t D) {
+  const int rc = check_cache_attn_shape(B, H, H_kv, T, max_pages, D);
+  if (rc) return -rc;
+  g_err.clear();
+  return (int64_t)sage::cache_attn_workspace_bytes(
+      sage::cache_attn_plan(B, H, H_kv, T, max_pages), D);
+}
+
+int sage_cache_attn(int dtype, int k_int8, const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sr,
+                    const void* k8, const float* sk, const void* v8, const float* sv,
+                    int64_t num_pages, const int32_t* block_table, int64_t t_sb,
+                    int64_t max_pages, const int32_t* kv_lens, const int32_t* q_lens,
+                    const void* mask, int64_t m_sb, int64_t m_sr, void* o, int64_t o_sb,
+                    int64_t o_sh, int64_t o_sr, int64_t B, int64_t H, int64_t T, int64_t H_kv,
+                    int64_t D, float sm_scale, float* lse, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  sage::CacheAttnArgs a = {};
+  int rc = check_pool(dtype, k_int8, k8, sk, v8, sv, num_pages, block_table, t_sb, max_pages, &a.pool);
+  if (rc) return rc;
+  if ((rc = check_cache_attn_shape(B, H, H_kv, T, max_pages, D))) return rc;
+  if ((rc = check_view("q", q, q_sb, q_sh, q_sr))) return rc;
+  if ((rc = check_view("o", o, o_sb, o_sh, o_sr))) return rc;
+  if (!kv_lens) return fail(SAGE_ERR_INVALID, "kv_lens is NULL");
+  if (mask && (m_sr < T || (m_sb != 0 && m_sb < T)))
+    return fail(SAGE_ERR_INVALID, "tree_mask: rows overlap (strides %lld, %lld for T=%lld)",
+                (long long)m_sb, (long long)m_sr, (long long)T);
+  if (!(sm_scale > 0.0f) || !(sm_scale < 3.0e38f))
+    return fail(SAGE_ERR_INVALID, "sm_scale: must be positive and finite (got %g)", (double)sm_scale);
+  if (lse && ((uintptr_t)lse & 3u))
+    return fail(SAGE_ERR_INVALID, "ptr_align: lse must be 4-byte aligned");
+  const size_t need = sage::cache_attn_workspace_bytes(
+      sage::cache_attn_plan(B, H, H_kv, T, max_pages), D);
+  if (need && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+    return fail(SAGE_ERR_INVALID, "workspace: need %zu bytes, 16-byte aligned (got %zu)", need,
+                workspace_bytes);
+  a.dtype = dtype;
+  a.q = q;
+  a.q_sb = q_sb;
+  a.q_sh = q_sh;
+  a.q_sr = q_sr;
+  a.o = o;
+  a.o_sb = o_sb;
+  a.o_sh = o_sh;
+  a.o_sr = o_sr;
+  a.B = B;
+  a.H = H;
+  a.T = T;
+  a.H_kv = H_kv;
+  a.D = D;
+  a.kv_lens = kv_lens;
+  a.q_lens = q_lens;
+  a.mask = mask;
+  a.m_sb = m_sb;
+  a.m_sr = m_sr;
+  a.sm_scale = sm_scale;
+  a.lse = lse;
+  a.workspace = workspace;
+  return hip_status(sage::launch_cache_attn(a, (hipStream_t)stream), "sage_cache_attn launch");
 }
 
 int sage_quant_q(int dtype, int qk_int8, const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sr,

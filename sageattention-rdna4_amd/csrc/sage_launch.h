@@ -97,4 +97,75 @@ hipError_t launch_layout_probe(const void* a, const void* bt, int32_t* c, const 
 hipError_t launch_mfma_peak(bool int8, int64_t blocks, int64_t iters, int64_t* clocks,
                             hipStream_t stream);
 
+// Rotary positions: a pair (a, b) of the first R columns becomes (a c - b s, b c + a s). `table` holds
+// R/2 cosines and R/2 sines per position; null where a cache write rotates nothing.
+struct RotaryArgs {
+  int dtype;
+  const void* x;
+  int64_t x_sb, x_sh, x_sr;
+  void* o;
+  int64_t o_sb, o_sh, o_sr;
+  const float* table;
+  int64_t rows, R;
+  const int32_t* positions;   // (B, N), rows p_sb apart
+  int64_t p_sb;
+  int64_t B, H, N, D;
+  int interleaved, inverse;
+};
+hipError_t launch_rotary(const RotaryArgs& a, hipStream_t stream);
+
+// A cache's pool of pages of 64 tokens, (num_pages, H_kv, 64, D) codes and (num_pages, H_kv, 64)
+// scales, and the page numbers of B sequences.
+struct CachePool {
+  int k_int8;
+  void* k8;
+  float* sk;
+  void* v8;
+  float* sv;
+  int64_t num_pages;
+  const int32_t* table;       // (B, max_pages), rows t_sb apart
+  int64_t t_sb, max_pages;
+};
+// Rows written to (k, v are read) or read from (k, v are written) positions start[b] + n of sequence
+// b, n < lens[b]. start null: 0 (reading only); lens null: all N (writing only).
+struct CacheRowsArgs {
+  int dtype;
+  void* k;
+  int64_t k_sb, k_sh, k_sr;
+  void* v;
+  int64_t v_sb, v_sh, v_sr;
+  int64_t B, H, N, D;
+  CachePool pool;
+  const int32_t* start;
+  const int32_t* lens;
+  RotaryArgs rotary;          // of K, when writing: table, rows, R, positions, p_sb, interleaved
+};
+hipError_t launch_cache_write(const CacheRowsArgs& a, hipStream_t stream);
+hipError_t launch_cache_read(const CacheRowsArgs& a, hipStream_t stream);
+
+struct CacheAttnArgs {
+  int dtype;
+  const void* q;
+  int64_t q_sb, q_sh, q_sr;
+  void* o;
+  int64_t o_sb, o_sh, o_sr;
+  int64_t B, H, T, H_kv, D;
+  CachePool pool;
+  const int32_t* kv_lens;
+  const int32_t* q_lens;      // null: T each
+  const void* mask;           // (B or 1, T, T) bytes; null: causal among the new tokens
+  int64_t m_sb, m_sr;
+  float sm_scale;
+  float* lse;                 // optional (B, H, T)
+  void* workspace;
+};
+// How a call is cut up: `rows` rows of a K/V head's T * H / H_kv per block, `splits` parts of each
+// sequence's pages. Sizes alone decide it, so a captured call and its workspace agree.
+struct CacheAttnPlan {
+  int64_t rows, row_blocks, splits, blocks;
+};
+CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_t max_pages);
+size_t cache_attn_workspace_bytes(const CacheAttnPlan& p, int64_t D);
+hipError_t launch_cache_attn(const CacheAttnArgs& a, hipStream_t stream);
+
 }  // namespace sage

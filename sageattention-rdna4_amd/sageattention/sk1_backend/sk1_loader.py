@@ -165,6 +165,20 @@ class SageLib:
         L.sage_mfma_peak_probe.argtypes = [i32, i64, i64, vp, vp]
         L.sage_attn_kernel_choice.restype = i32
         L.sage_attn_kernel_choice.argtypes = [i64, i64, i64, i64, i32, i64]
+        pool = [vp] * 4 + [i64, vp, i64, i64]     # k8, sk, v8, sv, num_pages, block_table
+        view = [vp, i64, i64, i64]
+        L.sage_rotary.restype = i32
+        L.sage_rotary.argtypes = [i32] + view * 2 + [i64] * 4 + [vp, i64, i64, vp, i64, i32, i32, vp]
+        L.sage_cache_write.restype = i32
+        L.sage_cache_write.argtypes = ([i32] * 2 + view * 2 + [i64] * 4 + pool
+                                       + [vp, vp, vp, i64, i64, vp, i64, i32, vp])
+        L.sage_cache_read.restype = i32
+        L.sage_cache_read.argtypes = [i32] * 2 + pool + [vp, vp] + view * 2 + [i64] * 4 + [vp]
+        L.sage_cache_attn.restype = i32
+        L.sage_cache_attn.argtypes = ([i32] * 2 + view + pool + [vp, vp, vp, i64, i64] + view
+                                      + [i64] * 5 + [f32, vp, vp, ctypes.c_size_t, vp])
+        L.sage_cache_attn_workspace_bytes.restype = i64
+        L.sage_cache_attn_workspace_bytes.argtypes = [i64] * 6
         self.version = int(L.sage_version())
         self.build_id = L.sage_build_id().decode()
         images = hip_runtime_images()
@@ -314,6 +328,74 @@ class SageLib:
             _ptr(mean), _ptr(workspace), int(workspace.numel() * workspace.element_size()),
             ctypes.c_void_p(torch_stream(k.device)))
         self._check(rc, "sage_kseq_mean")
+
+    # The serving entry points: q, k, v, x and o are logical (B, H, N, D) views, `cache` holds a pool
+    # (k8, sk, v8, sv, num_pages, int8), t_sb, p_sb, m_sb are elements between two sequences' rows.
+    def rotary(self, x, o, table, positions, p_sb, *, interleaved, inverse, stream):
+        """Rotary positions of `x` into `o` (see `sage_rotary`)."""
+        B, H, N, D = x.shape
+        x_sb, x_sh, x_sr, _ = x.stride()
+        o_sb, o_sh, o_sr, _ = o.stride()
+        rows, R = table.shape
+        rc = self.lib.sage_rotary(
+            _dtype_code(x.dtype), x.data_ptr(), x_sb, x_sh, x_sr, o.data_ptr(), o_sb, o_sh, o_sr,
+            B, H, N, D, table.data_ptr(), rows, R, positions.data_ptr(), p_sb,
+            int(bool(interleaved)), int(bool(inverse)), stream)
+        if rc:
+            self._check(rc, "sage_rotary")
+
+    def cache_write(self, cache, k, v, block_table, t_sb, start, lens, table, positions, p_sb, *,
+                    interleaved, stream):
+        """Rows of `k`, `v` quantized into the cache's pages (see `sage_cache_write`)."""
+        B, H, N, D = k.shape
+        k_sb, k_sh, k_sr, _ = k.stride()
+        v_sb, v_sh, v_sr, _ = v.stride()
+        rows, R = (0, 0) if table is None else table.shape
+        rc = self.lib.sage_cache_write(
+            _dtype_code(k.dtype), int(cache.int8), k.data_ptr(), k_sb, k_sh, k_sr, v.data_ptr(),
+            v_sb, v_sh, v_sr, B, H, N, D, cache.k8.data_ptr(), cache.sk.data_ptr(),
+            cache.v8.data_ptr(), cache.sv.data_ptr(), cache.num_pages, block_table.data_ptr(), t_sb,
+            block_table.shape[1], start.data_ptr(), None if lens is None else lens.data_ptr(),
+            None if table is None else table.data_ptr(), rows, R,
+            None if table is None else positions.data_ptr(), p_sb, int(bool(interleaved)), stream)
+        if rc:
+            self._check(rc, "sage_cache_write")
+
+    def cache_read(self, cache, k, v, block_table, t_sb, start, lens, *, stream):
+        """Cached rows into `k`, `v` (see `sage_cache_read`)."""
+        B, H, N, D = k.shape
+        k_sb, k_sh, k_sr, _ = k.stride()
+        v_sb, v_sh, v_sr, _ = v.stride()
+        rc = self.lib.sage_cache_read(
+            _dtype_code(k.dtype), int(cache.int8), cache.k8.data_ptr(), cache.sk.data_ptr(),
+            cache.v8.data_ptr(), cache.sv.data_ptr(), cache.num_pages, block_table.data_ptr(), t_sb,
+            block_table.shape[1], None if start is None else start.data_ptr(), lens.data_ptr(),
+            k.data_ptr(), k_sb, k_sh, k_sr, v.data_ptr(), v_sb, v_sh, v_sr, B, H, N, D, stream)
+        if rc:
+            self._check(rc, "sage_cache_read")
+
+    def cache_attn_workspace_bytes(self, B, H, H_kv, T, max_pages, D):
+        n = self.lib.sage_cache_attn_workspace_bytes(B, H, H_kv, T, max_pages, D)
+        if n < 0:
+            self._check(-n, "sage_cache_attn_workspace_bytes")
+        return n
+
+    def cache_attn(self, cache, q, o, block_table, t_sb, kv_lens, q_lens, mask, m_sb, m_sr, sm_scale,
+                   lse, workspace, workspace_bytes, *, stream):
+        """Attention of `q` over the cache into `o` (see `sage_cache_attn`)."""
+        B, H, T, D = q.shape
+        q_sb, q_sh, q_sr, _ = q.stride()
+        o_sb, o_sh, o_sr, _ = o.stride()
+        rc = self.lib.sage_cache_attn(
+            _dtype_code(q.dtype), int(cache.int8), q.data_ptr(), q_sb, q_sh, q_sr,
+            cache.k8.data_ptr(), cache.sk.data_ptr(), cache.v8.data_ptr(), cache.sv.data_ptr(),
+            cache.num_pages, block_table.data_ptr(), t_sb, block_table.shape[1], kv_lens.data_ptr(),
+            None if q_lens is None else q_lens.data_ptr(), None if mask is None else mask.data_ptr(),
+            m_sb, m_sr, o.data_ptr(), o_sb, o_sh, o_sr, B, H, T, cache.num_heads, D, sm_scale,
+            None if lse is None else lse.data_ptr(),
+            None if workspace is None else workspace.data_ptr(), workspace_bytes, stream)
+        if rc:
+            self._check(rc, "sage_cache_attn")
 
     def quant_q(self, q, sm_scale, *, qk_int8):
         """Q quantized exactly as the main loop quantizes it: `(q8, sq, cq)` on q's device."""
