@@ -12,12 +12,19 @@
 // what a bf16 weight would lose) without overflow, and 28 binades below a row's largest weight are
 // still normal numbers. Sums, maxima and outputs are fp32 until the one rounding of the output.
 //
-// Layout. A wave holds 16 R rows of one K/V head (row r: token r / G, head r % G of the group), and
-// takes a page of 64 keys at a time straight from memory to registers: S^T = K Q^T by 16x16x32 MFMAs
-// (keys down, rows across), whose results are, lane for lane, the B operand of O^T = V^T W^T when
-// the keys are taken in the order 4g .. 4g+3 of two 16-key tiles (g the lane's group of 16). Weights
-// never leave their lanes. A row of V is read 16 lanes wide and its bytes converted one by one into
-// the operand whose element is the key.
+// Layout. A wave holds 16 R rows of one K/V head (row r: token r / G, head r % G of the group) and
+// takes 64 keys, a page, at a time: S^T = K Q^T by 16x16x32 MFMAs (keys down, rows across), whose
+// results are, lane for lane, the B operand of O^T = V^T W^T when the keys are taken in the order
+// 4g .. 4g+3 of two 16-key tiles (g the lane's group of 16). Weights never leave their lanes. A row of
+// V is read 16 lanes wide and its bytes converted one by one into the operand whose element is the key.
+// What depends on a key alone (ks, lv, 1/SV) is worked out by one lane for each key.
+//
+// Two kernels share that step:
+//   stream: up to 32 rows of a K/V head (decoding, small trees). HBM-bound: each wave has pages of its
+//           own, straight from memory to registers, and a block's waves are merged through LDS.
+//   shared: more rows. MFMA- and VALU-bound: a block's four waves have rows of their own and share
+//           each page, of which every wave converts a quarter to 16 bits in LDS.
+// Either cuts a sequence's pages into S interleaved parts, which a second launch joins in order.
 #include "sage_device.h"
 #include "sage_launch.h"
 
@@ -29,7 +36,6 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-constexpr int WAVES = 4;            // of a block
 constexpr float W_SHIFT = 14.0f;    // weights are at most 2^14
 constexpr float SV_LEAST = 0x1p-100f;
 constexpr float NEG_INF = -__builtin_inff();
@@ -134,7 +140,7 @@ struct Shape {
   float* lse;
   float* part_o;    // (tiles, S, rows of a block, D)
   float* part_ml;   // (tiles, S, rows of a block, 2)
-  int H, H_kv, G, T, S, RB;
+  int H, H_kv, G, T, S, RB, units;
   float c;          // sm_scale log2 e
 };
 
@@ -154,89 +160,237 @@ __device__ __forceinline__ Lens lens_of(const Shape& p, int b) {
   return n;
 }
 
-// grid: block = (tile * S + split), tile = (b * H_kv + K/V head) * RB + row block of 16 R rows. The
-// block's waves take its pages in turn and are merged through LDS.
-template <typename T, bool KINT8, int D, int R>
-__global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(Shape p) {
+// Block -> (plane, part, row block): the row blocks of one part of a plane's pages run on one XCD (blocks
+// go round the 8 XCDs), whose L2 then holds the pages that they all read.
+struct Place {
+  int plane, b, hk, split, rb;
+  int64_t part;   // number of (plane, split, row block)
+  bool live;
+};
+__device__ __forceinline__ Place place_of(const Shape& p) {
+  Place w;
+  const u32 id = blockIdx.x, oct = id / (8u * (u32)p.RB), in = id - oct * 8u * (u32)p.RB;
+  w.rb = (int)(in / 8u);
+  const u32 unit = oct * 8u + in % 8u;
+  w.live = unit < (u32)p.units;
+  w.plane = (int)(unit / (u32)p.S);
+  w.split = (int)(unit - (u32)w.plane * (u32)p.S);
+  w.b = w.plane / p.H_kv;
+  w.hk = w.plane - w.b * p.H_kv;
+  w.part = (int64_t)unit * p.RB + w.rb;
+  return w;
+}
+
+// A wave's rows and running sums.
+template <typename T, int D, int R>
+struct Rows {
+  typename Frag<T>::type q[R][D / 32];
+  int token[R];
+  f32x4 acc[R][D / 16];
+  float m[R], l[R];
+
+  // lane l15 holds row l15 of each 16, columns 64c + 16g + 8s in k-step 2c + s
+  __device__ __forceinline__ void load(const Shape& p, int b, int hk, int row0, int l15, int g) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int row = row0 + 16 * r + l15;
+      token[r] = row / p.G;
+      const int h = hk * p.G + row - token[r] * p.G;
+      const bool live = token[r] < p.T;
+      const T* src = (const T*)p.q + b * p.q_sb + (live ? h * p.q_sh + token[r] * p.q_sr : 0) + 16 * g;
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t) {
+        u32x4 w = *(const u32x4*)(src + 64 * (t >> 1) + 8 * (t & 1));
+        if (!live) w = (u32x4){0, 0, 0, 0};
+        __builtin_memcpy(&q[r][t], &w, 16);
+      }
+      m[r] = NEG_INF, l[r] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) acc[r][e] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  }
+};
+
+// What the softmax needs of each key, by one lane a key, into 3 x 64 floats: SK sm_scale log2 e, log2 SV
+// and 1 / SV. A scale of 0 (a token never written) weighs as its key says and adds zeros; one of NaN (a
+// row that is not finite) makes the weights of the rows that see it NaN, and 1/SV 0, so that the
+// others' weights of 0 leave their sums alone. So do keys behind the sequence's end.
+__device__ __forceinline__ void key_consts(float* dst, int key, float sk, float sv, float c, bool held) {
+  const float v = sv < SV_LEAST ? SV_LEAST : sv;
+  dst[key] = sk * c;
+  dst[64 + key] = __builtin_amdgcn_logf(v);
+  dst[128 + key] = held ? fmaxf(__builtin_amdgcn_rcpf(v), 0.0f) : 0.0f;
+}
+
+// Scores to weights: u = t + log2 SV, where the page holds new tokens or ends the sequence only for the
+// keys that each row sees; then the running maximum and sum, and the weights as the PV MFMA takes them.
+template <typename T, int D, int R>
+__device__ __forceinline__ void softmax_step(const Shape& p, const Lens& n, int b, int key0,
+                                             const float* consts, int g, Rows<T, D, R>& w,
+                                             f32x4 (&s)[R][4], f16x8 (&wf)[R][2]) {
+  const int prefix = n.kv - n.tokens;    // tokens that every new token sees
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt) {
+    const f32x4 ks = *(const f32x4*)(consts + 16 * kt + 4 * g);
+    const f32x4 lv = *(const f32x4*)(consts + 64 + 16 * kt + 4 * g);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[r][kt][i] = __builtin_fmaf(s[r][kt][i], ks[i], lv[i]);
+  }
+  if (key0 + NPAD > prefix || key0 + NPAD > n.keys) {
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = key0 + 16 * kt + 4 * g + i, draft = key - prefix;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          bool seen = key < n.keys;
+          if (seen && draft >= 0) {
+            if (p.mask)
+              seen = w.token[r] < n.tokens && p.mask[b * p.m_sb + w.token[r] * p.m_sr + draft] != 0;
+            else
+              seen = draft <= w.token[r];
+          }
+          s[r][kt][i] = seen ? s[r][kt][i] : NEG_INF;
+        }
+      }
+  }
+  float top[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    top[r] = NEG_INF;
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top[r] = fmaxf(top[r], s[r][kt][i]);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) top[r] = max_groups(top[r]);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (__builtin_amdgcn_ballot_w64(top[r] > w.m[r])) {
+      const float now = fmaxf(top[r], w.m[r]);
+      // a row that has seen nothing keeps sums of zero
+      const float alpha = __builtin_amdgcn_exp2f(w.m[r] - (now == NEG_INF ? 0.0f : now));
+      w.m[r] = now;
+      w.l[r] *= alpha;
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) w.acc[r][e] *= alpha;
+    }
+    const float shift = (w.m[r] == NEG_INF ? 0.0f : w.m[r]) - W_SHIFT;
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      const f32x4 rsv = *(const f32x4*)(consts + 128 + 16 * kt + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = __builtin_amdgcn_exp2f(s[r][kt][i] - shift);
+        w.l[r] = __builtin_fmaf(x, rsv[i], w.l[r]);
+        wf[r][kt >> 1][4 * (kt & 1) + i] = (f16)x;
+      }
+    }
+  }
+}
+
+// N columns of an output row.
+template <typename T, int N>
+__device__ __forceinline__ void store_row(T* o, const float (&f)[N], float inv, bool some) {
+  T out[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) out[e] = (T)(some ? f[e] * inv : 0.0f);
+  if constexpr (N == 8) {
+    u32x4 w;
+    __builtin_memcpy(&w, out, 16);
+    *(u32x4*)o = w;
+  } else if constexpr (N == 4) {
+    u32x2 w;
+    __builtin_memcpy(&w, out, 8);
+    *(u32x2*)o = w;
+  } else {
+    u32 w;
+    __builtin_memcpy(&w, out, 4);
+    *(u32*)o = w;
+  }
+}
+
+__device__ __forceinline__ float lse_of(float top, float sum) {
+  return (top - W_SHIFT + __log2f(sum)) * LN2_F;
+}
+
+// A row's N columns from col on: to the output where the call has one part, else to the workspace
+// (at row `at` of the parts), where nothing is read that a part with a sum of 0 did not write.
+template <typename T, int D, int N>
+__device__ __forceinline__ void finish_row(const Shape& p, const Lens& n, int b, int hk, int row,
+                                           int64_t at, int col, const float (&f)[N], float top,
+                                           float sum) {
+  const int tok = row / p.G, h = hk * p.G + row - tok * p.G;
+  if (tok >= p.T) return;
+  if (p.S > 1) {
+    if (col == 0) *(float2*)(p.part_ml + 2 * at) = make_float2(top, sum);
+    if (sum != 0.0f) {
+#pragma unroll
+      for (int e = 0; e < N; e += 4)
+        *(f32x4*)(p.part_o + at * D + col + e) = (f32x4){f[e], f[e + 1], f[e + 2], f[e + 3]};
+    }
+    return;
+  }
+  const bool some = tok < n.tokens && sum != 0.0f;
+  store_row<T, N>((T*)p.o + b * p.o_sb + h * p.o_sh + tok * p.o_sr + col, f, some ? 1.0f / sum : 0.0f,
+                  some);
+  if (p.lse && col == 0)
+    p.lse[((int64_t)b * p.H + h) * p.T + tok] = some ? lse_of(top, sum) : NEG_INF;
+}
+
+// grid: one block per part of a plane (row blocks: 1). Wave w of part s takes pages s W + w, then every
+// (S W)-th: which these are does not wait for the sequence's length.
+template <typename T, bool KINT8, int D, int R, int W>
+__global__ __launch_bounds__(64 * W, 2) void cache_attn_stream_kernel(Shape p) {
   typedef typename Frag<T>::type frag;
-  constexpr int KC = D / 64, KT = D / 32, VE = D / 16, VW = VE / 4, ROWS = 16 * R, LD = D + 4;
-  __shared__ __attribute__((aligned(16))) float lds_o[WAVES][16][LD];
-  __shared__ float lds_ml[WAVES][16][2];
+  constexpr int KC = D / 64, KT = D / 32, VE = D / 16, VW = VE / 4, LD = D + 4;
+  __shared__ __attribute__((aligned(16))) float lds_o[W][16][LD];
+  __shared__ float lds_ml[W][16][2];
+  __shared__ __attribute__((aligned(16))) float lds_c[W][192];
 
   const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const u32 tile = blockIdx.x / (u32)p.S, split = blockIdx.x - tile * (u32)p.S;
-  const u32 plane = tile / (u32)p.RB;
-  const int rb = (int)(tile - plane * (u32)p.RB);
-  const int b = (int)(plane / (u32)p.H_kv), hk = (int)(plane - (u32)b * (u32)p.H_kv);
+  const Place at = place_of(p);
+  if (!at.live) return;
+  const int b = at.b, hk = at.hk;
   const Lens n = lens_of(p, b);
-  const int prefix = n.kv - n.tokens;    // tokens that every new token sees
-  const int row0 = rb * ROWS;
+  Rows<T, D, R> w;
+  w.load(p, b, hk, 0, l15, g);
 
-  // rows of Q: lane l15 holds row l15 of each 16, columns 64c + 16g + 8s in k-step 2c + s
-  frag qf[R][KT];
-  int token[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int row = row0 + 16 * r + l15;
-    token[r] = row / p.G;
-    const int h = hk * p.G + row - token[r] * p.G;
-    const bool live = token[r] < p.T;
-    const T* q = (const T*)p.q + b * p.q_sb + (live ? h * p.q_sh + token[r] * p.q_sr : 0) + 16 * g;
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      u32x4 w = *(const u32x4*)(q + 64 * (t >> 1) + 8 * (t & 1));
-      if (!live) w = (u32x4){0, 0, 0, 0};
-      __builtin_memcpy(&qf[r][t], &w, 16);
-    }
-  }
-
-  f32x4 acc[R][VE];
-  float m[R], l[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    m[r] = NEG_INF, l[r] = 0.0f;
-#pragma unroll
-    for (int e = 0; e < VE; ++e) acc[r][e] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-  }
-
-  const int pages = row0 < n.tokens * p.G ? (n.keys + NPAD - 1) / NPAD : 0;
-  const int per = (pages + p.S - 1) / p.S;
-  const int first = (int)split * per, last = first + per < pages ? first + per : pages;
+  const int pages = n.tokens > 0 ? (n.keys + NPAD - 1) / NPAD : 0;
   const int* table = p.table + b * p.t_sb;
-
-  for (int pg = first + wave; pg < last; pg += WAVES) {
+  for (int pg = at.split * W + wave; pg < pages; pg += p.S * W) {
     const int id = __builtin_amdgcn_readfirstlane(table[pg]);
     if (id < 0 || id >= p.num_pages) continue;   // no page: nothing to see
     const int64_t base = ((int64_t)id * p.H_kv + hk) * NPAD;
     const u8* kp = p.k8 + base * D + (int64_t)l15 * D + 16 * g;
     const u8* vp = p.v8 + base * D + (int64_t)(4 * g) * D + l15 * VE;
+    const float sk = p.sk[base + lane], sv = p.sv[base + lane];
     u32x4 kw[4][KC];
     u32 vw[4][VW][4];   // [key tile][word of the row's 4 VW bytes][key 4g + j]
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
       for (int c = 0; c < KC; ++c) kw[kt][c] = *(const u32x4*)(kp + 16 * kt * D + 64 * c);
-    f32x4 sk[4], sv[4];
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      sk[kt] = *(const f32x4*)(p.sk + base + 16 * kt + 4 * g);
-      sv[kt] = *(const f32x4*)(p.sv + base + 16 * kt + 4 * g);
-    }
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const u8* at = vp + (16 * kt + j) * D;
+        const u8* src = vp + (16 * kt + j) * D;
         if constexpr (VW == 2) {
-          const u32x2 w = *(const u32x2*)at;
-          vw[kt][0][j] = w[0], vw[kt][1][j] = w[1];
+          const u32x2 x = *(const u32x2*)src;
+          vw[kt][0][j] = x[0], vw[kt][1][j] = x[1];
         } else {
-          vw[kt][0][j] = *(const u32*)at;
+          vw[kt][0][j] = *(const u32*)src;
         }
       }
+    const int key0 = pg * NPAD;
+    key_consts(lds_c[wave], lane, sk, sv, p.c, key0 + lane < n.keys);
 
-    // S^T, then u = t + log2 SV
     f32x4 s[R][4];
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
@@ -246,80 +400,21 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(Shape p) {
       for (int t = 0; t < KT; ++t) {
         const frag kf = k_frag<T, KINT8>(kw[kt][t >> 1][2 * (t & 1)], kw[kt][t >> 1][2 * (t & 1) + 1]);
 #pragma unroll
-        for (int r = 0; r < R; ++r) s[r][kt] = mfma(kf, qf[r][t], s[r][kt]);
+        for (int r = 0; r < R; ++r) s[r][kt] = mfma(kf, w.q[r][t], s[r][kt]);
       }
     }
-    f32x4 rsv[4];
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // a scale of 0 (a token never written) weighs as its key says and adds zeros; one of NaN (a row
-        // that is not finite) makes the weights of the rows that see it NaN, and 1/SV 0, so that the
-        // others' weights of 0 leave their sums alone
-        const float v = sv[kt][i] < SV_LEAST ? SV_LEAST : sv[kt][i];
-        const float lv = __builtin_amdgcn_logf(v), ks = sk[kt][i] * p.c;
-        rsv[kt][i] = fmaxf(__builtin_amdgcn_rcpf(v), 0.0f);
-#pragma unroll
-        for (int r = 0; r < R; ++r) s[r][kt][i] = __builtin_fmaf(s[r][kt][i], ks, lv);
-      }
-
-    const int key0 = pg * NPAD;
-    if (key0 + NPAD > prefix || key0 + NPAD > n.keys) {
-      // the page holds new tokens or ends the sequence: each row sees what its mask leaves it
+    if (key0 + NPAD > n.keys) {   // whatever lies behind the end: no NaN may meet a weight of zero
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = key0 + 16 * kt + 4 * g + i, draft = key - prefix;
-          const bool held = key < n.keys;
-          if (!held) {   // whatever lies behind the sequence's end: no NaN may meet a zero weight
-            rsv[kt][i] = 0.0f;
+        for (int j = 0; j < 4; ++j)
+          if (key0 + 16 * kt + 4 * g + j >= n.keys) {
 #pragma unroll
-            for (int w = 0; w < VW; ++w) vw[kt][w][i] = 0;
+            for (int x = 0; x < VW; ++x) vw[kt][x][j] = 0;
           }
-#pragma unroll
-          for (int r = 0; r < R; ++r) {
-            bool seen = held;
-            if (held && draft >= 0) {
-              if (p.mask)
-                seen = token[r] < n.tokens && p.mask[b * p.m_sb + token[r] * p.m_sr + draft] != 0;
-              else
-                seen = draft <= token[r];
-            }
-            s[r][kt][i] = seen ? s[r][kt][i] : NEG_INF;
-          }
-        }
     }
-
     f16x8 wf[R][2];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float top = NEG_INF;
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[r][kt][i]);
-      top = max_groups(top);
-      if (__builtin_amdgcn_ballot_w64(top > m[r])) {
-        const float now = fmaxf(top, m[r]);
-        // a row that has seen nothing keeps sums of zero
-        const float alpha = __builtin_amdgcn_exp2f(m[r] - (now == NEG_INF ? 0.0f : now));
-        m[r] = now;
-        l[r] *= alpha;
-#pragma unroll
-        for (int e = 0; e < VE; ++e) acc[r][e] *= alpha;
-      }
-      const float shift = (m[r] == NEG_INF ? 0.0f : m[r]) - W_SHIFT;
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float w = __builtin_amdgcn_exp2f(s[r][kt][i] - shift);
-          l[r] = __builtin_fmaf(w, rsv[kt][i], l[r]);
-          wf[r][kt >> 1][4 * (kt & 1) + i] = (f16)w;
-        }
-    }
+    softmax_step<T, D, R>(p, n, b, key0, lds_c[wave], g, w, s, wf);
 
     // O^T += V^T W^T: tile e's row x is column VE x + e
     static_for<0, 2>([&](auto uc) {
@@ -328,76 +423,176 @@ __global__ __launch_bounds__(64 * WAVES) void cache_attn_kernel(Shape p) {
         constexpr int e = decltype(ec)::value;
         const f16x8 vf = v_frag<e % 4>(vw[2 * u][e / 4], vw[2 * u + 1][e / 4]);
 #pragma unroll
-        for (int r = 0; r < R; ++r) acc[r][e] = mfma(vf, wf[r][u], acc[r][e]);
+        for (int r = 0; r < R; ++r) w.acc[r][e] = mfma(vf, wf[r][u], w.acc[r][e]);
       });
     });
   }
 
-  // the waves' results merged, 16 rows at a time; thread tid: row tid / 16, columns VE (tid % 16)
-  const int tid = threadIdx.x, orow = tid >> 4, ocol = (tid & 15) * VE;
+  // the waves' results merged, 16 rows at a time; each thread has N columns of a row
+  constexpr int TPR = 4 * W, N = D / TPR;   // threads of a row
+  const int tid = threadIdx.x, orow = tid / TPR, ocol = (tid % TPR) * N;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const float total = sum_groups(l[r]);
+    const float total = sum_groups(w.l[r]);
     if (r) __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < VE; e += 4)
         *(f32x4*)&lds_o[wave][l15][VE * (4 * g + i) + e] =
-            (f32x4){acc[r][e][i], acc[r][e + 1][i], acc[r][e + 2][i], acc[r][e + 3][i]};
-    if (g == 0) lds_ml[wave][l15][0] = m[r], lds_ml[wave][l15][1] = total;
+            (f32x4){w.acc[r][e][i], w.acc[r][e + 1][i], w.acc[r][e + 2][i], w.acc[r][e + 3][i]};
+    if (g == 0) lds_ml[wave][l15][0] = w.m[r], lds_ml[wave][l15][1] = total;
     __syncthreads();
     float top = NEG_INF;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, lds_ml[w][orow][0]);
+    for (int x = 0; x < W; ++x) top = fmaxf(top, lds_ml[x][orow][0]);
     const float use = top == NEG_INF ? 0.0f : top;
-    float sum = 0.0f, f[8] = {};
+    float sum = 0.0f, f[N] = {};
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const float a = __builtin_amdgcn_exp2f(lds_ml[w][orow][0] - use);
-      sum += lds_ml[w][orow][1] * a;
+    for (int x = 0; x < W; ++x) {
+      const float a = __builtin_amdgcn_exp2f(lds_ml[x][orow][0] - use);
+      sum += lds_ml[x][orow][1] * a;
 #pragma unroll
-      for (int e = 0; e < VE; ++e) f[e] += lds_o[w][orow][ocol + e] * a;
+      for (int e = 0; e < N; ++e) f[e] += lds_o[x][orow][ocol + e] * a;
     }
-    const int row = row0 + 16 * r + orow, tok = row / p.G, h = hk * p.G + row - tok * p.G;
-    if (p.S > 1) {
-      const int64_t at = (int64_t)blockIdx.x * ROWS + 16 * r + orow;
-      if (ocol == 0) *(float2*)(p.part_ml + 2 * at) = make_float2(top, sum);
-      if (sum != 0.0f) {
+    finish_row<T, D, N>(p, n, b, hk, 16 * r + orow, at.part * (16 * R) + 16 * r + orow, ocol, f, top, sum);
+  }
+}
+
+// grid: row blocks of 64 R rows x parts of a plane. Part s takes pages s, s + S, ... The page in work
+// lies in LDS as the MFMAs' operands (K: key tile x k-step, V: half x column tile; 1 KB each, one
+// 16-byte piece a lane), the next one's bytes in registers: wave w converts key tile w of K and four
+// operands of V.
+template <typename T, bool KINT8, int D, int R>
+__global__ __launch_bounds__(256, 2) void cache_attn_shared_kernel(Shape p) {
+  typedef typename Frag<T>::type frag;
+  constexpr int KC = D / 64, KT = D / 32, VE = D / 16, NV = 2 * VE / 4, ROWS = 64 * R;
+  __shared__ __attribute__((aligned(16))) u32x4 lds_k[2][4][KT][64];
+  __shared__ __attribute__((aligned(16))) u32x4 lds_v[2][2][VE][64];
+  __shared__ __attribute__((aligned(16))) float lds_c[2][192];
+
+  const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Place at = place_of(p);
+  if (!at.live) return;
+  const int b = at.b, hk = at.hk;
+  const Lens n = lens_of(p, b);
+  const int row0 = at.rb * ROWS + 16 * R * wave;
+  Rows<T, D, R> w;
+  w.load(p, b, hk, row0, l15, g);
+
+  const int pages = at.rb * ROWS < n.tokens * p.G ? (n.keys + NPAD - 1) / NPAD : 0;
+  const int* table = p.table + b * p.t_sb;
+  // operands u = wave / 2, e = first .. first + NV - 1 of V: bytes of word `word` of a row's VE
+  const int vu = wave >> 1, vfirst = (wave & 1) * NV;
+  u32x4 kw[KC];
+  u32 vw[2][4];
+  float sk = 0.0f, sv = 0.0f;
+  bool there = false;
+  auto fetch = [&](int pg) {
+    const int id = pg < pages ? __builtin_amdgcn_readfirstlane(table[pg]) : -1;
+    there = id >= 0 && id < p.num_pages;
+    if (!there) return;
+    const int64_t base = ((int64_t)id * p.H_kv + hk) * NPAD;
+    const u8* kp = p.k8 + (base + 16 * wave + l15) * D + 16 * g;
 #pragma unroll
-        for (int e = 0; e < VE; e += 4)
-          *(f32x4*)(p.part_o + at * D + ocol + e) = (f32x4){f[e], f[e + 1], f[e + 2], f[e + 3]};
-      }
-    } else if (tok < p.T) {
-      const bool some = tok < n.tokens && sum != 0.0f;
-      const float inv = some ? 1.0f / sum : 0.0f;
-      T* o = (T*)p.o + b * p.o_sb + h * p.o_sh + tok * p.o_sr + ocol;
-      T out[VE];
+    for (int c = 0; c < KC; ++c) kw[c] = *(const u32x4*)(kp + 64 * c);
+    const u8* vp = p.v8 + (base + 32 * vu + 4 * g) * D + l15 * VE + (VE == 8 ? vfirst : 0);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) out[e] = (T)(some ? f[e] * inv : 0.0f);
-      if constexpr (VE == 8) {
-        u32x4 w;
-        __builtin_memcpy(&w, out, 16);
-        *(u32x4*)o = w;
-      } else {
-        u32x2 w;
-        __builtin_memcpy(&w, out, 8);
-        *(u32x2*)o = w;
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) vw[x][j] = *(const u32*)(vp + (16 * x + j) * D);
+    if (wave == 0) sk = p.sk[base + lane], sv = p.sv[base + lane];
+  };
+  auto convert = [&](int pg, int buf) {
+    if (!there) return;
+    const int key0 = pg * NPAD;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      const frag f = k_frag<T, KINT8>(kw[t >> 1][2 * (t & 1)], kw[t >> 1][2 * (t & 1) + 1]);
+      __builtin_memcpy(&lds_k[buf][wave][t][lane], &f, 16);
+    }
+    if (key0 + NPAD > n.keys) {   // whatever lies behind the end: no NaN may meet a weight of zero
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (key0 + 32 * vu + 16 * x + 4 * g + j >= n.keys) vw[x][j] = 0;
+    }
+    static_for<0, 4>([&](auto ec) {
+      constexpr int e = decltype(ec)::value;
+      if constexpr (NV == 4) {
+        const f16x8 f = v_frag<e>(vw[0], vw[1]);
+        __builtin_memcpy(&lds_v[buf][vu][vfirst + e][lane], &f, 16);
+      } else if (e / NV == (wave & 1)) {
+        const f16x8 f = v_frag<e>(vw[0], vw[1]);
+        __builtin_memcpy(&lds_v[buf][vu][e][lane], &f, 16);
       }
-      if (p.lse && ocol == 0)
-        p.lse[((int64_t)b * p.H + h) * p.T + tok] =
-            some ? (top - W_SHIFT + __log2f(sum)) * LN2_F : NEG_INF;
+    });
+    if (wave == 0) key_consts(lds_c[buf], lane, sk, sv, p.c, key0 + lane < n.keys);
+  };
+
+  int pg = at.split, buf = 0;
+  fetch(pg);
+  convert(pg, 0);
+  bool work = there;   // whether the page in LDS is one
+  __syncthreads();
+  for (; pg < pages; pg += p.S) {
+    fetch(pg + p.S);
+    if (work) {
+      f32x4 s[R][4];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r][kt] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          frag kf;
+          __builtin_memcpy(&kf, &lds_k[buf][kt][t][lane], 16);
+#pragma unroll
+          for (int r = 0; r < R; ++r) s[r][kt] = mfma(kf, w.q[r][t], s[r][kt]);
+        }
+      }
+      f16x8 wf[R][2];
+      softmax_step<T, D, R>(p, n, b, pg * NPAD, lds_c[buf], g, w, s, wf);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          f16x8 vf;
+          __builtin_memcpy(&vf, &lds_v[buf][u][e][lane], 16);
+#pragma unroll
+          for (int r = 0; r < R; ++r) w.acc[r][e] = mfma(vf, wf[r][u], w.acc[r][e]);
+        }
+    }
+    convert(pg + p.S, buf ^ 1);   // the other buffer: its readers passed the last barrier
+    work = there;
+    buf ^= 1;
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float sum = sum_groups(w.l[r]);
+    const int row = row0 + 16 * r + l15;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float f[VE];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) f[e] = w.acc[r][e][i];
+      finish_row<T, D, VE>(p, n, b, hk, row, at.part * ROWS + row - at.rb * ROWS, VE * (4 * g + i), f,
+                           w.m[r], sum);
     }
   }
 }
 
-// The splits' results joined, in the order of the splits: D/4 lanes per output row.
+// The parts joined, in their order: a wave per output row, D/64 columns a lane; lane s first has the
+// part s's maximum and sum (S is at most 64).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void cache_attn_join_kernel(Shape p, int rows_per_block, u32 rows) {
-  constexpr int LPR = D / 4;
-  const u32 t = blockIdx.x * 256u + threadIdx.x;
-  const u32 at = t / LPR;
-  const int c = (int)(t % LPR) * 4;
+  constexpr int N = D / 64;
+  const int lane = threadIdx.x & 63;
+  const u32 at = __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6));
   if (at >= rows) return;
   // rows in the order (b, K/V head, row of the plane)
   const u32 M = (u32)p.T * (u32)p.G;
@@ -405,39 +600,51 @@ __global__ __launch_bounds__(256) void cache_attn_join_kernel(Shape p, int rows_
   const int b = (int)(plane / (u32)p.H_kv), hk = (int)(plane - (u32)b * (u32)p.H_kv);
   const int tok = (int)(row / (u32)p.G), h = hk * p.G + (int)row - tok * p.G;
   const Lens n = lens_of(p, b);
-  const u32 rb = row / (u32)rows_per_block;
-  const int64_t first = (((int64_t)plane * p.RB + rb) * p.S) * rows_per_block +
-                        (row - rb * (u32)rows_per_block);
-  float top = NEG_INF, sum = 0.0f;
-  f32x4 f = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (tok < n.tokens) {
-    for (int s = 0; s < p.S; ++s) {
-      const float2 ml = *(const float2*)(p.part_ml + 2 * (first + (int64_t)s * rows_per_block));
-      top = fmaxf(top, ml.x);
+  const u32 rb = row / (u32)rows_per_block, in = row - rb * (u32)rows_per_block;
+  const int64_t first = ((int64_t)plane * p.S * p.RB + rb) * rows_per_block + in;
+  const int64_t step = (int64_t)p.RB * rows_per_block;
+  float2 ml = make_float2(NEG_INF, 0.0f);
+  if (lane < p.S) ml = *(const float2*)(p.part_ml + 2 * (first + lane * step));
+  float top = ml.x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  const float a = __builtin_amdgcn_exp2f(ml.x - (top == NEG_INF ? 0.0f : top));
+  const bool full = ml.y != 0.0f;
+  float sum = full ? ml.y * a : 0.0f;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+  const uint64_t parts = __builtin_amdgcn_ballot_w64(full);
+  float f[N] = {};
+  const float* src = p.part_o + first * D + lane * N;
+  for (int s0 = 0; s0 < p.S; s0 += 8) {   // eight parts requested together
+    float x[8][N];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int s = s0 + i < p.S ? s0 + i : p.S - 1;
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[i][e] = src[s * step * D + e];
     }
-    const float use = top == NEG_INF ? 0.0f : top;
-    for (int s = 0; s < p.S; ++s) {
-      const int64_t i = first + (int64_t)s * rows_per_block;
-      const float2 ml = *(const float2*)(p.part_ml + 2 * i);
-      if (ml.y == 0.0f) continue;
-      const float a = __builtin_amdgcn_exp2f(ml.x - use);
-      sum += ml.y * a;
-      f += *(const f32x4*)(p.part_o + i * D + c) * a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int s = s0 + i;
+      if (s >= p.S || !((parts >> s) & 1)) continue;
+      const float as = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(a), s));
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[e] += x[i][e] * as;
     }
   }
-  const bool some = sum != 0.0f;
+  const bool some = tok < n.tokens && sum != 0.0f;
   const float inv = some ? 1.0f / sum : 0.0f;
-  T out[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) out[e] = (T)(some ? f[e] * inv : 0.0f);
-  u32x2 w;
-  __builtin_memcpy(&w, out, 8);
-  *(u32x2*)((T*)p.o + b * p.o_sb + h * p.o_sh + tok * p.o_sr + c) = w;
-  if (p.lse && c == 0)
-    p.lse[((int64_t)b * p.H + h) * p.T + tok] = some ? (top - W_SHIFT + __log2f(sum)) * LN2_F : NEG_INF;
+  T* o = (T*)p.o + b * p.o_sb + h * p.o_sh + tok * p.o_sr + lane * N;
+  if constexpr (N == 2)
+    store_row<T, 2>(o, f, inv, some);
+  else
+    *o = (T)(some ? f[0] * inv : 0.0f);
+  if (p.lse && lane == 0)
+    p.lse[((int64_t)b * p.H + h) * p.T + tok] = some ? lse_of(top, sum) : NEG_INF;
 }
 
-template <typename T, bool KINT8, int D, int R>
+template <typename T, bool KINT8, int D>
 hipError_t run(const CacheAttnArgs& a, hipStream_t st) {
   const CacheAttnPlan plan = cache_attn_plan(a.B, a.H, a.H_kv, a.T, a.pool.max_pages);
   Shape p;
@@ -469,43 +676,55 @@ hipError_t run(const CacheAttnArgs& a, hipStream_t st) {
   p.T = (int)a.T;
   p.S = (int)plan.splits;
   p.RB = (int)plan.row_blocks;
+  p.units = (int)plan.units;
   p.c = a.sm_scale * LOG2E_F;
-  const int64_t blocks = plan.blocks;
   p.part_o = (float*)a.workspace;
-  p.part_ml = p.part_o + blocks * plan.rows * D;
-  cache_attn_kernel<T, KINT8, D, R><<<(u32)blocks, 64 * WAVES, 0, st>>>(p);
-  hipError_t e = hipGetLastError();
+  p.part_ml = p.part_o + plan.units * plan.row_blocks * plan.rows * D;
+  const u32 blocks = (u32)plan.blocks;
+  if (plan.rows == 16)
+    cache_attn_stream_kernel<T, KINT8, D, 1, 4><<<blocks, 256, 0, st>>>(p);
+  else if (plan.rows == 32)
+    cache_attn_stream_kernel<T, KINT8, D, 2, 4><<<blocks, 256, 0, st>>>(p);
+  else if (plan.rows == 64)
+    cache_attn_shared_kernel<T, KINT8, D, 1><<<blocks, 256, 0, st>>>(p);
+  else
+    cache_attn_shared_kernel<T, KINT8, D, 2><<<blocks, 256, 0, st>>>(p);
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess || plan.splits == 1) return e;
   const int64_t rows = a.B * a.H * a.T;
-  cache_attn_join_kernel<T, D><<<(u32)((rows * (D / 4) + 255) / 256), 256, 0, st>>>(
-      p, (int)plan.rows, (u32)rows);
+  cache_attn_join_kernel<T, D><<<(u32)((rows + 3) / 4), 256, 0, st>>>(p, (int)plan.rows, (u32)rows);
   return hipGetLastError();
 }
 
 template <int D>
 hipError_t run_d(const CacheAttnArgs& a, hipStream_t st) {
-  if (a.dtype == 1) return run<bf16, false, D, 1>(a, st);
-  return a.pool.k_int8 ? run<f16, true, D, 1>(a, st) : run<f16, false, D, 1>(a, st);
+  if (a.dtype == 1) return run<bf16, false, D>(a, st);
+  return a.pool.k_int8 ? run<f16, true, D>(a, st) : run<f16, false, D>(a, st);
 }
 
 }  // namespace
 
 CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_t max_pages) {
   CacheAttnPlan p;
-  p.rows = 16;
-  p.row_blocks = (T * (H / H_kv) + p.rows - 1) / p.rows;
-  const int64_t tiles = B * H_kv * p.row_blocks;
-  // two blocks per compute unit, and four pages at least for each block
-  int64_t s = (512 + tiles - 1) / tiles;
-  const int64_t most = (max_pages + WAVES - 1) / WAVES;
+  const int64_t M = T * (H / H_kv), planes = B * H_kv;
+  p.rows = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  p.row_blocks = (M + p.rows - 1) / p.rows;
+  const int64_t tiles = planes * p.row_blocks;
+  const bool stream = p.rows <= 32;
+  // stream: four blocks' worth of work for each compute unit, so that sequences of different lengths
+  // even out, and a page at least for each wave; shared: two
+  int64_t s = ((stream ? 1024 : 512) + tiles - 1) / tiles;
+  const int64_t most = stream ? (max_pages + 3) / 4 : max_pages;
   if (s > most) s = most;
+  if (s > 64) s = 64;
   p.splits = s < 1 ? 1 : s;
-  p.blocks = tiles * p.splits;
+  p.units = planes * p.splits;
+  p.blocks = (p.units + 7) / 8 * 8 * p.row_blocks;
   return p;
 }
 
 size_t cache_attn_workspace_bytes(const CacheAttnPlan& p, int64_t D) {
-  return p.splits > 1 ? (size_t)(p.blocks * p.rows * (D + 2)) * sizeof(float) : 0;
+  return p.splits > 1 ? (size_t)(p.units * p.row_blocks * p.rows * (D + 2)) * sizeof(float) : 0;
 }
 
 hipError_t launch_cache_attn(const CacheAttnArgs& a, hipStream_t st) {

@@ -160,9 +160,10 @@ struct CacheAttnArgs {
   void* workspace;
 };
 // How a call is cut up: `rows` rows of a K/V head's T * H / H_kv per block, `splits` parts of each
-// sequence's pages. Sizes alone decide it, so a captured call and its workspace agree.
+// sequence's pages, `units` = B * H_kv * splits. Sizes alone decide it, so a captured call and its
+// workspace agree.
 struct CacheAttnPlan {
-  int64_t rows, row_blocks, splits, blocks;
+  int64_t rows, row_blocks, splits, units, blocks;
 };
 CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_t max_pages);
 size_t cache_attn_workspace_bytes(const CacheAttnPlan& p, int64_t D);
