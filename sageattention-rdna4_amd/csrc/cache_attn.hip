@@ -24,7 +24,10 @@
 //           own, straight from memory to registers, and a block's waves are merged through LDS.
 //   shared: more rows. MFMA- and VALU-bound: a block's four waves have rows of their own and share
 //           each page, of which every wave converts a quarter to 16 bits in LDS.
-// Either cuts a sequence's pages into S interleaved parts, which a second launch joins in order.
+// Their blocks either take a plane each (a sequence's K/V head; a second block, and so on, for more rows
+// than one holds), or, spread, equal runs of the pages of all planes in a row, whatever the sequences'
+// lengths: about as many blocks as the card runs at once. A run may end one plane, hold others whole and
+// begin another; the planes that lie in several runs are joined by a second launch, in order.
 #include "sage_device.h"
 #include "sage_launch.h"
 
@@ -94,20 +97,23 @@ __device__ __forceinline__ typename Frag<T>::type k_frag(u32 lo, u32 hi) {
   return f;
 }
 
-// Byte E of four keys' words, and of four more, as 8 fp16 values (exact).
-template <int E>
-__device__ __forceinline__ f16x8 v_frag(const u32 (&a)[4], const u32 (&b)[4]) {
-  f16x8 f;
-  static_for<0, 4>([&](auto ic) {
-    constexpr int i = 2 * (decltype(ic)::value % 2);
-    const u32* w = decltype(ic)::value < 2 ? a : b;
-    f16x2 x = {};
-    x = __builtin_amdgcn_cvt_scalef32_f16_fp8(x, (int)w[i], 1.0f, E, false);
-    x = __builtin_amdgcn_cvt_scalef32_f16_fp8(x, (int)w[i + 1], 1.0f, E, true);
-    f[2 * decltype(ic)::value] = x[0];
-    f[2 * decltype(ic)::value + 1] = x[1];
-  });
-  return f;
+// Bytes of eight keys' words (keys 4g .. 4g+3 of two key tiles, x in a and b) as the operands of four
+// column tiles, byte e being tile e's: 16-bit halves of two keys' words interleaved by bytes convert
+// pairwise, 24 operations for 32 values. (Converted byte by byte, with the half-words that the
+// convert keeps set to zero first: 48.)
+__device__ __forceinline__ void v_frags(const u32 (&a)[4], const u32 (&b)[4], f16x8 (&f)[4]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {   // bytes 2h and 2h + 1
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const u32 k0 = i < 2 ? a[2 * i] : b[2 * i - 4], k1 = i < 2 ? a[2 * i + 1] : b[2 * i - 3];
+      const u32 w = __builtin_amdgcn_perm(k1, k0, h ? 0x07030602u : 0x05010400u);
+      const f16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
+      const f16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
+      f[2 * h][2 * i] = lo[0], f[2 * h][2 * i + 1] = lo[1];
+      f[2 * h + 1][2 * i] = hi[0], f[2 * h + 1][2 * i + 1] = hi[1];
+    }
+  }
 }
 
 __device__ __forceinline__ float max_groups(float x) {
@@ -138,9 +144,12 @@ struct Shape {
   void* o;
   int64_t o_sb, o_sh, o_sr;
   float* lse;
-  float* part_o;    // (tiles, S, rows of a block, D)
-  float* part_ml;   // (tiles, S, rows of a block, 2)
-  int H, H_kv, G, T, S, RB, units;
+  float* part_o;    // (runs, RB, 2, rows, D): a run's last part of a plane begun before it, and its
+  float* part_ml;   // part of the plane that goes on behind it; (runs, RB, 2, rows, 2)
+  int B, H, H_kv, G, T, RB;
+  int rows;         // of a row block
+  int units;        // planes, or runs
+  int least;        // pages of a run at least; 0: a block for each plane
   float c;          // sm_scale log2 e
 };
 
@@ -160,44 +169,141 @@ __device__ __forceinline__ Lens lens_of(const Shape& p, int b) {
   return n;
 }
 
-// Block -> (plane, part, row block): the row blocks of one part of a plane's pages run on one XCD (blocks
-// go round the 8 XCDs), whose L2 then holds the pages that they all read.
+__device__ __forceinline__ int pages_of(const Shape& p, int b) {
+  const Lens n = lens_of(p, b);
+  return n.tokens > 0 ? (n.keys + NPAD - 1) / NPAD : 0;
+}
+
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ u32 scan_lanes(u32 x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const u32 y = (u32)__shfl_up((int)x, o, 64);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+__device__ __forceinline__ u32 lane_of(u32 x, int lane) {
+  return (u32)__builtin_amdgcn_readlane((int)x, lane);
+}
+
+// All sequences' pages in a row (each H_kv times, plane after plane), and the runs' length. Every wave
+// works it out by itself, 64 sequences at a time; the entry point bounds the sum by 2^31.
+struct Runs {
+  u32 mine, upto;   // of sequence `lane`: its pages, and the pages up to its end
+  u32 total, per;
+};
+__device__ __forceinline__ Runs runs_of(const Shape& p, int lane) {
+  Runs r;
+  r.mine = lane < p.B ? (u32)pages_of(p, lane) : 0u;
+  r.upto = scan_lanes(r.mine, lane);
+  u32 pages = lane_of(r.upto, 63);
+  for (int b0 = 64; b0 < p.B; b0 += 64)
+    pages += lane_of(scan_lanes(b0 + lane < p.B ? (u32)pages_of(p, b0 + lane) : 0u, lane), 63);
+  r.total = pages * (u32)p.H_kv;
+  const u32 even = (r.total + (u32)p.units - 1) / (u32)p.units;
+  r.per = even < (u32)p.least ? (u32)p.least : even;
+  return r;
+}
+// The sequence that `pick` (of the pages up to a sequence's end, and its number) first holds for, with
+// its pages and those before it; there is one.
+struct Seq {
+  int b;
+  u32 pages, before;
+};
+template <typename F>
+__device__ __forceinline__ Seq find_seq(const Shape& p, const Runs& r, int lane, F&& pick) {
+  u32 mine = r.mine, upto = r.upto, base = 0;
+  for (int b0 = 0;;) {
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(b0 + lane < p.B && pick(base + upto, b0 + lane));
+    if (hit || b0 + 64 >= p.B) {
+      const int at = hit ? __builtin_ctzll(hit) : 0;
+      const u32 n = lane_of(mine, at);
+      return {b0 + at, n, base + lane_of(upto, at) - n};
+    }
+    base += lane_of(upto, 63);
+    b0 += 64;
+    mine = b0 + lane < p.B ? (u32)pages_of(p, b0 + lane) : 0u;
+    upto = scan_lanes(mine, lane);
+  }
+}
+
+// Block -> (plane or run, row block): the row blocks of one unit run on one XCD (blocks go round the 8
+// XCDs), whose L2 then holds the pages that they all read.
 struct Place {
-  int plane, b, hk, split, rb;
-  int64_t part;   // number of (plane, split, row block)
-  bool live;
+  u32 unit;
+  int rb;
 };
 __device__ __forceinline__ Place place_of(const Shape& p) {
-  Place w;
   const u32 id = blockIdx.x, oct = id / (8u * (u32)p.RB), in = id - oct * 8u * (u32)p.RB;
-  w.rb = (int)(in / 8u);
-  const u32 unit = oct * 8u + in % 8u;
-  w.live = unit < (u32)p.units;
-  w.plane = (int)(unit / (u32)p.S);
-  w.split = (int)(unit - (u32)w.plane * (u32)p.S);
-  w.b = w.plane / p.H_kv;
-  w.hk = w.plane - w.b * p.H_kv;
-  w.part = (int64_t)unit * p.RB + w.rb;
-  return w;
+  return {oct * 8u + in % 8u, (int)(in / 8u)};
+}
+
+// A block's part of a plane: pages first .. last - 1, the whole of it or not.
+struct Part {
+  int b, hk, first, last;
+  bool whole;
+  int64_t row;   // of the parts in the workspace
+};
+// Calls f(Part) for each part of the block's unit.
+template <typename F>
+__device__ __forceinline__ void for_parts(const Shape& p, const Place& at, int lane, F&& f) {
+  if (at.unit >= (u32)p.units) return;
+  u32 x = 0, end;   // of the pages in a row
+  int b, hk, first = 0, pages;
+  if (!p.least) {
+    b = (int)(at.unit / (u32)p.H_kv);
+    hk = (int)(at.unit - (u32)b * (u32)p.H_kv);
+    pages = pages_of(p, b);
+    end = (u32)pages;
+  } else {
+    const Runs r = runs_of(p, lane);
+    x = at.unit * r.per;   // below 2^31 + the pages of a run
+    if (x >= r.total) return;
+    end = x + r.per < r.total ? x + r.per : r.total;
+    const u32 y = x / (u32)p.H_kv;
+    const Seq q = find_seq(p, r, lane, [&](u32 upto, int) { return upto > y; });
+    const u32 in = x - q.before * (u32)p.H_kv;
+    b = q.b;
+    pages = (int)q.pages;
+    hk = (int)(in / q.pages);
+    first = (int)(in - (u32)hk * q.pages);
+  }
+  for (;;) {
+    const int left = (int)(end - x), last = pages - first < left ? pages : first + left;
+    f(Part{b, hk, first, last, first == 0 && last == pages,
+           (((int64_t)at.unit * p.RB + at.rb) * 2 + (first == 0)) * p.rows});
+    x += (u32)(last - first);
+    if (x >= end) return;
+    first = 0;
+    if (++hk == p.H_kv) {
+      hk = 0;
+      do {   // one with pages follows: x lies below the sum of all
+        if (++b >= p.B) return;
+        pages = pages_of(p, b);
+      } while (pages == 0);
+    }
+  }
 }
 
 // A wave's rows and running sums.
 template <typename T, int D, int R>
 struct Rows {
   typename Frag<T>::type q[R][D / 32];
-  int token[R];
+  int row0, step;   // lane l15 holds row row0 + step r + l15 of the plane in tile r
   f32x4 acc[R][D / 16];
   float m[R], l[R];
 
-  // lane l15 holds row l15 of each 16, columns 64c + 16g + 8s in k-step 2c + s
-  __device__ __forceinline__ void load(const Shape& p, int b, int hk, int row0, int l15, int g) {
+  // columns 64c + 16g + 8s of its row in k-step 2c + s
+  __device__ __forceinline__ void load(const Shape& p, int b, int hk, int first, int step_, int l15,
+                                       int g) {
+    row0 = first, step = step_;
+    asm volatile("" : "+v"(l15), "+v"(g));   // addresses are worked out here, not held from part to part
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int row = row0 + 16 * r + l15;
-      token[r] = row / p.G;
-      const int h = hk * p.G + row - token[r] * p.G;
-      const bool live = token[r] < p.T;
-      const T* src = (const T*)p.q + b * p.q_sb + (live ? h * p.q_sh + token[r] * p.q_sr : 0) + 16 * g;
+      const int row = row0 + step * r + l15, token = row / p.G, h = hk * p.G + row - token * p.G;
+      const bool live = token < p.T;
+      const T* src = (const T*)p.q + b * p.q_sb + (live ? h * p.q_sh + token * p.q_sr : 0) + 16 * g;
 #pragma unroll
       for (int t = 0; t < D / 32; ++t) {
         u32x4 w = *(const u32x4*)(src + 64 * (t >> 1) + 8 * (t & 1));
@@ -222,44 +328,70 @@ __device__ __forceinline__ void key_consts(float* dst, int key, float sk, float 
   dst[128 + key] = held ? fmaxf(__builtin_amdgcn_rcpf(v), 0.0f) : 0.0f;
 }
 
+// The keys of a page that this lane's row sees, a bit each; token: the row's new token. Under a mask, lane
+// x looks at key x for each of the 16 rows in turn (64 bytes of the mask at once), and every row's lanes
+// keep its ballot.
+__device__ __forceinline__ uint64_t seen_keys(const Shape& p, const Lens& n, int b, int key0, int token) {
+  const int prefix = n.kv - n.tokens;    // tokens that every new token sees
+  const int held = n.keys - key0;
+  if (!p.mask) {
+    const int upto = prefix + token + 1 - key0, count = upto < held ? upto : held;
+    return count >= 64 ? ~0ull : count <= 0 ? 0ull : (1ull << count) - 1;
+  }
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));   // what follows from it is worked out here, not held over the loop
+  const int draft = key0 + lane - prefix;
+  const u8* mask = p.mask + b * p.m_sb;
+  u8 at[16];
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    const int t = __builtin_amdgcn_readlane(token, x);
+    at[x] = draft < 0;
+    if (draft >= 0 && draft < n.tokens && t < n.tokens) at[x] = mask[t * p.m_sr + draft];
+  }
+  uint64_t seen = 0;
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    const uint64_t row = __builtin_amdgcn_ballot_w64(lane < held && at[x] != 0);
+    if ((lane & 15) == x) seen = row;
+  }
+  return seen;
+}
+
 // Scores to weights: u = t + log2 SV, where the page holds new tokens or ends the sequence only for the
 // keys that each row sees; then the running maximum and sum, and the weights as the PV MFMA takes them.
-template <typename T, int D, int R>
+// For the first NR of the wave's row tiles.
+template <int NR, typename T, int D, int R>
 __device__ __forceinline__ void softmax_step(const Shape& p, const Lens& n, int b, int key0,
                                              const float* consts, int g, Rows<T, D, R>& w,
-                                             f32x4 (&s)[R][4], f16x8 (&wf)[R][2]) {
-  const int prefix = n.kv - n.tokens;    // tokens that every new token sees
+                                             f32x4 (&s)[NR][4], f16x8 (&wf)[NR][2]) {
+  const int prefix = n.kv - n.tokens;
 #pragma unroll
   for (int kt = 0; kt < 4; ++kt) {
     const f32x4 ks = *(const f32x4*)(consts + 16 * kt + 4 * g);
     const f32x4 lv = *(const f32x4*)(consts + 64 + 16 * kt + 4 * g);
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < NR; ++r)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[r][kt][i] = __builtin_fmaf(s[r][kt][i], ks[i], lv[i]);
   }
   if (key0 + NPAD > prefix || key0 + NPAD > n.keys) {
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
+    for (int r = 0; r < NR; ++r) {
+      int row = w.row0 + w.step * r + (threadIdx.x & 15);
+      asm volatile("" : "+v"(row));   // its token is worked out here, not held over the loop
+      const uint64_t seen = seen_keys(p, n, b, key0, row / p.G);
+      const u32 half[2] = {(u32)seen >> (4 * g), (u32)(seen >> 32) >> (4 * g)};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = key0 + 16 * kt + 4 * g + i, draft = key - prefix;
+      for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          bool seen = key < n.keys;
-          if (seen && draft >= 0) {
-            if (p.mask)
-              seen = w.token[r] < n.tokens && p.mask[b * p.m_sb + w.token[r] * p.m_sr + draft] != 0;
-            else
-              seen = draft <= w.token[r];
-          }
-          s[r][kt][i] = seen ? s[r][kt][i] : NEG_INF;
-        }
-      }
+        for (int i = 0; i < 4; ++i)
+          s[r][kt][i] = (half[kt >> 1] >> (16 * (kt & 1) + i)) & 1 ? s[r][kt][i] : NEG_INF;
+    }
   }
-  float top[R];
+  float top[NR];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
+  for (int r = 0; r < NR; ++r) {
     top[r] = NEG_INF;
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt)
@@ -267,9 +399,9 @@ __device__ __forceinline__ void softmax_step(const Shape& p, const Lens& n, int 
       for (int i = 0; i < 4; ++i) top[r] = fmaxf(top[r], s[r][kt][i]);
   }
 #pragma unroll
-  for (int r = 0; r < R; ++r) top[r] = max_groups(top[r]);
+  for (int r = 0; r < NR; ++r) top[r] = max_groups(top[r]);
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
+  for (int r = 0; r < NR; ++r) {
     if (__builtin_amdgcn_ballot_w64(top[r] > w.m[r])) {
       const float now = fmaxf(top[r], w.m[r]);
       // a row that has seen nothing keeps sums of zero
@@ -318,34 +450,38 @@ __device__ __forceinline__ float lse_of(float top, float sum) {
   return (top - W_SHIFT + __log2f(sum)) * LN2_F;
 }
 
-// A row's N columns from col on: to the output where the call has one part, else to the workspace
+// A row's N columns from col on: to the output where the part is the whole plane, else to the workspace
 // (at row `at` of the parts), where nothing is read that a part with a sum of 0 did not write.
 template <typename T, int D, int N>
-__device__ __forceinline__ void finish_row(const Shape& p, const Lens& n, int b, int hk, int row,
+__device__ __forceinline__ void finish_row(const Shape& p, const Lens& n, const Part& part, int row,
                                            int64_t at, int col, const float (&f)[N], float top,
                                            float sum) {
-  const int tok = row / p.G, h = hk * p.G + row - tok * p.G;
+  const int tok = row / p.G, h = part.hk * p.G + row - tok * p.G;
   if (tok >= p.T) return;
-  if (p.S > 1) {
+  if (!part.whole) {
     if (col == 0) *(float2*)(p.part_ml + 2 * at) = make_float2(top, sum);
     if (sum != 0.0f) {
+      if constexpr (N % 4 == 0) {
 #pragma unroll
-      for (int e = 0; e < N; e += 4)
-        *(f32x4*)(p.part_o + at * D + col + e) = (f32x4){f[e], f[e + 1], f[e + 2], f[e + 3]};
+        for (int e = 0; e < N; e += 4)
+          *(f32x4*)(p.part_o + at * D + col + e) = (f32x4){f[e], f[e + 1], f[e + 2], f[e + 3]};
+      } else {
+        *(float2*)(p.part_o + at * D + col) = make_float2(f[0], f[1]);
+      }
     }
     return;
   }
   const bool some = tok < n.tokens && sum != 0.0f;
-  store_row<T, N>((T*)p.o + b * p.o_sb + h * p.o_sh + tok * p.o_sr + col, f, some ? 1.0f / sum : 0.0f,
-                  some);
+  store_row<T, N>((T*)p.o + part.b * p.o_sb + h * p.o_sh + tok * p.o_sr + col, f,
+                  some ? 1.0f / sum : 0.0f, some);
   if (p.lse && col == 0)
-    p.lse[((int64_t)b * p.H + h) * p.T + tok] = some ? lse_of(top, sum) : NEG_INF;
+    p.lse[((int64_t)part.b * p.H + h) * p.T + tok] = some ? lse_of(top, sum) : NEG_INF;
 }
 
-// grid: one block per part of a plane (row blocks: 1). Wave w of part s takes pages s W + w, then every
-// (S W)-th: which these are does not wait for the sequence's length.
+// Up to 16 R rows of a plane. Wave w of a part takes its pages first + w, then every W-th. The next
+// page's K is requested when the scores are done with this one's, its V when the products are.
 template <typename T, bool KINT8, int D, int R, int W>
-__global__ __launch_bounds__(64 * W, 2) void cache_attn_stream_kernel(Shape p) {
+__global__ __launch_bounds__(64 * W, (R == 2 && D == 128) ? 1 : 2) void cache_attn_stream_kernel(Shape p) {
   typedef typename Frag<T>::type frag;
   constexpr int KC = D / 64, KT = D / 32, VE = D / 16, VW = VE / 4, LD = D + 4;
   __shared__ __attribute__((aligned(16))) float lds_o[W][16][LD];
@@ -354,192 +490,61 @@ __global__ __launch_bounds__(64 * W, 2) void cache_attn_stream_kernel(Shape p) {
 
   const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Place at = place_of(p);
-  if (!at.live) return;
-  const int b = at.b, hk = at.hk;
-  const Lens n = lens_of(p, b);
-  Rows<T, D, R> w;
-  w.load(p, b, hk, 0, l15, g);
 
-  const int pages = n.tokens > 0 ? (n.keys + NPAD - 1) / NPAD : 0;
-  const int* table = p.table + b * p.t_sb;
-  for (int pg = at.split * W + wave; pg < pages; pg += p.S * W) {
-    const int id = __builtin_amdgcn_readfirstlane(table[pg]);
-    if (id < 0 || id >= p.num_pages) continue;   // no page: nothing to see
-    const int64_t base = ((int64_t)id * p.H_kv + hk) * NPAD;
-    const u8* kp = p.k8 + base * D + (int64_t)l15 * D + 16 * g;
-    const u8* vp = p.v8 + base * D + (int64_t)(4 * g) * D + l15 * VE;
-    const float sk = p.sk[base + lane], sv = p.sv[base + lane];
+  for_parts(p, place_of(p), lane, [&](const Part& part) {
+    const int b = part.b;
+    const int* table = p.table + b * p.t_sb;
+    int pg = part.first + wave;
+    int id = pg < p.max_pages ? table[pg] : -1;
+    const Lens n = lens_of(p, b);
+    Rows<T, D, R> w;
+    w.load(p, b, part.hk, 0, 16, l15, g);
+
     u32x4 kw[4][KC];
     u32 vw[4][VW][4];   // [key tile][word of the row's 4 VW bytes][key 4g + j]
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-      for (int c = 0; c < KC; ++c) kw[kt][c] = *(const u32x4*)(kp + 16 * kt * D + 64 * c);
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const u8* src = vp + (16 * kt + j) * D;
-        if constexpr (VW == 2) {
-          const u32x2 x = *(const u32x2*)src;
-          vw[kt][0][j] = x[0], vw[kt][1][j] = x[1];
-        } else {
-          vw[kt][0][j] = *(const u32*)src;
-        }
-      }
-    const int key0 = pg * NPAD;
-    key_consts(lds_c[wave], lane, sk, sv, p.c, key0 + lane < n.keys);
-
-    f32x4 s[R][4];
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-#pragma unroll
-      for (int r = 0; r < R; ++r) s[r][kt] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        const frag kf = k_frag<T, KINT8>(kw[kt][t >> 1][2 * (t & 1)], kw[kt][t >> 1][2 * (t & 1) + 1]);
-#pragma unroll
-        for (int r = 0; r < R; ++r) s[r][kt] = mfma(kf, w.q[r][t], s[r][kt]);
-      }
-    }
-    if (key0 + NPAD > n.keys) {   // whatever lies behind the end: no NaN may meet a weight of zero
+    float sk = 0.0f, sv = 0.0f;
+    auto load_k = [&](int64_t base) {
+      const u8* kp = p.k8 + base * D;
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (key0 + 16 * kt + 4 * g + j >= n.keys) {
+        for (int c = 0; c < KC; ++c)
+          kw[kt][c] = *(const u32x4*)(kp + (u32)(l15 * D + 16 * g + 16 * kt * D + 64 * c));
+      sk = (p.sk + base)[(u32)lane], sv = (p.sv + base)[(u32)lane];
+    };
+    auto load_v = [&](int64_t base) {
+      const u8* vp = p.v8 + base * D;
 #pragma unroll
-            for (int x = 0; x < VW; ++x) vw[kt][x][j] = 0;
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const u8* src = vp + (u32)(4 * g * D + l15 * VE + (16 * kt + j) * D);
+          if constexpr (VW == 2) {
+            const u32x2 x = *(const u32x2*)src;
+            vw[kt][0][j] = x[0], vw[kt][1][j] = x[1];
+          } else {
+            vw[kt][0][j] = *(const u32*)src;
           }
-    }
-    f16x8 wf[R][2];
-    softmax_step<T, D, R>(p, n, b, key0, lds_c[wave], g, w, s, wf);
-
-    // O^T += V^T W^T: tile e's row x is column VE x + e
-    static_for<0, 2>([&](auto uc) {
-      constexpr int u = decltype(uc)::value;
-      static_for<0, VE>([&](auto ec) {
-        constexpr int e = decltype(ec)::value;
-        const f16x8 vf = v_frag<e % 4>(vw[2 * u][e / 4], vw[2 * u + 1][e / 4]);
-#pragma unroll
-        for (int r = 0; r < R; ++r) w.acc[r][e] = mfma(vf, wf[r][u], w.acc[r][e]);
-      });
-    });
-  }
-
-  // the waves' results merged, 16 rows at a time; each thread has N columns of a row
-  constexpr int TPR = 4 * W, N = D / TPR;   // threads of a row
-  const int tid = threadIdx.x, orow = tid / TPR, ocol = (tid % TPR) * N;
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const float total = sum_groups(w.l[r]);
-    if (r) __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < VE; e += 4)
-        *(f32x4*)&lds_o[wave][l15][VE * (4 * g + i) + e] =
-            (f32x4){w.acc[r][e][i], w.acc[r][e + 1][i], w.acc[r][e + 2][i], w.acc[r][e + 3][i]};
-    if (g == 0) lds_ml[wave][l15][0] = w.m[r], lds_ml[wave][l15][1] = total;
-    __syncthreads();
-    float top = NEG_INF;
-#pragma unroll
-    for (int x = 0; x < W; ++x) top = fmaxf(top, lds_ml[x][orow][0]);
-    const float use = top == NEG_INF ? 0.0f : top;
-    float sum = 0.0f, f[N] = {};
-#pragma unroll
-    for (int x = 0; x < W; ++x) {
-      const float a = __builtin_amdgcn_exp2f(lds_ml[x][orow][0] - use);
-      sum += lds_ml[x][orow][1] * a;
-#pragma unroll
-      for (int e = 0; e < N; ++e) f[e] += lds_o[x][orow][ocol + e] * a;
-    }
-    finish_row<T, D, N>(p, n, b, hk, 16 * r + orow, at.part * (16 * R) + 16 * r + orow, ocol, f, top, sum);
-  }
-}
-
-// grid: row blocks of 64 R rows x parts of a plane. Part s takes pages s, s + S, ... The page in work
-// lies in LDS as the MFMAs' operands (K: key tile x k-step, V: half x column tile; 1 KB each, one
-// 16-byte piece a lane), the next one's bytes in registers: wave w converts key tile w of K and four
-// operands of V.
-template <typename T, bool KINT8, int D, int R>
-__global__ __launch_bounds__(256, 2) void cache_attn_shared_kernel(Shape p) {
-  typedef typename Frag<T>::type frag;
-  constexpr int KC = D / 64, KT = D / 32, VE = D / 16, NV = 2 * VE / 4, ROWS = 64 * R;
-  __shared__ __attribute__((aligned(16))) u32x4 lds_k[2][4][KT][64];
-  __shared__ __attribute__((aligned(16))) u32x4 lds_v[2][2][VE][64];
-  __shared__ __attribute__((aligned(16))) float lds_c[2][192];
-
-  const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Place at = place_of(p);
-  if (!at.live) return;
-  const int b = at.b, hk = at.hk;
-  const Lens n = lens_of(p, b);
-  const int row0 = at.rb * ROWS + 16 * R * wave;
-  Rows<T, D, R> w;
-  w.load(p, b, hk, row0, l15, g);
-
-  const int pages = at.rb * ROWS < n.tokens * p.G ? (n.keys + NPAD - 1) / NPAD : 0;
-  const int* table = p.table + b * p.t_sb;
-  // operands u = wave / 2, e = first .. first + NV - 1 of V: bytes of word `word` of a row's VE
-  const int vu = wave >> 1, vfirst = (wave & 1) * NV;
-  u32x4 kw[KC];
-  u32 vw[2][4];
-  float sk = 0.0f, sv = 0.0f;
-  bool there = false;
-  auto fetch = [&](int pg) {
-    const int id = pg < pages ? __builtin_amdgcn_readfirstlane(table[pg]) : -1;
-    there = id >= 0 && id < p.num_pages;
-    if (!there) return;
-    const int64_t base = ((int64_t)id * p.H_kv + hk) * NPAD;
-    const u8* kp = p.k8 + (base + 16 * wave + l15) * D + 16 * g;
-#pragma unroll
-    for (int c = 0; c < KC; ++c) kw[c] = *(const u32x4*)(kp + 64 * c);
-    const u8* vp = p.v8 + (base + 32 * vu + 4 * g) * D + l15 * VE + (VE == 8 ? vfirst : 0);
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) vw[x][j] = *(const u32*)(vp + (16 * x + j) * D);
-    if (wave == 0) sk = p.sk[base + lane], sv = p.sv[base + lane];
-  };
-  auto convert = [&](int pg, int buf) {
-    if (!there) return;
-    const int key0 = pg * NPAD;
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      const frag f = k_frag<T, KINT8>(kw[t >> 1][2 * (t & 1)], kw[t >> 1][2 * (t & 1) + 1]);
-      __builtin_memcpy(&lds_k[buf][wave][t][lane], &f, 16);
-    }
-    if (key0 + NPAD > n.keys) {   // whatever lies behind the end: no NaN may meet a weight of zero
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (key0 + 32 * vu + 16 * x + 4 * g + j >= n.keys) vw[x][j] = 0;
-    }
-    static_for<0, 4>([&](auto ec) {
-      constexpr int e = decltype(ec)::value;
-      if constexpr (NV == 4) {
-        const f16x8 f = v_frag<e>(vw[0], vw[1]);
-        __builtin_memcpy(&lds_v[buf][vu][vfirst + e][lane], &f, 16);
-      } else if (e / NV == (wave & 1)) {
-        const f16x8 f = v_frag<e>(vw[0], vw[1]);
-        __builtin_memcpy(&lds_v[buf][vu][e][lane], &f, 16);
+        }
+    };
+    // the next page of the wave that there is: its place in the pool, or -1
+    auto next_page = [&]() -> int64_t {
+      while (pg < part.last) {
+        const int cur = __builtin_amdgcn_readfirstlane(id);
+        pg += W;
+        id = pg < part.last ? table[pg] : -1;
+        if (cur >= 0 && cur < p.num_pages) return ((int64_t)cur * p.H_kv + part.hk) * NPAD;
       }
-    });
-    if (wave == 0) key_consts(lds_c[buf], lane, sk, sv, p.c, key0 + lane < n.keys);
-  };
-
-  int pg = at.split, buf = 0;
-  fetch(pg);
-  convert(pg, 0);
-  bool work = there;   // whether the page in LDS is one
-  __syncthreads();
-  for (; pg < pages; pg += p.S) {
-    fetch(pg + p.S);
-    if (work) {
+      return -1;
+    };
+    int64_t base = next_page();
+    int key0 = (pg - W) * NPAD;
+    if (base >= 0) {
+      load_k(base);
+      load_v(base);
+    }
+    while (base >= 0) {
+      key_consts(lds_c[wave], lane, sk, sv, p.c, key0 + lane < n.keys);
       f32x4 s[R][4];
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt) {
@@ -547,14 +552,169 @@ __global__ __launch_bounds__(256, 2) void cache_attn_shared_kernel(Shape p) {
         for (int r = 0; r < R; ++r) s[r][kt] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
-          frag kf;
-          __builtin_memcpy(&kf, &lds_k[buf][kt][t][lane], 16);
+          const frag kf = k_frag<T, KINT8>(kw[kt][t >> 1][2 * (t & 1)], kw[kt][t >> 1][2 * (t & 1) + 1]);
 #pragma unroll
           for (int r = 0; r < R; ++r) s[r][kt] = mfma(kf, w.q[r][t], s[r][kt]);
         }
       }
+      const int64_t next = next_page();
+      if (next >= 0) load_k(next);
+      if (key0 + NPAD > n.keys) {   // whatever lies behind the end: no NaN may meet a weight of zero
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (key0 + 16 * kt + 4 * g + j >= n.keys) {
+#pragma unroll
+              for (int x = 0; x < VW; ++x) vw[kt][x][j] = 0;
+            }
+      }
       f16x8 wf[R][2];
-      softmax_step<T, D, R>(p, n, b, pg * NPAD, lds_c[buf], g, w, s, wf);
+      softmax_step<R>(p, n, b, key0, lds_c[wave], g, w, s, wf);
+
+      // O^T += V^T W^T: tile e's row x is column VE x + e
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int x = 0; x < VW; ++x) {
+          f16x8 vf[4];
+          v_frags(vw[2 * u][x], vw[2 * u + 1][x], vf);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int r = 0; r < R; ++r) w.acc[r][4 * x + e] = mfma(vf[e], wf[r][u], w.acc[r][4 * x + e]);
+        }
+      if (next >= 0) load_v(next);
+      base = next;
+      key0 = (pg - W) * NPAD;
+    }
+
+    // the waves' results merged, 16 rows at a time; each thread has N columns of a row
+    constexpr int TPR = 4 * W, N = D / TPR;   // threads of a row
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));   // addresses are worked out here, not held over the loop
+    const int orow = tid / TPR, ocol = (tid % TPR) * N;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float total = sum_groups(w.l[r]);
+      __syncthreads();   // the readers of what was merged before
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < VE; e += 4)
+          *(f32x4*)&lds_o[wave][l15][VE * (4 * g + i) + e] =
+              (f32x4){w.acc[r][e][i], w.acc[r][e + 1][i], w.acc[r][e + 2][i], w.acc[r][e + 3][i]};
+      if (g == 0) lds_ml[wave][l15][0] = w.m[r], lds_ml[wave][l15][1] = total;
+      __syncthreads();
+      float top = NEG_INF;
+#pragma unroll
+      for (int x = 0; x < W; ++x) top = fmaxf(top, lds_ml[x][orow][0]);
+      const float use = top == NEG_INF ? 0.0f : top;
+      float sum = 0.0f, f[N] = {};
+#pragma unroll
+      for (int x = 0; x < W; ++x) {
+        const float a = __builtin_amdgcn_exp2f(lds_ml[x][orow][0] - use);
+        sum += lds_ml[x][orow][1] * a;
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] += lds_o[x][orow][ocol + e] * a;
+      }
+      finish_row<T, D, N>(p, n, part, 16 * r + orow, part.row + 16 * r + orow, ocol, f, top, sum);
+    }
+  });
+}
+
+// Row blocks of up to 64 R rows of a plane, the row tiles of 16 dealt to the four waves in turn. The page
+// in work lies in LDS as the MFMAs' operands (K: key tile x k-step, V: half x column tile; 1 KB each,
+// one 16-byte piece a lane), the next one's bytes in registers: wave w converts key tile w of K and
+// half w / 2 of V, four column tiles of it at D = 128 and two at 64.
+template <typename T, bool KINT8, int D, int R>
+__global__ __launch_bounds__(256, 2) void cache_attn_shared_kernel(Shape p) {
+  typedef typename Frag<T>::type frag;
+  constexpr int KC = D / 64, KT = D / 32, VE = D / 16;
+  __shared__ __attribute__((aligned(16))) u32x4 lds_k[2][4][KT][64];
+  __shared__ __attribute__((aligned(16))) u32x4 lds_v[2][2][VE][64];
+  __shared__ __attribute__((aligned(16))) float lds_c[2][192];
+
+  const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int vu = wave >> 1, odd = wave & 1;
+  const Place at = place_of(p);
+
+  for_parts(p, at, lane, [&](const Part& part) {
+    const int b = part.b;
+    const int* table = p.table + b * p.t_sb;
+    const Lens n = lens_of(p, b);
+    const int block0 = at.rb * p.rows, row0 = block0 + 16 * wave;
+    // rows of the block that are there, and the wave's tiles of them
+    const int rows = n.tokens * p.G - block0 < p.rows ? n.tokens * p.G - block0 : p.rows;
+    const int tiles = rows > 16 * wave ? (rows - 16 * wave + 63) / 64 : 0;
+    Rows<T, D, R> w;
+    w.load(p, b, part.hk, row0, 64, l15, g);
+
+    const int last = rows > 0 ? part.last : 0;
+    u32x4 kw[KC];
+    u32 vw[2][4];
+    float sk = 0.0f, sv = 0.0f;
+    bool there = false;
+    auto fetch = [&](int pg) {
+      const int id = pg < last ? __builtin_amdgcn_readfirstlane(table[pg]) : -1;
+      there = id >= 0 && id < p.num_pages;
+      if (!there) return;
+      const int64_t base = ((int64_t)id * p.H_kv + part.hk) * NPAD;
+      const u8* kp = p.k8 + (base + 16 * wave) * D;
+      const u8* vp = p.v8 + (base + 32 * vu) * D + (VE == 8 ? 4 * odd : 0);
+#pragma unroll
+      for (int c = 0; c < KC; ++c) kw[c] = *(const u32x4*)(kp + (u32)(l15 * D + 16 * g + 64 * c));
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          vw[x][j] = *(const u32*)(vp + (u32)(4 * g * D + l15 * VE + (16 * x + j) * D));
+      if (wave == 0) sk = (p.sk + base)[(u32)lane], sv = (p.sv + base)[(u32)lane];
+    };
+    auto convert = [&](int pg, int buf) {
+      if (!there) return;
+      const int key0 = pg * NPAD;
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        const frag f = k_frag<T, KINT8>(kw[t >> 1][2 * (t & 1)], kw[t >> 1][2 * (t & 1) + 1]);
+        __builtin_memcpy(&lds_k[buf][wave][t][lane], &f, 16);
+      }
+      if (key0 + NPAD > n.keys) {   // whatever lies behind the end: no NaN may meet a weight of zero
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (key0 + 32 * vu + 16 * x + 4 * g + j >= n.keys) vw[x][j] = 0;
+      }
+      f16x8 vf[4];
+      v_frags(vw[0], vw[1], vf);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (VE == 8)
+          __builtin_memcpy(&lds_v[buf][vu][(VE == 8 ? 4 * odd : 0) + e][lane], &vf[e], 16);
+        else if ((e >> 1) == odd)
+          __builtin_memcpy(&lds_v[buf][vu][e][lane], &vf[e], 16);
+      if (wave == 0) key_consts(lds_c[buf], lane, sk, sv, p.c, key0 + lane < n.keys);
+    };
+    // the page in LDS for the wave's first NR row tiles
+    auto page = [&](auto nr, int pg, int buf) {
+      constexpr int NR = decltype(nr)::value;
+      f32x4 s[NR][4];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) s[r][kt] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          frag kf;
+          __builtin_memcpy(&kf, &lds_k[buf][kt][t][lane], 16);
+#pragma unroll
+          for (int r = 0; r < NR; ++r) s[r][kt] = mfma(kf, w.q[r][t], s[r][kt]);
+        }
+      }
+      f16x8 wf[NR][2];
+      softmax_step<NR>(p, n, b, pg * NPAD, lds_c[buf], g, w, s, wf);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -562,78 +722,135 @@ __global__ __launch_bounds__(256, 2) void cache_attn_shared_kernel(Shape p) {
           f16x8 vf;
           __builtin_memcpy(&vf, &lds_v[buf][u][e][lane], 16);
 #pragma unroll
-          for (int r = 0; r < R; ++r) w.acc[r][e] = mfma(vf, wf[r][u], w.acc[r][e]);
+          for (int r = 0; r < NR; ++r) w.acc[r][e] = mfma(vf, wf[r][u], w.acc[r][e]);
         }
-    }
-    convert(pg + p.S, buf ^ 1);   // the other buffer: its readers passed the last barrier
-    work = there;
-    buf ^= 1;
-    __syncthreads();
-  }
+    };
 
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const float sum = sum_groups(w.l[r]);
-    const int row = row0 + 16 * r + l15;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float f[VE];
-#pragma unroll
-      for (int e = 0; e < VE; ++e) f[e] = w.acc[r][e][i];
-      finish_row<T, D, VE>(p, n, b, hk, row, at.part * ROWS + row - at.rb * ROWS, VE * (4 * g + i), f,
-                           w.m[r], sum);
+    int pg = part.first, buf = 0;
+    fetch(pg);
+    convert(pg, 0);
+    bool work = there;   // whether the page in LDS is one
+    __syncthreads();
+    for (; pg < last; ++pg) {
+      fetch(pg + 1);
+      if (work && tiles) {
+        if (R == 1 || tiles >= R)
+          page(std::integral_constant<int, R>{}, pg, buf);
+        else
+          page(std::integral_constant<int, 1>{}, pg, buf);
+      }
+      convert(pg + 1, buf ^ 1);   // the other buffer: its readers passed the last barrier
+      work = there;
+      buf ^= 1;
+      __syncthreads();
     }
-  }
+
+    int in0 = 16 * wave + l15, col0 = VE * 4 * g;
+    asm volatile("" : "+v"(in0), "+v"(col0));   // addresses are worked out here, not held over the loop
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float sum = sum_groups(w.l[r]);
+      const int in = 64 * r + in0;   // row of the block
+      if (in < p.rows) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float f[VE];
+#pragma unroll
+          for (int e = 0; e < VE; ++e) f[e] = w.acc[r][e][i];
+          finish_row<T, D, VE>(p, n, part, block0 + in, part.row + in, col0 + VE * i, f, w.m[r], sum);
+        }
+      }
+    }
+  });
 }
 
-// The parts joined, in their order: a wave per output row, D/64 columns a lane; lane s first has the
-// part s's maximum and sum (S is at most 64).
-template <typename T, int D>
-__global__ __launch_bounds__(256) void cache_attn_join_kernel(Shape p, int rows_per_block, u32 rows) {
-  constexpr int N = D / 64;
+// Planes in several runs joined, part after part, and the rows of those that have no pages cleared. WPR
+// waves to an output row, D/64 columns a lane; lane i first has part i's maximum and sum.
+template <typename T, int D, int WPR>
+__global__ __launch_bounds__(256) void cache_attn_join_kernel(Shape p, u32 out_rows) {
+  constexpr int N = D / 64, RPB = 4 / WPR;   // rows of a block
+  __shared__ float lds_f[4][64][N];
+  __shared__ float lds_ml[4][2];
   const int lane = threadIdx.x & 63;
-  const u32 at = __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6));
-  if (at >= rows) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = wave % WPR;
+  const u32 want = blockIdx.x * RPB + (u32)(wave / WPR);
+  const u32 at = want < out_rows ? want : out_rows - 1;   // its last wave takes part in the barrier
   // rows in the order (b, K/V head, row of the plane)
   const u32 M = (u32)p.T * (u32)p.G;
   const u32 plane = at / M, row = at - plane * M;
   const int b = (int)(plane / (u32)p.H_kv), hk = (int)(plane - (u32)b * (u32)p.H_kv);
   const int tok = (int)(row / (u32)p.G), h = hk * p.G + (int)row - tok * p.G;
-  const Lens n = lens_of(p, b);
-  const u32 rb = row / (u32)rows_per_block, in = row - rb * (u32)rows_per_block;
-  const int64_t first = ((int64_t)plane * p.S * p.RB + rb) * rows_per_block + in;
-  const int64_t step = (int64_t)p.RB * rows_per_block;
-  float2 ml = make_float2(NEG_INF, 0.0f);
-  if (lane < p.S) ml = *(const float2*)(p.part_ml + 2 * (first + lane * step));
-  float top = ml.x;
+  const u32 rb = row / (u32)p.rows, in = row - rb * (u32)p.rows;
+  const Runs r = runs_of(p, lane);
+  const Seq q = find_seq(p, r, lane, [&](u32, int x) { return x == b; });
+  const u32 x = q.before * (u32)p.H_kv + (u32)hk * q.pages;
+  const u32 run0 = x / r.per, run1 = q.pages ? (x + q.pages - 1) / r.per : run0;
+  const bool joined = q.pages == 0 || run0 != run1;
+  const int parts = q.pages ? (int)(run1 - run0) + 1 : 0;
+  const bool tokens = tok < lens_of(p, b).tokens;
+
+  // part i's row: of the first run its last part, of the others their first
+  auto row_of = [&](int i) {
+    return (((int64_t)(run0 + (u32)i) * p.RB + rb) * 2 + (i == 0)) * p.rows + in;
+  };
+  float top = NEG_INF, sum = 0.0f, f[N] = {};
+  for (int i0 = 64 * mine; i0 < (joined ? parts : 0); i0 += 64 * WPR) {
+    float2 ml = make_float2(NEG_INF, 0.0f);
+    const int count = parts - i0 < 64 ? parts - i0 : 64;
+    if (lane < count) ml = *(const float2*)(p.part_ml + 2 * row_of(i0 + lane));
+    float now = fmaxf(top, ml.x);
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-  const float a = __builtin_amdgcn_exp2f(ml.x - (top == NEG_INF ? 0.0f : top));
-  const bool full = ml.y != 0.0f;
-  float sum = full ? ml.y * a : 0.0f;
+    for (int o = 1; o < 64; o <<= 1) now = fmaxf(now, __shfl_xor(now, o, 64));
+    const float use = now == NEG_INF ? 0.0f : now;
+    const float a = __builtin_amdgcn_exp2f(ml.x - use), old = __builtin_amdgcn_exp2f(top - use);
+    const bool full = ml.y != 0.0f;
+    float add = full ? ml.y * a : 0.0f;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
-  const uint64_t parts = __builtin_amdgcn_ballot_w64(full);
-  float f[N] = {};
-  const float* src = p.part_o + first * D + lane * N;
-  for (int s0 = 0; s0 < p.S; s0 += 8) {   // eight parts requested together
-    float x[8][N];
+    for (int o = 1; o < 64; o <<= 1) add += __shfl_xor(add, o, 64);
+    sum = sum * old + add;
+    top = now;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int s = s0 + i < p.S ? s0 + i : p.S - 1;
+    for (int e = 0; e < N; ++e) f[e] *= old;
+    const uint64_t live = __builtin_amdgcn_ballot_w64(full);
+    for (int j0 = 0; j0 < count; j0 += 8) {   // eight parts requested together
+      float y[8][N];
 #pragma unroll
-      for (int e = 0; e < N; ++e) x[i][e] = src[s * step * D + e];
-    }
+      for (int j = 0; j < 8; ++j) {
+        const float* src = p.part_o + row_of(i0 + (j0 + j < count ? j0 + j : count - 1)) * D + lane * N;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int s = s0 + i;
-      if (s >= p.S || !((parts >> s) & 1)) continue;
-      const float as = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(a), s));
+        for (int e = 0; e < N; ++e) y[j][e] = src[e];
+      }
 #pragma unroll
-      for (int e = 0; e < N; ++e) f[e] += x[i][e] * as;
+      for (int j = 0; j < 8; ++j) {
+        if (j0 + j >= count || !((live >> (j0 + j)) & 1)) continue;
+        const float aj = __int_as_float((int)lane_of(__float_as_uint(a), j0 + j));
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] += y[j][e] * aj;
+      }
     }
   }
-  const bool some = tok < n.tokens && sum != 0.0f;
+  if constexpr (WPR > 1) {
+    if (lane == 0) lds_ml[wave][0] = top, lds_ml[wave][1] = sum;
+#pragma unroll
+    for (int e = 0; e < N; ++e) lds_f[wave][lane][e] = f[e];
+    __syncthreads();
+    if (mine != 0) return;
+#pragma unroll
+    for (int x2 = 0; x2 < WPR; ++x2) top = fmaxf(top, lds_ml[wave + x2][0]);
+    const float use = top == NEG_INF ? 0.0f : top;
+    sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = 0.0f;
+#pragma unroll
+    for (int x2 = 0; x2 < WPR; ++x2) {
+      const float a = __builtin_amdgcn_exp2f(lds_ml[wave + x2][0] - use);
+      sum += lds_ml[wave + x2][1] * a;
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[e] += lds_f[wave + x2][lane][e] * a;
+    }
+  }
+  if (!joined || want >= out_rows) return;   // its one run has written the plane
+  const bool some = tokens && sum != 0.0f;
   const float inv = some ? 1.0f / sum : 0.0f;
   T* o = (T*)p.o + b * p.o_sb + h * p.o_sh + tok * p.o_sr + lane * N;
   if constexpr (N == 2)
@@ -670,29 +887,42 @@ hipError_t run(const CacheAttnArgs& a, hipStream_t st) {
   p.o_sh = a.o_sh;
   p.o_sr = a.o_sr;
   p.lse = a.lse;
+  p.B = (int)a.B;
   p.H = (int)a.H;
   p.H_kv = (int)a.H_kv;
   p.G = (int)(a.H / a.H_kv);
   p.T = (int)a.T;
-  p.S = (int)plan.splits;
   p.RB = (int)plan.row_blocks;
+  p.rows = (int)plan.rows;
   p.units = (int)plan.units;
+  p.least = (int)plan.least;
   p.c = a.sm_scale * LOG2E_F;
   p.part_o = (float*)a.workspace;
-  p.part_ml = p.part_o + plan.units * plan.row_blocks * plan.rows * D;
+  p.part_ml = p.part_o + plan.part_rows * D;
   const u32 blocks = (u32)plan.blocks;
-  if (plan.rows == 16)
-    cache_attn_stream_kernel<T, KINT8, D, 1, 4><<<blocks, 256, 0, st>>>(p);
-  else if (plan.rows == 32)
-    cache_attn_stream_kernel<T, KINT8, D, 2, 4><<<blocks, 256, 0, st>>>(p);
-  else if (plan.rows == 64)
-    cache_attn_shared_kernel<T, KINT8, D, 1><<<blocks, 256, 0, st>>>(p);
-  else
-    cache_attn_shared_kernel<T, KINT8, D, 2><<<blocks, 256, 0, st>>>(p);
+  switch (plan.kernel) {
+    case CACHE_ATTN_STREAM16:
+      cache_attn_stream_kernel<T, KINT8, D, 1, 4><<<blocks, 256, 0, st>>>(p);
+      break;
+    case CACHE_ATTN_STREAM16_WIDE:
+      cache_attn_stream_kernel<T, KINT8, D, 1, 8><<<blocks, 512, 0, st>>>(p);
+      break;
+    case CACHE_ATTN_STREAM32:
+      cache_attn_stream_kernel<T, KINT8, D, 2, 4><<<blocks, 256, 0, st>>>(p);
+      break;
+    case CACHE_ATTN_SHARED64:
+      cache_attn_shared_kernel<T, KINT8, D, 1><<<blocks, 256, 0, st>>>(p);
+      break;
+    default:
+      cache_attn_shared_kernel<T, KINT8, D, 2><<<blocks, 256, 0, st>>>(p);
+  }
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || plan.splits == 1) return e;
-  const int64_t rows = a.B * a.H * a.T;
-  cache_attn_join_kernel<T, D><<<(u32)((rows + 3) / 4), 256, 0, st>>>(p, (int)plan.rows, (u32)rows);
+  if (e != hipSuccess || !plan.least) return e;
+  const u32 rows = (u32)(a.B * a.H * a.T);
+  if (plan.wide_join)
+    cache_attn_join_kernel<T, D, 4><<<rows, 256, 0, st>>>(p, rows);
+  else
+    cache_attn_join_kernel<T, D, 1><<<(rows + 3) / 4, 256, 0, st>>>(p, rows);
   return hipGetLastError();
 }
 
@@ -706,25 +936,36 @@ hipError_t run_d(const CacheAttnArgs& a, hipStream_t st) {
 
 CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_t max_pages) {
   CacheAttnPlan p;
-  const int64_t M = T * (H / H_kv), planes = B * H_kv;
-  p.rows = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  p.row_blocks = (M + p.rows - 1) / p.rows;
-  const int64_t tiles = planes * p.row_blocks;
-  const bool stream = p.rows <= 32;
-  // stream: four blocks' worth of work for each compute unit, so that sequences of different lengths
-  // even out, and a page at least for each wave; shared: two
-  int64_t s = ((stream ? 1024 : 512) + tiles - 1) / tiles;
-  const int64_t most = stream ? (max_pages + 3) / 4 : max_pages;
-  if (s > most) s = most;
-  if (s > 64) s = 64;
-  p.splits = s < 1 ? 1 : s;
-  p.units = planes * p.splits;
+  const int64_t M = T * (H / H_kv), planes = B * H_kv, tiles = (M + 15) / 16;
+  p.kernel = M <= 16 ? CACHE_ATTN_STREAM16 : M <= 32 ? CACHE_ATTN_STREAM32
+             : M <= 64 ? CACHE_ATTN_SHARED64 : CACHE_ATTN_SHARED128;
+  const bool stream = M <= 32;
+  const int64_t most = M <= 16 ? 1 : M <= 32 ? 2 : M <= 64 ? 4 : 8;   // tiles of a row block
+  p.row_blocks = (tiles + most - 1) / most;
+  p.rows = 16 * ((tiles + p.row_blocks - 1) / p.row_blocks);
+  const int64_t blocks = planes * p.row_blocks;
+  if (max_pages <= 8 || blocks >= 2048) {
+    p.units = planes;
+    p.least = 0;
+    p.part_rows = 0;
+    p.wide_join = false;
+    if (p.kernel == CACHE_ATTN_STREAM16 && blocks <= 256) p.kernel = CACHE_ATTN_STREAM16_WIDE;
+  } else {
+    p.least = stream ? 4 : 2;
+    int64_t runs = ((stream ? 1024 : 512) + p.row_blocks - 1) / p.row_blocks;
+    if (runs > (planes * max_pages + p.least - 1) / p.least)
+      runs = (planes * max_pages + p.least - 1) / p.least;
+    if (runs > 128 * planes) runs = 128 * planes;
+    p.units = runs;
+    p.part_rows = runs * p.row_blocks * 2 * p.rows;
+    p.wide_join = runs > 16 * planes;
+  }
   p.blocks = (p.units + 7) / 8 * 8 * p.row_blocks;
   return p;
 }
 
 size_t cache_attn_workspace_bytes(const CacheAttnPlan& p, int64_t D) {
-  return p.splits > 1 ? (size_t)(p.units * p.row_blocks * p.rows * (D + 2)) * sizeof(float) : 0;
+  return (size_t)(p.part_rows * (D + 2)) * sizeof(float);
 }
 
 hipError_t launch_cache_attn(const CacheAttnArgs& a, hipStream_t st) {

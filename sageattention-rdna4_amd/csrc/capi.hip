@@ -275,8 +275,11 @@ int check_cache_attn_shape(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_
   if (max_pages < 1 || max_pages > (1 << 24))
     return fail(SAGE_ERR_INVALID, "block_table: max_pages must be in [1, 2^24] (got %lld)",
                 (long long)max_pages);
-  // the join has a wave for each row
-  if ((rc = check_grid("the join", (B * H * T + 3) / 4, 256))) return rc;
+  // pages are counted in 32 bits; the join has up to a block for each row
+  if (max_pages > kInt32Max / (B * H_kv))
+    return fail(SAGE_ERR_INVALID, "block_table: %lld pages for %lld planes are too many",
+                (long long)max_pages, (long long)(B * H_kv));
+  if ((rc = check_grid("the join", B * H * T, 256))) return rc;
   return check_grid("the cached attention", sage::cache_attn_plan(B, H, H_kv, T, max_pages).blocks,
                     256);
 }

@@ -159,11 +159,20 @@ struct CacheAttnArgs {
   float* lse;                 // optional (B, H, T)
   void* workspace;
 };
-// How a call is cut up: `rows` rows of a K/V head's T * H / H_kv per block, `splits` parts of each
-// sequence's pages, `units` = B * H_kv * splits. Sizes alone decide it, so a captured call and its
-// workspace agree.
+// How a call is cut up: row blocks of `rows` of a K/V head's T * H / H_kv rows, and `units` planes (least
+// = 0) or equal runs of all planes' pages, of `least` pages or more, whose parts (part_rows rows of D
+// + 2 floats) a second launch joins. Sizes alone decide it, so a captured call and its workspace agree.
+enum CacheAttnKernel {
+  CACHE_ATTN_STREAM16,        // up to 16 rows, 4 waves
+  CACHE_ATTN_STREAM16_WIDE,   // 8 waves
+  CACHE_ATTN_STREAM32,        // up to 32 rows
+  CACHE_ATTN_SHARED64,        // row blocks of up to 64
+  CACHE_ATTN_SHARED128,       // and 128 rows
+};
 struct CacheAttnPlan {
-  int64_t rows, row_blocks, splits, units, blocks;
+  CacheAttnKernel kernel;
+  int64_t rows, row_blocks, units, least, part_rows, blocks;
+  bool wide_join;
 };
 CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_t max_pages);
 size_t cache_attn_workspace_bytes(const CacheAttnPlan& p, int64_t D);

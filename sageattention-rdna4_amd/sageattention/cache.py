@@ -20,16 +20,19 @@ there, zeros are read from it, and nobody attends to it. A row of K or V that ho
 infinity is held as NaN: so come out the rows that attend to it, and only they.
 """
 import math
-from contextlib import nullcontext
 
 import torch
 
 from . import sk1_backend as _sk1
-from .sk1_backend.sk1_loader import SageLib, _dtype_code, strided_view_reason, torch_stream
+from .sk1_backend.sk1_loader import SageLib, strided_view_reason, torch_stream
 
 PAGE = 64
 
 _HEAD_DIMS = (64, 128)
+_DTYPES = (torch.float16, torch.bfloat16)
+
+#: device index -> the library, once the device is known to be served
+_LIBRARIES = {}
 
 
 def _refuse(what, reason):
@@ -38,61 +41,78 @@ def _refuse(what, reason):
 
 def _library(what, device):
     """The library, where it serves this device."""
-    if not _sk1.arch_supported(device):
-        raise RuntimeError("%s: device arch is %r; libsagemi355.so is built for %s" % (
-            what, _sk1.device_arch(device) or "<unknown>", ", ".join(_sk1.SUPPORTED_ARCHS)))
-    return SageLib.get()
+    lib = _LIBRARIES.get(device.index)
+    if lib is None:
+        if not _sk1.arch_supported(device):
+            raise RuntimeError("%s: device arch is %r; libsagemi355.so is built for %s" % (
+                what, _sk1.device_arch(device) or "<unknown>", ", ".join(_sk1.SUPPORTED_ARCHS)))
+        lib = _LIBRARIES[device.index] = SageLib.get()
+    return lib
 
 
-def _on(device):
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _launch(device, call, *args, **kwargs):
+    """The call on the device's current stream, with the device current."""
+    if device.index == torch.cuda.current_device():
+        call(*args, stream=torch_stream(device), **kwargs)
+    else:
+        with torch.cuda.device(device):
+            call(*args, stream=torch_stream(device), **kwargs)
 
 
-def _views(what, tensor_layout, **tensors):
-    """The tensors as (B, H, N, D) views on one device, of one served dtype and head_dim."""
-    if tensor_layout not in ("HND", "NHD"):
+def _view(what, tensor_layout, name, t):
+    """The tensor as a (B, H, N, D) view of a served dtype and head_dim."""
+    if tensor_layout != "HND" and tensor_layout != "NHD":
         _refuse(what, "layout: tensor_layout must be HND or NHD (got %r)" % (tensor_layout,))
-    out, first = [], None
-    for name, t in tensors.items():
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            _refuse(what, "device: %s must be a tensor on the GPU" % name)
-        if t.dim() != 4:
-            _refuse(what, "rank: %s must have 4 dimensions (got %d)" % (name, t.dim()))
-        if t.dtype not in (torch.float16, torch.bfloat16):
-            _refuse(what, "dtype: %s is %s (fp16 and bf16 are served)" % (name, t.dtype))
-        first = t if first is None else first
-        if t.device != first.device:
-            _refuse(what, "device: %s is on %s, not %s" % (name, t.device, first.device))
-        if t.dtype != first.dtype:
-            _refuse(what, "dtype: %s is %s, not %s" % (name, t.dtype, first.dtype))
-        if min(t.shape) < 1:
-            _refuse(what, "seq_len: %s is empty %s" % (name, tuple(t.shape)))
-        if t.shape[3] not in _HEAD_DIMS:
-            _refuse(what, "head_dim: %s has %d (64 and 128 are served)" % (name, t.shape[3]))
-        t = t if tensor_layout == "HND" else t.transpose(1, 2)
-        reason = strided_view_reason(t, name)
-        if reason is not None:
-            _refuse(what, "%s: %s %s" % (reason, name, tuple(t.stride())))
-        out.append(t)
-    return out
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _refuse(what, "device: %s must be a tensor on the GPU" % name)
+    if t.dim() != 4:
+        _refuse(what, "rank: %s must have 4 dimensions (got %d)" % (name, t.dim()))
+    if t.dtype not in _DTYPES:
+        _refuse(what, "dtype: %s is %s (fp16 and bf16 are served)" % (name, t.dtype))
+    if not t.numel():
+        _refuse(what, "seq_len: %s is empty %s" % (name, tuple(t.shape)))
+    if t.shape[3] not in _HEAD_DIMS:
+        _refuse(what, "head_dim: %s has %d (64 and 128 are served)" % (name, t.shape[3]))
+    if tensor_layout == "NHD":
+        t = t.transpose(1, 2)
+    reason = strided_view_reason(t, name)
+    if reason is not None:
+        _refuse(what, "%s: %s %s" % (reason, name, tuple(t.stride())))
+    return t
 
 
-def _ints(what, name, t, device, *shape):
-    """Checks an int32 tensor of this shape (-1: any size) whose rows are contiguous; returns the
-    elements between its rows, 0 where there is one."""
+def _empty(shape, like):
+    """A new tensor of this shape, of `like`'s dtype and device."""
+    if like.is_contiguous() and like.shape == shape:
+        return torch.empty_like(like)
+    return torch.empty(shape, device=like.device, dtype=like.dtype)
+
+
+def _ints(what, name, t, device, rows, columns=None):
+    """Checks an int32 tensor (rows,), or (rows, columns) with contiguous rows (columns -1: any);
+    returns the elements between two rows, 0 where there is one."""
     if not isinstance(t, torch.Tensor) or t.device != device:
         _refuse(what, "device: %s must be a tensor on %s" % (name, device))
     if t.dtype != torch.int32:
         _refuse(what, "dtype: %s must be int32 (got %s)" % (name, t.dtype))
-    if t.dim() != len(shape) or any(n not in (-1, m) for n, m in zip(shape, t.shape)):
-        _refuse(what, "shape: %s is %s, not %s" % (name, tuple(t.shape), shape))
-    if t.shape[-1] < 1 or (t.shape[-1] > 1 and t.stride(-1) != 1):
-        _refuse(what, "stride_last: %s must have contiguous rows" % name)
-    if len(shape) == 1 or t.shape[0] == 1:
+    shape = t.shape
+    if columns is None:
+        if len(shape) != 1 or shape[0] != rows:
+            _refuse(what, "shape: %s is %s, not (%d,)" % (name, tuple(shape), rows))
+        if rows > 1 and t.stride(0) != 1:
+            _refuse(what, "stride_last: %s must be contiguous" % name)
         return 0
-    if t.stride(0) < t.shape[1] and t.stride(0) != 0:
+    if len(shape) != 2 or shape[0] != rows or columns not in (-1, shape[1]) or shape[1] < 1:
+        _refuse(what, "shape: %s is %s, not (%d, %s)" % (
+            name, tuple(shape), rows, "..." if columns < 0 else columns))
+    step, last = t.stride()
+    if last != 1 and shape[1] > 1:
+        _refuse(what, "stride_last: %s must have contiguous rows" % name)
+    if rows == 1:
+        return 0
+    if step < shape[1] and step != 0:
         _refuse(what, "stride_overlap: rows of %s overlap" % name)
-    return t.stride(0)
+    return step
 
 
 def _check_table(what, table, positions, device, B, N, D):
@@ -107,8 +127,7 @@ def _check_table(what, table, positions, device, B, N, D):
         _refuse(what, "table: %s: R must be a multiple of 16 up to the head_dim %d" % (
             tuple(table.shape), D))
     if isinstance(positions, torch.Tensor) and positions.dim() == 1:
-        _ints(what, "positions", positions, device, N)
-        return 0
+        return _ints(what, "positions", positions, device, N)
     return _ints(what, "positions", positions, device, B, N)
 
 
@@ -163,16 +182,14 @@ def apply_rotary(x, table, positions, tensor_layout="HND", interleaved=False, in
     `inverse` turns by the negative angle: the gradient of x from that of the result.
     """
     what = "apply_rotary"
-    xx, = _views(what, tensor_layout, x=x)
-    B, H, N, D = xx.shape
+    xx = _view(what, tensor_layout, "x", x)
+    B, _, N, D = xx.shape
     dev = x.device
     p_sb = _check_table(what, table, positions, dev, B, N, D)
     lib = _library(what, dev)
-    out = torch.empty(x.shape, device=dev, dtype=x.dtype)
-    oo = out if tensor_layout == "HND" else out.transpose(1, 2)
-    with _on(dev):
-        lib.rotary(xx, oo, table, positions, p_sb, interleaved=interleaved, inverse=inverse,
-                   stream=torch_stream(dev))
+    out = _empty(x.shape, x)
+    _launch(dev, lib.rotary, xx, out if tensor_layout == "HND" else out.transpose(1, 2), table,
+            positions, p_sb, interleaved=interleaved, inverse=inverse)
     return out
 
 
@@ -243,25 +260,25 @@ class KVCache:
         may go to the same place (two sequences that share a page and both write to it).
         """
         what = "KVCache.write"
-        kk, vv = _views(what, tensor_layout, k=k, v=v)
+        kk, vv = _view(what, tensor_layout, "k", k), _view(what, tensor_layout, "v", v)
         self._check_rows(what, kk)
+        self._check_rows(what, vv)
+        dev = self.device
         B, H, N, D = kk.shape
         if vv.shape != kk.shape or H != self.num_heads:
             _refuse(what, "heads: k %s and v %s for a cache of %d heads" % (
                 tuple(kk.shape), tuple(vv.shape), self.num_heads))
-        t_sb = _ints(what, "block_table", block_table, self.device, B, -1)
-        _ints(what, "start", start, self.device, B)
+        t_sb = _ints(what, "block_table", block_table, dev, B, -1)
+        _ints(what, "start", start, dev, B)
         if lens is not None:
-            _ints(what, "lens", lens, self.device, B)
+            _ints(what, "lens", lens, dev, B)
         p_sb = 0
         if table is not None:
-            p_sb = _check_table(what, table, positions, self.device, B, N, D)
+            p_sb = _check_table(what, table, positions, dev, B, N, D)
         elif positions is not None:
             _refuse(what, "table: positions are given without a rotary table")
-        lib = _library(what, self.device)
-        with _on(self.device):
-            lib.cache_write(self, kk, vv, block_table, t_sb, start, lens, table, positions, p_sb,
-                            interleaved=interleaved, stream=torch_stream(self.device))
+        _launch(dev, _library(what, dev).cache_write, self, kk, vv, block_table, t_sb, start, lens,
+                table, positions, p_sb, interleaved=interleaved)
 
     def read(self, block_table, lens, n, start=None, tensor_layout="HND"):
         """(k, v), the cached rows in 16 bits: row i < lens[b] of sequence b is position `start[b] +
@@ -274,21 +291,21 @@ class KVCache:
         n = int(n)
         if n < 1:
             _refuse(what, "seq_len: n must be at least 1 (got %d)" % n)
-        t_sb = _ints(what, "block_table", block_table, self.device, -1, -1)
-        B = block_table.shape[0]
-        if B < 1:
-            _refuse(what, "shape: block_table has no rows")
-        _ints(what, "lens", lens, self.device, B)
+        if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2 \
+                or block_table.shape[0] < 1:
+            _refuse(what, "shape: block_table must be a (B, max_pages) tensor")
+        dev, B, H, D = self.device, block_table.shape[0], self.num_heads, self.head_dim
+        t_sb = _ints(what, "block_table", block_table, dev, B, -1)
+        _ints(what, "lens", lens, dev, B)
         if start is not None:
-            _ints(what, "start", start, self.device, B)
-        lib = _library(what, self.device)
+            _ints(what, "start", start, dev, B)
+        lib = _library(what, dev)
         hnd = tensor_layout == "HND"
-        shape = (B, self.num_heads, n, self.head_dim) if hnd else (B, n, self.num_heads, self.head_dim)
-        k = torch.empty(shape, device=self.device, dtype=self.dtype)
-        v = torch.empty(shape, device=self.device, dtype=self.dtype)
-        with _on(self.device):
-            lib.cache_read(self, k if hnd else k.transpose(1, 2), v if hnd else v.transpose(1, 2),
-                           block_table, t_sb, start, lens, stream=torch_stream(self.device))
+        # both in one allocation: every row is a multiple of 128 bytes
+        kv = torch.empty((2, B, H, n, D) if hnd else (2, B, n, H, D), device=dev, dtype=self.dtype)
+        k, v = kv.unbind(0)
+        _launch(dev, lib.cache_read, self, k if hnd else k.transpose(1, 2),
+                v if hnd else v.transpose(1, 2), block_table, t_sb, start, lens)
         return k, v
 
 
@@ -309,14 +326,14 @@ def sageattn_cached(q, cache, block_table, kv_lens, tensor_layout="HND", q_lens=
     zeros and -inf. Queries are not quantized: the result is that of the cached values to 16 bits.
     """
     what = "sageattn_cached"
-    qq, = _views(what, tensor_layout, q=q)
+    qq = _view(what, tensor_layout, "q", q)
     if not isinstance(cache, KVCache):
         _refuse(what, "cache: a KVCache is needed (got %s)" % type(cache).__name__)
     cache._check_rows(what, qq)
     B, H, T, D = qq.shape
     if H % cache.num_heads:
         _refuse(what, "heads: %d query heads for %d K/V heads" % (H, cache.num_heads))
-    dev = q.device
+    dev = cache.device
     t_sb = _ints(what, "block_table", block_table, dev, B, -1)
     _ints(what, "kv_lens", kv_lens, dev, B)
     if q_lens is not None:
@@ -327,21 +344,19 @@ def sageattn_cached(q, cache, block_table, kv_lens, tensor_layout="HND", q_lens=
             _refuse(what, "device: tree_mask must be a tensor on %s" % dev)
         if tree_mask.dtype not in (torch.bool, torch.uint8):
             _refuse(what, "dtype: tree_mask must be bool or uint8 (got %s)" % tree_mask.dtype)
-        if tuple(tree_mask.shape) not in ((T, T), (B, T, T)):
+        if tree_mask.shape != (T, T) and tree_mask.shape != (B, T, T):
             _refuse(what, "shape: tree_mask is %s, not (%d, %d) or (%d, %d, %d)" % (
                 tuple(tree_mask.shape), T, T, B, T, T))
         m_sr = tree_mask.stride(-2) if T > 1 else 1
         m_sb = tree_mask.stride(0) if tree_mask.dim() == 3 and B > 1 else 0
         if (T > 1 and tree_mask.stride(-1) != 1) or m_sr < T or 0 < m_sb < T:
             _refuse(what, "stride_last: tree_mask must have contiguous rows that do not overlap")
-    sm = float(sm_scale if sm_scale is not None else D ** -0.5)
+    sm = D ** -0.5 if sm_scale is None else float(sm_scale)
     lib = _library(what, dev)
-    out = torch.empty(q.shape, device=dev, dtype=q.dtype)
-    oo = out if tensor_layout == "HND" else out.transpose(1, 2)
-    lse = torch.empty(B, H, T, device=dev, dtype=torch.float32) if return_lse else None
     need = lib.cache_attn_workspace_bytes(B, H, cache.num_heads, T, block_table.shape[1], D)
+    out = _empty(q.shape, q)
+    lse = torch.empty((B, H, T), device=dev, dtype=torch.float32) if return_lse else None
     tmp = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
-    with _on(dev):
-        lib.cache_attn(cache, qq, oo, block_table, t_sb, kv_lens, q_lens, tree_mask, m_sb, m_sr, sm,
-                       lse, tmp, need, stream=torch_stream(dev))
+    _launch(dev, lib.cache_attn, cache, qq, out if tensor_layout == "HND" else out.transpose(1, 2),
+            block_table, t_sb, kv_lens, q_lens, tree_mask, m_sb, m_sr, sm, lse, tmp, need)
     return (out, lse) if return_lse else out

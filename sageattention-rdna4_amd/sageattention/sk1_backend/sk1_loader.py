@@ -10,6 +10,7 @@ Every launch goes on `torch.cuda.current_stream()` with no host synchronization
 (`sk1_loader.py:17-19`, `:301-303` of the reference).
 """
 import ctypes
+import functools
 import os
 import threading
 
@@ -374,7 +375,9 @@ class SageLib:
         if rc:
             self._check(rc, "sage_cache_read")
 
+    @functools.lru_cache(maxsize=4096)
     def cache_attn_workspace_bytes(self, B, H, H_kv, T, max_pages, D):
+        """Bytes of `sage_cache_attn`'s workspace, a function of the sizes alone."""
         n = self.lib.sage_cache_attn_workspace_bytes(B, H, H_kv, T, max_pages, D)
         if n < 0:
             self._check(-n, "sage_cache_attn_workspace_bytes")

@@ -434,6 +434,38 @@ def test_long_sequences_are_split_and_joined(L, B, H_kv):
     ref.check_attention(o[0].cpu(), p @ v, err * (p @ v.abs()), torch.float16)
 
 
+@pytest.mark.parametrize("dtype,int8", KINDS, ids=KIND_IDS)
+@pytest.mark.parametrize("H,H_kv,T,D", [(2, 2, 1, 128), (4, 1, 1, 64), (8, 2, 6, 128), (20, 2, 5, 64),
+                                        (16, 1, 9, 128)])
+@pytest.mark.parametrize("B", [5, 70, 131])
+def test_ragged_batches(dtype, int8, H, H_kv, T, D, B):
+    # many sequences of every length, none and fewer tokens than new ones among them: equal shares of all
+    # their pages, each of which may end one sequence, hold several and begin another
+    from sageattention import sageattn_cached
+    gen = torch.Generator().manual_seed(B + T)
+    pick = [0, 1, 63, 64, 65, 130, 200, 641, 1000]
+    lens = [pick[int(i)] for i in torch.randint(0, len(pick), (B,), generator=gen)]
+    lens[B // 2], lens[0], lens[B - 1] = 1500, 0, 0
+    cache, table = _filled(dtype, int8, H_kv, D, lens, gen)
+    q, qg = _randn((B, H, T, D), dtype, "HND", gen, 2.0)
+    q_lens = torch.randint(0, T + 1, (B,), generator=gen).int() if T > 1 else None
+    o, lse = sageattn_cached(qg, cache, table, _lens(*lens), return_lse=True,
+                             q_lens=None if q_lens is None else q_lens.cuda())
+    some = [0, 1, B // 2, B - 2, B - 1] + [int(i) for i in torch.randint(0, B, (8,), generator=gen)]
+    want, wl, slack = ref.attention(q[some], cache, table.cpu()[some], [lens[b] for b in some],
+                                    None if q_lens is None else q_lens[some])
+    ref.check_attention(o.cpu()[some], want, slack[0], dtype)
+    ref.check_lse(lse.cpu()[some], wl, slack[1])
+    # and each as it comes out alone
+    one = [b for b in range(B) if b % 7 == 0]
+    for b in one:
+        alone = sageattn_cached(qg[b:b + 1], cache, table[b:b + 1], _lens(lens[b]),
+                                q_lens=None if q_lens is None else q_lens[b:b + 1].cuda())
+        off = (alone[0].double() - o[b].double()).abs().cpu()
+        assert (off <= 4 * ref.HALF_STEP[dtype] * o[b].double().abs().cpu()
+                + 2 ** -10 * o[b].double().abs().max().cpu() + 1e-7).all()
+
+
 def test_pools_beyond_32_bits():
     # codes of more than 2^32 bytes: pages at both ends, written, read and attended to
     from sageattention import KVCache, sageattn_cached
