@@ -146,6 +146,7 @@ struct Shape {
   float* lse;
   float* part_o;    // (runs, RB, 2, rows, D): a run's last part of a plane begun before it, and its
   float* part_ml;   // part of the plane that goes on behind it; (runs, RB, 2, rows, 2)
+  uint2* starts;    // (planes): where its pages begin in the row of all, and the runs' length
   int B, H, H_kv, G, T, RB;
   int rows;         // of a row block
   int units;        // planes, or runs
@@ -249,7 +250,7 @@ struct Part {
 template <typename F>
 __device__ __forceinline__ void for_parts(const Shape& p, const Place& at, int lane, F&& f) {
   if (at.unit >= (u32)p.units) return;
-  u32 x = 0, end;   // of the pages in a row
+  u32 x = 0, end, per = 0;   // of the pages in a row
   int b, hk, first = 0, pages;
   if (!p.least) {
     b = (int)(at.unit / (u32)p.H_kv);
@@ -258,6 +259,7 @@ __device__ __forceinline__ void for_parts(const Shape& p, const Place& at, int l
     end = (u32)pages;
   } else {
     const Runs r = runs_of(p, lane);
+    per = r.per;
     x = at.unit * r.per;   // below 2^31 + the pages of a run
     if (x >= r.total) return;
     end = x + r.per < r.total ? x + r.per : r.total;
@@ -271,6 +273,8 @@ __device__ __forceinline__ void for_parts(const Shape& p, const Place& at, int l
   }
   for (;;) {
     const int left = (int)(end - x), last = pages - first < left ? pages : first + left;
+    if (p.least && first == 0 && at.rb == 0 && threadIdx.x == 0)
+      p.starts[b * p.H_kv + hk] = make_uint2(x, per);   // for the join
     f(Part{b, hk, first, last, first == 0 && last == pages,
            (((int64_t)at.unit * p.RB + at.rb) * 2 + (first == 0)) * p.rows});
     x += (u32)(last - first);
@@ -764,100 +768,88 @@ __global__ __launch_bounds__(256, 2) void cache_attn_shared_kernel(Shape p) {
   });
 }
 
-// Planes in several runs joined, part after part, and the rows of those that have no pages cleared. WPR
-// waves to an output row, D/64 columns a lane; lane i first has part i's maximum and sum.
-template <typename T, int D, int WPR>
-__global__ __launch_bounds__(256) void cache_attn_join_kernel(Shape p, u32 out_rows) {
-  constexpr int N = D / 64, RPB = 4 / WPR;   // rows of a block
-  __shared__ float lds_f[4][64][N];
-  __shared__ float lds_ml[4][2];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = wave % WPR;
-  const u32 want = blockIdx.x * RPB + (u32)(wave / WPR);
-  const u32 at = want < out_rows ? want : out_rows - 1;   // its last wave takes part in the barrier
-  // rows in the order (b, K/V head, row of the plane)
-  const u32 M = (u32)p.T * (u32)p.G;
-  const u32 plane = at / M, row = at - plane * M;
+// Planes in several runs joined, part after part, and the rows of those that have no pages cleared. grid:
+// (row tile, plane), D/4 lanes to a row and SL slices of its parts; 8 parts are requested at a time.
+template <typename T, int D, int SL>
+__global__ __launch_bounds__(256) void cache_attn_join_kernel(Shape p, u32 row_tiles) {
+  constexpr int LPR = D / 4, ROWS = 256 / (LPR * SL);
+  __shared__ __attribute__((aligned(16))) f32x4 lds_f[SL > 1 ? 256 : 1];
+  __shared__ float2 lds_ml[SL > 1 ? 256 : 1];
+  const int tid = threadIdx.x, col = tid % LPR * 4, slice = tid / LPR % SL;
+  const u32 plane = blockIdx.x / row_tiles, rt = blockIdx.x - plane * row_tiles;
   const int b = (int)(plane / (u32)p.H_kv), hk = (int)(plane - (u32)b * (u32)p.H_kv);
-  const int tok = (int)(row / (u32)p.G), h = hk * p.G + (int)row - tok * p.G;
-  const u32 rb = row / (u32)p.rows, in = row - rb * (u32)p.rows;
-  const Runs r = runs_of(p, lane);
-  const Seq q = find_seq(p, r, lane, [&](u32, int x) { return x == b; });
-  const u32 x = q.before * (u32)p.H_kv + (u32)hk * q.pages;
-  const u32 run0 = x / r.per, run1 = q.pages ? (x + q.pages - 1) / r.per : run0;
-  const bool joined = q.pages == 0 || run0 != run1;
-  const int parts = q.pages ? (int)(run1 - run0) + 1 : 0;
-  const bool tokens = tok < lens_of(p, b).tokens;
-
+  const int row = (int)rt * ROWS + tid / (LPR * SL);
+  const u32 pages = (u32)pages_of(p, b);
+  u32 run0 = 0;
+  int parts = 0;
+  if (pages) {
+    const uint2 at = p.starts[plane];
+    run0 = at.x / at.y;
+    parts = (int)((at.x + pages - 1) / at.y - run0) + 1;
+    if (parts == 1) return;   // its one run has written the plane
+  }
+  const int tok = row / p.G, h = hk * p.G + row - tok * p.G;
+  const bool live = tok < p.T;
+  const int rb = row / p.rows, in = row - rb * p.rows;
   // part i's row: of the first run its last part, of the others their first
   auto row_of = [&](int i) {
     return (((int64_t)(run0 + (u32)i) * p.RB + rb) * 2 + (i == 0)) * p.rows + in;
   };
-  float top = NEG_INF, sum = 0.0f, f[N] = {};
-  for (int i0 = 64 * mine; i0 < (joined ? parts : 0); i0 += 64 * WPR) {
-    float2 ml = make_float2(NEG_INF, 0.0f);
-    const int count = parts - i0 < 64 ? parts - i0 : 64;
-    if (lane < count) ml = *(const float2*)(p.part_ml + 2 * row_of(i0 + lane));
-    float now = fmaxf(top, ml.x);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) now = fmaxf(now, __shfl_xor(now, o, 64));
-    const float use = now == NEG_INF ? 0.0f : now;
-    const float a = __builtin_amdgcn_exp2f(ml.x - use), old = __builtin_amdgcn_exp2f(top - use);
-    const bool full = ml.y != 0.0f;
-    float add = full ? ml.y * a : 0.0f;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) add += __shfl_xor(add, o, 64);
-    sum = sum * old + add;
-    top = now;
-#pragma unroll
-    for (int e = 0; e < N; ++e) f[e] *= old;
-    const uint64_t live = __builtin_amdgcn_ballot_w64(full);
-    for (int j0 = 0; j0 < count; j0 += 8) {   // eight parts requested together
-      float y[8][N];
+  float top = NEG_INF, sum = 0.0f;
+  f32x4 f = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (live) {
+    for (int i0 = slice; i0 < parts; i0 += 8 * SL) {
+      float2 ml[8];
+      f32x4 y[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float* src = p.part_o + row_of(i0 + (j0 + j < count ? j0 + j : count - 1)) * D + lane * N;
-#pragma unroll
-        for (int e = 0; e < N; ++e) y[j][e] = src[e];
+        const int i = i0 + j * SL;
+        const int64_t at = row_of(i < parts ? i : i0);
+        ml[j] = *(const float2*)(p.part_ml + 2 * at);
+        y[j] = *(const f32x4*)(p.part_o + at * D + col);
+        if (i >= parts) ml[j] = make_float2(NEG_INF, 0.0f);
       }
+      float now = top;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) now = fmaxf(now, ml[j].x);
+      const float use = now == NEG_INF ? 0.0f : now, old = __builtin_amdgcn_exp2f(top - use);
+      top = now;
+      sum *= old;
+      f *= old;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if (j0 + j >= count || !((live >> (j0 + j)) & 1)) continue;
-        const float aj = __int_as_float((int)lane_of(__float_as_uint(a), j0 + j));
+        const float a = __builtin_amdgcn_exp2f(ml[j].x - use);
+        const bool full = ml[j].y != 0.0f;   // else nothing was written there
+        sum += full ? ml[j].y * a : 0.0f;
 #pragma unroll
-        for (int e = 0; e < N; ++e) f[e] += y[j][e] * aj;
+        for (int e = 0; e < 4; ++e) f[e] += full ? y[j][e] * a : 0.0f;
       }
     }
   }
-  if constexpr (WPR > 1) {
-    if (lane == 0) lds_ml[wave][0] = top, lds_ml[wave][1] = sum;
-#pragma unroll
-    for (int e = 0; e < N; ++e) lds_f[wave][lane][e] = f[e];
+  if constexpr (SL > 1) {
+    lds_f[tid] = f;
+    lds_ml[tid] = make_float2(top, sum);
     __syncthreads();
-    if (mine != 0) return;
+    if (slice != 0) return;
 #pragma unroll
-    for (int x2 = 0; x2 < WPR; ++x2) top = fmaxf(top, lds_ml[wave + x2][0]);
+    for (int x = 1; x < SL; ++x) top = fmaxf(top, lds_ml[tid + x * LPR].x);
     const float use = top == NEG_INF ? 0.0f : top;
     sum = 0.0f;
+    f = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int e = 0; e < N; ++e) f[e] = 0.0f;
-#pragma unroll
-    for (int x2 = 0; x2 < WPR; ++x2) {
-      const float a = __builtin_amdgcn_exp2f(lds_ml[wave + x2][0] - use);
-      sum += lds_ml[wave + x2][1] * a;
-#pragma unroll
-      for (int e = 0; e < N; ++e) f[e] += lds_f[wave + x2][lane][e] * a;
+    for (int x = 0; x < SL; ++x) {
+      const float2 ml = lds_ml[tid + x * LPR];
+      const float a = __builtin_amdgcn_exp2f(ml.x - use);
+      sum += ml.y * a;
+      f += lds_f[tid + x * LPR] * a;
     }
   }
-  if (!joined || want >= out_rows) return;   // its one run has written the plane
-  const bool some = tokens && sum != 0.0f;
-  const float inv = some ? 1.0f / sum : 0.0f;
-  T* o = (T*)p.o + b * p.o_sb + h * p.o_sh + tok * p.o_sr + lane * N;
-  if constexpr (N == 2)
-    store_row<T, 2>(o, f, inv, some);
-  else
-    *o = (T)(some ? f[0] * inv : 0.0f);
-  if (p.lse && lane == 0)
+  if (!live) return;
+  const bool some = tok < lens_of(p, b).tokens && sum != 0.0f;
+  const float out[4] = {f[0], f[1], f[2], f[3]};
+  store_row<T, 4>((T*)p.o + b * p.o_sb + h * p.o_sh + tok * p.o_sr + col, out, some ? 1.0f / sum : 0.0f,
+                  some);
+  if (p.lse && col == 0)
     p.lse[((int64_t)b * p.H + h) * p.T + tok] = some ? lse_of(top, sum) : NEG_INF;
 }
 
@@ -899,6 +891,7 @@ hipError_t run(const CacheAttnArgs& a, hipStream_t st) {
   p.c = a.sm_scale * LOG2E_F;
   p.part_o = (float*)a.workspace;
   p.part_ml = p.part_o + plan.part_rows * D;
+  p.starts = (uint2*)(p.part_ml + plan.part_rows * 2);
   const u32 blocks = (u32)plan.blocks;
   switch (plan.kernel) {
     case CACHE_ATTN_STREAM16:
@@ -918,11 +911,16 @@ hipError_t run(const CacheAttnArgs& a, hipStream_t st) {
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !plan.least) return e;
-  const u32 rows = (u32)(a.B * a.H * a.T);
-  if (plan.wide_join)
-    cache_attn_join_kernel<T, D, 4><<<rows, 256, 0, st>>>(p, rows);
-  else
-    cache_attn_join_kernel<T, D, 1><<<(rows + 3) / 4, 256, 0, st>>>(p, rows);
+  const u32 M = (u32)(a.T * (a.H / a.H_kv)), planes = (u32)(a.B * a.H_kv);
+  if (plan.wide_join) {
+    constexpr u32 ROWS = 256 / (D / 4 * 8);
+    const u32 tiles = (M + ROWS - 1) / ROWS;
+    cache_attn_join_kernel<T, D, 8><<<planes * tiles, 256, 0, st>>>(p, tiles);
+  } else {
+    constexpr u32 ROWS = 256 / (D / 4);
+    const u32 tiles = (M + ROWS - 1) / ROWS;
+    cache_attn_join_kernel<T, D, 1><<<planes * tiles, 256, 0, st>>>(p, tiles);
+  }
   return hipGetLastError();
 }
 
@@ -944,14 +942,15 @@ CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int
   p.row_blocks = (tiles + most - 1) / most;
   p.rows = 16 * ((tiles + p.row_blocks - 1) / p.row_blocks);
   const int64_t blocks = planes * p.row_blocks;
-  if (max_pages <= 8 || blocks >= 2048) {
+  const int64_t single = M <= 16 ? (blocks <= 256 ? 48 : 16) : stream ? 12 : 6;
+  if (max_pages <= single || blocks >= 2048) {
     p.units = planes;
     p.least = 0;
     p.part_rows = 0;
     p.wide_join = false;
-    if (p.kernel == CACHE_ATTN_STREAM16 && blocks <= 256) p.kernel = CACHE_ATTN_STREAM16_WIDE;
+    if (M <= 16 && blocks <= 256) p.kernel = CACHE_ATTN_STREAM16_WIDE;
   } else {
-    p.least = stream ? 4 : 2;
+    p.least = stream ? 8 : 2;
     int64_t runs = ((stream ? 1024 : 512) + p.row_blocks - 1) / p.row_blocks;
     if (runs > (planes * max_pages + p.least - 1) / p.least)
       runs = (planes * max_pages + p.least - 1) / p.least;
@@ -960,12 +959,13 @@ CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int
     p.part_rows = runs * p.row_blocks * 2 * p.rows;
     p.wide_join = runs > 16 * planes;
   }
+  p.planes = planes;
   p.blocks = (p.units + 7) / 8 * 8 * p.row_blocks;
   return p;
 }
 
 size_t cache_attn_workspace_bytes(const CacheAttnPlan& p, int64_t D) {
-  return (size_t)(p.part_rows * (D + 2)) * sizeof(float);
+  return p.least ? (size_t)(p.part_rows * (D + 2) + 2 * p.planes) * sizeof(float) : 0;
 }
 
 hipError_t launch_cache_attn(const CacheAttnArgs& a, hipStream_t st) {

@@ -171,7 +171,7 @@ enum CacheAttnKernel {
 };
 struct CacheAttnPlan {
   CacheAttnKernel kernel;
-  int64_t rows, row_blocks, units, least, part_rows, blocks;
+  int64_t rows, row_blocks, planes, units, least, part_rows, blocks;
   bool wide_join;
 };
 CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_t max_pages);
