@@ -101,7 +101,7 @@ __device__ __forceinline__ typename Frag<T>::type k_frag(u32 lo, u32 hi) {
 // column tiles, byte e being tile e's: 16-bit halves of two keys' words interleaved by bytes convert
 // pairwise, 24 operations for 32 values. (Converted byte by byte, with the half-words that the
 // convert keeps set to zero first: 48.)
-__device__ __forceinline__ void v_frags(const u32 (&a)[4], const u32 (&b)[4], f16x8 (&f)[4]) {
+__device__ __forceinline__ void v_frags(const u32x4 a, const u32x4 b, f16x8 (&f)[4]) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {   // bytes 2h and 2h + 1
 #pragma unroll
@@ -273,7 +273,9 @@ __device__ __forceinline__ void for_parts(const Shape& p, const Place& at, int l
   }
   for (;;) {
     const int left = (int)(end - x), last = pages - first < left ? pages : first + left;
-    if (p.least && first == 0 && at.rb == 0 && threadIdx.x == 0)
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    if (p.least && first == 0 && at.rb == 0 && tid == 0)
       p.starts[b * p.H_kv + hk] = make_uint2(x, per);   // for the join
     f(Part{b, hk, first, last, first == 0 && last == pages,
            (((int64_t)at.unit * p.RB + at.rb) * 2 + (first == 0)) * p.rows});
@@ -290,6 +292,22 @@ __device__ __forceinline__ void for_parts(const Shape& p, const Place& at, int l
   }
 }
 
+// N operands from LDS, each used once, three more requested ahead of the one in use. The memory clobber
+// keeps each request where it stands: left to itself the compiler reads every operand into the same
+// registers, right before its use, and waits for LDS N times in a row.
+template <int N, typename Read, typename Use>
+__device__ __forceinline__ void run_operands(Read&& read, Use&& use) {
+  u32x4 x[4];
+#pragma unroll
+  for (int j = 0; j < 3; ++j) x[j] = read(j);
+  static_for<0, N>([&](auto jc) {
+    constexpr int j = decltype(jc)::value;
+    if constexpr (j + 3 < N) x[(j + 3) & 3] = read(j + 3);
+    asm volatile("" : "+v"(x[j & 3]) : : "memory");
+    use(jc, x[j & 3]);
+  });
+}
+
 // A wave's rows and running sums.
 template <typename T, int D, int R>
 struct Rows {
@@ -299,10 +317,11 @@ struct Rows {
   float m[R], l[R];
 
   // columns 64c + 16g + 8s of its row in k-step 2c + s
-  __device__ __forceinline__ void load(const Shape& p, int b, int hk, int first, int step_, int l15,
-                                       int g) {
+  __device__ __forceinline__ void load(const Shape& p, int b, int hk, int first, int step_) {
     row0 = first, step = step_;
-    asm volatile("" : "+v"(l15), "+v"(g));   // addresses are worked out here, not held from part to part
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));   // addresses are worked out here, not held from part to part
+    const int l15 = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int row = row0 + step * r + l15, token = row / p.G, h = hk * p.G + row - token * p.G;
@@ -324,11 +343,12 @@ struct Rows {
 // What the softmax needs of each key, by one lane a key, into 3 x 64 floats: SK sm_scale log2 e, log2 SV
 // and 1 / SV. A scale of 0 (a token never written) weighs as its key says and adds zeros; one of NaN (a
 // row that is not finite) makes the weights of the rows that see it NaN, and 1/SV 0, so that the
-// others' weights of 0 leave their sums alone. So do keys behind the sequence's end.
+// others' weights of 0 leave their sums alone. Keys that are not held weigh nothing: with a score of 0,
+// which is neither infinite nor NaN, their u is -infinity.
 __device__ __forceinline__ void key_consts(float* dst, int key, float sk, float sv, float c, bool held) {
   const float v = sv < SV_LEAST ? SV_LEAST : sv;
-  dst[key] = sk * c;
-  dst[64 + key] = __builtin_amdgcn_logf(v);
+  dst[key] = held ? sk * c : 0.0f;
+  dst[64 + key] = held ? __builtin_amdgcn_logf(v) : NEG_INF;
   dst[128 + key] = held ? fmaxf(__builtin_amdgcn_rcpf(v), 0.0f) : 0.0f;
 }
 
@@ -368,23 +388,29 @@ __device__ __forceinline__ uint64_t seen_keys(const Shape& p, const Lens& n, int
 template <int NR, typename T, int D, int R>
 __device__ __forceinline__ void softmax_step(const Shape& p, const Lens& n, int b, int key0,
                                              const float* consts, int g, Rows<T, D, R>& w,
-                                             f32x4 (&s)[NR][4], f16x8 (&wf)[NR][2]) {
+                                             f32x4 (&s)[R][4], f16x8 (&wf)[R][2]) {
   const int prefix = n.kv - n.tokens;
+  f32x4 ks[4], lv[4], rsv[4];
 #pragma unroll
   for (int kt = 0; kt < 4; ++kt) {
-    const f32x4 ks = *(const f32x4*)(consts + 16 * kt + 4 * g);
-    const f32x4 lv = *(const f32x4*)(consts + 64 + 16 * kt + 4 * g);
+    ks[kt] = *(const f32x4*)(consts + 16 * kt + 4 * g);
+    lv[kt] = *(const f32x4*)(consts + 64 + 16 * kt + 4 * g);
+  }
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt) rsv[kt] = *(const f32x4*)(consts + 128 + 16 * kt + 4 * g);
+  asm volatile("" : : : "memory");   // all requested here
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
     for (int r = 0; r < NR; ++r)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[r][kt][i] = __builtin_fmaf(s[r][kt][i], ks[i], lv[i]);
-  }
+      for (int i = 0; i < 4; ++i) s[r][kt][i] = __builtin_fmaf(s[r][kt][i], ks[kt][i], lv[kt][i]);
   if (key0 + NPAD > prefix || key0 + NPAD > n.keys) {
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      int row = w.row0 + w.step * r + (threadIdx.x & 15);
-      asm volatile("" : "+v"(row));   // its token is worked out here, not held over the loop
-      const uint64_t seen = seen_keys(p, n, b, key0, row / p.G);
+      int tid = threadIdx.x, G = p.G;
+      asm volatile("" : "+v"(tid), "+s"(G));   // the row's token is worked out here, not held over the loop
+      const uint64_t seen = seen_keys(p, n, b, key0, (w.row0 + w.step * r + (tid & 15)) / G);
       const u32 half[2] = {(u32)seen >> (4 * g), (u32)(seen >> 32) >> (4 * g)};
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
@@ -418,11 +444,10 @@ __device__ __forceinline__ void softmax_step(const Shape& p, const Lens& n, int 
     const float shift = (w.m[r] == NEG_INF ? 0.0f : w.m[r]) - W_SHIFT;
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
-      const f32x4 rsv = *(const f32x4*)(consts + 128 + 16 * kt + 4 * g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float x = __builtin_amdgcn_exp2f(s[r][kt][i] - shift);
-        w.l[r] = __builtin_fmaf(x, rsv[i], w.l[r]);
+        w.l[r] = __builtin_fmaf(x, rsv[kt][i], w.l[r]);
         wf[r][kt >> 1][4 * (kt & 1) + i] = (f16)x;
       }
     }
@@ -485,7 +510,7 @@ __device__ __forceinline__ void finish_row(const Shape& p, const Lens& n, const 
 // Up to 16 R rows of a plane. Wave w of a part takes its pages first + w, then every W-th. The next
 // page's K is requested when the scores are done with this one's, its V when the products are.
 template <typename T, bool KINT8, int D, int R, int W>
-__global__ __launch_bounds__(64 * W, (R == 2 && D == 128) ? 1 : 2) void cache_attn_stream_kernel(Shape p) {
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu((R == 2 && D == 128) ? 1 : 2, (R == 2 && D == 128) ? 1 : 2))) void cache_attn_stream_kernel(Shape p) {
   typedef typename Frag<T>::type frag;
   constexpr int KC = D / 64, KT = D / 32, VE = D / 16, VW = VE / 4, LD = D + 4;
   __shared__ __attribute__((aligned(16))) float lds_o[W][16][LD];
@@ -502,10 +527,10 @@ __global__ __launch_bounds__(64 * W, (R == 2 && D == 128) ? 1 : 2) void cache_at
     int id = pg < p.max_pages ? table[pg] : -1;
     const Lens n = lens_of(p, b);
     Rows<T, D, R> w;
-    w.load(p, b, part.hk, 0, 16, l15, g);
+    w.load(p, b, part.hk, 0, 16);
 
     u32x4 kw[4][KC];
-    u32 vw[4][VW][4];   // [key tile][word of the row's 4 VW bytes][key 4g + j]
+    u32x4 vw[4][VW];   // [key tile][word of the row's 4 VW bytes][key 4g + j]
     float sk = 0.0f, sv = 0.0f;
     auto load_k = [&](int64_t base) {
       const u8* kp = p.k8 + base * D;
@@ -630,127 +655,160 @@ __global__ __launch_bounds__(64 * W, (R == 2 && D == 128) ? 1 : 2) void cache_at
 // Row blocks of up to 64 R rows of a plane, the row tiles of 16 dealt to the four waves in turn. The page
 // in work lies in LDS as the MFMAs' operands (K: key tile x k-step, V: half x column tile; 1 KB each,
 // one 16-byte piece a lane), the next one's bytes in registers: wave w converts key tile w of K and
-// half w / 2 of V, four column tiles of it at D = 128 and two at 64.
+// half w / 2 of V, four column tiles of it at D = 128 and two at 64. One barrier a page: the page after
+// it goes to the other half of the buffers, whose readers passed the barrier before. Two blocks share a
+// CU, whose matrix cores and vector units each serve one while the other waits.
 template <typename T, bool KINT8, int D, int R>
-__global__ __launch_bounds__(256, 2) void cache_attn_shared_kernel(Shape p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void cache_attn_shared_kernel(Shape p) {
   typedef typename Frag<T>::type frag;
   constexpr int KC = D / 64, KT = D / 32, VE = D / 16;
   __shared__ __attribute__((aligned(16))) u32x4 lds_k[2][4][KT][64];
   __shared__ __attribute__((aligned(16))) u32x4 lds_v[2][2][VE][64];
   __shared__ __attribute__((aligned(16))) float lds_c[2][192];
 
-  const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int vu = wave >> 1, odd = wave & 1;
   const Place at = place_of(p);
 
   for_parts(p, at, lane, [&](const Part& part) {
     const int b = part.b;
-    const int* table = p.table + b * p.t_sb;
     const Lens n = lens_of(p, b);
     const int block0 = at.rb * p.rows, row0 = block0 + 16 * wave;
     // rows of the block that are there, and the wave's tiles of them
     const int rows = n.tokens * p.G - block0 < p.rows ? n.tokens * p.G - block0 : p.rows;
     const int tiles = rows > 16 * wave ? (rows - 16 * wave + 63) / 64 : 0;
     Rows<T, D, R> w;
-    w.load(p, b, part.hk, row0, 64, l15, g);
+    w.load(p, b, part.hk, row0, 64);
 
-    const int last = rows > 0 ? part.last : 0;
+    const int last = rows > 0 ? part.last : part.first;
+    // this wave's share of the next page, and the keys' scales, by lane
     u32x4 kw[KC];
-    u32 vw[2][4];
-    float sk = 0.0f, sv = 0.0f;
-    bool there = false;
+    u32 vw[8];
+    float sk, sv;
+    int held;   // keys of that page, 0 where there is none (and 64 or more: all)
+    // page numbers are requested a page before they are used, ahead of that page's bytes
+    const int* numbers = p.table + b * p.t_sb;
+    int number = 0;
+    // Requests page pg's share (the last page's again behind it), without a branch: nothing but the
+    // conversion waits for these loads. Offsets that hang on the lane or the wave are worked out here and
+    // in convert, not held over the loop, where registers are short.
     auto fetch = [&](int pg) {
-      const int id = pg < last ? __builtin_amdgcn_readfirstlane(table[pg]) : -1;
-      there = id >= 0 && id < p.num_pages;
-      if (!there) return;
-      const int64_t base = ((int64_t)id * p.H_kv + part.hk) * NPAD;
-      const u8* kp = p.k8 + (base + 16 * wave) * D;
-      const u8* vp = p.v8 + (base + 32 * vu) * D + (VE == 8 ? 4 * odd : 0);
+      const int cur = __builtin_amdgcn_readfirstlane(number);
+      const bool there = cur >= 0 && cur < p.num_pages;
+      number = numbers[pg + 1 < last ? pg + 1 : last - 1];
+      held = there ? n.keys - pg * NPAD : 0;
+      const int64_t base = ((int64_t)(there ? cur : 0) * p.H_kv + part.hk) * NPAD;
+      int ln = lane, me = wave;
+      asm volatile("" : "+v"(ln), "+s"(me));
+      const u8* kp = p.k8 + base * D;
+      const u8* vp = p.v8 + base * D;
+      u32 ko = (u32)((16 * me + (ln & 15)) * D + (ln >> 4) * 16);
+      u32 vo = (u32)((32 * (me >> 1) + (ln >> 4) * 4) * D + (ln & 15) * VE + (VE == 8 ? 4 * (me & 1) : 0));
+      asm volatile("" : "+v"(ko), "+v"(vo));
 #pragma unroll
-      for (int c = 0; c < KC; ++c) kw[c] = *(const u32x4*)(kp + (u32)(l15 * D + 16 * g + 64 * c));
+      for (int c = 0; c < KC; ++c) kw[c] = *(const u32x4*)(kp + (ko + 64 * c));
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          vw[x][j] = *(const u32*)(vp + (u32)(4 * g * D + l15 * VE + (16 * x + j) * D));
-      if (wave == 0) sk = (p.sk + base)[(u32)lane], sv = (p.sv + base)[(u32)lane];
+      for (int i = 0; i < 8; ++i) vw[i] = *(const u32*)(vp + (vo + (16 * (i >> 2) + (i & 3)) * D));
+      sk = (p.sk + base)[(u32)ln];
+      sv = (p.sv + base)[(u32)ln];
     };
-    auto convert = [&](int pg, int buf) {
-      if (!there) return;
-      const int key0 = pg * NPAD;
+    // The requested page to LDS. What lies behind the sequence's end, or on no page, is zeros under the
+    // constants of a key that weighs nothing: no NaN may meet a weight of zero.
+    auto convert = [&](int pg) {
+      const int buf = pg & 1;
+      int ln = lane, me = wave;
+      asm volatile("" : "+v"(ln), "+s"(me));
+      if (held < NPAD) {
+        const int left = held - 32 * (me >> 1) - (ln >> 4) * 4;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vw[i] = 16 * (i >> 2) + (i & 3) < left ? vw[i] : 0u;
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+          if (16 * me + (ln & 15) >= held) kw[c] = (u32x4){0, 0, 0, 0};
+      }
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
         const frag f = k_frag<T, KINT8>(kw[t >> 1][2 * (t & 1)], kw[t >> 1][2 * (t & 1) + 1]);
-        __builtin_memcpy(&lds_k[buf][wave][t][lane], &f, 16);
-      }
-      if (key0 + NPAD > n.keys) {   // whatever lies behind the end: no NaN may meet a weight of zero
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (key0 + 32 * vu + 16 * x + 4 * g + j >= n.keys) vw[x][j] = 0;
+        __builtin_memcpy(&lds_k[buf][me][t][ln], &f, 16);
       }
       f16x8 vf[4];
-      v_frags(vw[0], vw[1], vf);
+      v_frags((u32x4){vw[0], vw[1], vw[2], vw[3]}, (u32x4){vw[4], vw[5], vw[6], vw[7]}, vf);
+      if constexpr (VE == 8) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (VE == 8)
-          __builtin_memcpy(&lds_v[buf][vu][(VE == 8 ? 4 * odd : 0) + e][lane], &vf[e], 16);
-        else if ((e >> 1) == odd)
-          __builtin_memcpy(&lds_v[buf][vu][e][lane], &vf[e], 16);
-      if (wave == 0) key_consts(lds_c[buf], lane, sk, sv, p.c, key0 + lane < n.keys);
-    };
-    // the page in LDS for the wave's first NR row tiles
-    auto page = [&](auto nr, int pg, int buf) {
-      constexpr int NR = decltype(nr)::value;
-      f32x4 s[NR][4];
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-#pragma unroll
-        for (int r = 0; r < NR; ++r) s[r][kt] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          frag kf;
-          __builtin_memcpy(&kf, &lds_k[buf][kt][t][lane], 16);
-#pragma unroll
-          for (int r = 0; r < NR; ++r) s[r][kt] = mfma(kf, w.q[r][t], s[r][kt]);
-        }
+        for (int e = 0; e < 4; ++e) __builtin_memcpy(&lds_v[buf][me >> 1][4 * (me & 1) + e][ln], &vf[e], 16);
+      } else {   // both waves of a half have all four tiles, and write two each
+        const bool odd = me & 1;
+        const f16x8 v0 = odd ? vf[2] : vf[0], v1 = odd ? vf[3] : vf[1];
+        __builtin_memcpy(&lds_v[buf][me >> 1][2 * (me & 1)][ln], &v0, 16);
+        __builtin_memcpy(&lds_v[buf][me >> 1][2 * (me & 1) + 1][ln], &v1, 16);
       }
-      f16x8 wf[NR][2];
-      softmax_step<NR>(p, n, b, pg * NPAD, lds_c[buf], g, w, s, wf);
+      if (me == 0) key_consts(lds_c[buf], ln, sk, sv, p.c, ln < held);
+    };
+    f32x4 s[R][4];
+    f16x8 wf[R][2];
+    auto scores = [&](auto nr, int pg) {
+      constexpr int NR = decltype(nr)::value;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int r = 0; r < NR; ++r)
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          f16x8 vf;
-          __builtin_memcpy(&vf, &lds_v[buf][u][e][lane], 16);
+        for (int kt = 0; kt < 4; ++kt) s[r][kt] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+      // two key tiles at a time, so that no MFMA waits for the one before it
+      auto tile = [](int i) { return i / (2 * KT) * 2 + (i & 1); };
+      auto step = [](int i) { return i % (2 * KT) / 2; };
+      const auto* k = lds_k[pg & 1];
+      run_operands<4 * KT>([&](int i) { return k[tile(i)][step(i)][lane]; },
+                           [&](auto i, const u32x4& x) {
+                             constexpr int I = decltype(i)::value;
+                             frag kf;
+                             __builtin_memcpy(&kf, &x, 16);
 #pragma unroll
-          for (int r = 0; r < NR; ++r) w.acc[r][e] = mfma(vf, wf[r][u], w.acc[r][e]);
+                             for (int r = 0; r < NR; ++r)
+                               s[r][tile(I)] = mfma(kf, w.q[r][step(I)], s[r][tile(I)]);
+                           });
+    };
+    auto values = [&](auto nr, int pg) {
+      constexpr int NR = decltype(nr)::value;
+      const auto* v = lds_v[pg & 1];
+      run_operands<2 * VE>([&](int i) { return v[i / VE][i % VE][lane]; },
+                           [&](auto i, const u32x4& x) {
+                             constexpr int I = decltype(i)::value;
+                             f16x8 vf;
+                             __builtin_memcpy(&vf, &x, 16);
+#pragma unroll
+                             for (int r = 0; r < NR; ++r)
+                               w.acc[r][I % VE] = mfma(vf, wf[r][I / VE], w.acc[r][I % VE]);
+                           });
+    };
+    // all pages for the wave's first NR row tiles
+    auto pages = [&](auto nr) {
+      constexpr int NR = decltype(nr)::value;
+      for (int pg = part.first; pg < last; ++pg) {
+        fetch(pg + 1);
+        if constexpr (NR > 0) {
+          scores(nr, pg);
+          softmax_step<NR>(p, n, b, pg * NPAD, lds_c[pg & 1], g, w, s, wf);
+          values(nr, pg);
         }
+        if (pg + 1 < last) convert(pg + 1);
+        __syncthreads();
+      }
     };
 
-    int pg = part.first, buf = 0;
-    fetch(pg);
-    convert(pg, 0);
-    bool work = there;   // whether the page in LDS is one
-    __syncthreads();
-    for (; pg < last; ++pg) {
-      fetch(pg + 1);
-      if (work && tiles) {
-        if (R == 1 || tiles >= R)
-          page(std::integral_constant<int, R>{}, pg, buf);
-        else
-          page(std::integral_constant<int, 1>{}, pg, buf);
-      }
-      convert(pg + 1, buf ^ 1);   // the other buffer: its readers passed the last barrier
-      work = there;
-      buf ^= 1;
+    if (part.first < last) {
+      number = numbers[part.first];
+      fetch(part.first);
+      convert(part.first);   // the readers of the part before have passed its last barrier
       __syncthreads();
+      // (two tiles a wave are taken for five or more, so that a wave without any is rare there)
+      if (tiles == R)
+        pages(std::integral_constant<int, R>{});
+      else
+        pages(std::integral_constant<int, R - 1>{});
     }
 
-    int in0 = 16 * wave + l15, col0 = VE * 4 * g;
-    asm volatile("" : "+v"(in0), "+v"(col0));   // addresses are worked out here, not held over the loop
+    int ln = threadIdx.x & 63;
+    asm volatile("" : "+v"(ln));   // addresses are worked out here, not held over the loop
+    const int in0 = 16 * wave + (ln & 15), col0 = VE * 4 * (ln >> 4);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const float sum = sum_groups(w.l[r]);

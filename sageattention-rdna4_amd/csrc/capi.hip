@@ -281,7 +281,7 @@ int check_cache_attn_shape(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_
                 (long long)max_pages, (long long)(B * H_kv));
   if ((rc = check_grid("the join", B * H * T, 256))) return rc;
   return check_grid("the cached attention", sage::cache_attn_plan(B, H, H_kv, T, max_pages).blocks,
-                    256);
+                    512);
 }
 
 }  // namespace
