@@ -355,9 +355,9 @@ __device__ __forceinline__ void key_consts(float* dst, int key, float sk, float 
 // The keys of a page that this lane's row sees, a bit each; token: the row's new token. Under a mask, lane
 // x looks at key x for each of the 16 rows in turn (64 bytes of the mask at once), and every row's lanes
 // keep its ballot.
-__device__ __forceinline__ uint64_t seen_keys(const Shape& p, const Lens& n, int b, int key0, int token) {
+__device__ __forceinline__ uint64_t seen_keys(const Shape& p, const Lens& n, int b, int key0, int held,
+                                              int token) {
   const int prefix = n.kv - n.tokens;    // tokens that every new token sees
-  const int held = n.keys - key0;
   if (!p.mask) {
     const int upto = prefix + token + 1 - key0, count = upto < held ? upto : held;
     return count >= 64 ? ~0ull : count <= 0 ? 0ull : (1ull << count) - 1;
@@ -366,17 +366,18 @@ __device__ __forceinline__ uint64_t seen_keys(const Shape& p, const Lens& n, int
   asm volatile("" : "+v"(lane));   // what follows from it is worked out here, not held over the loop
   const int draft = key0 + lane - prefix;
   const u8* mask = p.mask + b * p.m_sb;
+  // every row's byte at once, from a place that there is; n.tokens is 1 or more here
+  const u32 col = (u32)(draft < 0 ? 0 : draft < n.tokens ? draft : n.tokens - 1);
   u8 at[16];
 #pragma unroll
   for (int x = 0; x < 16; ++x) {
     const int t = __builtin_amdgcn_readlane(token, x);
-    at[x] = draft < 0;
-    if (draft >= 0 && draft < n.tokens && t < n.tokens) at[x] = mask[t * p.m_sr + draft];
+    at[x] = (mask + (t < n.tokens ? t : n.tokens - 1) * p.m_sr)[col];
   }
   uint64_t seen = 0;
 #pragma unroll
   for (int x = 0; x < 16; ++x) {
-    const uint64_t row = __builtin_amdgcn_ballot_w64(lane < held && at[x] != 0);
+    const uint64_t row = __builtin_amdgcn_ballot_w64(lane < held && (draft < 0 || at[x] != 0));
     if ((lane & 15) == x) seen = row;
   }
   return seen;
@@ -386,7 +387,7 @@ __device__ __forceinline__ uint64_t seen_keys(const Shape& p, const Lens& n, int
 // keys that each row sees; then the running maximum and sum, and the weights as the PV MFMA takes them.
 // For the first NR of the wave's row tiles.
 template <int NR, typename T, int D, int R>
-__device__ __forceinline__ void softmax_step(const Shape& p, const Lens& n, int b, int key0,
+__device__ __forceinline__ void softmax_step(const Shape& p, const Lens& n, int b, int key0, int held,
                                              const float* consts, int g, Rows<T, D, R>& w,
                                              f32x4 (&s)[R][4], f16x8 (&wf)[R][2]) {
   const int prefix = n.kv - n.tokens;
@@ -405,12 +406,12 @@ __device__ __forceinline__ void softmax_step(const Shape& p, const Lens& n, int 
     for (int r = 0; r < NR; ++r)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[r][kt][i] = __builtin_fmaf(s[r][kt][i], ks[kt][i], lv[kt][i]);
-  if (key0 + NPAD > prefix || key0 + NPAD > n.keys) {
+  if (key0 + NPAD > prefix || held < NPAD) {
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       int tid = threadIdx.x, G = p.G;
       asm volatile("" : "+v"(tid), "+s"(G));   // the row's token is worked out here, not held over the loop
-      const uint64_t seen = seen_keys(p, n, b, key0, (w.row0 + w.step * r + (tid & 15)) / G);
+      const uint64_t seen = seen_keys(p, n, b, key0, held, (w.row0 + w.step * r + (tid & 15)) / G);
       const u32 half[2] = {(u32)seen >> (4 * g), (u32)(seen >> 32) >> (4 * g)};
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
@@ -522,32 +523,51 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu((R == 2 
 
   for_parts(p, place_of(p), lane, [&](const Part& part) {
     const int b = part.b;
-    const int* table = p.table + b * p.t_sb;
-    int pg = part.first + wave;
-    int id = pg < p.max_pages ? table[pg] : -1;
     const Lens n = lens_of(p, b);
     Rows<T, D, R> w;
     w.load(p, b, part.hk, 0, 16);
 
+    // The page in work and what is known of the next one: its place, and the keys that it holds (0 where
+    // there is no page; 64 or more: all). Its number is requested a page before that, ahead of all bytes.
+    // Loads stand in no branch, where the compiler would wait for them at its end: a wave without a next
+    // page asks for one line of its last one again.
     u32x4 kw[4][KC];
     u32x4 vw[4][VW];   // [key tile][word of the row's 4 VW bytes][key 4g + j]
-    float sk = 0.0f, sv = 0.0f;
-    auto load_k = [&](int64_t base) {
+    float sk, sv;
+    const int* numbers = p.table + b * p.t_sb;
+    int pg = part.first + wave;
+    const int end = part.last;
+    int number = numbers[pg < p.max_pages ? pg : 0], held = 0;
+    int64_t base = 0;
+    bool more = false;
+    auto look_ahead = [&](int page) {   // at page's number, and request the next one's
+      const int cur = __builtin_amdgcn_readfirstlane(number);
+      const bool there = cur >= 0 && cur < p.num_pages;
+      more = page < end;
+      number = numbers[page + W < end ? page + W : 0];
+      held = there && more ? n.keys - page * NPAD : 0;
+      base = more ? ((int64_t)(there ? cur : 0) * p.H_kv + part.hk) * NPAD : base;
+    };
+    auto load_k = [&]() {
       const u8* kp = p.k8 + base * D;
+      u32 at = more ? (u32)(l15 * D + 16 * g) : 0u;
+      asm volatile("" : "+v"(at));
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-        for (int c = 0; c < KC; ++c)
-          kw[kt][c] = *(const u32x4*)(kp + (u32)(l15 * D + 16 * g + 16 * kt * D + 64 * c));
-      sk = (p.sk + base)[(u32)lane], sv = (p.sv + base)[(u32)lane];
+        for (int c = 0; c < KC; ++c) kw[kt][c] = *(const u32x4*)(kp + (at + 16 * kt * D + 64 * c));
+      sk = (p.sk + base)[(u32)lane];
+      sv = (p.sv + base)[(u32)lane];
     };
-    auto load_v = [&](int64_t base) {
+    auto load_v = [&]() {
       const u8* vp = p.v8 + base * D;
+      u32 at = more ? (u32)(4 * g * D + l15 * VE) : 0u;
+      asm volatile("" : "+v"(at));
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const u8* src = vp + (u32)(4 * g * D + l15 * VE + (16 * kt + j) * D);
+          const u8* src = vp + (at + (16 * kt + j) * D);
           if constexpr (VW == 2) {
             const u32x2 x = *(const u32x2*)src;
             vw[kt][0][j] = x[0], vw[kt][1][j] = x[1];
@@ -556,24 +576,14 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu((R == 2 
           }
         }
     };
-    // the next page of the wave that there is: its place in the pool, or -1
-    auto next_page = [&]() -> int64_t {
-      while (pg < part.last) {
-        const int cur = __builtin_amdgcn_readfirstlane(id);
-        pg += W;
-        id = pg < part.last ? table[pg] : -1;
-        if (cur >= 0 && cur < p.num_pages) return ((int64_t)cur * p.H_kv + part.hk) * NPAD;
-      }
-      return -1;
-    };
-    int64_t base = next_page();
-    int key0 = (pg - W) * NPAD;
-    if (base >= 0) {
-      load_k(base);
-      load_v(base);
+    if (pg < end) {
+      look_ahead(pg);
+      load_k();
+      load_v();
     }
-    while (base >= 0) {
-      key_consts(lds_c[wave], lane, sk, sv, p.c, key0 + lane < n.keys);
+    for (; pg < end; pg += W) {
+      const int key0 = pg * NPAD, now = held;
+      key_consts(lds_c[wave], lane, sk, sv, p.c, lane < now);
       f32x4 s[R][4];
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt) {
@@ -586,20 +596,19 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu((R == 2 
           for (int r = 0; r < R; ++r) s[r][kt] = mfma(kf, w.q[r][t], s[r][kt]);
         }
       }
-      const int64_t next = next_page();
-      if (next >= 0) load_k(next);
-      if (key0 + NPAD > n.keys) {   // whatever lies behind the end: no NaN may meet a weight of zero
+      look_ahead(pg + W);
+      load_k();
+      if (now < NPAD) {   // whatever lies behind the end, or on no page: no NaN may meet a weight of zero
+        const int left = now - 4 * g;
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (key0 + 16 * kt + 4 * g + j >= n.keys) {
 #pragma unroll
-              for (int x = 0; x < VW; ++x) vw[kt][x][j] = 0;
-            }
+            for (int x = 0; x < VW; ++x) vw[kt][x][j] = 16 * kt + j < left ? vw[kt][x][j] : 0u;
       }
       f16x8 wf[R][2];
-      softmax_step<R>(p, n, b, key0, lds_c[wave], g, w, s, wf);
+      softmax_step<R>(p, n, b, key0, now, lds_c[wave], g, w, s, wf);
 
       // O^T += V^T W^T: tile e's row x is column VE x + e
 #pragma unroll
@@ -613,9 +622,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu((R == 2 
 #pragma unroll
             for (int r = 0; r < R; ++r) w.acc[r][4 * x + e] = mfma(vf[e], wf[r][u], w.acc[r][4 * x + e]);
         }
-      if (next >= 0) load_v(next);
-      base = next;
-      key0 = (pg - W) * NPAD;
+      load_v();
     }
 
     // the waves' results merged, 16 rows at a time; each thread has N columns of a row
@@ -783,10 +790,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     auto pages = [&](auto nr) {
       constexpr int NR = decltype(nr)::value;
       for (int pg = part.first; pg < last; ++pg) {
+        const int now = held;
         fetch(pg + 1);
         if constexpr (NR > 0) {
           scores(nr, pg);
-          softmax_step<NR>(p, n, b, pg * NPAD, lds_c[pg & 1], g, w, s, wf);
+          softmax_step<NR>(p, n, b, pg * NPAD, now, lds_c[pg & 1], g, w, s, wf);
           values(nr, pg);
         }
         if (pg + 1 < last) convert(pg + 1);
