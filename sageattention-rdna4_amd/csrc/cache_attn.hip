@@ -146,11 +146,12 @@ struct Shape {
   float* lse;
   float* part_o;    // (runs, RB, 2, rows, D): a run's last part of a plane begun before it, and its
   float* part_ml;   // part of the plane that goes on behind it; (runs, RB, 2, rows, 2)
-  uint2* starts;    // (planes): where its pages begin in the row of all, and the runs' length
+  uint2* starts;    // (planes): where its pages begin in the row of all planes, and the runs' length
   int B, H, H_kv, G, T, RB;
   int rows;         // of a row block
   int units;        // planes, or runs
-  int least;        // pages of a run at least; 0: a block for each plane
+  int least;        // length of a run at least; 0: a block for each plane
+  int ahead;        // cost of beginning a plane, in pages
   float c;          // sm_scale log2 e
 };
 
@@ -188,43 +189,46 @@ __device__ __forceinline__ u32 lane_of(u32 x, int lane) {
   return (u32)__builtin_amdgcn_readlane((int)x, lane);
 }
 
-// All sequences' pages in a row (each H_kv times, plane after plane), and the runs' length. Every wave
-// works it out by itself, 64 sequences at a time; the entry point bounds the sum by 2^31.
+// All planes in a row: each is as long as its pages and, ahead of them, what it costs to begin a plane,
+// in pages (so that the runs that hold many short planes do not end last). Every wave works it out by
+// itself, 64 sequences at a time; the entry point bounds the sum by 2^31.
 struct Runs {
-  u32 mine, upto;   // of sequence `lane`: its pages, and the pages up to its end
-  u32 total, per;
+  u32 mine, upto;   // length of sequence `lane`'s planes, and of those up to its own, one of each head
+  u32 total, per;   // of the row, and of a run
 };
+__device__ __forceinline__ u32 length_of(const Shape& p, int b) {
+  const u32 pages = b < p.B ? (u32)pages_of(p, b) : 0u;
+  return pages ? pages + (u32)p.ahead : 0u;
+}
 __device__ __forceinline__ Runs runs_of(const Shape& p, int lane) {
   Runs r;
-  r.mine = lane < p.B ? (u32)pages_of(p, lane) : 0u;
+  r.mine = length_of(p, lane);
   r.upto = scan_lanes(r.mine, lane);
-  u32 pages = lane_of(r.upto, 63);
+  u32 length = lane_of(r.upto, 63);
   for (int b0 = 64; b0 < p.B; b0 += 64)
-    pages += lane_of(scan_lanes(b0 + lane < p.B ? (u32)pages_of(p, b0 + lane) : 0u, lane), 63);
-  r.total = pages * (u32)p.H_kv;
+    length += lane_of(scan_lanes(length_of(p, b0 + lane), lane), 63);
+  r.total = length * (u32)p.H_kv;
   const u32 even = (r.total + (u32)p.units - 1) / (u32)p.units;
   r.per = even < (u32)p.least ? (u32)p.least : even;
   return r;
 }
-// The sequence that `pick` (of the pages up to a sequence's end, and its number) first holds for, with
-// its pages and those before it; there is one.
+// The sequence at y of the row with one plane of each, its planes' length and that of those before it.
 struct Seq {
   int b;
-  u32 pages, before;
+  u32 length, before;
 };
-template <typename F>
-__device__ __forceinline__ Seq find_seq(const Shape& p, const Runs& r, int lane, F&& pick) {
+__device__ __forceinline__ Seq find_seq(const Shape& p, const Runs& r, int lane, u32 y) {
   u32 mine = r.mine, upto = r.upto, base = 0;
   for (int b0 = 0;;) {
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(b0 + lane < p.B && pick(base + upto, b0 + lane));
-    if (hit || b0 + 64 >= p.B) {
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(base + upto > y);
+    if (hit || b0 + 64 >= p.B) {   // y lies below the sum: there is one
       const int at = hit ? __builtin_ctzll(hit) : 0;
       const u32 n = lane_of(mine, at);
       return {b0 + at, n, base + lane_of(upto, at) - n};
     }
     base += lane_of(upto, 63);
     b0 += 64;
-    mine = b0 + lane < p.B ? (u32)pages_of(p, b0 + lane) : 0u;
+    mine = length_of(p, b0 + lane);
     upto = scan_lanes(mine, lane);
   }
 }
@@ -250,41 +254,46 @@ struct Part {
 template <typename F>
 __device__ __forceinline__ void for_parts(const Shape& p, const Place& at, int lane, F&& f) {
   if (at.unit >= (u32)p.units) return;
-  u32 x = 0, end, per = 0;   // of the pages in a row
-  int b, hk, first = 0, pages;
+  u32 left, per = 0;          // of the run; its length
+  int b, hk, pages, at0 = 0;   // plane, its pages, and the page (from -ahead on) where the run is
+  u32 x = 0;                   // place of the plane's page 0 in the row
   if (!p.least) {
     b = (int)(at.unit / (u32)p.H_kv);
     hk = (int)(at.unit - (u32)b * (u32)p.H_kv);
     pages = pages_of(p, b);
-    end = (u32)pages;
+    left = (u32)pages;
   } else {
     const Runs r = runs_of(p, lane);
     per = r.per;
-    x = at.unit * r.per;   // below 2^31 + the pages of a run
-    if (x >= r.total) return;
-    end = x + r.per < r.total ? x + r.per : r.total;
-    const u32 y = x / (u32)p.H_kv;
-    const Seq q = find_seq(p, r, lane, [&](u32 upto, int) { return upto > y; });
-    const u32 in = x - q.before * (u32)p.H_kv;
+    const u32 begin = at.unit * per;   // below 2^31 + the length of a run
+    if (begin >= r.total) return;
+    left = r.total - begin < per ? r.total - begin : per;
+    const Seq q = find_seq(p, r, lane, begin / (u32)p.H_kv);
+    const u32 in = begin - q.before * (u32)p.H_kv;
     b = q.b;
-    pages = (int)q.pages;
-    hk = (int)(in / q.pages);
-    first = (int)(in - (u32)hk * q.pages);
+    hk = (int)(in / q.length);
+    pages = (int)q.length - p.ahead;
+    at0 = (int)(in - (u32)hk * q.length) - p.ahead;
+    x = begin - (u32)at0;
   }
   for (;;) {
-    const int left = (int)(end - x), last = pages - first < left ? pages : first + left;
+    const u32 rest = (u32)(pages - at0);   // of the plane
+    const int first = at0 < 0 ? 0 : at0, last = rest < left ? pages : at0 + (int)left;
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));
-    if (p.least && first == 0 && at.rb == 0 && tid == 0)
-      p.starts[b * p.H_kv + hk] = make_uint2(x, per);   // for the join
-    f(Part{b, hk, first, last, first == 0 && last == pages,
-           (((int64_t)at.unit * p.RB + at.rb) * 2 + (first == 0)) * p.rows});
-    x += (u32)(last - first);
-    if (x >= end) return;
-    first = 0;
+    if (last > first || !p.least) {
+      if (p.least && first == 0 && at.rb == 0 && tid == 0)
+        p.starts[b * p.H_kv + hk] = make_uint2(x, per);   // for the join
+      f(Part{b, hk, first, last, first == 0 && last == pages,
+             (((int64_t)at.unit * p.RB + at.rb) * 2 + (first == 0)) * p.rows});
+    }
+    if (rest >= left) return;
+    left -= rest;
+    x += (u32)pages + (u32)p.ahead;
+    at0 = -p.ahead;
     if (++hk == p.H_kv) {
       hk = 0;
-      do {   // one with pages follows: x lies below the sum of all
+      do {   // one with pages follows: the run ends below the row's length
         if (++b >= p.B) return;
         pages = pages_of(p, b);
       } while (pages == 0);
@@ -954,6 +963,7 @@ hipError_t run(const CacheAttnArgs& a, hipStream_t st) {
   p.rows = (int)plan.rows;
   p.units = (int)plan.units;
   p.least = (int)plan.least;
+  p.ahead = CACHE_ATTN_AHEAD;
   p.c = a.sm_scale * LOG2E_F;
   p.part_o = (float*)a.workspace;
   p.part_ml = p.part_o + plan.part_rows * D;

@@ -169,6 +169,8 @@ enum CacheAttnKernel {
   CACHE_ATTN_SHARED64,        // row blocks of up to 64
   CACHE_ATTN_SHARED128,       // and 128 rows
 };
+// What beginning a plane costs a run, in pages of its own (see cache_attn.hip).
+constexpr int CACHE_ATTN_AHEAD = 4;
 struct CacheAttnPlan {
   CacheAttnKernel kernel;
   int64_t rows, row_blocks, planes, units, least, part_rows, blocks;
