@@ -930,7 +930,7 @@ __global__ __launch_bounds__(256) void cache_attn_join_kernel(Shape p, u32 row_t
 
 template <typename T, bool KINT8, int D>
 hipError_t run(const CacheAttnArgs& a, hipStream_t st) {
-  const CacheAttnPlan plan = cache_attn_plan(a.B, a.H, a.H_kv, a.T, a.pool.max_pages);
+  const CacheAttnPlan plan = cache_attn_plan(a.B, a.H, a.H_kv, a.T, a.pool.max_pages, D);
   Shape p;
   p.k8 = (const u8*)a.pool.k8;
   p.sk = a.pool.sk;
@@ -1008,7 +1008,18 @@ hipError_t run_d(const CacheAttnArgs& a, hipStream_t st) {
 
 }  // namespace
 
-CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_t max_pages) {
+// Which kernel: by the rows M that read one K/V head. Up to 32 rows leave the matrix cores idle enough
+// for every wave to convert its own pages (stream); more share the conversion. Measured, 8 sequences of
+// 8192 tokens, 8 K/V heads, us: M = 32 stream 37, shared 48; M = 64 shared 55.
+//
+// Which cut: as many runs as blocks are resident at once (512 threads' registers of a CU hold two blocks
+// of 4 waves, but one of the 32-row kernel at head_dim 128), so that all runs begin and end together.
+// 8 x 3000 tokens, M = 4: 512 runs 20 us, 1024 runs 26; 8 x 8192, M = 32: 256 runs 37, 1024 runs 61. Runs
+// shorter than a page for each wave (or two pages, shared) cost more in their beginnings than they save.
+// Short sequences, and more planes than fill the card four times, take a block for each plane and no
+// second launch: 16 pages in one launch of 8 waves a plane 13 us, spread 14; 32 pages 18 and 13.
+CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_t max_pages,
+                              int64_t D) {
   CacheAttnPlan p;
   const int64_t M = T * (H / H_kv), planes = B * H_kv, tiles = (M + 15) / 16;
   p.kernel = M <= 16 ? CACHE_ATTN_STREAM16 : M <= 32 ? CACHE_ATTN_STREAM32
@@ -1017,25 +1028,26 @@ CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int
   const int64_t most = M <= 16 ? 1 : M <= 32 ? 2 : M <= 64 ? 4 : 8;   // tiles of a row block
   p.row_blocks = (tiles + most - 1) / most;
   p.rows = 16 * ((tiles + p.row_blocks - 1) / p.row_blocks);
+  p.planes = planes;
   const int64_t blocks = planes * p.row_blocks;
-  const int64_t single = M <= 16 ? (blocks <= 256 ? 48 : 16) : stream ? 12 : 6;
-  if (max_pages <= single || blocks >= 2048) {
+  if (max_pages <= (M <= 16 ? 16 : stream ? 12 : 6) || blocks >= 2048) {
     p.units = planes;
     p.least = 0;
     p.part_rows = 0;
     p.wide_join = false;
+    // fewer planes than CUs: twice the waves for each
     if (M <= 16 && blocks <= 256) p.kernel = CACHE_ATTN_STREAM16_WIDE;
   } else {
-    p.least = stream ? 8 : 2;
-    int64_t runs = ((stream ? 1024 : 512) + p.row_blocks - 1) / p.row_blocks;
-    if (runs > (planes * max_pages + p.least - 1) / p.least)
-      runs = (planes * max_pages + p.least - 1) / p.least;
-    if (runs > 128 * planes) runs = 128 * planes;
+    p.least = stream ? 4 : 2;
+    const int64_t resident = p.kernel == CACHE_ATTN_STREAM32 && D == 128 ? 256 : 512;
+    int64_t runs = (resident + p.row_blocks - 1) / p.row_blocks;
+    const int64_t longest = (planes * (max_pages + CACHE_ATTN_AHEAD) + p.least - 1) / p.least;
+    if (runs > longest) runs = longest;
+    if (runs > 128 * planes) runs = 128 * planes;   // parts of a plane that the join reads
     p.units = runs;
     p.part_rows = runs * p.row_blocks * 2 * p.rows;
     p.wide_join = runs > 16 * planes;
   }
-  p.planes = planes;
   p.blocks = (p.units + 7) / 8 * 8 * p.row_blocks;
   return p;
 }

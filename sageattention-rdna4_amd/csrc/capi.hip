@@ -280,7 +280,7 @@ int check_cache_attn_shape(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_
     return fail(SAGE_ERR_INVALID, "block_table: %lld pages for %lld planes are too many",
                 (long long)max_pages, (long long)(B * H_kv));
   if ((rc = check_grid("the join", B * H * T, 256))) return rc;
-  return check_grid("the cached attention", sage::cache_attn_plan(B, H, H_kv, T, max_pages).blocks,
+  return check_grid("the cached attention", sage::cache_attn_plan(B, H, H_kv, T, max_pages, D).blocks,
                     512);
 }
 
@@ -713,7 +713,7 @@ int64_t sage_cache_attn_workspace_bytes(int64_t B, int64_t H, int64_t H_kv, int6
   if (rc) return -rc;
   g_err.clear();
   return (int64_t)sage::cache_attn_workspace_bytes(
-      sage::cache_attn_plan(B, H, H_kv, T, max_pages), D);
+      sage::cache_attn_plan(B, H, H_kv, T, max_pages, D), D);
 }
 
 int sage_cache_attn(int dtype, int k_int8, const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sr,
@@ -739,7 +739,7 @@ int sage_cache_attn(int dtype, int k_int8, const void* q, int64_t q_sb, int64_t 
   if (lse && ((uintptr_t)lse & 3u))
     return fail(SAGE_ERR_INVALID, "ptr_align: lse must be 4-byte aligned");
   const size_t need = sage::cache_attn_workspace_bytes(
-      sage::cache_attn_plan(B, H, H_kv, T, max_pages), D);
+      sage::cache_attn_plan(B, H, H_kv, T, max_pages, D), D);
   if (need && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
     return fail(SAGE_ERR_INVALID, "workspace: need %zu bytes, 16-byte aligned (got %zu)", need,
                 workspace_bytes);

@@ -176,7 +176,8 @@ struct CacheAttnPlan {
   int64_t rows, row_blocks, planes, units, least, part_rows, blocks;
   bool wide_join;
 };
-CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_t max_pages);
+CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_t max_pages,
+                              int64_t D);
 size_t cache_attn_workspace_bytes(const CacheAttnPlan& p, int64_t D);
 hipError_t launch_cache_attn(const CacheAttnArgs& a, hipStream_t stream);
 
