@@ -301,6 +301,14 @@ __device__ __forceinline__ void for_parts(const Shape& p, const Place& at, int l
   }
 }
 
+// Time for the last products to be written before anything else may read them (a copy on the way out of
+// a loop, say): the 16 cycles that such an MFMA takes, where the compiler's table has 8 wait states.
+__device__ __forceinline__ void results_done() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15" : : : "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // N operands from LDS, each used once, three more requested ahead of the one in use. The memory clobber
 // keeps each request where it stands: left to itself the compiler reads every operand into the same
 // registers, right before its use, and waits for LDS N times in a row.
@@ -632,6 +640,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu((R == 2 
             for (int r = 0; r < R; ++r) w.acc[r][4 * x + e] = mfma(vf[e], wf[r][u], w.acc[r][4 * x + e]);
         }
       load_v();
+      results_done();
     }
 
     // the waves' results merged, 16 rows at a time; each thread has N columns of a row

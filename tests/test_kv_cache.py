@@ -9,7 +9,8 @@ import pytest
 import torch
 
 import kv_cache_ref as ref
-from test_codegen import PKG, _assembly, _kernel_resources, masked_mfmas, undefined_converts
+from test_codegen import (PKG, _assembly, _kernel_resources, early_mfma_reads, masked_mfmas,
+                          undefined_converts)
 
 
 # ------------------------------------------------------------------------------------- tables
@@ -191,12 +192,19 @@ def test_the_reference_rotations_agree():
 
 # ---------------------------------------------------------------------------- generated code
 # The rules of the main loops' code hold for the cache's kernels: every MFMA runs with the whole wave
-# active, nothing spills, no
-# flat accesses, converts into a half-word keep a defined other half.
+# active, no result is read before its MFMA is done, nothing spills, no flat accesses, converts into a
+# half-word keep a defined other half.
 def test_attention_mfmas_run_with_the_whole_wave():
     asm = _assembly(os.path.join(PKG, "csrc", "cache_attn.hip"))
     assert "v_mfma_f32_16x16x32_f16" in asm and "v_mfma_f32_16x16x32_bf16" in asm
     assert masked_mfmas(asm) == []
+
+
+def test_attention_products_are_read_after_they_are_done():
+    # 16 cycles a 16x16x32 MFMA of 16-bit operands, counted as for the main loops' MFMAs
+    asm = _assembly(os.path.join(PKG, "csrc", "cache_attn.hip"))
+    bad = early_mfma_reads(asm, min_other=16)
+    assert not bad, bad[:4]
 
 
 @pytest.mark.parametrize("source", ["cache_attn.hip", "kv_cache.hip"])
