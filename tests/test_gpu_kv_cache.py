@@ -409,29 +409,73 @@ def test_tokens_never_written_count_as_zeros():
     assert (lse.double() - torch.log(torch.tensor(10.0))).abs().max() <= 1e-5
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [3, 8, 40])
 @pytest.mark.parametrize("L,B,H_kv", [(5000, 1, 2), (1100, 3, 1), (40000, 1, 1)])
-def test_long_sequences_are_split_and_joined(L, B, H_kv):
-    # split over many blocks: against the sum in float64 on the GPU, all rows at once
+def test_long_sequences_are_split_and_joined(L, B, H_kv, T, D):
+    # split over many blocks, 12 to 160 rows of a K/V head
     from sageattention import sageattn_cached
     gen = torch.Generator().manual_seed(L)
     lens = [L - 97 * b for b in range(B)]
-    cache, table = _filled(torch.float16, True, H_kv, 128, lens, gen)
-    q, qg = _randn((B, 4 * H_kv, 3, 128), torch.float16, "HND", gen, 2.0)
+    cache, table = _filled(torch.float16, True, H_kv, D, lens, gen)
+    q, qg = _randn((B, 4 * H_kv, T, D), torch.float16, "HND", gen, 2.0)
     o, lse = sageattn_cached(qg, cache, table, _lens(*lens), return_lse=True)
     again = sageattn_cached(qg, cache, table, _lens(*lens))
     assert torch.equal(o, again)       # sums have one order
-    want, wl, slack = ref.attention(q, cache, table.cpu(), lens) if L < 10000 else (None,) * 3
-    if want is not None:
+    if L < 10000 and T == 3:
+        want, wl, slack = ref.attention(q, cache, table.cpu(), lens)
         ref.check_attention(o.cpu(), want, slack[0], torch.float16)
         ref.check_lse(lse.cpu(), wl, slack[1])
         return
-    k, v, _ = ref.gather(cache, table.cpu(), 0, L)
-    s = q[0].double() @ k.transpose(1, 2) / 128 ** 0.5
-    s[:, 0, L - 2:] = s[:, 1, L - 1:] = -torch.inf
-    p = torch.softmax(s, -1)
-    # the bound of kv_cache_ref.attention with A <= 60 for these inputs
-    err = 2 * (132 * 2.0 ** -23 * 60 + 2.0 ** -20) + 2.0 ** -12 + L * 2.0 ** -23
-    ref.check_attention(o[0].cpu(), p @ v, err * (p @ v.abs()), torch.float16)
+    for b in range(B):   # all rows of a sequence at once
+        n = lens[b]
+        k, v, _ = ref.gather(cache, table.cpu(), b, n)
+        k, v = k.repeat_interleave(4, 0), v.repeat_interleave(4, 0)
+        s = q[b].double() @ k.transpose(1, 2) / D ** 0.5
+        a = (q[b].double().abs() @ k.abs().transpose(1, 2) / D ** 0.5).amax()
+        late = torch.arange(n) > n - T + torch.arange(T)[:, None]
+        s[:, late] = -torch.inf
+        p = torch.softmax(s, -1)
+        # the bound of kv_cache_ref.attention
+        err = 2 * ((D + 4) * 2.0 ** -23 * a + 2.0 ** -20) + 2.0 ** -12 + n * 2.0 ** -23
+        ref.check_attention(o[b].cpu(), p @ v, err * (p @ v.abs()), torch.float16)
+        assert ((lse[b].cpu().double() - torch.logsumexp(s, -1)).abs() <= err + 1e-5).all()
+
+
+def test_more_planes_than_the_card_holds():
+    # 2200 planes: a block for each, of any length
+    from sageattention import sageattn_cached
+    gen = torch.Generator().manual_seed(21)
+    B, pick = 1100, [0, 1, 64, 300, 1030]
+    lens = [pick[int(i)] for i in torch.randint(0, 5, (B,), generator=gen)]
+    lens[B - 1] = 1030
+    cache, table = _filled(torch.float16, True, 2, 64, lens, gen)
+    q, qg = _randn((B, 6, 1, 64), torch.float16, "HND", gen, 2.0)
+    o, lse = sageattn_cached(qg, cache, table, _lens(*lens), return_lse=True)
+    some = [0, 1, 2, 3, 4, 5, 550, 800, B - 1]
+    want, wl, slack = ref.attention(q[some], cache, table.cpu()[some], [lens[b] for b in some])
+    ref.check_attention(o.cpu()[some], want, slack[0], torch.float16)
+    ref.check_lse(lse.cpu()[some], wl, slack[1])
+
+
+@pytest.mark.parametrize("T", [1, 20])
+def test_sequences_that_share_pages_and_fused_queries(T):
+    # a common prefix's pages in both tables, queries as a view of a fused projection
+    from sageattention import KVCache, sageattn_cached
+    gen = torch.Generator().manual_seed(22)
+    cache = KVCache.allocate(40, 2, 128, torch.bfloat16)
+    own = torch.randperm(40, generator=gen).int()
+    table = torch.stack((own[:20], torch.cat((own[:12], own[20:28])))).cuda()
+    _, k = _randn((2, 2, 1280, 128), torch.bfloat16, "HND", gen)
+    _, v = _randn((2, 2, 1280, 128), torch.bfloat16, "HND", gen)
+    lens = [1271, 1240]
+    cache.write(k[:1], v[:1], table[:1], _lens(0), _lens(lens[0]))
+    cache.write(k[1:, :, 768:], v[1:, :, 768:], table[1:], _lens(768), _lens(lens[1] - 768))
+    fused = torch.randn(2, T, 3, 6, 128, generator=gen).bfloat16().cuda()
+    for i in range(3):
+        o = sageattn_cached(fused[:, :, i], cache, table, _lens(*lens), "NHD")
+        want, _, slack = ref.attention(fused[:, :, i].transpose(1, 2).cpu(), cache, table.cpu(), lens)
+        ref.check_attention(o.transpose(1, 2).cpu(), want, slack[0], torch.bfloat16)
 
 
 @pytest.mark.parametrize("dtype,int8", KINDS, ids=KIND_IDS)
