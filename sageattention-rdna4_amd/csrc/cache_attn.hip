@@ -1023,7 +1023,9 @@ hipError_t run_d(const CacheAttnArgs& a, hipStream_t st) {
 //
 // Which cut: as many runs as blocks are resident at once (512 threads' registers of a CU hold two blocks
 // of 4 waves, but one of the 32-row kernel at head_dim 128), so that all runs begin and end together.
-// 8 x 3000 tokens, M = 4: 512 runs 20 us, 1024 runs 26; 8 x 8192, M = 32: 256 runs 37, 1024 runs 61. Runs
+// 8 x 3000 tokens, M = 4: 512 runs 20 us, 1024 runs 26; 8 x 8192, M = 32: 256 runs 37, 1024 runs 61. The
+// row blocks of a run share an XCD, so the runs are as many as each of the 8 XCDs holds whole: three row
+// blocks (M = 384) in 168 runs 176 us, in 171 (two XCDs with blocks left for a second turn) 237. Runs
 // shorter than a page for each wave (or two pages, shared) cost more in their beginnings than they save.
 // Short sequences, and more planes than fill the card four times, take a block for each plane and no
 // second launch: 16 pages in one launch of 8 waves a plane 13 us, spread 14; 32 pages 18 and 13.
@@ -1049,7 +1051,8 @@ CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int
   } else {
     p.least = stream ? 4 : 2;
     const int64_t resident = p.kernel == CACHE_ATTN_STREAM32 && D == 128 ? 256 : 512;
-    int64_t runs = (resident + p.row_blocks - 1) / p.row_blocks;
+    int64_t runs = resident / 8 / p.row_blocks * 8;
+    if (runs < 8) runs = resident / p.row_blocks > 1 ? resident / p.row_blocks : 1;
     const int64_t longest = (planes * (max_pages + CACHE_ATTN_AHEAD) + p.least - 1) / p.least;
     if (runs > longest) runs = longest;
     if (runs > 128 * planes) runs = 128 * planes;   // parts of a plane that the join reads

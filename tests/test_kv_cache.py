@@ -179,6 +179,21 @@ def test_workspace_sizes():
 
 
 # ------------------------------------------------------------------------------------ oracles
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [33, 64, 66, 96, 100, 128, 144, 200, 400])
+def test_runs_fill_the_card_once(T, D):
+    # two blocks a CU, 32 CUs to each of the 8 XCDs that runs are dealt to with all their row blocks
+    B, H, H_kv, pages = 8, 32, 8, 128
+    tiles = -(-T * (H // H_kv) // 16)
+    blocks = -(-tiles // 8)
+    rows = 16 * -(-tiles // blocks)
+    floats = _lib().sage_cache_attn_workspace_bytes(B, H, H_kv, T, pages, D) // 4
+    parts = (floats - 2 * B * H_kv) // (D + 2)
+    runs = parts // (blocks * 2 * rows)
+    assert floats == runs * blocks * 2 * rows * (D + 2) + 2 * B * H_kv
+    assert 0.8 * 64 < -(-runs // 8) * blocks <= 64
+
+
 def test_the_reference_rotations_agree():
     gen = torch.Generator().manual_seed(0)
     from sageattention import rotary_table
