@@ -339,6 +339,44 @@ def test_attention_of_trees(dtype, int8, D, H, H_kv, T, lens):
                                           tree_mask=wide[:, :T, :T], sm_scale=0.11))
 
 
+@pytest.mark.parametrize("H", [1, 4, 12])
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 6, 9, 64, 67, 131])
+def test_masks_at_every_place_of_a_page(T, H):
+    # drafted tokens that begin anywhere in a page, masks of any bytes at any alignment, short drafts
+    from sageattention import sageattn_cached
+    gen = torch.Generator().manual_seed(1000 * H + T)
+    starts = list(range(0, 67, 3)) + [126, 127, 128, 129, 190] + [-1, -T // 2]
+    B, D = len(starts), 64
+    q_lens = [T if b % 3 else max(1, T - b // 3) for b in range(B)]
+    lens = [max(0, s + t) for s, t in zip(starts, q_lens)]
+    cache, table = _filled(torch.float16, True, 1, D, lens, gen)
+    q, qg = _randn((B, H, T, D), torch.float16, "HND", gen, 2.0)
+    kinds = torch.tensor([0, 0, 0, 1, 1, 2, 127, 128, 129, 255], dtype=torch.uint8)
+    pool = kinds[torch.randint(0, 10, (B, T, T + 5), generator=gen)].cuda()
+    for at in (0, 1, 5):
+        mask = pool[:, :, at:at + T]
+        o, lse = sageattn_cached(qg, cache, table, _lens(*lens), q_lens=_lens(*q_lens), tree_mask=mask,
+                                 return_lse=True)
+        for b in range(B):
+            n, t = lens[b], q_lens[b]
+            k, v, _ = ref.gather(cache, table.cpu(), b, n)
+            s = q[b].double() @ k[0].T / D ** 0.5
+            draft = torch.arange(n) - (n - t)
+            seen = (draft < 0) | (mask[b].cpu() != 0)[:, draft.clamp(min=0)]
+            s[:, ~seen] = -torch.inf
+            empty = ~seen.any(1) | (torch.arange(T) >= t)
+            p = torch.softmax(s, -1)
+            p[:, empty] = 0.0
+            a = (q[b].double().abs() @ k[0].abs().T / D ** 0.5).amax() if n else 0.0
+            # the bound of kv_cache_ref.attention
+            err = 2 * ((D + 4) * 2.0 ** -23 * a + 2.0 ** -20) + 2.0 ** -12 + n * 2.0 ** -23
+            spread = n * 2.0 ** -39 * v[0].abs().amax() if n else 0.0
+            ref.check_attention(o[b].cpu(), p @ v[0], err * (p @ v[0].abs()) + spread, torch.float16)
+            want = torch.logsumexp(s, -1)
+            want[:, empty] = -torch.inf
+            ref.check_lse(lse[b].cpu(), want, torch.full_like(want, err + 1e-5))
+
+
 @pytest.mark.parametrize("dtype,int8", KINDS, ids=KIND_IDS)
 def test_a_chain_mask_is_the_default(dtype, int8):
     from sageattention import sageattn_cached
