@@ -16,7 +16,8 @@
 // takes 64 keys, a page, at a time: S^T = K Q^T by 16x16x32 MFMAs (keys down, rows across), whose
 // results are, lane for lane, the B operand of O^T = V^T W^T when the keys are taken in the order
 // 4g .. 4g+3 of two 16-key tiles (g the lane's group of 16). Weights never leave their lanes. A row of
-// V is read 16 lanes wide and its bytes converted one by one into the operand whose element is the key.
+// V is read 16 lanes wide and its bytes converted, pairs of keys at a time, into the operand whose element
+// is the key.
 // What depends on a key alone (ks, lv, 1/SV) is worked out by one lane for each key.
 //
 // Two kernels share that step:
@@ -562,7 +563,11 @@ __device__ __forceinline__ void finish_row(const Shape& p, const Lens& n, const 
 }
 
 // Up to 16 R rows of a plane. Wave w of a part takes its pages first + w, then every W-th. The next
-// page's K is requested when the scores are done with this one's, its V when the products are.
+// page's K is requested when the scores are done with this one's, its V when the products are: a wave has
+// 17 KB in flight at head_dim 128, a CU 8 waves. Bound by HBM where there are enough pages: 64 sequences
+// of up to 8192 tokens, 8 K/V heads, M = 4: 103 us, 5.4 TB/s; 4 of 131072, M = 6: 191 us, 5.8 TB/s (a
+// large copy: 4.9, read and written). A call of a few pages is a chain of latencies (lengths, page number,
+// K and V, the waves' exchange): 517 tokens 10 us.
 template <typename T, bool KINT8, int D, int R, int W>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu((R == 2 && D == 128) ? 1 : 2, (R == 2 && D == 128) ? 1 : 2))) void cache_attn_stream_kernel(Shape p) {
   typedef typename Frag<T>::type frag;
@@ -719,6 +724,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu((R == 2 
 // half w / 2 of V, four column tiles of it at D = 128 and two at 64. One barrier a page: the page after
 // it goes to the other half of the buffers, whose readers passed the barrier before. Two blocks share a
 // CU, whose matrix cores and vector units each serve one while the other waits.
+// 8 sequences of 32768 tokens, 4 K/V heads, M = 512: 345 us, 0.80 PFLOP/s (a large matrix product: 1.21).
+// Of a page's time for a SIMD's two waves, 128 MFMAs are 2048 cycles and 680 vector operations, 64 of them
+// exponentials, about 3500; the two overlap little. More rows to a block would share the conversion, a
+// third of those operations, further, but: 8 waves in two groups, one at its products while the other is
+// at its softmax, took 404 us or more, three row tiles a wave (one block a CU) 1095 for want of registers
+// and of a second block, the conversion spread among the second products 2 % more.
 template <typename T, bool KINT8, int D, int R>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void cache_attn_shared_kernel(Shape p) {
   typedef typename Frag<T>::type frag;

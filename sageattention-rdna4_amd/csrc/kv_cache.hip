@@ -1,7 +1,12 @@
 // Rotary positions, and K and V quantized into the pages of a cache and read back (gfx950).
 //
 // All three are bound by HBM: every value is read once and written once, and a row of D elements is
-// held by CG = D/8 adjacent lanes, 8 elements (16 bytes of 16-bit values, 8 bytes of codes) each.
+// held by CG = D/8 adjacent lanes, 8 elements (16 bytes of 16-bit values, 8 bytes of codes) each. No row
+// waits for another, so there is no LDS and no loop: as many waves as a CU holds hide the latency.
+// Measured (a large copy reaches 4.9 TB/s read and written): 2.3 million rotated rows of 128 fp16 values
+// 203 us, 5.8 TB/s; 128 thousand rows of K and V written in 23 us, 4.4 TB/s, and read back in 19 us, 5.3
+// TB/s; 262 thousand rows read in 33 us, 6.1 TB/s. The smallest calls take 3 to 5 us, the rest of their
+// time is the launch.
 //
 // A cache page holds 64 tokens of every K/V head: K8 and V8 (pages, H, 64, D) codes, SK and SV (pages,
 // H, 64) fp32. Position p of sequence b lies in page table[b][p / 64], row p % 64. A page number
@@ -114,7 +119,8 @@ __device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
 }
 
 // grid: units of one token and HPT heads, CG lanes each. The angles are loaded once for the unit's
-// heads; heads of a unit lie HG = ceil(H / HPT) apart, so that adjacent units are adjacent rows.
+// heads; heads of a unit lie HG = ceil(H / HPT) apart, so that adjacent units are adjacent rows. Without
+// it every row's fp32 angles are twice its own bytes, from L2.
 template <typename T, int D, int HPT>
 __global__ __launch_bounds__(THREADS) void rotary_kernel(const T* X, T* O, Rotary r,
                                                          u32 units, u32 H, u32 HG, u32 N,
@@ -184,7 +190,8 @@ __device__ __forceinline__ float quantize8(const float (&f)[8], u32x2& codes) {
   return s;
 }
 
-// grid: one unit per row of K and V.
+// grid: one unit per row of K and V, which share the place that they go to: one look at the table for
+// both, and twice the loads in flight.
 template <typename T, bool KINT8, int D>
 __global__ __launch_bounds__(THREADS) void cache_write_kernel(
     const T* __restrict__ K, const T* __restrict__ V, u8* __restrict__ K8, float* __restrict__ SK,
@@ -239,7 +246,7 @@ __device__ __forceinline__ void codes8(const u32x2 w, float (&f)[8]) {
   }
 }
 
-// grid: one unit per row of K and V. Each value is code * scale, rounded once to T.
+// grid: one unit per row of K and V, as in writing. Each value is code * scale, rounded once to T.
 template <typename T, bool KINT8, int D>
 __global__ __launch_bounds__(THREADS) void cache_read_kernel(
     const u8* __restrict__ K8, const float* __restrict__ SK, const u8* __restrict__ V8,
@@ -285,6 +292,9 @@ Rotary rotary_of(const RotaryArgs& a) {
   return r;
 }
 
+// One head a thread while the rows do not fill the card (32768 rows of 128 are 2048 blocks), else four:
+// 16384 rows 5.5 us by one, 6.8 by four; 32768 rows 7.3 and 6.7; 2.3 million 266 and 207 (two: 221, eight:
+// 219).
 template <typename T, int D>
 hipError_t rotary_d(const RotaryArgs& a, hipStream_t st) {
   constexpr int HPT = 4;
