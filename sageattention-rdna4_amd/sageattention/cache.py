@@ -179,7 +179,8 @@ def apply_rotary(x, table, positions, tensor_layout="HND", interleaved=False, in
     of 16), the others copied. positions: int32 (B, N), or (N,) for all sequences alike; where one lies
     outside the table, the rotated columns are NaN. A pair (a, b), columns (i, i + R/2) or, `interleaved`,
     (2i, 2i + 1), becomes (a c - b s, b c + a s), in fp32 with one rounding to x's dtype at the end.
-    `inverse` turns by the negative angle: the gradient of x from that of the result.
+    `inverse` turns by the negative angle: the gradient of x from that of the result (autograd records
+    neither this call nor the others here).
     """
     what = "apply_rotary"
     xx = _view(what, tensor_layout, "x", x)
