@@ -1019,7 +1019,7 @@ hipError_t run(const CacheAttnArgs& a, hipStream_t st) {
   p.rows = (int)plan.rows;
   p.units = (int)plan.units;
   p.least = (int)plan.least;
-  p.ahead = CACHE_ATTN_AHEAD;
+  p.ahead = plan.ahead;
   p.c = a.sm_scale * LOG2E_F;
   p.part_o = (float*)a.workspace;
   p.part_ml = p.part_o + plan.part_rows * D;
@@ -1074,8 +1074,20 @@ hipError_t run_d(const CacheAttnArgs& a, hipStream_t st) {
 // row blocks of a run share an XCD, so the runs are as many as each of the 8 XCDs holds whole: three row
 // blocks (M = 384) in 168 runs 176 us, in 171 (two XCDs with blocks left for a second turn) 237. Runs
 // shorter than a page for each wave (or two pages, shared) cost more in their beginnings than they save.
-// Short sequences, and more planes than fill the card four times, take a block for each plane and no
-// second launch: 16 pages in one launch of 8 waves a plane 13 us, spread 14; 32 pages 18 and 13.
+// A run's beginning of a plane counts as `ahead` pages: the more, the less else a CU has to do meanwhile.
+// M = 32 at head_dim 128 (one block a CU), 64 ragged sequences of up to 8192 tokens: 4 pages 180 us, 8
+// 146, 12 126, 16 130; head_dim 64: 4 pages 86, 8 64, 16 65. M = 4, up to 4096 tokens, head_dim 64: 4
+// pages 35, 8 33, 16 35; head_dim 128: 2 pages 64, 4 53, 8 54, 16 57. Shared, M = 128, 16 of up to 4096: 4
+// pages 56, 8 58, 16 61. No more than a run is long: no run can begin a plane for another (49 planes of 19
+// ragged pages, M = 30, 4 pages 14.9, 12 pages 16.7).
+//
+// A block for each plane saves the second launch and the parts' way through memory, but waits for the
+// longest: taken for tables of up to so many pages as either takes as long (us, one launch / spread), the
+// more the better the planes fill the card. 8 K/V heads, M = 4, 12 pages, 1 sequence 11.4 / 11.6, 8
+// sequences 11.7 / 11.9; 16 pages 13.1 / 11.7 and 13.4 / 14.4; 32 ragged sequences, 16 pages 14.9 / 18.9,
+// 32 pages 21.6 / 24.1, 64 pages 33.6 / 33.7. M = 32, 8 sequences, 16 pages 17.9 / 18.5, 24 pages 22.1 /
+// 19.3. M = 128, 8 sequences, 8 pages 24.9 / 29.3, 16 pages 40.6 / 33.5; 32 ragged, 16 pages 43.6 / 49.0, 32
+// pages 74 / 62; 64 ragged, 32 pages 92 / 100. Planes that fill the card four times always take it.
 CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_t max_pages,
                               int64_t D) {
   CacheAttnPlan p;
@@ -1088,7 +1100,13 @@ CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int
   p.rows = 16 * ((tiles + p.row_blocks - 1) / p.row_blocks);
   p.planes = planes;
   const int64_t blocks = planes * p.row_blocks;
-  if (max_pages <= (M <= 16 ? 16 : stream ? 12 : 6) || blocks >= 2048) {
+  int64_t one_launch;   // pages
+  if (stream)
+    one_launch = blocks >= 256 ? 32 : blocks >= 32 ? 16 : (M <= 16 ? 12 : 8) * (128 / D);
+  else
+    one_launch = blocks >= 512 ? 32 : blocks >= 256 ? 16 : blocks >= 64 ? 10 : 4;
+  p.ahead = CACHE_ATTN_LEAST_AHEAD;
+  if (max_pages <= one_launch || blocks >= 2048) {
     p.units = planes;
     p.least = 0;
     p.part_rows = 0;
@@ -1100,10 +1118,14 @@ CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int
     const int64_t resident = p.kernel == CACHE_ATTN_STREAM32 && D == 128 ? 256 : 512;
     int64_t runs = resident / 8 / p.row_blocks * 8;
     if (runs < 8) runs = resident / p.row_blocks > 1 ? resident / p.row_blocks : 1;
-    const int64_t longest = (planes * (max_pages + CACHE_ATTN_AHEAD) + p.least - 1) / p.least;
+    const int64_t longest = (planes * (max_pages + CACHE_ATTN_LEAST_AHEAD) + p.least - 1) / p.least;
     if (runs > longest) runs = longest;
     if (runs > 128 * planes) runs = 128 * planes;   // parts of a plane that the join reads
     p.units = runs;
+    const int64_t most_ahead = !stream ? 4 : D == 64 ? 8 : M <= 16 ? 4 : CACHE_ATTN_MOST_AHEAD;
+    const int64_t length = planes * max_pages / runs;   // of a run, at most
+    p.ahead = (int)(length < CACHE_ATTN_LEAST_AHEAD ? CACHE_ATTN_LEAST_AHEAD
+                    : length < most_ahead ? length : most_ahead);
     p.part_rows = runs * p.row_blocks * 2 * p.rows;
     p.wide_join = runs > 16 * planes;
   }

@@ -276,7 +276,7 @@ int check_cache_attn_shape(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_
     return fail(SAGE_ERR_INVALID, "block_table: max_pages must be in [1, 2^24] (got %lld)",
                 (long long)max_pages);
   // pages are counted in 32 bits; the join has up to a block for each row
-  if (max_pages + sage::CACHE_ATTN_AHEAD > kInt32Max / (B * H_kv))
+  if (max_pages + sage::CACHE_ATTN_MOST_AHEAD > kInt32Max / (B * H_kv))
     return fail(SAGE_ERR_INVALID, "block_table: %lld pages for %lld planes are too many",
                 (long long)max_pages, (long long)(B * H_kv));
   if ((rc = check_grid("the join", B * H * T, 256))) return rc;

@@ -169,11 +169,12 @@ enum CacheAttnKernel {
   CACHE_ATTN_SHARED64,        // row blocks of up to 64
   CACHE_ATTN_SHARED128,       // and 128 rows
 };
-// What beginning a plane costs a run, in pages of its own (see cache_attn.hip).
-constexpr int CACHE_ATTN_AHEAD = 4;
+// What beginning a plane costs a run, in pages of its own (CacheAttnPlan::ahead).
+constexpr int CACHE_ATTN_LEAST_AHEAD = 4, CACHE_ATTN_MOST_AHEAD = 12;
 struct CacheAttnPlan {
   CacheAttnKernel kernel;
   int64_t rows, row_blocks, planes, units, least, part_rows, blocks;
+  int ahead;
   bool wide_join;
 };
 CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_t max_pages,

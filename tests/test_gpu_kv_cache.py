@@ -480,6 +480,39 @@ def test_long_sequences_are_split_and_joined(L, B, H_kv, T, D):
         assert ((lse[b].cpu().double() - torch.logsumexp(s, -1)).abs() <= err + 1e-5).all()
 
 
+@pytest.mark.parametrize("H,H_kv,T,D", [(16, 4, 8, 128), (16, 4, 8, 64), (8, 4, 1, 64), (4, 4, 3, 128),
+                                        (4, 2, 50, 128), (8, 1, 40, 64)])
+def test_many_ragged_sequences_in_runs(H, H_kv, T, D):
+    # runs that end one plane, hold short ones whole and begin another; sequences without a token between
+    from sageattention import sageattn_cached
+    gen = torch.Generator().manual_seed(23)
+    B = 68
+    lens = [int(x) for x in torch.randint(0, 2600, (B,), generator=gen)]
+    lens[::5] = [int(x) for x in torch.randint(0, 70, (len(lens[::5]),), generator=gen)]
+    lens[0], lens[7], lens[8], lens[66], lens[67] = 2600, 0, 0, 1, 0
+    cache, table = _filled(torch.bfloat16, False, H_kv, D, lens, gen)
+    q, qg = _randn((B, H, T, D), torch.bfloat16, "HND", gen, 2.0)
+    o, lse = sageattn_cached(qg, cache, table, _lens(*lens), return_lse=True)
+    o, lse, at = o.cpu(), lse.cpu(), table.cpu()
+    for b in range(B):
+        n = lens[b]
+        k, v, _ = ref.gather(cache, at, b, n)
+        k, v = k.repeat_interleave(H // H_kv, 0), v.repeat_interleave(H // H_kv, 0)
+        s = q[b].double() @ k.transpose(1, 2) / D ** 0.5
+        a = (q[b].double().abs() @ k.abs().transpose(1, 2) / D ** 0.5).amax() if n else 0.0
+        s[:, torch.arange(n) > n - T + torch.arange(T)[:, None]] = -torch.inf
+        empty = torch.arange(T) < T - n
+        p = torch.softmax(s, -1)
+        p[:, empty] = 0.0
+        # the bound of kv_cache_ref.attention
+        err = 2 * ((D + 4) * 2.0 ** -23 * a + 2.0 ** -20) + 2.0 ** -12 + n * 2.0 ** -23
+        spread = n * 2.0 ** -39 * v.abs().amax() if n else 0.0
+        ref.check_attention(o[b], p @ v, err * (p @ v.abs()) + spread, torch.bfloat16)
+        want = torch.logsumexp(s, -1) if n else torch.full((H, T), -torch.inf).double()
+        want[:, empty] = -torch.inf
+        ref.check_lse(lse[b], want, torch.full_like(want, err + 1e-5))
+
+
 def test_more_planes_than_the_card_holds():
     # 2200 planes: a block for each, of any length
     from sageattention import sageattn_cached
