@@ -50,13 +50,13 @@ def _library(what, device):
     return lib
 
 
-def _launch(device, call, *args, **kwargs):
+def _launch(device, call, *args):
     """The call on the device's current stream, with the device current."""
     if device.index == torch.cuda.current_device():
-        call(*args, stream=torch_stream(device), **kwargs)
+        call(*args, torch_stream(device))
     else:
         with torch.cuda.device(device):
-            call(*args, stream=torch_stream(device), **kwargs)
+            call(*args, torch_stream(device))
 
 
 def _view(what, tensor_layout, name, t):
@@ -81,11 +81,9 @@ def _view(what, tensor_layout, name, t):
     return t
 
 
-def _empty(shape, like):
-    """A new tensor of this shape, of `like`'s dtype and device."""
-    if like.is_contiguous() and like.shape == shape:
-        return torch.empty_like(like)
-    return torch.empty(shape, device=like.device, dtype=like.dtype)
+def _empty(like):
+    """A new contiguous tensor of `like`'s shape, dtype and device."""
+    return torch.empty_like(like) if like.is_contiguous() else like.new_empty(like.shape)
 
 
 def _ints(what, name, t, device, rows, columns=None):
@@ -122,8 +120,8 @@ def _check_table(what, table, positions, device, B, N, D):
     if table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous() \
             or table.data_ptr() & 15:
         _refuse(what, "table: a contiguous fp32 (positions, R) tensor is needed, as rotary_table's")
-    R = table.shape[1]
-    if table.shape[0] < 1 or R % 16 or not 16 <= R <= D:
+    rows, R = table.shape
+    if rows < 1 or R % 16 or not 16 <= R <= D:
         _refuse(what, "table: %s: R must be a multiple of 16 up to the head_dim %d" % (
             tuple(table.shape), D))
     if isinstance(positions, torch.Tensor) and positions.dim() == 1:
@@ -188,9 +186,9 @@ def apply_rotary(x, table, positions, tensor_layout="HND", interleaved=False, in
     dev = x.device
     p_sb = _check_table(what, table, positions, dev, B, N, D)
     lib = _library(what, dev)
-    out = _empty(x.shape, x)
+    out = _empty(x)
     _launch(dev, lib.rotary, xx, out if tensor_layout == "HND" else out.transpose(1, 2), table,
-            positions, p_sb, interleaved=interleaved, inverse=inverse)
+            positions, p_sb, interleaved, inverse)
     return out
 
 
@@ -279,7 +277,7 @@ class KVCache:
         elif positions is not None:
             _refuse(what, "table: positions are given without a rotary table")
         _launch(dev, _library(what, dev).cache_write, self, kk, vv, block_table, t_sb, start, lens,
-                table, positions, p_sb, interleaved=interleaved)
+                table, positions, p_sb, interleaved)
 
     def read(self, block_table, lens, n, start=None, tensor_layout="HND"):
         """(k, v), the cached rows in 16 bits: row i < lens[b] of sequence b is position `start[b] +
@@ -355,7 +353,7 @@ def sageattn_cached(q, cache, block_table, kv_lens, tensor_layout="HND", q_lens=
     sm = D ** -0.5 if sm_scale is None else float(sm_scale)
     lib = _library(what, dev)
     need = lib.cache_attn_workspace_bytes(B, H, cache.num_heads, T, block_table.shape[1], D)
-    out = _empty(q.shape, q)
+    out = _empty(q)
     lse = torch.empty((B, H, T), device=dev, dtype=torch.float32) if return_lse else None
     tmp = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
     _launch(dev, lib.cache_attn, cache, qq, out if tensor_layout == "HND" else out.transpose(1, 2),

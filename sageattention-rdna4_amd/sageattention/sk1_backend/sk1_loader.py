@@ -332,7 +332,7 @@ class SageLib:
 
     # The serving entry points: q, k, v, x and o are logical (B, H, N, D) views, `cache` holds a pool
     # (k8, sk, v8, sv, num_pages, int8), t_sb, p_sb, m_sb are elements between two sequences' rows.
-    def rotary(self, x, o, table, positions, p_sb, *, interleaved, inverse, stream):
+    def rotary(self, x, o, table, positions, p_sb, interleaved, inverse, stream):
         """Rotary positions of `x` into `o` (see `sage_rotary`)."""
         B, H, N, D = x.shape
         x_sb, x_sh, x_sr, _ = x.stride()
@@ -345,7 +345,7 @@ class SageLib:
         if rc:
             self._check(rc, "sage_rotary")
 
-    def cache_write(self, cache, k, v, block_table, t_sb, start, lens, table, positions, p_sb, *,
+    def cache_write(self, cache, k, v, block_table, t_sb, start, lens, table, positions, p_sb,
                     interleaved, stream):
         """Rows of `k`, `v` quantized into the cache's pages (see `sage_cache_write`)."""
         B, H, N, D = k.shape
@@ -362,7 +362,7 @@ class SageLib:
         if rc:
             self._check(rc, "sage_cache_write")
 
-    def cache_read(self, cache, k, v, block_table, t_sb, start, lens, *, stream):
+    def cache_read(self, cache, k, v, block_table, t_sb, start, lens, stream):
         """Cached rows into `k`, `v` (see `sage_cache_read`)."""
         B, H, N, D = k.shape
         k_sb, k_sh, k_sr, _ = k.stride()
@@ -384,7 +384,7 @@ class SageLib:
         return n
 
     def cache_attn(self, cache, q, o, block_table, t_sb, kv_lens, q_lens, mask, m_sb, m_sr, sm_scale,
-                   lse, workspace, workspace_bytes, *, stream):
+                   lse, workspace, workspace_bytes, stream):
         """Attention of `q` over the cache into `o` (see `sage_cache_attn`)."""
         B, H, T, D = q.shape
         q_sb, q_sh, q_sr, _ = q.stride()
