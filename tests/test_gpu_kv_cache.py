@@ -480,6 +480,35 @@ def test_long_sequences_are_split_and_joined(L, B, H_kv, T, D):
         assert ((lse[b].cpu().double() - torch.logsumexp(s, -1)).abs() <= err + 1e-5).all()
 
 
+@pytest.mark.parametrize("H,H_kv,D", [(8, 2, 128), (3, 3, 64)])
+@pytest.mark.parametrize("T,past", [(300, 0), (257, 700), (601, 5), (128, 1500)])
+def test_a_prompts_parts(T, past, H, H_kv, D):
+    # many new tokens in causal order, after others or by themselves, of sequences that have fewer of them
+    from sageattention import sageattn_cached
+    gen = torch.Generator().manual_seed(T + past)
+    q_lens = [T, T - 1, T - 130 if T > 140 else 3, 1, 0, T]
+    lens = [past + t for t in q_lens[:5]] + [T // 2]
+    cache, table = _filled(torch.float16, True, H_kv, D, lens, gen)
+    q, qg = _randn((6, H, T, D), torch.float16, "HND", gen, 2.0)
+    o, lse = sageattn_cached(qg, cache, table, _lens(*lens), q_lens=_lens(*q_lens), return_lse=True)
+    for b, (n, t) in enumerate(zip(lens, q_lens)):
+        k, v, _ = ref.gather(cache, table.cpu(), b, n)
+        k, v = k.repeat_interleave(H // H_kv, 0), v.repeat_interleave(H // H_kv, 0)
+        s = q[b].double() @ k.transpose(1, 2) / D ** 0.5
+        a = (q[b].double().abs() @ k.abs().transpose(1, 2) / D ** 0.5).amax() if n else 0.0
+        s[:, torch.arange(n) > n - t + torch.arange(T)[:, None]] = -torch.inf
+        empty = (torch.arange(T) >= t) | (torch.arange(T) < t - n)
+        p = torch.softmax(s, -1)
+        p[:, empty] = 0.0
+        # the bound of kv_cache_ref.attention
+        err = 2 * ((D + 4) * 2.0 ** -23 * a + 2.0 ** -20) + 2.0 ** -12 + n * 2.0 ** -23
+        spread = n * 2.0 ** -39 * v.abs().amax() if n else 0.0
+        ref.check_attention(o[b].cpu(), p @ v, err * (p @ v.abs()) + spread, torch.float16)
+        want = torch.logsumexp(s, -1) if n else torch.full((H, T), -torch.inf).double()
+        want[:, empty] = -torch.inf
+        ref.check_lse(lse[b].cpu(), want, torch.full_like(want, err + 1e-5))
+
+
 @pytest.mark.parametrize("H,H_kv,T,D", [(16, 4, 8, 128), (16, 4, 8, 64), (8, 4, 1, 64), (4, 4, 3, 128),
                                         (4, 2, 50, 128), (8, 1, 40, 64)])
 def test_many_ragged_sequences_in_runs(H, H_kv, T, D):
