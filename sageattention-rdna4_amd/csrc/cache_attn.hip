@@ -41,7 +41,10 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 constexpr float W_SHIFT = 14.0f;    // weights are at most 2^14
-constexpr float SV_LEAST = 0x1p-100f;
+// What a value scale of less counts as (0: a token never written; the scheme's own are 1e-12 or more). Its
+// key's share of a row's sum is at most 2^(14 + 64), so that the 2^30 tokens that a table may have pages
+// for add up to no more than 2^108.
+constexpr float SV_LEAST = 0x1p-64f;
 constexpr float NEG_INF = -__builtin_inff();
 constexpr float LN2_F = 0.6931471805599453f;
 

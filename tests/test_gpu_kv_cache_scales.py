@@ -1,0 +1,97 @@
+"""Attention over cached rows whose value scales are 0 or lie very far apart (GPU), against 64-bit
+results. A weight carries its value's scale, and the sum that it is divided by does not: these are the
+caches where the two drift apart.
+"""
+import math
+
+import pytest
+import torch
+
+import kv_cache_ref as ref
+from sage_testutil import have_gfx950
+
+pytestmark = [pytest.mark.gpu,
+              pytest.mark.skipif(not have_gfx950(), reason="needs a gfx950 GPU")]
+
+
+def _ints(*n):
+    return torch.tensor(n, dtype=torch.int32, device="cuda")
+
+
+def _attend(q, k, v, seen, blank, sm):
+    """(o, lse, slack_o, slack_l) in 64 bits: q (H, T, D) over rows k, v (H, n, D) where `seen` (T, n), and
+    over `blank` more rows of zeros that all see.
+
+    The slack is `kv_cache_ref.attention`'s: a score of at most a = sum |q_d k_d| sm is off by (D + 4) 2^-23
+    a, its logarithm, exponential and reciprocal by 2^-20, a weight and the sum that divides it by that each;
+    the fp16 rounding of a weight is 2^-11 of it, and 2^-39 of the row's largest weight below 2^-28
+    of that; an fp32 sum of n terms is off by n 2^-23.
+    """
+    n, D = blank + k.shape[1], q.shape[2]
+    q = q.double()
+    s = (q @ k.transpose(1, 2) * sm).masked_fill(~seen, -torch.inf)
+    a = (q.abs() @ k.abs().transpose(1, 2) * sm).amax()
+    top = s.amax(-1, keepdim=True).clamp(min=0.0 if blank else -1e300)
+    total = (s - top).exp().sum(-1, keepdim=True) + blank * (-top).exp()
+    p = (s - top).exp() / total
+    lse = (top + total.log())[..., 0]
+    err = (D + 4) * 2.0 ** -23 * a + 2.0 ** -20
+    slack = (2 * err + 2.0 ** -11 + n * 2.0 ** -23) * (p @ v.abs()) \
+        + n * 2.0 ** -39 * (p[..., None] * v.abs()[:, None]).amax((-1, -2))[..., None]
+    return p @ v, lse, slack, err + (n + 8) * 2.0 ** -23 + 2.0 ** -22 * lse.abs()
+
+
+# ------------------------------------------------------------------------ tokens never written
+@pytest.mark.parametrize("blank", [16384, 40000])
+@pytest.mark.parametrize("T", [1, 8, 16, 40])
+@pytest.mark.parametrize("B", [1, 2048])
+def test_nothing_but_tokens_never_written(B, T, blank):
+    # in runs (1 sequence) and by a block for each plane (2048), 4 to 160 rows of a K/V head
+    from sageattention import KVCache, sageattn_cached
+    cache = KVCache.allocate(1, 1, 64)
+    pages = -(-blank // 64)
+    table = torch.zeros(1, pages, dtype=torch.int32, device="cuda").expand(B, pages)
+    lens = torch.full((B,), 64, dtype=torch.int32, device="cuda")
+    lens[B // 2] = blank
+    q = torch.randn(B, 4, T, 64, generator=torch.Generator().manual_seed(T)).half().cuda()
+    o, lse = sageattn_cached(q, cache, table, lens, return_lse=True)
+    assert not o.any()
+    for b, n in ((B // 2, blank), (B - 1, blank if B == 1 else 64)):
+        # token i sees all tokens but the T - 1 - i last ones
+        want = torch.tensor([math.log(n - T + 1 + i) for i in range(T)], dtype=torch.float64)
+        bound = 2.0 ** -20 + (n + 8) * 2.0 ** -23 + 2.0 ** -22 * want
+        assert ((lse[b].double().cpu() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("T", [1, 8, 16, 40])
+@pytest.mark.parametrize("B,blank", [(1, 16384), (1, 40001), (1, 2 ** 21 + 70), (2048, 16384),
+                                     (2048, 40001)])
+def test_tokens_never_written_before_others(B, blank, T):
+    # the first is in runs of a few pages, and of 256 or more for 2^21 tokens; 2048 a block for each plane
+    from sageattention import KVCache, sageattn_cached
+    gen, D, H, n = torch.Generator().manual_seed(T + blank), 64, 4, 6 + T
+    pages = -(-(blank + n) // 64)
+    cache = KVCache.allocate(5, 1, D)
+    table = torch.zeros(1, pages, dtype=torch.int32, device="cuda")
+    first = blank // 64
+    table[0, first:] = torch.arange(1, 1 + pages - first)
+    k, v = (torch.randn(1, 1, n, D, generator=gen).mul(x).half().cuda() for x in (3.0, 1.0))
+    cache.write(k, v, table, _ints(blank))
+    at = B // 2
+    lens = torch.full((B,), 64, dtype=torch.int32, device="cuda")
+    lens[at] = blank + n
+    q = torch.randn(B, H, T, D, generator=gen).mul(3.0).half()
+    o, lse = sageattn_cached(q.cuda(), cache, table.expand(B, pages), lens, return_lse=True)
+    kk, vv = (x[0, 0].cpu() for x in cache.read(table, _ints(n), n, start=_ints(blank)))
+    # the codes' own values: 16-bit reads of them round
+    at_page, slot = table[0, (blank + torch.arange(n)) // 64].long(), (blank + torch.arange(n)).cuda() % 64
+    k64 = (cache.k8[at_page, 0, slot].double() * cache.sk[at_page, 0, slot].double()[:, None]).cpu()
+    v64 = (cache.v8.view(torch.uint8)[at_page, 0, slot].cpu().view(torch.float8_e4m3fn).double()
+           * cache.sv[at_page, 0, slot].double().cpu()[:, None])
+    assert torch.equal(k64.half(), kk) and torch.equal(v64.half(), vv)
+    seen = torch.arange(n) <= n - T + torch.arange(T)[:, None]
+    want, wl, slack, slack_l = _attend(q[at], k64.expand(H, n, D), v64.expand(H, n, D), seen, blank,
+                                       D ** -0.5)
+    assert want.abs().max() > 0.05      # the written ones weigh something
+    ref.check_attention(o[at].cpu(), want, slack, torch.float16)
+    ref.check_lse(lse[at].cpu(), wl, slack_l)
