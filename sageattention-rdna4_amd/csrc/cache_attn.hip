@@ -45,6 +45,17 @@ constexpr float W_SHIFT = 14.0f;    // weights are at most 2^14
 // key's share of a row's sum is at most 2^(14 + 64), so that the 2^30 tokens that a table may have pages
 // for add up to no more than 2^108.
 constexpr float SV_LEAST = 0x1p-64f;
+// A float's exponential ends at 2^-126, and in a bf16 cache value scales may lie 2^183 apart: a row of zeros
+// (1e-12) that scores as a row of bf16's largest values does has a weight that low, but half of the sum. So
+// from the first scale of a part over this one on (values over 3e13), its sums are added up and scaled by
+// square roots, one after the other, which end at 2^-252; all sums of bf16 are merged so. Up to it, what
+// falls under 2^-126 is 2^(-126 + 36 + 64) = 2^-26 of the largest share of the sum or less. (fp16 values have
+// scales of 2^7.2 at most.) A branch in the loop that scales sums took 5 to 12 % longer than a loop of its
+// own does, which costs other bf16 calls 0 to 1 %: 64 sequences of up to 8192 tokens, M = 4, 109.8 us and
+// 109.6 without.
+constexpr float SV_FAR = 0x1p36f;
+template <typename T>
+constexpr bool MAY_BE_FAR = std::is_same_v<T, bf16>;
 constexpr float NEG_INF = -__builtin_inff();
 constexpr float LN2_F = 0.6931471805599453f;
 
@@ -128,6 +139,17 @@ __device__ __forceinline__ float sum_groups(float x) {
   x += __shfl_xor(x, 16, 64);
   return x + __shfl_xor(x, 32, 64);
 }
+
+// 2^d, d at most 0, for accumulators (a) and for sums: in bf16 as two square roots, down to d = -252.
+template <typename T>
+struct Down {
+  float root, a;
+  __device__ __forceinline__ explicit Down(float d) {
+    root = __builtin_amdgcn_exp2f(MAY_BE_FAR<T> ? 0.5f * d : d);
+    a = MAY_BE_FAR<T> ? root * root : root;
+  }
+  __device__ __forceinline__ float sum(float y) const { return MAY_BE_FAR<T> ? y * root * root : y * a; }
+};
 
 struct Shape {
   // pool
@@ -431,8 +453,8 @@ __device__ __forceinline__ Seen seen_masked(const Shape& p, const Lens& n, const
 
 // Scores to weights: u = t + log2 SV, where the page holds new tokens or ends the sequence only for the
 // keys that each row sees; then the running maximum and sum, and the weights as the PV MFMA takes them.
-// For the first NR of the wave's row tiles.
-template <int NR, typename T, int D, int R>
+// For the first NR of the wave's row tiles. FAR: one of the part's value scales is over SV_FAR.
+template <int NR, bool FAR, typename T, int D, int R>
 __device__ __forceinline__ void softmax_step(const Shape& p, const Lens& n, int b, int key0, int held,
                                              const float* consts, int g, Rows<T, D, R>& w,
                                              f32x4 (&s)[R][4], f16x8 (&wf)[R][2]) {
@@ -493,11 +515,11 @@ __device__ __forceinline__ void softmax_step(const Shape& p, const Lens& n, int 
     if (__builtin_amdgcn_ballot_w64(top[r] > w.m[r])) {
       const float now = fmaxf(top[r], w.m[r]);
       // a row that has seen nothing keeps sums of zero
-      const float alpha = __builtin_amdgcn_exp2f(w.m[r] - (now == NEG_INF ? 0.0f : now));
+      const std::conditional_t<FAR, Down<T>, Down<f16>> alpha(w.m[r] - (now == NEG_INF ? 0.0f : now));
       w.m[r] = now;
-      w.l[r] *= alpha;
+      w.l[r] = alpha.sum(w.l[r]);
 #pragma unroll
-      for (int e = 0; e < D / 16; ++e) w.acc[r][e] *= alpha;
+      for (int e = 0; e < D / 16; ++e) w.acc[r][e] *= alpha.a;
     }
     const float shift = (w.m[r] == NEG_INF ? 0.0f : w.m[r]) - W_SHIFT;
 #pragma unroll
@@ -505,7 +527,12 @@ __device__ __forceinline__ void softmax_step(const Shape& p, const Lens& n, int 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float x = __builtin_amdgcn_exp2f(s[r][kt][i] - shift);
-        w.l[r] = __builtin_fmaf(x, rsv[kt][i], w.l[r]);
+        if constexpr (FAR) {
+          const float root = __builtin_amdgcn_exp2f(0.5f * (s[r][kt][i] - shift));
+          w.l[r] = __builtin_fmaf(root * rsv[kt][i], root, w.l[r]);
+        } else {
+          w.l[r] = __builtin_fmaf(x, rsv[kt][i], w.l[r]);
+        }
         wf[r][kt >> 1][4 * (kt & 1) + i] = (f16)x;
       }
     }
@@ -613,12 +640,13 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu((R == 2 
       const u8* kp = p.k8 + base * D;
       u32 at = more ? (u32)(l15 * D + 16 * g) : 0u;
       asm volatile("" : "+v"(at));
+      sk = (p.sk + base)[(u32)lane];
+      sv = (p.sv + base)[(u32)lane];
+      asm volatile("" : : : "memory");   // ahead of the rows, so that the look at them waits for no row
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
         for (int c = 0; c < KC; ++c) kw[kt][c] = *(const u32x4*)(kp + (at + 16 * kt * D + 64 * c));
-      sk = (p.sk + base)[(u32)lane];
-      sv = (p.sv + base)[(u32)lane];
     };
     auto load_v = [&]() {
       const u8* vp = p.v8 + base * D;
@@ -637,54 +665,61 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu((R == 2 
           }
         }
     };
+    auto pages = [&](auto fc) {   // up to the first one with a scale over SV_FAR, or from there on
+      constexpr bool FAR = decltype(fc)::value;
+      for (; pg < end; pg += W) {
+        const int key0 = pg * NPAD, now = held;
+        if constexpr (MAY_BE_FAR<T> && !FAR)
+          if (__builtin_amdgcn_ballot_w64(lane < now && sv > SV_FAR)) return;
+        key_consts(lds_c[wave], lane, sk, sv, p.c, lane < now);
+        f32x4 s[R][4];
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) s[r][kt] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int t = 0; t < KT; ++t) {
+            const frag kf = k_frag<T, KINT8>(kw[kt][t >> 1][2 * (t & 1)], kw[kt][t >> 1][2 * (t & 1) + 1]);
+#pragma unroll
+            for (int r = 0; r < R; ++r) s[r][kt] = mfma(kf, w.q[r][t], s[r][kt]);
+          }
+        }
+        look_ahead(pg + W);
+        load_k();
+        if (now < NPAD) {   // whatever lies behind the end, or on no page: no NaN may meet a weight of zero
+          const int left = now - 4 * g;
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int x = 0; x < VW; ++x) vw[kt][x][j] = 16 * kt + j < left ? vw[kt][x][j] : 0u;
+        }
+        f16x8 wf[R][2];
+        softmax_step<R, FAR>(p, n, b, key0, now, lds_c[wave], g, w, s, wf);
+
+        // O^T += V^T W^T: tile e's row x is column VE x + e
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int x = 0; x < VW; ++x) {
+            f16x8 vf[4];
+            v_frags(vw[2 * u][x], vw[2 * u + 1][x], vf);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int r = 0; r < R; ++r) w.acc[r][4 * x + e] = mfma(vf[e], wf[r][u], w.acc[r][4 * x + e]);
+          }
+        load_v();
+        results_done();
+      }
+    };
     if (pg < end) {
       look_ahead(pg);
       load_k();
       load_v();
-    }
-    for (; pg < end; pg += W) {
-      const int key0 = pg * NPAD, now = held;
-      key_consts(lds_c[wave], lane, sk, sv, p.c, lane < now);
-      f32x4 s[R][4];
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) s[r][kt] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          const frag kf = k_frag<T, KINT8>(kw[kt][t >> 1][2 * (t & 1)], kw[kt][t >> 1][2 * (t & 1) + 1]);
-#pragma unroll
-          for (int r = 0; r < R; ++r) s[r][kt] = mfma(kf, w.q[r][t], s[r][kt]);
-        }
-      }
-      look_ahead(pg + W);
-      load_k();
-      if (now < NPAD) {   // whatever lies behind the end, or on no page: no NaN may meet a weight of zero
-        const int left = now - 4 * g;
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int x = 0; x < VW; ++x) vw[kt][x][j] = 16 * kt + j < left ? vw[kt][x][j] : 0u;
-      }
-      f16x8 wf[R][2];
-      softmax_step<R>(p, n, b, key0, now, lds_c[wave], g, w, s, wf);
-
-      // O^T += V^T W^T: tile e's row x is column VE x + e
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int x = 0; x < VW; ++x) {
-          f16x8 vf[4];
-          v_frags(vw[2 * u][x], vw[2 * u + 1][x], vf);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int r = 0; r < R; ++r) w.acc[r][4 * x + e] = mfma(vf[e], wf[r][u], w.acc[r][4 * x + e]);
-        }
-      load_v();
-      results_done();
+      pages(std::false_type{});
+      if constexpr (MAY_BE_FAR<T>) pages(std::true_type{});
     }
 
     // the waves' results merged, 16 rows at a time; each thread has N columns of a row
@@ -711,10 +746,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu((R == 2 
       float sum = 0.0f, f[N] = {};
 #pragma unroll
       for (int x = 0; x < W; ++x) {
-        const float a = __builtin_amdgcn_exp2f(lds_ml[x][orow][0] - use);
-        sum += lds_ml[x][orow][1] * a;
+        const Down<T> to(lds_ml[x][orow][0] - use);
+        sum += to.sum(lds_ml[x][orow][1]);
 #pragma unroll
-        for (int e = 0; e < N; ++e) f[e] += lds_o[x][orow][ocol + e] * a;
+        for (int e = 0; e < N; ++e) f[e] += lds_o[x][orow][ocol + e] * to.a;
       }
       finish_row<T, D, N>(p, n, part, 16 * r + orow, part.row + 16 * r + orow, ocol, f, top, sum);
     }
@@ -765,6 +800,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     u32 vw[8];
     float sk, sv;
     int held;   // keys of that page, 0 where there is none (and 64 or more: all)
+    bool far = false;
     // page numbers are requested a page before they are used, ahead of that page's bytes
     const int* numbers = p.table + b * p.t_sb;
     int number = 0;
@@ -822,6 +858,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         __builtin_memcpy(&lds_v[buf][me >> 1][2 * (me & 1) + 1][ln], &v1, 16);
       }
       if (me == 0) key_consts(lds_c[buf], ln, sk, sv, p.c, ln < held);
+      if constexpr (MAY_BE_FAR<T>) far |= __builtin_amdgcn_ballot_w64(ln < held && sv > SV_FAR) != 0;
     };
     f32x4 s[R][4];
     f16x8 wf[R][2];
@@ -858,15 +895,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                                w.acc[r][I % VE] = mfma(vf, wf[r][I / VE], w.acc[r][I % VE]);
                            });
     };
-    // all pages for the wave's first NR row tiles
-    auto pages = [&](auto nr) {
+    int pg = part.first;
+    // pages for the wave's first NR row tiles: up to the first one with a scale over SV_FAR, which all
+    // waves have read, or from there on
+    auto pages = [&](auto nr, auto fc) {
       constexpr int NR = decltype(nr)::value;
-      for (int pg = part.first; pg < last; ++pg) {
+      constexpr bool FAR = decltype(fc)::value;
+      for (; pg < last; ++pg) {
+        if constexpr (MAY_BE_FAR<T> && !FAR)
+          if (far) return;
         const int now = held;
         fetch(pg + 1);
         if constexpr (NR > 0) {
           scores(nr, pg);
-          softmax_step<NR>(p, n, b, pg * NPAD, now, lds_c[pg & 1], g, w, s, wf);
+          softmax_step<NR, FAR>(p, n, b, pg * NPAD, now, lds_c[pg & 1], g, w, s, wf);
           values(nr, pg);
         }
         if (pg + 1 < last) convert(pg + 1);
@@ -880,10 +922,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       convert(part.first);   // the readers of the part before have passed its last barrier
       __syncthreads();
       // (two tiles a wave are taken for five or more, so that a wave without any is rare there)
+      auto all = [&](auto nr) {
+        pages(nr, std::false_type{});
+        if constexpr (MAY_BE_FAR<T>) pages(nr, std::true_type{});
+      };
       if (tiles == R)
-        pages(std::integral_constant<int, R>{});
+        all(std::integral_constant<int, R>{});
       else
-        pages(std::integral_constant<int, R - 1>{});
+        all(std::integral_constant<int, R - 1>{});
     }
 
     int ln = threadIdx.x & 63;
@@ -950,17 +996,18 @@ __global__ __launch_bounds__(256) void cache_attn_join_kernel(Shape p, u32 row_t
       float now = top;
 #pragma unroll
       for (int j = 0; j < 8; ++j) now = fmaxf(now, ml[j].x);
-      const float use = now == NEG_INF ? 0.0f : now, old = __builtin_amdgcn_exp2f(top - use);
+      const float use = now == NEG_INF ? 0.0f : now;
+      const Down<T> old(top - use);
       top = now;
-      sum *= old;
-      f *= old;
+      sum = old.sum(sum);
+      f *= old.a;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float a = __builtin_amdgcn_exp2f(ml[j].x - use);
+        const Down<T> to(ml[j].x - use);
         const bool full = ml[j].y != 0.0f;   // else nothing was written there
-        sum += full ? ml[j].y * a : 0.0f;
+        sum += full ? to.sum(ml[j].y) : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] += full ? y[j][e] * a : 0.0f;
+        for (int e = 0; e < 4; ++e) f[e] += full ? y[j][e] * to.a : 0.0f;
       }
     }
   }
@@ -977,9 +1024,9 @@ __global__ __launch_bounds__(256) void cache_attn_join_kernel(Shape p, u32 row_t
 #pragma unroll
     for (int x = 0; x < SL; ++x) {
       const float2 ml = lds_ml[tid + x * LPR];
-      const float a = __builtin_amdgcn_exp2f(ml.x - use);
-      sum += ml.y * a;
-      f += lds_f[tid + x * LPR] * a;
+      const Down<T> to(ml.x - use);
+      sum += to.sum(ml.y);
+      f += lds_f[tid + x * LPR] * to.a;
     }
   }
   if (!live) return;

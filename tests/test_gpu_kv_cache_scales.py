@@ -95,3 +95,76 @@ def test_tokens_never_written_before_others(B, blank, T):
     assert want.abs().max() > 0.05      # the written ones weigh something
     ref.check_attention(o[at].cpu(), want, slack, torch.float16)
     ref.check_lse(lse[at].cpu(), wl, slack_l)
+
+
+# ------------------------------------------------------------------------ scales far apart
+def _far_apart(n, D, gen):
+    """V rows (1, 1, n, D) of bf16: a third of zeros (a scale of 1e-12), a third ordinary, a third between
+    1e-30 and 1e30."""
+    size = 10.0 ** torch.randint(-30, 31, (n,), generator=gen).float()
+    size[torch.arange(n) % 3 == 0], size[torch.arange(n) % 3 == 1] = 0, 1
+    return (torch.randn(1, 1, n, D, generator=gen) * size[:, None]).bfloat16()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [1, 8, 16, 40])
+@pytest.mark.parametrize("n", [63, 300, 3000])
+@pytest.mark.parametrize("where", ["first", "middle", "late", "all"])
+def test_bf16_values_of_every_size(where, n, T, D):
+    """Rows of up to bf16's largest value beside rows of zeros at like scores: every row counts in the sum
+    that a result is divided by. In one launch (n = 63, 300 at up to 32 rows of a K/V head) and in runs.
+
+    Beyond `_attend`'s slack: log2 of scales between 2^-40 and 2^119.2 and scores below 2^6 make numbers of
+    up to 2^8, whose logarithm, sum, maximum's shift and difference are rounded at 2^-17 each: 4 of them
+    move a weight by less than 2^-15 of it, and the sum by as much.
+    """
+    from sageattention import KVCache, sageattn_cached
+    gen, H = torch.Generator().manual_seed(1000 * n + T + D), 4
+    past = max(0, n - T)
+    top = torch.finfo(torch.bfloat16).max
+    big = {"first": [1], "middle": [past // 2], "late": [n - 1 - T // 2], "all": range(2, n, 7)}[where]
+    k = torch.randn(1, 1, n, D, generator=gen).bfloat16()
+    v = _far_apart(n, D, gen)
+    for i, at in enumerate(big):
+        v[0, 0, at] = torch.randn(D, generator=gen).clamp(-3, 3).mul(1e38 * 4.0 ** -(i % 20)).bfloat16()
+    v[0, 0, list(big)[-1], D // 3] = -top
+    pages = -(-n // 64)
+    cache = KVCache.allocate(pages, 1, D, torch.bfloat16)
+    table = torch.randperm(pages, generator=gen).int()[None].cuda()
+    cache.write(k.cuda(), v.cuda(), table, _ints(0))
+    q = torch.randn(1, H, T, D, generator=gen).mul(2.0).bfloat16()
+    o, lse = sageattn_cached(q.cuda(), cache, table, _ints(n), return_lse=True)
+    k64, v64, _ = ref.gather(cache, table.cpu(), 0, n)
+    seen = torch.arange(n) <= n - T + torch.arange(T)[:, None]
+    want, wl, slack, slack_l = _attend(q[0], k64.expand(H, n, D), v64.expand(H, n, D), seen, 0, D ** -0.5)
+    far = 2.0 ** -15
+    spread = torch.softmax((q[0].double() @ k64.transpose(1, 2) * D ** -0.5).masked_fill(~seen, -torch.inf),
+                           -1) @ v64.abs()
+    ref.check_attention(o[0].cpu(), want, slack + 2 * far * spread, torch.bfloat16)
+    ref.check_lse(lse[0].cpu(), wl, slack_l + far)
+
+
+@pytest.mark.parametrize("T", [1, 8, 16, 40])
+def test_bf16_values_of_every_size_in_ragged_runs(T):
+    # 70 sequences: runs that end one plane and begin another, with and without large values
+    from sageattention import KVCache, sageattn_cached
+    gen, B, H, D = torch.Generator().manual_seed(T), 70, 4, 64
+    lens = [int(x) for x in torch.randint(T, 2400, (B,), generator=gen)]
+    width = -(-max(lens) // 64)
+    cache = KVCache.allocate(B * width, 1, D, torch.bfloat16)
+    table = torch.randperm(B * width, generator=gen).int().view(B, width).cuda()
+    k = torch.randn(B, 1, max(lens), D, generator=gen).bfloat16()
+    v = torch.cat([_far_apart(max(lens), D, gen) for _ in range(B)])
+    for b in range(0, B, 2):
+        v[b, 0, lens[b] * (b % 5) // 6] = torch.randn(D, generator=gen).mul(2e37).bfloat16()
+    cache.write(k.cuda(), v.cuda(), table, torch.zeros(B, dtype=torch.int32, device="cuda"))
+    q = torch.randn(B, H, T, D, generator=gen).mul(2.0).bfloat16()
+    o, lse = sageattn_cached(q.cuda(), cache, table, _ints(*lens), return_lse=True)
+    for b in range(0, B, 3):
+        n = lens[b]
+        k64, v64, _ = ref.gather(cache, table.cpu(), b, n)
+        seen = torch.arange(n) <= n - T + torch.arange(T)[:, None]
+        want, wl, slack, slack_l = _attend(q[b], k64.expand(H, n, D), v64.expand(H, n, D), seen, 0, 0.125)
+        p = torch.softmax((q[b].double() @ k64.transpose(1, 2) * 0.125).masked_fill(~seen, -torch.inf), -1)
+        ref.check_attention(o[b].cpu(), want, slack + 2.0 ** -14 * (p @ v64.abs()), torch.bfloat16)
+        ref.check_lse(lse[b].cpu(), wl, slack_l + 2.0 ** -15)
