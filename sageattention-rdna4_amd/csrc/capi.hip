@@ -275,13 +275,14 @@ int check_cache_attn_shape(int64_t B, int64_t H, int64_t H_kv, int64_t T, int64_
   if (max_pages < 1 || max_pages > (1 << 24))
     return fail(SAGE_ERR_INVALID, "block_table: max_pages must be in [1, 2^24] (got %lld)",
                 (long long)max_pages);
-  // pages are counted in 32 bits; the join has up to a block for each row
+  // pages are counted in 32 bits
   if (max_pages + sage::CACHE_ATTN_MOST_AHEAD > kInt32Max / (B * H_kv))
     return fail(SAGE_ERR_INVALID, "block_table: %lld pages for %lld planes are too many",
                 (long long)max_pages, (long long)(B * H_kv));
-  if ((rc = check_grid("the join", B * H * T, 256))) return rc;
+  // 512 threads are for up to 256 blocks, and a join, of up to a block for each row, for fewer than 2048
+  // blocks of up to 128 rows
   return check_grid("the cached attention", sage::cache_attn_plan(B, H, H_kv, T, max_pages, D).blocks,
-                    512);
+                    256);
 }
 
 }  // namespace

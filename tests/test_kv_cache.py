@@ -178,6 +178,21 @@ def test_workspace_sizes():
     assert lib.sage_cache_attn_workspace_bytes(1, 32, 8, 1, 0, 128) == -1
 
 
+@pytest.mark.parametrize("B,H,H_kv,T,max_pages,D,served", [
+    # many prompts' parts, a block for each plane and 128 rows: the rows' limit, D/8 threads each
+    (64, 32, 8, 8192, 128, 128, True), (512, 32, 8, 8192, 128, 128, True),
+    (1024, 32, 8, 8192, 128, 128, False), (1024, 32, 8, 8192, 128, 64, True),
+    # decoding of as many planes as a launch has blocks of 256 threads
+    (2 ** 21 - 1, 8, 8, 1, 1, 64, True), (2 ** 21, 8, 8, 1, 1, 64, False),
+    # one K/V head: eight blocks for each 128 rows
+    (1, 2 ** 20, 1, 255, 1, 64, True), (1, 2 ** 20, 1, 256, 1, 64, False),
+])
+def test_sizes_are_refused_by_the_launch_that_they_need(B, H, H_kv, T, max_pages, D, served):
+    lib = _lib()
+    n = lib.sage_cache_attn_workspace_bytes(B, H, H_kv, T, max_pages, D)
+    assert n == 0 if served else n == -1 and b"grid" in lib.sage_last_error()
+
+
 # ------------------------------------------------------------------------------------ oracles
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("T", [33, 64, 66, 96, 100, 128, 144, 200, 400])
