@@ -539,12 +539,18 @@ __device__ __forceinline__ void softmax_step(const Shape& p, const Lens& n, int 
   }
 }
 
-// N columns of an output row.
+// N columns of an output row. A mean of fp16 values is no larger than fp16's largest, 65504, but with weights
+// rounded up by 2^-11 it may come out as up to 65536, an infinity: such ones are 65504. (bf16 would need 2^-9.)
 template <typename T, int N>
 __device__ __forceinline__ void store_row(T* o, const float (&f)[N], float inv, bool some) {
   T out[N];
 #pragma unroll
-  for (int e = 0; e < N; ++e) out[e] = (T)(some ? f[e] * inv : 0.0f);
+  for (int e = 0; e < N; ++e) {
+    float x = some ? f[e] * inv : 0.0f;
+    if constexpr (std::is_same_v<T, f16>)
+      x = fabsf(x) < 65568.0f ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x;
+    out[e] = (T)x;
+  }
   if constexpr (N == 8) {
     u32x4 w;
     __builtin_memcpy(&w, out, 16);

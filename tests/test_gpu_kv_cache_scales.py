@@ -168,3 +168,30 @@ def test_bf16_values_of_every_size_in_ragged_runs(T):
         p = torch.softmax((q[b].double() @ k64.transpose(1, 2) * 0.125).masked_fill(~seen, -torch.inf), -1)
         ref.check_attention(o[b].cpu(), want, slack + 2.0 ** -14 * (p @ v64.abs()), torch.bfloat16)
         ref.check_lse(lse[b].cpu(), wl, slack_l + 2.0 ** -15)
+
+
+# ----------------------------------------------------------------------------- largest values
+@pytest.mark.parametrize("int8", [True, False])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [1, 8, 16, 40])
+@pytest.mark.parametrize("n", [700, 5000])
+def test_fp16_largest_values_stay_finite(n, T, D, int8):
+    """A mean of fp16's largest value is that value, also where all weights are rounded up: one token of 32
+    weighs 1 and the others exp(-2 sm) = (1 + 1.05 2^-11) / 2, which fp16 takes for (1 + 2^-10) / 2."""
+    from sageattention import KVCache, sageattn_cached
+    sm = -0.5 * math.log(0.5 * (1 + 1.05 * 2.0 ** -11))
+    top = torch.finfo(torch.float16).max
+    k, v = torch.zeros(2, 1, 1, n, D, dtype=torch.float16)
+    k[..., 0], k[:, :, ::32, 0] = -1, 1
+    v[..., 0], v[..., 1], v[..., 2] = top, -top, 1
+    pages = -(-n // 64)
+    cache = KVCache.allocate(pages, 1, D, int8=int8)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    cache.write(k.cuda(), v.cuda(), table, _ints(0))
+    q = torch.zeros(1, 4, T, D, device="cuda", dtype=torch.float16)
+    q[..., 0] = 1
+    o = sageattn_cached(q, cache, table, _ints(n), sm_scale=sm).cpu()
+    for column, want in ((0, top), (1, -top)):
+        # the weights' 2^-11 and the result's own half step
+        off = (o[..., column].double() - want).abs()
+        assert torch.isfinite(o[..., column]).all() and (off <= 2.0 ** -10 * top).all()
