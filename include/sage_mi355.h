@@ -322,7 +322,9 @@ int sage_cache_read(int dtype, int k_int8, const void* k8, const float* sk, cons
  *   mask      (B, T, T) bytes, strides m_sb, m_sr in elements (m_sb 0: one mask for all), last stride 1
  *   lse       optional (B, H, T) fp32: the natural logsumexp of each row's scores times sm_scale
  *   workspace sage_cache_attn_workspace_bytes bytes, 16-byte aligned; NULL where that is 0
- * Rows that see nothing, and rows of tokens i >= q_lens[b], are zeros with a logsumexp of -infinity.
+ * Rows that see nothing, and rows of tokens i >= q_lens[b], are zeros with a logsumexp of -infinity; a
+ * score of -infinity counts as not seen. Tokens never written (scales of 0) are seen as rows of zeros; any
+ * other scales that sage_cache_write makes may stand side by side.
  * Q is not quantized: scores are exact products of 16-bit queries and 8-bit codes, summed in fp32.
  */
 int sage_cache_attn(int dtype, int k_int8, const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sr,

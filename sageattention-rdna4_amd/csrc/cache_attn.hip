@@ -8,9 +8,9 @@
 // of its own. The weight that meets V8 includes V's scale: with u_j = t_j + log2 SV_j and the running
 // row maximum m of u,
 //     w_j = 2^(u_j - m + 14),   o = (sum_j w_j V8_j) / (sum_j w_j / SV_j):
-// w is at most 2^14 whatever the scales, so it is rounded to fp16 (half a step of 2^-11, a quarter of
-// what a bf16 weight would lose) without overflow, and 28 binades below a row's largest weight are
-// still normal numbers. Sums, maxima and outputs are fp32 until the one rounding of the output.
+// w is at most 2^14 whatever the scales, so it is rounded to fp16 (by 2^-11 of it at most, an eighth of what
+// a bf16 weight would lose) without overflow, and 28 binades below a row's largest weight are still
+// normal numbers. Sums, maxima and outputs are fp32 until the one rounding of the output.
 //
 // Layout. A wave holds 16 R rows of one K/V head (row r: token r / G, head r % G of the group) and
 // takes 64 keys, a page, at a time: S^T = K Q^T by 16x16x32 MFMAs (keys down, rows across), whose
@@ -768,9 +768,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu((R == 2 
 // half w / 2 of V, four column tiles of it at D = 128 and two at 64. One barrier a page: the page after
 // it goes to the other half of the buffers, whose readers passed the barrier before. Two blocks share a
 // CU, whose matrix cores and vector units each serve one while the other waits.
-// 8 sequences of 32768 tokens, 4 K/V heads, M = 512: 345 us, 0.80 PFLOP/s (a large matrix product: 1.21).
-// Of a page's time for a SIMD's two waves, 128 MFMAs are 2048 cycles and 680 vector operations, 64 of them
-// exponentials, about 3500; the two overlap little. More rows to a block would share the conversion, a
+// 8 sequences of 32768 tokens, 4 K/V heads, M = 512: 345 to 369 us by the card, 0.80 to 0.75 PFLOP/s (a large
+// matrix product: 1.21). Of a page's time for a SIMD's two waves, 128 MFMAs are 2048 cycles and 680 vector
+// operations, 64 of them exponentials, about 3500; the two overlap little (matrix cores busy for 32 % of
+// the cycles, vector units for 52 %). More rows to a block would share the conversion, a
 // third of those operations, further, but: 8 waves in two groups, one at its products while the other is
 // at its softmax, took 404 us or more, three row tiles a wave (one block a CU) 1095 for want of registers
 // and of a second block, the conversion spread among the second products 2 % more.
@@ -1128,11 +1129,15 @@ hipError_t run_d(const CacheAttnArgs& a, hipStream_t st) {
 // for every wave to convert its own pages (stream); more share the conversion. Measured, 8 sequences of
 // 8192 tokens, 8 K/V heads, us: M = 32 stream 37, shared 48; M = 64 shared 55.
 //
-// Which cut: as many runs as blocks are resident at once (512 threads' registers of a CU hold two blocks
+// Which cut (for the whole card, 256 CUs in 8 XCDs; on a part of it calls are served, but not filled so): as
+// many runs as blocks are resident at once (512 threads' registers of a CU hold two blocks
 // of 4 waves, but one of the 32-row kernel at head_dim 128), so that all runs begin and end together.
 // 8 x 3000 tokens, M = 4: 512 runs 20 us, 1024 runs 26; 8 x 8192, M = 32: 256 runs 37, 1024 runs 61. The
 // row blocks of a run share an XCD, so the runs are as many as each of the 8 XCDs holds whole: three row
-// blocks (M = 384) in 168 runs 176 us, in 171 (two XCDs with blocks left for a second turn) 237. Runs
+// blocks (M = 384) in 168 runs 176 us, in 171 (two XCDs with blocks left for a second turn) 237. From 65 row
+// blocks on (M over 8192: a prompt's part of over 2048 tokens, 4 heads to a K/V head) none holds a run whole,
+// and there are as few runs as make about 512 blocks, or one: less than 8 leave XCDs without work (4096
+// tokens: 4 runs of 128 row blocks on 4 of the 8), as do fewer than 8 planes of a block each. Runs
 // shorter than a page for each wave (or two pages, shared) cost more in their beginnings than they save.
 // A run's beginning of a plane counts as `ahead` pages: the more, the less else a CU has to do meanwhile.
 // M = 32 at head_dim 128 (one block a CU), 64 ragged sequences of up to 8192 tokens: 4 pages 180 us, 8

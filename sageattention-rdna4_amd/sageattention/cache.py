@@ -178,7 +178,8 @@ def apply_rotary(x, table, positions, tensor_layout="HND", interleaved=False, in
     outside the table, the rotated columns are NaN. A pair (a, b), columns (i, i + R/2) or, `interleaved`,
     (2i, 2i + 1), becomes (a c - b s, b c + a s), in fp32 with one rounding to x's dtype at the end.
     `inverse` turns by the negative angle: the gradient of x from that of the result (autograd records
-    neither this call nor the others here).
+    neither this call nor the others here). It gives x back from the result where the table's pairs are of
+    size 1; a "yarn" table's are larger, and x comes back times their size squared.
     """
     what = "apply_rotary"
     xx = _view(what, tensor_layout, "x", x)
@@ -322,7 +323,9 @@ def sageattn_cached(q, cache, block_table, kv_lens, tensor_layout="HND", q_lens=
 
     Returns the output in q's layout and dtype; with `return_lse=True` the pair `(out, lse)`, lse (B,
     H, T) fp32 as `sageattn` defines it. A token that sees nothing, and tokens from q_lens[b] on, give
-    zeros and -inf. Queries are not quantized: the result is that of the cached values to 16 bits.
+    zeros and -inf; a score of -infinity counts as not seen, one of +infinity or NaN makes the row NaN. A
+    token that was never written (a scale of 0) is seen as a row of zeros. Queries are not quantized: the
+    result is that of the cached values to 16 bits.
     """
     what = "sageattn_cached"
     qq = _view(what, tensor_layout, "q", q)
