@@ -195,3 +195,27 @@ def test_fp16_largest_values_stay_finite(n, T, D, int8):
         # the weights' 2^-11 and the result's own half step
         off = (o[..., column].double() - want).abs()
         assert torch.isfinite(o[..., column]).all() and (off <= 2.0 ** -10 * top).all()
+
+
+# --------------------------------------------------------------------------- infinite scores
+@pytest.mark.parametrize("dtype,int8", [(torch.float16, True), (torch.float16, False),
+                                        (torch.bfloat16, False)])
+@pytest.mark.parametrize("T", [1, 8, 16, 40])
+@pytest.mark.parametrize("n", [100, 3000])
+def test_infinite_scores(n, T, dtype, int8):
+    # a query's infinity meets a column of negative keys, or one that is positive in the newest token's row
+    from sageattention import KVCache, sageattn_cached
+    gen, pages = torch.Generator().manual_seed(n + T), -(-n // 64)
+    cache = KVCache.allocate(pages, 1, 64, dtype, int8)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    k, v = (torch.randn(1, 1, n, 64, generator=gen).to(dtype) for _ in range(2))
+    k[..., 0], k[..., 1], k[0, 0, n - 1, 1] = -1, -1, 1
+    cache.write(k.cuda(), v.cuda(), table, _ints(0))
+    q = torch.randn(1, 4, T, 64, generator=gen).to(dtype)
+    q[:, 1, :, 0] = q[:, 2, :, 1] = torch.inf
+    o, lse = (x.cpu() for x in sageattn_cached(q.cuda(), cache, table, _ints(n), return_lse=True))
+    assert torch.isfinite(o[:, [0, 3]]).all() and torch.isfinite(lse[:, [0, 3]]).all()
+    assert not o[:, 1].any() and torch.isneginf(lse[:, 1]).all()     # as if nothing were seen
+    # only the last token sees the newest
+    assert not o[:, 2, :-1].any() and torch.isneginf(lse[:, 2, :-1]).all()
+    assert torch.isnan(o[:, 2, -1]).all() and torch.isnan(lse[:, 2, -1]).all()
