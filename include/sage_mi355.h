@@ -341,6 +341,40 @@ int64_t sage_cache_attn_workspace_bytes(int64_t B, int64_t H, int64_t H_kv, int6
                                         int64_t max_pages, int64_t D);
 
 /*
+ * Attention's backward pass: the gradients of q, k and v from that of the output, in two or three
+ * launches. No counterpart in the reference, whose kernels have no gradients. With
+ * P_ij = exp(sm_scale q_i.k_j - lse_i) (0 for j > i when causal) and d_i = dout_i.o_i - dlse_i:
+ *   dv_j = sum_i P_ij dout_i,  dS_ij = P_ij (dout_i.v_j - d_i),
+ *   dq_i = sm_scale sum_j dS_ij k_j,  dk_j = sm_scale sum_i dS_ij q_i,
+ * k's and v's summed over the query heads of their group.
+ *   q, o, dout, dq   logical (B, H, N, D) views, D = 64 or 128; k, v, dk, dv (B, H_kv, N_kv, D); rows
+ *                    less than 2^24 elements apart; the outputs overlap nothing else
+ *   lse              (B, H, N) fp32: the forward call's, or that of a larger set of keys that these are
+ *                    part of (o and dout are then those of the whole); -infinity: the row saw nothing
+ *   dlse             optional (B, H, N) fp32: the gradient of lse
+ *   workspace        sage_attn_bwd_workspace_bytes bytes, 256-byte aligned
+ * P and dS are rounded to `dtype` ahead of their products (fp16: scaled by powers of two that keep
+ * them in range), every sum is fp32, and the results are rounded once. They are the same from call to
+ * call. Where P is 0 its other factor has to be finite: 0 times a NaN or an infinity is NaN.
+ */
+int sage_attn_bwd(int dtype, int causal,
+                  const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sr,
+                  const void* k, int64_t k_sb, int64_t k_sh, int64_t k_sr,
+                  const void* v, int64_t v_sb, int64_t v_sh, int64_t v_sr,
+                  const void* o, int64_t o_sb, int64_t o_sh, int64_t o_sr,
+                  const void* dout, int64_t do_sb, int64_t do_sh, int64_t do_sr,
+                  const float* lse, const float* dlse,
+                  void* dq, int64_t dq_sb, int64_t dq_sh, int64_t dq_sr,
+                  void* dk, int64_t dk_sb, int64_t dk_sh, int64_t dk_sr,
+                  void* dv, int64_t dv_sb, int64_t dv_sh, int64_t dv_sr,
+                  int64_t B, int64_t H, int64_t N, int64_t H_kv, int64_t N_kv, int64_t D,
+                  float sm_scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace of a sage_attn_bwd call of these sizes, or -SAGE_ERR_INVALID. */
+int64_t sage_attn_bwd_workspace_bytes(int dtype, int causal, int64_t B, int64_t H, int64_t N,
+                                      int64_t H_kv, int64_t N_kv, int64_t D);
+
+/*
  * MFMA accumulator layout probe (known-answer test of the fragment layouts the main loop relies
  * on). One wave computes C = A(32x32, int8) * B(32x32, int8) with v_mfma_i32_32x32x32_i8 and
  * D = E(32x64, fp8) * F(64x32, fp8) with v_mfma_scale_f32_32x32x64_f8f6f4, loading operands in

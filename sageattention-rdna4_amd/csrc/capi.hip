@@ -86,18 +86,41 @@ int check_main_grid(int64_t B, int64_t H, int64_t N) {
   return check_grid("the 256-query main loop", B * H * ((N + 255) / 256), 512);
 }
 
+int check_head_dim(int64_t D) {
+  if (D != 64 && D != 128)
+    return fail(SAGE_ERR_INVALID, "head_dim: D must be 64 or 128 (got %lld)", (long long)D);
+  return SAGE_OK;
+}
+
+// The sizes of a backward call: those of the forward call, and grids within HIP's bounds.
+constexpr int64_t kMaxRowStride = (1 << 24) - 8;
+int check_attn_bwd(int dtype, int causal, int64_t B, int64_t H, int64_t N, int64_t H_kv, int64_t N_kv,
+                   int64_t D) {
+  if (dtype != SAGE_F16 && dtype != SAGE_BF16)
+    return fail(SAGE_ERR_INVALID, "dtype: unsupported dtype code %d", dtype);
+  int rc = check_head_dim(D);
+  if (rc) return rc;
+  if ((rc = check_shape(B, H, N, (N + 63) / 64 * 64))) return rc;
+  if (H_kv < 1 || H % H_kv != 0)
+    return fail(SAGE_ERR_INVALID, "heads: H (%lld) must be a multiple of H_kv (%lld)", (long long)H,
+                (long long)H_kv);
+  if ((rc = check_shape(B, H_kv, N_kv, (N_kv + 63) / 64 * 64))) return rc;
+  if (causal && N != N_kv)
+    return fail(SAGE_ERR_INVALID, "seq_len: causal attention needs N == N_kv (N=%lld N_kv=%lld)",
+                (long long)N, (long long)N_kv);
+  // the rows launch, a block per 64 rows of each tensor; the main launch has fewer blocks, or few
+  const int64_t tiles = B * H * ((N + 63) / 64), tiles_kv = B * H_kv * ((N_kv + 63) / 64);
+  if ((rc = check_grid("the backward pass", tiles + tiles_kv, 256))) return rc;
+  const sage::AttnBwdPlan p = sage::attn_bwd_plan(B, H, H_kv, N, N_kv, D, causal != 0);
+  return check_grid("the backward pass", p.k_blocks + p.q_blocks, 256);
+}
+
 // The prologue's two passes: C1 and C2 blocks per plane of 256 threads.
 int check_prologue_grid(int64_t BH, int64_t N, int64_t N_pad) {
   const sage::PrologueGeom g = sage::prologue_geom(BH, N, N_pad);
   const int64_t c = g.C1 > g.C2 ? g.C1 : g.C2;
   if (c > kInt32Max / BH) return check_grid("the prologue", kInt32Max, 256);
   return check_grid("the prologue", c * BH, 256);
-}
-
-int check_head_dim(int64_t D) {
-  if (D != 64 && D != 128)
-    return fail(SAGE_ERR_INVALID, "head_dim: D must be 64 or 128 (got %lld)", (long long)D);
-  return SAGE_OK;
 }
 
 }  // namespace
@@ -767,6 +790,72 @@ int sage_cache_attn(int dtype, int k_int8, const void* q, int64_t q_sb, int64_t 
   a.lse = lse;
   a.workspace = workspace;
   return hip_status(sage::launch_cache_attn(a, (hipStream_t)stream), "sage_cache_attn launch");
+}
+
+int64_t sage_attn_bwd_workspace_bytes(int dtype, int causal, int64_t B, int64_t H, int64_t N,
+                                      int64_t H_kv, int64_t N_kv, int64_t D) {
+  const int rc = check_attn_bwd(dtype, causal, B, H, N, H_kv, N_kv, D);
+  if (rc) return -rc;
+  g_err.clear();
+  return sage::attn_bwd_workspace_bytes(sage::attn_bwd_plan(B, H, H_kv, N, N_kv, D, causal != 0),
+                                        dtype, B * H, B * H_kv, D);
+}
+
+int sage_attn_bwd(int dtype, int causal, const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sr,
+                  const void* k, int64_t k_sb, int64_t k_sh, int64_t k_sr, const void* v,
+                  int64_t v_sb, int64_t v_sh, int64_t v_sr, const void* o, int64_t o_sb,
+                  int64_t o_sh, int64_t o_sr, const void* dout, int64_t do_sb, int64_t do_sh,
+                  int64_t do_sr, const float* lse, const float* dlse, void* dq, int64_t dq_sb,
+                  int64_t dq_sh, int64_t dq_sr, void* dk, int64_t dk_sb, int64_t dk_sh,
+                  int64_t dk_sr, void* dv, int64_t dv_sb, int64_t dv_sh, int64_t dv_sr, int64_t B,
+                  int64_t H, int64_t N, int64_t H_kv, int64_t N_kv, int64_t D, float sm_scale,
+                  void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_attn_bwd(dtype, causal, B, H, N, H_kv, N_kv, D);
+  if (rc) return rc;
+  sage::AttnBwdArgs a = {};
+  a.q = {q, q_sb, q_sh, q_sr};
+  a.k = {k, k_sb, k_sh, k_sr};
+  a.v = {v, v_sb, v_sh, v_sr};
+  a.o = {o, o_sb, o_sh, o_sr};
+  a.dout = {dout, do_sb, do_sh, do_sr};
+  a.dq = {dq, dq_sb, dq_sh, dq_sr};
+  a.dk = {dk, dk_sb, dk_sh, dk_sr};
+  a.dv = {dv, dv_sb, dv_sh, dv_sr};
+  const struct {
+    const char* name;
+    const sage::View* view;
+  } views[] = {{"q", &a.q}, {"k", &a.k}, {"v", &a.v}, {"o", &a.o}, {"dout", &a.dout},
+               {"dq", &a.dq}, {"dk", &a.dk}, {"dv", &a.dv}};
+  for (const auto& x : views) {
+    if ((rc = check_view(x.name, x.view->p, x.view->sb, x.view->sh, x.view->sr))) return rc;
+    // the 64 rows of a tile are reached by 32-bit offsets from its first
+    if (x.view->sr > kMaxRowStride)
+      return fail(SAGE_ERR_INVALID, "%s: stride_int32 (rows %lld elements apart, at most %lld are served)",
+                  x.name, (long long)x.view->sr, (long long)kMaxRowStride);
+  }
+  if (!lse) return fail(SAGE_ERR_INVALID, "lse is NULL");
+  if (((uintptr_t)lse & 3u) || ((uintptr_t)dlse & 3u))
+    return fail(SAGE_ERR_INVALID, "ptr_align: lse and dlse must be 4-byte aligned");
+  if (!(sm_scale > 0.0f) || !(sm_scale < 3.0e38f))
+    return fail(SAGE_ERR_INVALID, "sm_scale: must be positive and finite (got %g)", (double)sm_scale);
+  const int64_t need = sage::attn_bwd_workspace_bytes(
+      sage::attn_bwd_plan(B, H, H_kv, N, N_kv, D, causal != 0), dtype, B * H, B * H_kv, D);
+  if (workspace == nullptr || workspace_bytes < (size_t)need || ((uintptr_t)workspace & 255u))
+    return fail(SAGE_ERR_INVALID, "workspace: need %lld bytes, 256-byte aligned (got %zu)",
+                (long long)need, workspace_bytes);
+  a.dtype = dtype;
+  a.causal = causal ? 1 : 0;
+  a.lse = lse;
+  a.dlse = dlse;
+  a.B = B;
+  a.H = H;
+  a.N = N;
+  a.H_kv = H_kv;
+  a.N_kv = N_kv;
+  a.D = D;
+  a.sm_scale = sm_scale;
+  a.workspace = workspace;
+  return hip_status(sage::launch_attn_bwd(a, (hipStream_t)stream), "sage_attn_bwd launch");
 }
 
 int sage_quant_q(int dtype, int qk_int8, const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sr,

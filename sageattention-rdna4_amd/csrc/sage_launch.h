@@ -182,4 +182,31 @@ CacheAttnPlan cache_attn_plan(int64_t B, int64_t H, int64_t H_kv, int64_t T, int
 size_t cache_attn_workspace_bytes(const CacheAttnPlan& p, int64_t D);
 hipError_t launch_cache_attn(const CacheAttnArgs& a, hipStream_t stream);
 
+// A (B, H, N, D) view with contiguous columns.
+struct View {
+  const void* p;
+  int64_t sb, sh, sr;
+};
+struct AttnBwdArgs {
+  int dtype, causal;
+  View q, k, v, o, dout;      // read
+  View dq, dk, dv;            // written
+  const float* lse;           // (B, H, N)
+  const float* dlse;          // optional (B, H, N)
+  int64_t B, H, H_kv, N, N_kv, D;
+  float sm_scale;
+  void* workspace;
+};
+// How a call is cut up: tiles of 64 rows in a plane, blocks of k_rows keys and of q_rows queries,
+// each one's loop in k_split or q_split parts. Sizes alone decide it, so a captured call and its
+// workspace agree.
+struct AttnBwdPlan {
+  int64_t nb_q, nb_kv, k_rows, q_rows, k_tiles, q_tiles, k_split, q_split, k_blocks, q_blocks;
+};
+AttnBwdPlan attn_bwd_plan(int64_t B, int64_t H, int64_t H_kv, int64_t N, int64_t N_kv, int64_t D,
+                          bool causal);
+int64_t attn_bwd_workspace_bytes(const AttnBwdPlan& p, int dtype, int64_t planes_q, int64_t planes_kv,
+                                 int64_t D);
+hipError_t launch_attn_bwd(const AttnBwdArgs& a, hipStream_t stream);
+
 }  // namespace sage

@@ -180,6 +180,11 @@ class SageLib:
                                       + [i64] * 5 + [f32, vp, vp, ctypes.c_size_t, vp])
         L.sage_cache_attn_workspace_bytes.restype = i64
         L.sage_cache_attn_workspace_bytes.argtypes = [i64] * 6
+        L.sage_attn_bwd.restype = i32
+        L.sage_attn_bwd.argtypes = ([i32] * 2 + view * 5 + [vp, vp] + view * 3 + [i64] * 6
+                                    + [f32, vp, ctypes.c_size_t, vp])
+        L.sage_attn_bwd_workspace_bytes.restype = i64
+        L.sage_attn_bwd_workspace_bytes.argtypes = [i32] * 2 + [i64] * 6
         self.version = int(L.sage_version())
         self.build_id = L.sage_build_id().decode()
         images = hip_runtime_images()
@@ -399,6 +404,31 @@ class SageLib:
             None if workspace is None else workspace.data_ptr(), workspace_bytes, stream)
         if rc:
             self._check(rc, "sage_cache_attn")
+
+    @functools.lru_cache(maxsize=4096)
+    def attn_bwd_workspace_bytes(self, dtype, causal, B, H, N, H_kv, N_kv, D):
+        """Bytes of `sage_attn_bwd`'s workspace, a function of the sizes alone."""
+        n = self.lib.sage_attn_bwd_workspace_bytes(_dtype_code(dtype), int(bool(causal)), B, H, N,
+                                                   H_kv, N_kv, D)
+        if n < 0:
+            self._check(-n, "sage_attn_bwd_workspace_bytes")
+        return n
+
+    def attn_bwd(self, q, k, v, o, dout, lse, dlse, dq, dk, dv, causal, sm_scale, workspace, stream):
+        """The gradients of `q`, `k`, `v` into `dq`, `dk`, `dv` (see `sage_attn_bwd`)."""
+        B, H, N, D = q.shape
+        _, H_kv, N_kv, _ = k.shape
+        args = []
+        for t in (q, k, v, o, dout):
+            args += (t.data_ptr(),) + t.stride()[:3]
+        args += (lse.data_ptr(), None if dlse is None else dlse.data_ptr())
+        for t in (dq, dk, dv):
+            args += (t.data_ptr(),) + t.stride()[:3]
+        rc = self.lib.sage_attn_bwd(
+            _dtype_code(q.dtype), int(bool(causal)), *args, B, H, N, H_kv, N_kv, D, sm_scale,
+            workspace.data_ptr(), workspace.numel(), stream)
+        if rc:
+            self._check(rc, "sage_attn_bwd")
 
     def quant_q(self, q, sm_scale, *, qk_int8):
         """Q quantized exactly as the main loop quantizes it: `(q8, sq, cq)` on q's device."""

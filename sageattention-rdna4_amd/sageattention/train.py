@@ -1,0 +1,113 @@
+"""Training with `sageattn`: its backward pass.
+
+    out = sageattn_train(q, k, v, is_causal=True)      # as sageattn, recorded by autograd
+    out.backward(dout)
+
+`sageattn_backward` is the pass itself, for a program that keeps the forward call's output and
+logsumexp on its own. It recomputes the probabilities from Q, K and the logsumexp in 16 bits (the
+forward call's 8-bit codes are not kept), takes two or three launches on the current stream and
+synchronizes nothing, so that it can be captured into a graph. A call that is not served raises
+`ValueError` with the reason.
+"""
+import math
+
+import torch
+
+from .cache import _launch, _library, _refuse, _view
+from .core import sageattn
+
+
+def _row_floats(what, name, t, shape, device):
+    """Checks a contiguous fp32 tensor of one value per row."""
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        _refuse(what, "device: %s must be a tensor on %s" % (name, device))
+    if t.dtype != torch.float32:
+        _refuse(what, "dtype: %s must be float32 (got %s)" % (name, t.dtype))
+    if tuple(t.shape) != tuple(shape):
+        _refuse(what, "shape: %s is %s, not %s" % (name, tuple(t.shape), tuple(shape)))
+    if not t.is_contiguous():
+        _refuse(what, "stride_last: %s must be contiguous" % name)
+
+
+def sageattn_backward(dout, q, k, v, out, lse, tensor_layout="HND", is_causal=False, sm_scale=None,
+                      dlse=None):
+    """The gradients `(dq, dk, dv)` of `sageattn(q, k, v, ...)` from `dout`, that of its output.
+
+    q, k, v, tensor_layout, is_causal, sm_scale: as the forward call had them. out, lse: what it returned
+    with `return_lse=True`. dlse (B, H, N) fp32: the gradient of lse, where the caller used it. out and
+    dout have q's shape and dtype (any strides that `sageattn` takes), the gradients are contiguous, of
+    q's, k's and v's shapes and dtype.
+
+    Keys that are one part of those a query sees (attention over parts, merged by their logsumexp)
+    have their gradients from calls with the merged out and lse, a call for each part; dq is the calls'
+    sum. A row with a logsumexp of -infinity saw nothing and counts for nothing. Values have to be finite,
+    those of a padded batch's unused rows too: 0 times a NaN or an infinity is NaN.
+    """
+    what = "sageattn_backward"
+    views = [_view(what, tensor_layout, name, t) for name, t in
+             (("q", q), ("k", k), ("v", v), ("out", out), ("dout", dout))]
+    qq, kk, vv, oo, gg = views
+    dev, dtype = q.device, q.dtype
+    for name, t in (("k", k), ("v", v), ("out", out), ("dout", dout)):
+        if t.device != dev:
+            _refuse(what, "device: %s is on %s, q on %s" % (name, t.device, dev))
+        if t.dtype != dtype:
+            _refuse(what, "dtype: %s is %s, q %s" % (name, t.dtype, dtype))
+    B, H, N, D = qq.shape
+    H_kv, N_kv = kk.shape[1], kk.shape[2]
+    if kk.shape != vv.shape:
+        _refuse(what, "shape: k is %s, v %s" % (tuple(k.shape), tuple(v.shape)))
+    for name, t in (("out", out), ("dout", dout)):
+        if t.shape != q.shape:
+            _refuse(what, "shape: %s is %s, q %s" % (name, tuple(t.shape), tuple(q.shape)))
+    if kk.shape[0] != B or kk.shape[3] != D:
+        _refuse(what, "shape: k is %s, q %s" % (tuple(k.shape), tuple(q.shape)))
+    if H % H_kv:
+        _refuse(what, "heads: %d query heads on %d K/V heads" % (H, H_kv))
+    if is_causal and N != N_kv:
+        _refuse(what, "seq_len: causal attention needs as many queries as keys (%d, %d)" % (N, N_kv))
+    _row_floats(what, "lse", lse, (B, H, N), dev)
+    if dlse is not None:
+        _row_floats(what, "dlse", dlse, (B, H, N), dev)
+    sm = D ** -0.5 if sm_scale is None else float(sm_scale)
+    if not 0.0 < sm < math.inf:
+        _refuse(what, "sm_scale: must be positive and finite (got %r)" % (sm_scale,))
+    lib = _library(what, dev)
+    grads = [t.new_empty(t.shape) for t in (q, k, v)]
+    into = grads if tensor_layout == "HND" else [t.transpose(1, 2) for t in grads]
+    work = torch.empty(lib.attn_bwd_workspace_bytes(dtype, bool(is_causal), B, H, N, H_kv, N_kv, D),
+                       dtype=torch.uint8, device=dev)
+    _launch(dev, lib.attn_bwd, qq, kk, vv, oo, gg, lse, dlse, *into, is_causal, sm, work)
+    return tuple(grads)
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, tensor_layout, is_causal, sm_scale, options):
+        out, lse = sageattn(q, k, v, tensor_layout, is_causal, sm_scale, return_lse=True, **options)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.call = (tensor_layout, bool(is_causal), sm_scale)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dlse):
+        q, k, v, out, lse = ctx.saved_tensors
+        if dout is None and dlse is None:
+            return (None,) * 7
+        dout = torch.zeros_like(out) if dout is None else dout.contiguous()
+        dlse = None if dlse is None else dlse.contiguous()
+        return sageattn_backward(dout, q, k, v, out, lse, *ctx.call, dlse=dlse) + (None,) * 4
+
+
+def sageattn_train(q, k, v, tensor_layout="HND", is_causal=False, sm_scale=None, return_lse=False,
+                   **kwargs):
+    """`sageattn` as an operation that autograd records: the same arguments and results, with gradients
+    to q, k and v (from the logsumexp's gradient too, with `return_lse`).
+
+    The gradients are those of attention itself: the forward call's rounding to 8 bits counts as the
+    identity. Gradients of gradients are not served.
+    """
+    out, lse = _Attention.apply(q, k, v, tensor_layout, is_causal, sm_scale, kwargs)
+    return (out, lse) if return_lse else out
