@@ -15,7 +15,7 @@
 // the card each one's loop is cut into parts, whose fp32 sums `join` adds in order. So results are the
 // same from call to call.
 //
-// Layout. A wave owns 32 T columns (keys, or queries) of 16-bit operands in registers and multiplies
+// Layout. A wave owns 32 columns (keys, or queries) of 16-bit operands in registers and multiplies
 // them with 32 rows of the other side at a time by 32x32x16 MFMAs. The result has a column per lane,
 // its rows in the lane's registers: converted to 16 bits it is, lane for lane, the operand of the second
 // product when that takes its inner index in the order {16t + 4g + 0..3, 16t + 8 + 4g + 0..3} (g the
@@ -62,7 +62,11 @@ __device__ __forceinline__ bf16x4 read_tr(const bf16* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)p);
 }
 
+constexpr int BC = 128;                // columns (keys, or queries) that a block owns: 32 a wave
 constexpr int BT = 64;                 // rows of the other side in an LDS tile
+// Halves of a tile in the loop's code.
+template <int D>
+constexpr int U = D == 64 ? 2 : 1;
 constexpr float NEG_INF = -__builtin_inff();
 // fp16 operands: P is held times 2^12, so that it is a normal number from 2^-26 up and may pass 1 by a
 // factor of 15 (a logsumexp of quantized scores is off by some hundredths), dS times a power of two
@@ -96,14 +100,14 @@ struct Args {
   int k_tiles, q_tiles, k_split, q_split, k_blocks;
   float sm_scale, c;
   // workspace
-  float* nl;        // (planes_q, NP): P_SHIFT - lse log2 e
+  float* nl;        // (planes_q, NP): (P_SHIFT - lse log2 e) / c
   float* nd;        // (planes_q, NP): -d
   float* max_do;    // fp16: (planes_q, nb_q): a tile's largest |dout|^2, |d|, and (planes_kv, nb_kv) |v|^2
   float* max_d;
   float* max_v;
-  float* part_k;    // (k_split, planes_kv, k_tiles KB, D) sums of dK, of dV, where k_split > 1
+  float* part_k;    // (k_split, planes_kv, k_tiles BC, D) sums of dK, of dV, where k_split > 1
   float* part_v;
-  float* part_q;    // (q_split, planes_q, q_tiles QB, D)
+  float* part_q;    // (q_split, planes_q, q_tiles BC, D)
 };
 
 template <typename T>
@@ -161,7 +165,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const Args a) {
       if (r < n_rows) {
         const int64_t row = (int64_t)p * a.N + r;
         const float l = a.lse[row];
-        nl = l == NEG_INF ? NEG_INF : __builtin_fmaf(-LOG2E_F, l, P_SHIFT<T>);
+        nl = l == NEG_INF ? NEG_INF : __builtin_fmaf(-LOG2E_F, l, P_SHIFT<T>) / a.c;
         nd = (a.dlse ? a.dlse[row] : 0.0f) - dot;
       }
       if (cg == 0) {
@@ -224,113 +228,164 @@ __device__ __forceinline__ float scale_for(float bound) {
 template <int D>
 constexpr int LDS_BYTES = 4 * BT * D * 2 + 2 * 2 * BT * 4;
 
-// One tile of BT rows of x from row r0 on into LDS, a quarter by each wave; rows from `n` on are row
-// n - 1 again (what they would add is multiplied by P = 0).
-template <typename T, int D>
-__device__ __forceinline__ void stage(const T* x, int64_t sr, int r0, int n, uint32_t lds, int w,
-                                      int lane) {
-  constexpr int CPR = D / 8, RPI = 64 / CPR, IT = 16 / RPI;
-  const T* base = x + (int64_t)r0 * sr;
-  const int last = n - 1 - r0;
-#pragma unroll
-  for (int i = 0; i < IT; ++i) {
-    const int r = 16 * w + RPI * i + lane / CPR, c = (lane % CPR) ^ swz<D>(r);
-    dma16(base, (uint32_t)(min(r, last) * (int)(2 * sr) + 16 * c),
-          lds + (16 * w + RPI * i) * D * 2);
-  }
+// The lane's number, formed where it stands: what follows from it is not kept in registers over the
+// main loop (head_dim 128, where all 256 are in use).
+__device__ __forceinline__ int lane_anew() {
+  int x;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+  return x;
 }
 
-// Offsets, in elements, of a lane's operands within a tile.
-template <int D>
-struct Offsets {
-  int row[D / 16];       // rows lane % 32: chunk 2s + g
-  int tr[D / 32][2];     // transposed: 4 rows from 4g (+ 8) on, columns 32 dt .. + 31
-  __device__ __forceinline__ Offsets(int lane) {
-    const int r = lane & 31, g = lane >> 5, l16 = lane & 15, j = (lane >> 4) & 1;
+// A tile of BT rows of a plane on its way into LDS, a quarter by each wave, 1 KB a request: 64 lanes of
+// 16 bytes, RPI rows.
+template <typename T, int D>
+struct Staging {
+  static constexpr int CPR = D / 8, RPI = 64 / CPR, IT = 16 / RPI;
+  int lane, w;
+  __device__ __forceinline__ Staging(int lane, int w) : lane(lane), w(w) {}
+  // Rows from r0 on (`x`: row 0) to LDS address `lds`. Rows from n on are row n - 1 again: what they would
+  // add is multiplied by P = 0.
+  __device__ __forceinline__ void operator()(const T* x, int64_t sr, int r0, int n, uint32_t lds) const {
+    const int l = D == 128 ? lane_anew() : lane;
+    const int step = (int)(2 * sr), own = l / CPR;
+    const int chunk = 16 * ((l % CPR) ^ swz<D>(own));
+    const T* base = x + (int64_t)(r0 + 16 * w) * sr;
+    lds = __builtin_amdgcn_readfirstlane(lds + 16 * w * D * 2);
+    // (At head_dim 128 the branch costs more than the clamps: 7.20 ms for 6.94, 32 heads of 16384.)
+    if (D == 64 && r0 + BT <= n) {
+      const int at = own * step;
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) row[s] = r * D + 8 * ((2 * s + g) ^ swz<D>(r));
+      for (int i = 0; i < IT; ++i)
+        dma16(base + (int64_t)(RPI * i) * sr, (uint32_t)(at + (chunk ^ 16 * swz<D>(RPI * i))),
+              lds + RPI * i * D * 2);
+    } else {
+      base = x + (int64_t)r0 * sr;
+      const int last = n - 1 - r0;
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-      for (int hi = 0; hi < 2; ++hi) {
-        const int rr = 4 * g + (l16 >> 2) + 8 * hi;
-        tr[dt][hi] = rr * D + 8 * ((4 * dt + 2 * j + ((l16 & 3) >> 1)) ^ swz<D>(rr)) + 4 * (l16 & 1);
-      }
+      for (int i = 0; i < IT; ++i)
+        dma16(base, (uint32_t)(min(16 * w + RPI * i + own, last) * step + (chunk ^ 16 * swz<D>(RPI * i))),
+              lds + RPI * i * D * 2);
+    }
   }
 };
 
-// The transposed operand of 16 rows (from `tile` on) and columns 32 dt .. + 31.
-template <typename T, int D>
-__device__ __forceinline__ typename Vec<T>::x8 transposed(const T* tile, const Offsets<D>& of, int dt) {
-  const auto lo = read_tr(tile + of.tr[dt][0]), hi = read_tr(tile + of.tr[dt][1]);
-  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-
-// A wave's 32 KT columns of x (rows of memory from r0 on; from n on row n - 1 again) as operands.
-template <typename T, int D, int KT>
-__device__ __forceinline__ void load_columns(const T* x, int64_t sr, int r0, int n, int lane,
-                                             typename Vec<T>::x8 (&f)[KT][D / 16]) {
-#pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
-    const T* p = x + (int64_t)min(r0 + 32 * kt + (lane & 31), n - 1) * sr + 8 * (lane >> 5);
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) f[kt][s] = *(const typename Vec<T>::x8*)(p + 16 * s);
+// Where a lane's operands lie in a tile, in bytes; the chunk's number is part of the address by
+// exclusive or alone.
+template <int D>
+struct Offsets {
+  int row, lo, hi;
+  __device__ __forceinline__ Offsets(int lane) {
+    const int r = lane & 31, g = lane >> 5, l16 = lane & 15, j = (lane >> 4) & 1;
+    row = r * D * 2 + 16 * (g ^ swz<D>(r));
+    const int r4 = 4 * g + (l16 >> 2), c = 2 * j + ((l16 & 3) >> 1);
+    lo = r4 * D * 2 + 16 * (c ^ swz<D>(r4)) + 8 * (l16 & 1);
+    hi = (r4 + 8) * D * 2 + 16 * (c ^ swz<D>(r4 + 8)) + 8 * (l16 & 1);
   }
-}
-
-// A wave's sums, columns of D values each, times f, into rows from r0 on of a 16-bit view or of fp32
-// parts.
-template <typename T, int D, int KT>
-__device__ __forceinline__ void store_columns(const f32x16 (&acc)[KT][D / 32], const float (&f)[KT],
-                                              const Out& o, int b, int h, float* part, int r0, int n,
-                                              int lane) {
-#pragma unroll
-  for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt) keep_live(acc[kt][dt]);
-#pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
-    const int r = r0 + 32 * kt + (lane & 31);
-    if (r >= n) continue;
-    const int col = 4 * (lane >> 5);
-    if (part) {
-      float* p = part + (int64_t)r * D + col;
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          f32x4 x;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = acc[kt][dt][4 * i + e] * f[kt];
-          *(f32x4*)(p + 32 * dt + 8 * i) = x;
-        }
-    } else {
-      T* p = (T*)o.p + (int64_t)b * o.sb + (int64_t)h * o.sh + (int64_t)r * o.sr + col;
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          typename Vec<T>::x4 x;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = (T)(acc[kt][dt][4 * i + e] * f[kt]);
-          *(typename Vec<T>::x4*)(p + 32 * dt + 8 * i) = x;
-        }
+  // In the 32 rows at `at`, a multiple of a row. At head_dim 128 the addresses of a chunk are worked
+  // out for its read, at 64 each has a register and `at` stands in the instruction.
+  __device__ __forceinline__ Offsets rows(int& at) const {
+    Offsets x = *this;
+    if (D == 128) {
+      asm volatile("" : "+s"(at));
+      x.row += at;
+      x.lo += at;
+      x.hi += at;
+      at = 0;
     }
+    return x;
+  }
+};
+// Rows lane % 32 of 32, columns 16 s + 8 g .. + 7; `at`: the place of the rows.
+template <typename T>
+__device__ __forceinline__ typename Vec<T>::x8 row_operand(const u8* smem, int off, int at, int s) {
+  return *(const typename Vec<T>::x8*)(smem + (off ^ (32 * s)) + at);
+}
+// The transposed operand of 16 rows and columns 32 dt .. + 31.
+template <typename T>
+__device__ __forceinline__ typename Vec<T>::x8 transposed(const u8* smem, int lo, int hi, int at, int dt) {
+  const auto a = read_tr((const T*)(smem + (lo ^ (64 * dt)) + at)),
+             b = read_tr((const T*)(smem + (hi ^ (64 * dt)) + at));
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// A wave's 32 columns of x (rows of memory from r0 on; from n on row n - 1 again) as operands.
+template <typename T, int D>
+__device__ __forceinline__ void load_columns(const T* x, int64_t sr, int r0, int n, int lane,
+                                             typename Vec<T>::x8 (&f)[D / 16]) {
+  const T* p = x + (int64_t)min(r0 + (lane & 31), n - 1) * sr + 8 * (lane >> 5);
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) f[s] = *(const typename Vec<T>::x8*)(p + 16 * s);
+}
+
+// A wave's sums, 32 columns of D values each, times f, into rows from r0 on of a 16-bit view or of fp32
+// parts.
+template <typename T, int D>
+__device__ __forceinline__ void store_columns(const f32x16 (&acc)[D / 32], float f, const Out& o, int b,
+                                              int h, float* part, int r0, int n, int lane) {
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) keep_live(acc[dt]);
+  const int r = r0 + (lane & 31), col = 4 * (lane >> 5);
+  if (r >= n) return;
+  if (part) {
+    float* p = part + (int64_t)r * D + col;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = acc[dt][4 * i + e] * f;
+        *(f32x4*)(p + 32 * dt + 8 * i) = x;
+      }
+  } else {
+    T* p = (T*)o.p + (int64_t)b * o.sb + (int64_t)h * o.sh + (int64_t)r * o.sr + col;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        typename Vec<T>::x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = (T)(acc[dt][4 * i + e] * f);
+        *(typename Vec<T>::x4*)(p + 32 * dt + 8 * i) = x;
+      }
   }
 }
 
-template <int N>
-__device__ __forceinline__ void clear(f32x16 (&x)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) x[i][r] = 0.0f;
+// Between the phases of a step: what the compiler moves across costs it registers, at head_dim 64 (a
+// 4096-token image at 20 heads: 356 us with, 372 without) and where no branch for masks parts the
+// phases (spills). Not for causal calls at head_dim 128: 4 sequences of 2048, 32 heads, 551 us with, 544
+// without.
+template <int D, bool CAUSAL>
+__device__ __forceinline__ void fence() {
+  if (D == 64 || !CAUSAL) __builtin_amdgcn_sched_barrier(0);
 }
 
-// A block that owns 128 KT keys of a K/V head.
-template <typename T, int D, int KT, bool CAUSAL>
+__device__ __forceinline__ void clear(f32x16& x) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) x[r] = 0.0f;
+}
+
+// The requests of the tile at hand have landed, in all waves, and everyone is done with the other one.
+__device__ __forceinline__ void next_tile() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// A constant of each of a result's rows, 8 (r / 4) + 4 g + r % 4; `rows`: from 4 g on.
+__device__ __forceinline__ f32x16 row_constants(const float* rows) {
+  f32x16 x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x4 y = *(const f32x4*)(rows + 8 * i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[4 * i + e] = y[e];
+  }
+  return x;
+}
+
+// A block that owns 128 keys of a K/V head.
+template <typename T, int D, bool CAUSAL>
 __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
-  constexpr int KB = 128 * KT, TILE = BT * D;
+  constexpr int TILE = BT * D * 2;
   constexpr bool F16 = std::is_same_v<T, f16>;
   typedef typename Vec<T>::x8 x8;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -338,8 +393,8 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
   const int pl = block % a.planes_kv, ts = block / a.planes_kv;
   const int tile = ts / a.k_split, sp = ts - tile * a.k_split;
   const int b = pl / a.H_kv, hk = pl - b * a.H_kv;
-  const int k0 = tile * KB, kw = k0 + 32 * KT * w;
-  // iterations: tiles of queries, head after head of the group
+  const int k0 = tile * BC, kw = k0 + 32 * w;
+  // tiles of queries, head after head of the group
   const int first = CAUSAL ? k0 / BT : 0, per = a.nb_q - first;
   const int n = per * a.G;
   const int it0 = (int)((int64_t)n * sp / a.k_split), it1 = (int)((int64_t)n * (sp + 1) / a.k_split);
@@ -355,118 +410,102 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
   }
   const float fs = scale * __builtin_ldexpf(1.0f, -(int)P_SHIFT<T>);
 
-  T* lds = (T*)smem;
-  float* lds_rows = (float*)(lds + 4 * TILE);
+  // LDS: two tiles of Q, two of dout, and of the rows' two constants
+  const float* lds_rows = (const float*)(smem + 4 * TILE);
   const uint32_t lds0 = lds_addr(smem);
+  const Staging<T, D> stage(lane, w);
   int gi = it0 / per, ti = first + it0 - gi * per;   // of the next tile to be requested
   auto request = [&](int buf) {
     const int h = hk * a.G + gi, q0 = ti * BT;
-    stage<T, D>(plane<T>(a.q, b, h), a.q.sr, q0, a.N, lds0 + buf * TILE * 2, w, lane);
-    stage<T, D>(plane<T>(a.dout, b, h), a.dout.sr, q0, a.N, lds0 + (2 + buf) * TILE * 2, w, lane);
+    stage(plane<T>(a.q, b, h), a.q.sr, q0, a.N, lds0 + buf * TILE);
+    stage(plane<T>(a.dout, b, h), a.dout.sr, q0, a.N, lds0 + (2 + buf) * TILE);
     const int64_t row = (int64_t)(b * a.H + h) * a.NP + q0;
     if (w < 2)
-      dma4((w ? a.nd : a.nl) + row, 4 * lane, lds0 + 8 * TILE + (2 * buf + w) * BT * 4);
+      dma4((w ? a.nd : a.nl) + row, 4 * (D == 128 ? lane_anew() : lane),
+           lds0 + 4 * TILE + (2 * buf + w) * BT * 4);
     if (++ti == a.nb_q) {
       ti = first;
       ++gi;
     }
   };
 
-  const Offsets<D> of(lane);
-  x8 kf[KT][D / 16], vf[KT][D / 16];
-  load_columns<T, D, KT>(plane<T>(a.k, b, hk), a.k.sr, kw, a.N_kv, lane, kf);
-  load_columns<T, D, KT>(plane<T>(a.v, b, hk), a.v.sr, kw, a.N_kv, lane, vf);
-  f32x16 dk[KT][D / 32], dv[KT][D / 32];
+  const Offsets<D> offsets(lane);
+  x8 kf[D / 16], vf[D / 16];
+  load_columns<T, D>(plane<T>(a.k, b, hk), a.k.sr, kw, a.N_kv, lane, kf);
+  load_columns<T, D>(plane<T>(a.v, b, hk), a.v.sr, kw, a.N_kv, lane, vf);
+  f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
-    clear(dk[kt]);
-    clear(dv[kt]);
+  for (int dt = 0; dt < D / 32; ++dt) {
+    clear(dk[dt]);
+    clear(dv[dt]);
   }
+  // 32 queries from qu on, which lie at `at`
+  auto step = [&](int qu, int at, const float* rows) {
+    const Offsets<D> of = offsets.rows(at);
+    const int at_do = at + 2 * TILE;
+    f32x16 s = row_constants(rows), dp;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) s = mfma16(row_operand<T>(smem, of.row, at, i), kf[i], s);
+    if (CAUSAL && qu < kw + 31) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (qu + 8 * (r / 4) + 4 * g + r % 4 < kw + (lane & 31)) s[r] = NEG_INF;
+    }
+    fence<D, CAUSAL>();
+    dp = row_constants(rows + BT);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) dp = mfma16(row_operand<T>(smem, of.row, at_do, i), vf[i], dp);
+    fence<D, CAUSAL>();
+    x8 pf[2], df[2];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      float p = __builtin_amdgcn_exp2f(s[r] * a.c);
+      pf[r / 8][r % 8] = (T)p;
+      if (F16) p *= fs;
+      df[r / 8][r % 8] = (T)(p * dp[r]);
+    }
+    fence<D, CAUSAL>();
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) {
+        dv[dt] = mfma16(transposed<T>(smem, of.lo, of.hi, at_do + 32 * t * D, dt), pf[t], dv[dt]);
+        dk[dt] = mfma16(transposed<T>(smem, of.lo, of.hi, at + 32 * t * D, dt), df[t], dk[dt]);
+      }
+  };
   int tc = ti;                                       // the tile at hand
+  // what was loaded so far is here: in the loop the compiler has nothing of its own to wait for
+  __builtin_amdgcn_s_waitcnt(0);
   if (it0 < it1) request(0);
-  int buf = 0;
-  for (int it = it0; it < it1; ++it) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  auto tile_of = [&](int it, int buf) {
+    next_tile();
     const int q0 = tc * BT;
     tc = ti;
     if (it + 1 < it1) request(buf ^ 1);
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int qu = q0 + 32 * u;
-      if (CAUSAL && qu + 31 < kw) continue;
-      const T* tq = lds + buf * TILE + 32 * u * D;
-      const T* to = tq + 2 * TILE;
-      const float* rows = lds_rows + 2 * buf * BT + 32 * u + 4 * g;
-      f32x16 nl, nd;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4 x = *(const f32x4*)(rows + 8 * i), y = *(const f32x4*)(rows + BT + 8 * i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          nl[4 * i + e] = x[e];
-          nd[4 * i + e] = y[e];
-        }
-      }
-      f32x16 s[KT], dp[KT];
-      clear(s);
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) dp[kt] = nd;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const x8 x = *(const x8*)(tq + of.row[i]);
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) s[kt] = mfma16(x, kf[kt][i], s[kt]);
-      }
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const x8 x = *(const x8*)(to + of.row[i]);
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) dp[kt] = mfma16(x, vf[kt][i], dp[kt]);
-      }
-      x8 pf[KT][2], df[KT][2];
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        const int key = kw + 32 * kt + (lane & 31);
-        const bool diagonal = CAUSAL && qu < kw + 32 * kt + 31;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], a.c, nl[r]));
-          if (diagonal && qu + 8 * (r / 4) + 4 * g + r % 4 < key) p = 0.0f;
-          pf[kt][r / 8][r % 8] = (T)p;
-          if (F16) p *= fs;
-          df[kt][r / 8][r % 8] = (T)(p * dp[kt][r]);
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) {
-          const x8 x = transposed<T, D>(to + 16 * t * D, of, dt);
-          const x8 y = transposed<T, D>(tq + 16 * t * D, of, dt);
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt) {
-            dv[kt][dt] = mfma16(x, pf[kt][t], dv[kt][dt]);
-            dk[kt][dt] = mfma16(y, df[kt][t], dk[kt][dt]);
-          }
-        }
+    const float* rows = lds_rows + 2 * buf * BT + 4 * g;
+#pragma unroll U<D>
+    for (int u = 0; u < 2; ++u)
+      if (!CAUSAL || q0 + 32 * u + 31 >= kw) step(q0 + 32 * u, (buf * BT + 32 * u) * D * 2, rows + 32 * u);
+  };
+  if (D == 64) {
+    for (int it = it0; it < it1; it += 2) {
+      tile_of(it, 0);
+      if (it + 1 < it1) tile_of(it + 1, 1);
     }
-    buf ^= 1;
+  } else {
+    for (int it = it0; it < it1; ++it) tile_of(it, (it - it0) & 1);
   }
-  float fk[KT], fv[KT];
-#pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
-    fk[kt] = a.sm_scale / scale;
-    fv[kt] = __builtin_ldexpf(1.0f, -(int)P_SHIFT<T>);
-  }
-  const int64_t part = ((int64_t)sp * a.planes_kv + pl) * a.k_tiles * KB * D;
-  store_columns<T, D, KT>(dk, fk, a.dk, b, hk, a.k_split > 1 ? a.part_k + part : nullptr, kw, a.N_kv, lane);
-  store_columns<T, D, KT>(dv, fv, a.dv, b, hk, a.k_split > 1 ? a.part_v + part : nullptr, kw, a.N_kv, lane);
+  const int64_t part = ((int64_t)sp * a.planes_kv + pl) * a.k_tiles * BC * D;
+  store_columns<T, D>(dk, a.sm_scale / scale, a.dk, b, hk, a.k_split > 1 ? a.part_k + part : nullptr, kw,
+                      a.N_kv, lane);
+  store_columns<T, D>(dv, __builtin_ldexpf(1.0f, -(int)P_SHIFT<T>), a.dv, b, hk,
+                      a.k_split > 1 ? a.part_v + part : nullptr, kw, a.N_kv, lane);
 }
 
-// A block that owns 128 QT queries of a head.
-template <typename T, int D, int QT, bool CAUSAL>
+// A block that owns 128 queries of a head.
+template <typename T, int D, bool CAUSAL>
 __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block) {
-  constexpr int QB = 128 * QT, TILE = BT * D;
+  constexpr int TILE = BT * D * 2;
   constexpr bool F16 = std::is_same_v<T, f16>;
   typedef typename Vec<T>::x8 x8;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -475,8 +514,8 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
   // the longest tiles, the last of a causal plane, begin first
   const int tile = a.q_tiles - 1 - ts / a.q_split, sp = ts % a.q_split;
   const int b = pl / a.H, h = pl - b * a.H, hk = h / a.G;
-  const int q0 = tile * QB, qw = q0 + 32 * QT * w;
-  const int n = CAUSAL ? min((q0 + QB + BT - 1) / BT, a.nb_kv) : a.nb_kv;
+  const int q0 = tile * BC, qw = q0 + 32 * w;
+  const int n = CAUSAL ? min((q0 + BC) / BT, a.nb_kv) : a.nb_kv;
   const int it0 = (int)((int64_t)n * sp / a.q_split), it1 = (int)((int64_t)n * (sp + 1) / a.q_split);
 
   float mv = 0.0f;
@@ -484,112 +523,107 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
     mv = sqrtf(block_max(a.max_v + (int64_t)(b * a.H_kv + hk) * a.nb_kv, a.nb_kv, (float*)smem));
     __syncthreads();
   }
-  T* lds = (T*)smem;
+  // LDS: two tiles of K, two of V
   const uint32_t lds0 = lds_addr(smem);
   const T* pk = plane<T>(a.k, b, hk);
   const T* pv = plane<T>(a.v, b, hk);
+  const Staging<T, D> stage(lane, w);
   auto request = [&](int it, int buf) {
-    stage<T, D>(pk, a.k.sr, it * BT, a.N_kv, lds0 + buf * TILE * 2, w, lane);
-    stage<T, D>(pv, a.v.sr, it * BT, a.N_kv, lds0 + (2 + buf) * TILE * 2, w, lane);
+    stage(pk, a.k.sr, it * BT, a.N_kv, lds0 + buf * TILE);
+    stage(pv, a.v.sr, it * BT, a.N_kv, lds0 + (2 + buf) * TILE);
   };
 
-  const Offsets<D> of(lane);
-  x8 qf[QT][D / 16], of_do[QT][D / 16];
-  load_columns<T, D, QT>(plane<T>(a.q, b, h), a.q.sr, qw, a.N, lane, qf);
-  load_columns<T, D, QT>(plane<T>(a.dout, b, h), a.dout.sr, qw, a.N, lane, of_do);
-  float nl[QT], nd[QT], fs[QT], fq[QT];
+  const Offsets<D> offsets(lane);
+  x8 qf[D / 16], gf[D / 16];
+  load_columns<T, D>(plane<T>(a.q, b, h), a.q.sr, qw, a.N, lane, qf);
+  load_columns<T, D>(plane<T>(a.dout, b, h), a.dout.sr, qw, a.N, lane, gf);
+  const int64_t row = (int64_t)pl * a.NP + min(qw + (lane & 31), a.NP - 1);
+  const float nl1 = a.nl[row], nd1 = a.nd[row];
+  float scale = 1.0f;
+  if (F16) {
+    float sq = 0.0f;
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    const int64_t row = (int64_t)pl * a.NP + min(qw + 32 * qt + (lane & 31), a.NP - 1);
-    nl[qt] = a.nl[row];
-    nd[qt] = a.nd[row];
-    float scale = 1.0f;
-    if (F16) {
-      float sq = 0.0f;
+    for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = (float)of_do[qt][i][e];
-          sq = __builtin_fmaf(x, x, sq);
-        }
-      sq += __shfl_xor(sq, 32, 64);
-      scale = scale_for(sqrtf(sq) * mv + fabsf(nd[qt]));
-    }
-    fs[qt] = scale * __builtin_ldexpf(1.0f, -(int)P_SHIFT<T>);
-    fq[qt] = a.sm_scale / scale;
+      for (int e = 0; e < 8; ++e) {
+        const float x = (float)gf[i][e];
+        sq = __builtin_fmaf(x, x, sq);
+      }
+    sq += __shfl_xor(sq, 32, 64);
+    scale = scale_for(sqrtf(sq) * mv + fabsf(nd1));
   }
-  f32x16 dq[QT][D / 32];
+  const float fs = scale * __builtin_ldexpf(1.0f, -(int)P_SHIFT<T>);
+  f32x16 dq[D / 32];
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) clear(dq[qt]);
+  for (int dt = 0; dt < D / 32; ++dt) clear(dq[dt]);
+  // what S and dP begin with: a register for each row, all alike
+  f32x16 nl, nd;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    nl[r] = nl1;
+    nd[r] = nd1;
+  }
+  // 32 keys from ku on, which lie at `at`
+  auto step = [&](int ku, int at) {
+    const Offsets<D> of = offsets.rows(at);
+    f32x16 s = nl, dp = nd;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) s = mfma16(row_operand<T>(smem, of.row, at, i), qf[i], s);
+    if (ku + 31 >= (CAUSAL ? qw + 1 : a.N_kv)) {
+      const int query = qw + (lane & 31), end = CAUSAL ? min(query + 1, a.N_kv) : a.N_kv;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (ku + 8 * (r / 4) + 4 * g + r % 4 >= end) s[r] = NEG_INF;
+    }
+    fence<D, CAUSAL>();
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+      dp = mfma16(row_operand<T>(smem, of.row, at + 2 * TILE, i), gf[i], dp);
+    fence<D, CAUSAL>();
+    x8 df[2];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      float p = __builtin_amdgcn_exp2f(s[r] * a.c);
+      if (F16) p *= fs;
+      df[r / 8][r % 8] = (T)(p * dp[r]);
+    }
+    fence<D, CAUSAL>();
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+        dq[dt] = mfma16(transposed<T>(smem, of.lo, of.hi, at + 32 * t * D, dt), df[t], dq[dt]);
+  };
+  __builtin_amdgcn_s_waitcnt(0);                     // as in keys_block
   if (it0 < it1) request(it0, 0);
-  int buf = 0;
-  for (int it = it0; it < it1; ++it) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const int k0 = it * BT;
+  const int end = CAUSAL ? min(qw + 32, a.N_kv) : a.N_kv;
+  auto tile_of = [&](int it, int buf) {
+    next_tile();
     if (it + 1 < it1) request(it + 1, buf ^ 1);
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int ku = k0 + 32 * u;
-      if (ku >= a.N_kv || (CAUSAL && ku > qw + 32 * QT - 1)) continue;
-      const T* tk = lds + buf * TILE + 32 * u * D;
-      const T* tv = tk + 2 * TILE;
-      f32x16 s[QT], dp[QT];
-      clear(s);
-#pragma unroll
-      for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dp[qt][r] = nd[qt];
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const x8 x = *(const x8*)(tk + of.row[i]);
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) s[qt] = mfma16(x, qf[qt][i], s[qt]);
-      }
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const x8 x = *(const x8*)(tv + of.row[i]);
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) dp[qt] = mfma16(x, of_do[qt][i], dp[qt]);
-      }
-      x8 df[QT][2];
-      const bool ragged = ku + 32 > a.N_kv;
-#pragma unroll
-      for (int qt = 0; qt < QT; ++qt) {
-        const int query = qw + 32 * qt + (lane & 31);
-        const bool diagonal = CAUSAL && ku + 31 > qw + 32 * qt;
-        const int end = CAUSAL ? min(query + 1, a.N_kv) : a.N_kv;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qt][r], a.c, nl[qt]));
-          if ((ragged || diagonal) && ku + 8 * (r / 4) + 4 * g + r % 4 >= end) p = 0.0f;
-          if (F16) p *= fs[qt];
-          df[qt][r / 8][r % 8] = (T)(p * dp[qt][r]);
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) {
-          const x8 x = transposed<T, D>(tk + 16 * t * D, of, dt);
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) dq[qt][dt] = mfma16(x, df[qt][t], dq[qt][dt]);
-        }
+#pragma unroll U<D>
+    for (int u = 0; u < 2; ++u)
+      if (it * BT + 32 * u < end) step(it * BT + 32 * u, (buf * BT + 32 * u) * D * 2);
+  };
+  if (D == 64) {
+    for (int it = it0; it < it1; it += 2) {
+      tile_of(it, 0);
+      if (it + 1 < it1) tile_of(it + 1, 1);
     }
-    buf ^= 1;
+  } else {
+    for (int it = it0; it < it1; ++it) tile_of(it, (it - it0) & 1);
   }
-  const int64_t part = ((int64_t)sp * a.planes_q + pl) * a.q_tiles * QB * D;
-  store_columns<T, D, QT>(dq, fq, a.dq, b, h, a.q_split > 1 ? a.part_q + part : nullptr, qw, a.N, lane);
+  const int64_t part = ((int64_t)sp * a.planes_q + pl) * a.q_tiles * BC * D;
+  store_columns<T, D>(dq, a.sm_scale / scale, a.dq, b, h, a.q_split > 1 ? a.part_q + part : nullptr, qw, a.N,
+                      lane);
 }
 
-
-template <typename T, int D, int KT, bool CAUSAL>
-__global__ void __launch_bounds__(256, 3 - KT) main_kernel(const Args a) {
-  __shared__ __align__(16) u8 smem[LDS_BYTES<D>];
+template <typename T, int D, bool CAUSAL>
+__global__ void __launch_bounds__(256, D == 64 ? 3 : 2) main_kernel(const Args a) {
+  __shared__ __align__(1024) u8 smem[LDS_BYTES<D>];
   if ((int)blockIdx.x < a.k_blocks)
-    keys_block<T, D, KT, CAUSAL>(a, smem, blockIdx.x);
+    keys_block<T, D, CAUSAL>(a, smem, blockIdx.x);
   else
-    queries_block<T, D, KT, CAUSAL>(a, smem, blockIdx.x - a.k_blocks);
+    queries_block<T, D, CAUSAL>(a, smem, blockIdx.x - a.k_blocks);
 }
 
 // ------------------------------------------------------------------------------------- join
@@ -627,12 +661,12 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
                           (int64_t)r * a.out[x].sr + col) = y;
 }
 
-template <typename T, int D, int KT>
+template <typename T, int D>
 void launch_main(const Args& a, bool causal, int blocks, hipStream_t s) {
   if (causal)
-    hipLaunchKernelGGL((main_kernel<T, D, KT, true>), dim3(blocks), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((main_kernel<T, D, true>), dim3(blocks), dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((main_kernel<T, D, KT, false>), dim3(blocks), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((main_kernel<T, D, false>), dim3(blocks), dim3(256), 0, s, a);
 }
 
 template <typename T, int D>
@@ -641,7 +675,7 @@ hipError_t launch(const AttnBwdArgs& x, const AttnBwdPlan& p, const Args& a, hip
   hipLaunchKernelGGL((rows_kernel<T, D>), dim3(rows), dim3(256), 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  launch_main<T, D, 1>(a, x.causal, (int)(p.k_blocks + p.q_blocks), s);
+  launch_main<T, D>(a, x.causal, (int)(p.k_blocks + p.q_blocks), s);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   JoinArgs j = {};
   j.part[0] = a.part_k;
@@ -702,7 +736,7 @@ AttnBwdPlan attn_bwd_plan(int64_t B, int64_t H, int64_t H_kv, int64_t N, int64_t
   AttnBwdPlan p;
   p.nb_q = ceil_div(N, BT);
   p.nb_kv = ceil_div(N_kv, BT);
-  p.k_rows = p.q_rows = 128;
+  p.k_rows = p.q_rows = BC;
   p.k_tiles = ceil_div(N_kv, p.k_rows);
   p.q_tiles = ceil_div(N, p.q_rows);
   // As many parts as bring each block's steps (four products over a tile for keys, three for queries)
