@@ -82,6 +82,14 @@ __device__ __forceinline__ int swz(int r) {
                   : (((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1) | ((r >> 3) & 1);
 }
 
+// The lane's number, formed where it stands: what follows from it is not kept in registers over the
+// main loop, which needs them all.
+__device__ __forceinline__ int lane_anew() {
+  int x;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+  return x;
+}
+
 struct Rows {                          // a (B, H, N, D) view
   const void* p;
   int64_t sb, sh, sr;
@@ -228,14 +236,6 @@ __device__ __forceinline__ float scale_for(float bound) {
 template <int D>
 constexpr int LDS_BYTES = 4 * BT * D * 2 + 2 * 2 * BT * 4;
 
-// The lane's number, formed where it stands: what follows from it is not kept in registers over the
-// main loop (head_dim 128, where all 256 are in use).
-__device__ __forceinline__ int lane_anew() {
-  int x;
-  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
-  return x;
-}
-
 // A tile of BT rows of a plane on its way into LDS, a quarter by each wave, 1 KB a request: 64 lanes of
 // 16 bytes, RPI rows.
 template <typename T, int D>
@@ -321,10 +321,10 @@ __device__ __forceinline__ void load_columns(const T* x, int64_t sr, int r0, int
 // parts.
 template <typename T, int D>
 __device__ __forceinline__ void store_columns(const f32x16 (&acc)[D / 32], float f, const Out& o, int b,
-                                              int h, float* part, int r0, int n, int lane) {
+                                              int h, float* part, int r0, int n) {
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) keep_live(acc[dt]);
-  const int r = r0 + (lane & 31), col = 4 * (lane >> 5);
+  const int lane = lane_anew(), r = r0 + (lane & 31), col = 4 * (lane >> 5);
   if (r >= n) return;
   if (part) {
     float* p = part + (int64_t)r * D + col;
@@ -421,7 +421,7 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
     stage(plane<T>(a.dout, b, h), a.dout.sr, q0, a.N, lds0 + (2 + buf) * TILE);
     const int64_t row = (int64_t)(b * a.H + h) * a.NP + q0;
     if (w < 2)
-      dma4((w ? a.nd : a.nl) + row, 4 * (D == 128 ? lane_anew() : lane),
+      dma4((w ? a.nd : a.nl) + row, 4 * lane_anew(),
            lds0 + 4 * TILE + (2 * buf + w) * BT * 4);
     if (++ti == a.nb_q) {
       ti = first;
@@ -447,9 +447,10 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) s = mfma16(row_operand<T>(smem, of.row, at, i), kf[i], s);
     if (CAUSAL && qu < kw + 31) {
+      const int l = lane_anew(), ahead = kw + (l & 31) - qu - 4 * (l >> 5);
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        if (qu + 8 * (r / 4) + 4 * g + r % 4 < kw + (lane & 31)) s[r] = NEG_INF;
+        if (8 * (r / 4) + r % 4 < ahead) s[r] = NEG_INF;
     }
     fence<D, CAUSAL>();
     dp = row_constants(rows + BT);
@@ -497,9 +498,9 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
   }
   const int64_t part = ((int64_t)sp * a.planes_kv + pl) * a.k_tiles * BC * D;
   store_columns<T, D>(dk, a.sm_scale / scale, a.dk, b, hk, a.k_split > 1 ? a.part_k + part : nullptr, kw,
-                      a.N_kv, lane);
+                      a.N_kv);
   store_columns<T, D>(dv, __builtin_ldexpf(1.0f, -(int)P_SHIFT<T>), a.dv, b, hk,
-                      a.k_split > 1 ? a.part_v + part : nullptr, kw, a.N_kv, lane);
+                      a.k_split > 1 ? a.part_v + part : nullptr, kw, a.N_kv);
 }
 
 // A block that owns 128 queries of a head.
@@ -509,7 +510,6 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
   constexpr bool F16 = std::is_same_v<T, f16>;
   typedef typename Vec<T>::x8 x8;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = lane >> 5;
   const int pl = block % a.planes_q, ts = block / a.planes_q;
   // the longest tiles, the last of a causal plane, begin first
   const int tile = a.q_tiles - 1 - ts / a.q_split, sp = ts % a.q_split;
@@ -570,10 +570,11 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) s = mfma16(row_operand<T>(smem, of.row, at, i), qf[i], s);
     if (ku + 31 >= (CAUSAL ? qw + 1 : a.N_kv)) {
-      const int query = qw + (lane & 31), end = CAUSAL ? min(query + 1, a.N_kv) : a.N_kv;
+      const int l = lane_anew(), query = qw + (l & 31);
+      const int left = (CAUSAL ? min(query + 1, a.N_kv) : a.N_kv) - ku - 4 * (l >> 5);
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        if (ku + 8 * (r / 4) + 4 * g + r % 4 >= end) s[r] = NEG_INF;
+        if (8 * (r / 4) + r % 4 >= left) s[r] = NEG_INF;
     }
     fence<D, CAUSAL>();
 #pragma unroll
@@ -613,8 +614,7 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
     for (int it = it0; it < it1; ++it) tile_of(it, (it - it0) & 1);
   }
   const int64_t part = ((int64_t)sp * a.planes_q + pl) * a.q_tiles * BC * D;
-  store_columns<T, D>(dq, a.sm_scale / scale, a.dq, b, h, a.q_split > 1 ? a.part_q + part : nullptr, qw, a.N,
-                      lane);
+  store_columns<T, D>(dq, a.sm_scale / scale, a.dq, b, h, a.q_split > 1 ? a.part_q + part : nullptr, qw, a.N);
 }
 
 template <typename T, int D, bool CAUSAL>
