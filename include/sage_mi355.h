@@ -375,6 +375,42 @@ int64_t sage_attn_bwd_workspace_bytes(int dtype, int causal, int64_t B, int64_t 
                                       int64_t H_kv, int64_t N_kv, int64_t D);
 
 /*
+ * Root-mean-square norm of d0 x d1 x d2 rows of n values, in one launch. No counterpart in the reference.
+ * In fp32: t = x + residual, r = 1 / sqrt(mean t^2 + eps), y = t r w, rounded once.
+ *   x, residual  rows of `dtype`, 16-byte aligned, strides (outermost first) multiples of 8 elements; residual
+ *                optional
+ *   n            a multiple of 8 up to 32768
+ *   w            (n) of `dtype`, or fp32 with w_fp32; 16-byte aligned
+ *   out          0: y in `dtype`; codes with a scale per row by the prologue's scheme (scale =
+ *                max(max|y| / 127 or 448, 1e-12), y / scale rounded half to even): 1 int8, 2 e4m3. A row that
+ *                holds a NaN or an infinity: zero codes under a NaN scale
+ *   y, scales, sum, rstd   contiguous (rows, n), (rows) fp32 with codes, (rows, n) t in `dtype`
+ *                (optional), (rows) r (optional)
+ */
+int sage_rms_norm(int dtype, int w_fp32, int out, const void* x, int64_t x_s0, int64_t x_s1,
+                  int64_t x_s2, const void* residual, int64_t r_s0, int64_t r_s1, int64_t r_s2,
+                  const void* w, int64_t d0, int64_t d1, int64_t d2, int64_t n, float eps, void* y,
+                  float* scales, void* sum, float* rstd, void* stream);
+
+/*
+ * Its gradients, in two launches: with t the rows that were normed (x; with a residual the sum), r as
+ * sage_rms_norm gave it and g = dy w:
+ *   dx = r (g - t r mean(g t r)) + dsum (the gradient of x and of the residual alike),
+ *   dw = sum over the rows of dy t r, in fp32 and an order that the sizes decide, as w is held.
+ *   dy, x, dsum  rows as above; dsum (the gradient of t where it was used further on) optional
+ *   rstd         (rows) fp32; dx (rows, n) contiguous
+ *   workspace    sage_rms_norm_bwd_workspace_bytes bytes, 16-byte aligned
+ */
+int sage_rms_norm_bwd(int dtype, int w_fp32, const void* dy, int64_t g_s0, int64_t g_s1,
+                      int64_t g_s2, const void* x, int64_t x_s0, int64_t x_s1, int64_t x_s2,
+                      const void* dsum, int64_t s_s0, int64_t s_s1, int64_t s_s2, const void* w,
+                      const float* rstd, int64_t d0, int64_t d1, int64_t d2, int64_t n, void* dx,
+                      void* dw, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace of a sage_rms_norm_bwd call of these sizes, or -SAGE_ERR_INVALID. */
+int64_t sage_rms_norm_bwd_workspace_bytes(int64_t rows, int64_t n);
+
+/*
  * MFMA accumulator layout probe (known-answer test of the fragment layouts the main loop relies
  * on). One wave computes C = A(32x32, int8) * B(32x32, int8) with v_mfma_i32_32x32x32_i8 and
  * D = E(32x64, fp8) * F(64x32, fp8) with v_mfma_scale_f32_32x32x64_f8f6f4, loading operands in

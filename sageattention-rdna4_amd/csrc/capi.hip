@@ -115,6 +115,31 @@ int check_attn_bwd(int dtype, int causal, int64_t B, int64_t H, int64_t N, int64
   return check_grid("the backward pass", p.k_blocks + p.q_blocks, 256);
 }
 
+// The rows of a norm: in three dimensions, with 32-bit row numbers.
+constexpr int64_t kMaxNorm = 32768, kMaxNormRows = 1 << 30;
+int check_norm(int dtype, int64_t d0, int64_t d1, int64_t d2, int64_t n) {
+  if (dtype != SAGE_F16 && dtype != SAGE_BF16)
+    return fail(SAGE_ERR_INVALID, "dtype: unsupported dtype code %d", dtype);
+  if (n < 8 || n % 8 || n > kMaxNorm)
+    return fail(SAGE_ERR_INVALID, "row: %lld values (a multiple of 8 up to %lld is needed)", (long long)n,
+                (long long)kMaxNorm);
+  if (d0 < 1 || d1 < 1 || d2 < 1 || d0 > kMaxNormRows || d1 > kMaxNormRows ||
+      d2 > kMaxNormRows || d0 * d1 > kMaxNormRows || d0 * d1 * d2 > kMaxNormRows)
+    return fail(SAGE_ERR_INVALID, "rows: %lld x %lld x %lld (1 to 2^30 are served)", (long long)d0,
+                (long long)d1, (long long)d2);
+  // a block of 256 threads for up to 8 rows at least, of 1024 for longer rows
+  const int64_t rows = d0 * d1 * d2;
+  return n > 8192 ? check_grid("the norm", rows, 1024)
+                  : check_grid("the norm", n <= 1024 ? (rows + 3) / 4 : rows, 256);
+}
+int check_rows_view(const char* name, const sage::RowsView& v) {
+  if (!v.p) return fail(SAGE_ERR_INVALID, "%s is NULL", name);
+  if (!aligned16(v.p)) return fail(SAGE_ERR_INVALID, "%s: ptr_align (pointer not 16-byte aligned)", name);
+  if ((v.s[0] | v.s[1] | v.s[2]) & 7)
+    return fail(SAGE_ERR_INVALID, "%s: stride_align (strides must be multiples of 8 elements)", name);
+  return SAGE_OK;
+}
+
 // The prologue's two passes: C1 and C2 blocks per plane of 256 threads.
 int check_prologue_grid(int64_t BH, int64_t N, int64_t N_pad) {
   const sage::PrologueGeom g = sage::prologue_geom(BH, N, N_pad);
@@ -856,6 +881,83 @@ int sage_attn_bwd(int dtype, int causal, const void* q, int64_t q_sb, int64_t q_
   a.sm_scale = sm_scale;
   a.workspace = workspace;
   return hip_status(sage::launch_attn_bwd(a, (hipStream_t)stream), "sage_attn_bwd launch");
+}
+
+int sage_rms_norm(int dtype, int w_fp32, int out, const void* x, int64_t x_s0, int64_t x_s1,
+                  int64_t x_s2, const void* residual, int64_t r_s0, int64_t r_s1, int64_t r_s2,
+                  const void* w, int64_t d0, int64_t d1, int64_t d2, int64_t n, float eps, void* y,
+                  float* scales, void* sum, float* rstd, void* stream) {
+  int rc = check_norm(dtype, d0, d1, d2, n);
+  if (rc) return rc;
+  if (out < 0 || out > 2) return fail(SAGE_ERR_INVALID, "out: unsupported output code %d", out);
+  sage::NormArgs a = {};
+  a.x = {x, {x_s0, x_s1, x_s2}};
+  a.residual = {residual, {r_s0, r_s1, r_s2}};
+  if ((rc = check_rows_view("x", a.x))) return rc;
+  if (residual && (rc = check_rows_view("residual", a.residual))) return rc;
+  if (!w || !y || (out && !scales)) return fail(SAGE_ERR_INVALID, "a pointer is NULL");
+  if (!aligned16(w) || !aligned16(y) || !aligned16(sum))
+    return fail(SAGE_ERR_INVALID, "ptr_align: weight and outputs must be 16-byte aligned");
+  if (((uintptr_t)scales & 3u) || ((uintptr_t)rstd & 3u))
+    return fail(SAGE_ERR_INVALID, "ptr_align: scales and rstd must be 4-byte aligned");
+  if (!(eps >= 0.0f) || !(eps < 3.0e38f))
+    return fail(SAGE_ERR_INVALID, "eps: must be finite and not negative (got %g)", (double)eps);
+  a.dtype = dtype;
+  a.w32 = w_fp32 ? 1 : 0;
+  a.out = out;
+  a.w = w;
+  a.rows = d0 * d1 * d2;
+  a.d1 = d1;
+  a.d2 = d2;
+  a.n = n;
+  a.eps = eps;
+  a.y = y;
+  a.scales = scales;
+  a.sum = sum;
+  a.rstd = rstd;
+  return hip_status(sage::launch_rms_norm(a, (hipStream_t)stream), "sage_rms_norm launch");
+}
+
+int64_t sage_rms_norm_bwd_workspace_bytes(int64_t rows, int64_t n) {
+  const int rc = check_norm(SAGE_F16, 1, 1, rows, n);
+  if (rc) return -rc;
+  g_err.clear();
+  return sage::norm_grad_blocks(rows, n) * n * 4;
+}
+
+int sage_rms_norm_bwd(int dtype, int w_fp32, const void* dy, int64_t g_s0, int64_t g_s1,
+                      int64_t g_s2, const void* x, int64_t x_s0, int64_t x_s1, int64_t x_s2,
+                      const void* dsum, int64_t s_s0, int64_t s_s1, int64_t s_s2, const void* w,
+                      const float* rstd, int64_t d0, int64_t d1, int64_t d2, int64_t n, void* dx,
+                      void* dw, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_norm(dtype, d0, d1, d2, n);
+  if (rc) return rc;
+  sage::NormGradArgs a = {};
+  a.dy = {dy, {g_s0, g_s1, g_s2}};
+  a.x = {x, {x_s0, x_s1, x_s2}};
+  a.dsum = {dsum, {s_s0, s_s1, s_s2}};
+  if ((rc = check_rows_view("dy", a.dy))) return rc;
+  if ((rc = check_rows_view("x", a.x))) return rc;
+  if (dsum && (rc = check_rows_view("dsum", a.dsum))) return rc;
+  if (!w || !rstd || !dx || !dw) return fail(SAGE_ERR_INVALID, "a pointer is NULL");
+  if (!aligned16(w) || !aligned16(dx) || ((uintptr_t)rstd & 3u) || ((uintptr_t)dw & 3u))
+    return fail(SAGE_ERR_INVALID, "ptr_align: weight and dx must be 16-byte aligned, rstd and dw 4-byte");
+  const int64_t rows = d0 * d1 * d2, need = sage::norm_grad_blocks(rows, n) * n * 4;
+  if (workspace == nullptr || workspace_bytes < (size_t)need || !aligned16(workspace))
+    return fail(SAGE_ERR_INVALID, "workspace: need %lld bytes, 16-byte aligned (got %zu)",
+                (long long)need, workspace_bytes);
+  a.dtype = dtype;
+  a.w32 = w_fp32 ? 1 : 0;
+  a.w = w;
+  a.rstd = rstd;
+  a.rows = rows;
+  a.d1 = d1;
+  a.d2 = d2;
+  a.n = n;
+  a.dx = dx;
+  a.dw = dw;
+  a.workspace = workspace;
+  return hip_status(sage::launch_rms_norm_grad(a, (hipStream_t)stream), "sage_rms_norm_bwd launch");
 }
 
 int sage_quant_q(int dtype, int qk_int8, const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sr,

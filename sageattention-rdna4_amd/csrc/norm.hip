@@ -1,0 +1,413 @@
+// Root-mean-square norm (gfx950), with the residual's addition ahead of it and 16-bit or 8-bit output, and
+// its gradients.
+//
+// For a row of n values and the weights w, in fp32:
+//     t = x + residual,   r = 1 / sqrt(mean t^2 + eps),   y = t r w.
+// 8-bit output is the library's per-token scheme: scale = max(max|y| / 127 or 448, 1e-12), codes
+// rne(y / scale) or e4m3(y / scale). With dy, and dsum where t itself was used further on:
+//     g = dy w,   dx = r (g - t r mean(g t r)) + dsum,   dw = sum over the rows of dy t r.
+//
+// Every row is read once and kept in registers between its sum (for codes: its largest, too) and its
+// output, 16 bytes a lane and chunk: TPR lanes or threads to a row, C chunks each. All are bound by memory
+// (a large copy's 5.0 TB/s), small calls by their launch.
+#include "sage_device.h"
+#include "sage_launch.h"
+
+namespace sage {
+namespace {
+
+struct Norm {
+  const void* x;
+  const void* res;
+  const void* w;
+  void* y;
+  float* scales;
+  void* sum;
+  float* rstd;
+  int64_t xs[3], rs[3];      // strides of the rows' three dimensions
+  int rows, d1, d2, n, w32;
+  float eps;
+};
+struct NormGrad {
+  const void* dy;
+  const void* x;
+  const void* dsum;
+  const void* w;
+  const float* rstd;
+  void* dx;
+  float* part;               // (blocks, n)
+  int64_t gs[3], xs[3], ds[3];
+  int rows, d1, d2, n, w32;
+};
+
+// Element offset of row r; with one dimension alone (d2 = rows) nothing is divided.
+__device__ __forceinline__ int64_t row_at(const int64_t (&s)[3], int r, int rows, int d1, int d2) {
+  if (d2 == rows) return r * s[2];
+  const int q = r / d2, c = r - q * d2, a = q / d1, b = q - a * d1;
+  return a * s[0] + b * s[1] + c * s[2];
+}
+
+__device__ __forceinline__ void load_weights(const void* w, int w32, int col, float (&f)[8], f16) {
+  if (w32) {
+    const f32x4 a = *(const f32x4*)((const float*)w + col), b = *(const f32x4*)((const float*)w + col + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[e] = a[e];
+      f[4 + e] = b[e];
+    }
+  } else {
+    unpack8<f16>(*(const u32x4*)((const f16*)w + col), f);
+  }
+}
+__device__ __forceinline__ void load_weights(const void* w, int w32, int col, float (&f)[8], bf16) {
+  if (w32)
+    load_weights(w, w32, col, f, f16());
+  else
+    unpack8<bf16>(*(const u32x4*)((const bf16*)w + col), f);
+}
+
+template <typename T>
+__device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
+  typedef T T8 __attribute__((ext_vector_type(8)));
+  T8 x;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = (T)f[e];
+  return __builtin_bit_cast(u32x4, x);
+}
+
+// Combines a value over the TPR threads of a row, in an order that the sizes alone decide. Over more than
+// a wave: through `lds`, which has a float per wave and is used once by each call.
+template <int TPR, typename F>
+__device__ __forceinline__ float combine(float v, float* lds, F&& f) {
+  v = f(v, dpp_mov<0xB1>(v));                       // lanes l ^ 1, l ^ 2
+  v = f(v, dpp_mov<0x4E>(v));
+  v = f(v, dpp_mov<0x141>(v));                      // the other quad of 8 lanes
+  if (TPR >= 16) v = f(v, dpp_mov<0x140>(v));       // the other half of 16
+  if (TPR >= 32) v = f(v, __shfl_xor(v, 16, 64));
+  if (TPR >= 64) v = f(v, __shfl_xor(v, 32, 64));
+  if (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = lds[0];
+#pragma unroll
+    for (int i = 1; i < TPR / 64; ++i) v = f(v, lds[i]);
+  }
+  return v;
+}
+__device__ __forceinline__ float add(float a, float b) { return a + b; }
+// Larger absolute value, by its bits: a NaN is larger than infinity.
+__device__ __forceinline__ float larger(float a, float b) {
+  return __uint_as_float(umax(__float_as_uint(a) & 0x7fffffffu, __float_as_uint(b) & 0x7fffffffu));
+}
+
+enum { OUT16, OUT_I8, OUT_F8 };
+
+template <typename T, int OUT, int TPR, int C>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_kernel(const Norm a) {
+  constexpr int THREADS = TPR > 256 ? TPR : 256, RPB = THREADS / TPR;
+  __shared__ float lds[3][THREADS / 64];
+  const int l = threadIdx.x % TPR;
+  const int row = blockIdx.x * RPB + threadIdx.x / TPR;
+  // rows past the last one: the last one again, up to the stores, so that every lane takes part
+  const int r = min(row, a.rows - 1);
+  const T* x = (const T*)a.x + row_at(a.xs, r, a.rows, a.d1, a.d2);
+  const T* res = a.res ? (const T*)a.res + row_at(a.rs, r, a.rows, a.d1, a.d2) : nullptr;
+  float t[C][8];
+  u32x4 vx[C], vr[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int col = 8 * (l + TPR * c);
+    vx[c] = vr[c] = (u32x4){0, 0, 0, 0};
+    if (col < a.n) {
+      vx[c] = *(const u32x4*)(x + col);
+      if (res) vr[c] = *(const u32x4*)(res + col);
+    }
+  }
+  float ss = 0.0f;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    float f[8];
+    unpack8<T>(vx[c], t[c]);
+    if (res) {
+      unpack8<T>(vr[c], f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t[c][e] += f[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(t[c][e], t[c][e], ss);
+  }
+  ss = combine<TPR>(ss, lds[0], add);
+  float rstd = 1.0f / sqrtf(ss / (float)a.n + a.eps);
+  // bf16 rows of 1e19 and over: the squares' sum ends at 3e38, that of values 2^80 times smaller does not
+  // (eps is nothing beside it). The row's threads all have the same sum, so all go this way.
+  if (!std::is_same_v<T, f16> && !(ss < __builtin_inff())) {
+    ss = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float s = t[c][e] * 0x1p-80f;
+        ss = __builtin_fmaf(s, s, ss);
+      }
+    ss = combine<TPR>(ss, lds[1], add);
+    rstd = 1.0f / sqrtf(ss / (float)a.n) * 0x1p-80f;
+  }
+  const int64_t base = (int64_t)row * a.n;
+  const bool live = row < a.rows;
+  if (live && l == 0 && a.rstd) a.rstd[row] = rstd;
+  float top = 0.0f;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int col = 8 * (l + TPR * c);
+    if (col >= a.n) continue;
+    float w[8];
+    load_weights(a.w, a.w32, col, w, T());
+    if (live && a.sum) *(u32x4*)((T*)a.sum + base + col) = pack8<T>(t[c]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      t[c][e] = t[c][e] * rstd * w[e];
+      if (OUT != OUT16) top = larger(top, t[c][e]);
+    }
+    if (OUT == OUT16 && live) *(u32x4*)((T*)a.y + base + col) = pack8<T>(t[c]);
+  }
+  if (OUT == OUT16) return;
+  top = combine<TPR>(top, lds[2], larger);
+  const float most = OUT == OUT_I8 ? I8_MAX : P_SCALE;
+  const bool finite = top < __builtin_inff();
+  const float scale = fmaxf(__fdiv_rn(top, most), SCALE_FLOOR), inv = __fdiv_rn(1.0f, scale);
+  // a row with a NaN or an infinity: zero codes under a NaN scale, as the cache holds one
+  if (live && l == 0) a.scales[row] = finite ? scale : __builtin_nanf("");
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int col = 8 * (l + TPR * c);
+    if (!live || col >= a.n) continue;
+    float z[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      z[e] = finite ? div_by(t[c][e], scale, inv) : 0.0f;
+      if (OUT == OUT_F8) z[e] = __builtin_amdgcn_fmed3f(z[e], -P_SCALE, P_SCALE);
+    }
+    *(u32x2*)((u8*)a.y + base + col) =
+        OUT == OUT_I8 ? (u32x2){i8x4(z[0], z[1], z[2], z[3]), i8x4(z[4], z[5], z[6], z[7])}
+                      : (u32x2){fp8x4(z[0], z[1], z[2], z[3]), fp8x4(z[4], z[5], z[6], z[7])};
+  }
+}
+
+// Each block takes every gridDim.x-th group of rows, and keeps its columns' share of dw.
+template <typename T, int TPR, int C>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_grad_kernel(const NormGrad a) {
+  constexpr int THREADS = TPR > 256 ? TPR : 256, RPB = THREADS / TPR;
+  __shared__ float lds[2][THREADS / 64];
+  __shared__ float cols[RPB > 1 ? THREADS * 8 * C : 1];
+  const int l = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  float w[C][8], dw[C][8];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int col = 8 * (l + TPR * c);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[c][e] = w[c][e] = 0.0f;
+    if (col < a.n) load_weights(a.w, a.w32, col, w[c], T());
+  }
+  int turn = 0;
+  for (int first = blockIdx.x * RPB; first < a.rows; first += gridDim.x * RPB, turn ^= 1) {
+    const int row = first + sub, r = min(row, a.rows - 1);
+    const bool live = row < a.rows;
+    const T* x = (const T*)a.x + row_at(a.xs, r, a.rows, a.d1, a.d2);
+    const T* dy = (const T*)a.dy + row_at(a.gs, r, a.rows, a.d1, a.d2);
+    const T* ds = a.dsum ? (const T*)a.dsum + row_at(a.ds, r, a.rows, a.d1, a.d2) : nullptr;
+    const float rstd = a.rstd[r];
+    u32x4 vx[C], vg[C], vd[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = 8 * (l + TPR * c);
+      vx[c] = vg[c] = vd[c] = (u32x4){0, 0, 0, 0};
+      if (col < a.n) {
+        vx[c] = *(const u32x4*)(x + col);
+        vg[c] = *(const u32x4*)(dy + col);
+        if (ds) vd[c] = *(const u32x4*)(ds + col);
+      }
+    }
+    float m = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float fx[8], fg[8];
+      unpack8<T>(vx[c], fx);
+      unpack8<T>(vg[c], fg);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float h = fx[e] * rstd;
+        m = __builtin_fmaf(fg[e] * w[c][e], h, m);
+        dw[c][e] += live ? fg[e] * h : 0.0f;
+      }
+    }
+    // (a sum's slots are used again two rows on: a barrier lies between)
+    m = combine<TPR>(m, lds[turn], add) / (float)a.n;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = 8 * (l + TPR * c);
+      if (!live || col >= a.n) continue;
+      float fx[8], fg[8], fd[8], o[8];
+      unpack8<T>(vx[c], fx);
+      unpack8<T>(vg[c], fg);
+      unpack8<T>(vd[c], fd);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        o[e] = rstd * (fg[e] * w[c][e] - fx[e] * rstd * m);
+        if (ds) o[e] += fd[e];
+      }
+      *(u32x4*)((T*)a.dx + (int64_t)row * a.n + col) = pack8<T>(o);
+    }
+  }
+  float* part = a.part + (int64_t)blockIdx.x * a.n;
+  if constexpr (RPB == 1) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = 8 * (l + TPR * c);
+      if (col < a.n) {
+        *(f32x4*)(part + col) = (f32x4){dw[c][0], dw[c][1], dw[c][2], dw[c][3]};
+        *(f32x4*)(part + col + 4) = (f32x4){dw[c][4], dw[c][5], dw[c][6], dw[c][7]};
+      }
+    }
+  } else {
+    // the block's row groups, added in order: column `col` of group s at s * TPR * 8 C + col
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) cols[sub * (TPR * 8 * C) + 8 * (l + TPR * c) + e] = dw[c][e];
+    __syncthreads();
+    for (int col = threadIdx.x; col < a.n; col += THREADS) {
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < RPB; ++i) s += cols[i * (TPR * 8 * C) + col];
+      part[col] = s;
+    }
+  }
+}
+
+// dw: the blocks' shares added, 32 columns a block, in 32 runs and those in order.
+template <typename W>
+__global__ void __launch_bounds__(256) norm_dw_kernel(const float* part, int blocks, int n, W* dw) {
+  __shared__ f32x4 lds[256];
+  const int q = threadIdx.x & 7, run = threadIdx.x >> 3;
+  const int col = blockIdx.x * 32 + 4 * q;
+  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (col < n)
+    for (int b = run; b < blocks; b += 32) s += *(const f32x4*)(part + (int64_t)b * n + col);
+  lds[threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.x < 8 && col < n) {
+#pragma unroll
+    for (int i = 1; i < 32; ++i) s += lds[8 * i + q];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) dw[col + e] = (W)s[e];
+  }
+}
+
+// Calls f(TPR, C) for rows of n values: a group of lanes up to 512, a wave up to 4096 where there are
+// rows for all, blocks otherwise.
+template <typename F>
+hipError_t by_shape(int64_t rows, int64_t n, F&& f) {
+#define SAGE_SHAPE(TPR, C) f(std::integral_constant<int, TPR>(), std::integral_constant<int, C>())
+  if (n <= 64) return SAGE_SHAPE(8, 1);
+  if (n <= 128) return SAGE_SHAPE(16, 1);
+  if (n <= 256) return SAGE_SHAPE(32, 1);
+  if (n <= 512) return SAGE_SHAPE(64, 1);
+  if (n <= 1024) return SAGE_SHAPE(64, 2);
+  if (n <= 2048) return SAGE_SHAPE(256, 1);
+  if (n <= 4096) return SAGE_SHAPE(256, 2);
+  if (n <= 8192) return SAGE_SHAPE(256, 4);
+  if (n <= 16384) return SAGE_SHAPE(1024, 2);
+  return SAGE_SHAPE(1024, 4);
+#undef SAGE_SHAPE
+}
+
+template <typename T, int OUT>
+hipError_t launch_out(const Norm& a, hipStream_t s) {
+  return by_shape(a.rows, a.n, [&](auto tpr, auto c) {
+    constexpr int TPR = tpr.value, THREADS = TPR > 256 ? TPR : 256, RPB = THREADS / TPR;
+    hipLaunchKernelGGL((norm_kernel<T, OUT, TPR, c.value>), dim3((a.rows + RPB - 1) / RPB), dim3(THREADS), 0, s,
+                       a);
+    return hipGetLastError();
+  });
+}
+template <typename T>
+hipError_t launch_norm(const NormArgs& x, const Norm& a, hipStream_t s) {
+  if (x.out == OUT_I8) return launch_out<T, OUT_I8>(a, s);
+  if (x.out == OUT_F8) return launch_out<T, OUT_F8>(a, s);
+  return launch_out<T, OUT16>(a, s);
+}
+
+template <typename T>
+hipError_t launch_grad(const NormGradArgs& x, const NormGrad& a, hipStream_t s) {
+  const int blocks = (int)norm_grad_blocks(a.rows, a.n);
+  hipError_t e = by_shape(a.rows, a.n, [&](auto tpr, auto c) {
+    constexpr int TPR = tpr.value, THREADS = TPR > 256 ? TPR : 256;
+    hipLaunchKernelGGL((norm_grad_kernel<T, TPR, c.value>), dim3(blocks), dim3(THREADS), 0, s, a);
+    return hipGetLastError();
+  });
+  if (e != hipSuccess) return e;
+  const dim3 grid((a.n + 31) / 32);
+  if (a.w32)
+    hipLaunchKernelGGL((norm_dw_kernel<float>), grid, dim3(256), 0, s, a.part, blocks, a.n, (float*)x.dw);
+  else
+    hipLaunchKernelGGL((norm_dw_kernel<T>), grid, dim3(256), 0, s, a.part, blocks, a.n, (T*)x.dw);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t norm_grad_blocks(int64_t rows, int64_t n) {
+  int64_t per = 1;
+  (void)by_shape(rows, n, [&](auto tpr, auto) {
+    per = tpr.value > 256 ? 1 : 256 / tpr.value;
+    return hipSuccess;
+  });
+  const int64_t groups = (rows + per - 1) / per, most = n > 8192 ? 512 : 2048;
+  return groups < most ? groups : most;
+}
+
+hipError_t launch_rms_norm(const NormArgs& x, hipStream_t s) {
+  Norm a = {};
+  a.x = x.x.p;
+  a.res = x.residual.p;
+  a.w = x.w;
+  a.y = x.y;
+  a.scales = x.scales;
+  a.sum = x.sum;
+  a.rstd = x.rstd;
+  for (int i = 0; i < 3; ++i) {
+    a.xs[i] = x.x.s[i];
+    a.rs[i] = x.residual.s[i];
+  }
+  a.rows = (int)x.rows;
+  a.d1 = (int)x.d1;
+  a.d2 = (int)x.d2;
+  a.n = (int)x.n;
+  a.w32 = x.w32;
+  a.eps = x.eps;
+  return x.dtype == 0 ? launch_norm<f16>(x, a, s) : launch_norm<bf16>(x, a, s);
+}
+
+hipError_t launch_rms_norm_grad(const NormGradArgs& x, hipStream_t s) {
+  NormGrad a = {};
+  a.dy = x.dy.p;
+  a.x = x.x.p;
+  a.dsum = x.dsum.p;
+  a.w = x.w;
+  a.rstd = x.rstd;
+  a.dx = x.dx;
+  a.part = (float*)x.workspace;
+  for (int i = 0; i < 3; ++i) {
+    a.gs[i] = x.dy.s[i];
+    a.xs[i] = x.x.s[i];
+    a.ds[i] = x.dsum.s[i];
+  }
+  a.rows = (int)x.rows;
+  a.d1 = (int)x.d1;
+  a.d2 = (int)x.d2;
+  a.n = (int)x.n;
+  a.w32 = x.w32;
+  return x.dtype == 0 ? launch_grad<f16>(x, a, s) : launch_grad<bf16>(x, a, s);
+}
+
+}  // namespace sage

@@ -209,4 +209,35 @@ int64_t attn_bwd_workspace_bytes(const AttnBwdPlan& p, int dtype, int64_t planes
                                  int64_t D);
 hipError_t launch_attn_bwd(const AttnBwdArgs& a, hipStream_t stream);
 
+// Rows of n contiguous values in up to three dimensions, the last of d2 rows, the middle one of d1.
+struct RowsView {
+  const void* p;
+  int64_t s[3];               // strides, outermost first
+};
+struct NormArgs {
+  int dtype, w32, out;        // weights in fp32; out 0: `dtype`, 1: int8, 2: e4m3
+  RowsView x, residual;       // residual.p optional
+  const void* w;
+  int64_t rows, d1, d2, n;
+  float eps;
+  void* y;                    // written, contiguous: y or codes, and scales (rows) with codes;
+  float* scales;
+  void* sum;                  // optional: x + residual,
+  float* rstd;                // and (rows) 1 / root mean square
+};
+hipError_t launch_rms_norm(const NormArgs& a, hipStream_t stream);
+
+struct NormGradArgs {
+  int dtype, w32;
+  RowsView dy, x, dsum;       // dsum.p optional
+  const void* w;
+  const float* rstd;
+  int64_t rows, d1, d2, n;
+  void* dx;
+  void* dw;
+  void* workspace;            // norm_grad_blocks * n floats
+};
+int64_t norm_grad_blocks(int64_t rows, int64_t n);
+hipError_t launch_rms_norm_grad(const NormGradArgs& a, hipStream_t stream);
+
 }  // namespace sage

@@ -185,6 +185,14 @@ class SageLib:
                                     + [f32, vp, ctypes.c_size_t, vp])
         L.sage_attn_bwd_workspace_bytes.restype = i64
         L.sage_attn_bwd_workspace_bytes.argtypes = [i32] * 2 + [i64] * 6
+        rows = [vp, i64, i64, i64]
+        L.sage_rms_norm.restype = i32
+        L.sage_rms_norm.argtypes = [i32] * 3 + rows * 2 + [vp] + [i64] * 4 + [f32] + [vp] * 5
+        L.sage_rms_norm_bwd.restype = i32
+        L.sage_rms_norm_bwd.argtypes = ([i32] * 2 + rows * 3 + [vp, vp] + [i64] * 4
+                                        + [vp] * 3 + [ctypes.c_size_t, vp])
+        L.sage_rms_norm_bwd_workspace_bytes.restype = i64
+        L.sage_rms_norm_bwd_workspace_bytes.argtypes = [i64] * 2
         self.version = int(L.sage_version())
         self.build_id = L.sage_build_id().decode()
         images = hip_runtime_images()
@@ -429,6 +437,34 @@ class SageLib:
             workspace.data_ptr(), workspace.numel(), stream)
         if rc:
             self._check(rc, "sage_attn_bwd")
+
+    # The norm: rows of n values in dims (d0, d1, d2), each tensor with its three strides.
+    def rms_norm(self, x, x_s, residual, r_s, w, dims, n, eps, out, y, scales, total, rstd, stream):
+        """The norm of `x` (+ `residual`) into `y` and the optional outputs (see `sage_rms_norm`)."""
+        rc = self.lib.sage_rms_norm(
+            _dtype_code(x.dtype), int(w.dtype == torch.float32), out, x.data_ptr(), *x_s,
+            None if residual is None else residual.data_ptr(), *r_s, w.data_ptr(), *dims, n, eps,
+            y.data_ptr(), None if scales is None else scales.data_ptr(),
+            None if total is None else total.data_ptr(), None if rstd is None else rstd.data_ptr(), stream)
+        if rc:
+            self._check(rc, "sage_rms_norm")
+
+    @functools.lru_cache(maxsize=4096)
+    def rms_norm_bwd_workspace_bytes(self, rows, n):
+        """Bytes of `sage_rms_norm_bwd`'s workspace, a function of the sizes alone."""
+        size = self.lib.sage_rms_norm_bwd_workspace_bytes(rows, n)
+        if size < 0:
+            self._check(-size, "sage_rms_norm_bwd_workspace_bytes")
+        return size
+
+    def rms_norm_bwd(self, dy, g_s, x, x_s, dsum, s_s, w, rstd, dims, n, dx, dw, workspace, stream):
+        """The norm's gradients into `dx` and `dw` (see `sage_rms_norm_bwd`)."""
+        rc = self.lib.sage_rms_norm_bwd(
+            _dtype_code(x.dtype), int(w.dtype == torch.float32), dy.data_ptr(), *g_s, x.data_ptr(), *x_s,
+            None if dsum is None else dsum.data_ptr(), *s_s, w.data_ptr(), rstd.data_ptr(), *dims, n,
+            dx.data_ptr(), dw.data_ptr(), workspace.data_ptr(), workspace.numel(), stream)
+        if rc:
+            self._check(rc, "sage_rms_norm_bwd")
 
     def quant_q(self, q, sm_scale, *, qk_int8):
         """Q quantized exactly as the main loop quantizes it: `(q8, sq, cq)` on q's device."""
