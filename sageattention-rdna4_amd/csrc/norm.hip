@@ -38,6 +38,7 @@ struct NormGrad {
   float* part;               // (blocks, n)
   int64_t gs[3], xs[3], ds[3];
   int rows, d1, d2, n, w32;
+  float inv_n;
 };
 
 // Element offset of row r; with one dimension alone (d2 = rows) nothing is divided.
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_kernel(const Norm 
     for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(t[c][e], t[c][e], ss);
   }
   ss = combine<TPR>(ss, lds[0], add);
-  float rstd = 1.0f / sqrtf(ss / (float)a.n + a.eps);
+  float rstd = rsqrtf(__fadd_rn(__fdiv_rn(ss, (float)a.n), a.eps));
   // bf16 rows of 1e19 and over: the squares' sum ends at 3e38, that of values 2^80 times smaller does not
   // (eps is nothing beside it). The row's threads all have the same sum, so all go this way.
   if (!std::is_same_v<T, f16> && !(ss < __builtin_inff())) {
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_kernel(const Norm 
         ss = __builtin_fmaf(s, s, ss);
       }
     ss = combine<TPR>(ss, lds[1], add);
-    rstd = 1.0f / sqrtf(ss / (float)a.n) * 0x1p-80f;
+    rstd = rsqrtf(__fdiv_rn(ss, (float)a.n)) * 0x1p-80f;
   }
   const int64_t base = (int64_t)row * a.n;
   const bool live = row < a.rows;
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_grad_kernel(const 
       }
     }
     // (a sum's slots are used again two rows on: a barrier lies between)
-    m = combine<TPR>(m, lds[turn], add) / (float)a.n;
+    m = combine<TPR>(m, lds[turn], add) * a.inv_n;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int col = 8 * (l + TPR * c);
@@ -406,6 +407,7 @@ hipError_t launch_rms_norm_grad(const NormGradArgs& x, hipStream_t s) {
   a.d1 = (int)x.d1;
   a.d2 = (int)x.d2;
   a.n = (int)x.n;
+  a.inv_n = 1.0f / (float)x.n;
   a.w32 = x.w32;
   return x.dtype == 0 ? launch_grad<f16>(x, a, s) : launch_grad<bf16>(x, a, s);
 }
