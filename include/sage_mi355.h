@@ -352,6 +352,7 @@ int64_t sage_cache_attn_workspace_bytes(int64_t B, int64_t H, int64_t H_kv, int6
  *   lse              (B, H, N) fp32: the forward call's, or that of a larger set of keys that these are
  *                    part of (o and dout are then those of the whole); -infinity: the row saw nothing
  *   dlse             optional (B, H, N) fp32: the gradient of lse
+ *   sm_scale         from 1e-30 to 1e30
  *   workspace        sage_attn_bwd_workspace_bytes bytes, 256-byte aligned
  * P and dS are rounded to `dtype` ahead of their products (fp16: scaled by powers of two that keep
  * them in range), every sum is fp32, and the results are rounded once. They are the same from call to

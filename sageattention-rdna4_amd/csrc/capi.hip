@@ -861,8 +861,8 @@ int sage_attn_bwd(int dtype, int causal, const void* q, int64_t q_sb, int64_t q_
   if (!lse) return fail(SAGE_ERR_INVALID, "lse is NULL");
   if (((uintptr_t)lse & 3u) || ((uintptr_t)dlse & 3u))
     return fail(SAGE_ERR_INVALID, "ptr_align: lse and dlse must be 4-byte aligned");
-  if (!(sm_scale > 0.0f) || !(sm_scale < 3.0e38f))
-    return fail(SAGE_ERR_INVALID, "sm_scale: must be positive and finite (got %g)", (double)sm_scale);
+  if (!(sm_scale >= 1e-30f) || !(sm_scale <= 1e30f))   // the logsumexp is divided by it
+    return fail(SAGE_ERR_INVALID, "sm_scale: must lie between 1e-30 and 1e30 (got %g)", (double)sm_scale);
   const int64_t need = sage::attn_bwd_workspace_bytes(
       sage::attn_bwd_plan(B, H, H_kv, N, N_kv, D, causal != 0), dtype, B * H, B * H_kv, D);
   if (workspace == nullptr || workspace_bytes < (size_t)need || ((uintptr_t)workspace & 255u))

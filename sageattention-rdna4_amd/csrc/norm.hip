@@ -209,15 +209,15 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_grad_kernel(const 
     for (int e = 0; e < 8; ++e) dw[c][e] = w[c][e] = 0.0f;
     if (col < a.n) load_weights(a.w, a.w32, col, w[c], T());
   }
-  int turn = 0;
-  for (int first = blockIdx.x * RPB; first < a.rows; first += gridDim.x * RPB, turn ^= 1) {
-    const int row = first + sub, r = min(row, a.rows - 1);
-    const bool live = row < a.rows;
+  // the next rows are requested ahead of the sum over the ones at hand
+  u32x4 vx[C], vg[C], vd[C];
+  float rstd;
+  auto load = [&](int first) {
+    const int r = min(first + sub, a.rows - 1);
     const T* x = (const T*)a.x + row_at(a.xs, r, a.rows, a.d1, a.d2);
     const T* dy = (const T*)a.dy + row_at(a.gs, r, a.rows, a.d1, a.d2);
     const T* ds = a.dsum ? (const T*)a.dsum + row_at(a.ds, r, a.rows, a.d1, a.d2) : nullptr;
-    const float rstd = a.rstd[r];
-    u32x4 vx[C], vg[C], vd[C];
+    rstd = a.rstd[r];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int col = 8 * (l + TPR * c);
@@ -228,15 +228,30 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_grad_kernel(const 
         if (ds) vd[c] = *(const u32x4*)(ds + col);
       }
     }
+  };
+  int turn = 0;
+  load(blockIdx.x * RPB);
+  for (int first = blockIdx.x * RPB; first < a.rows; first += gridDim.x * RPB, turn ^= 1) {
+    const int row = first + sub;
+    const bool live = row < a.rows;
+    u32x4 x[C], g[C], d[C];
+    const float r = rstd;
     float m = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
+      x[c] = vx[c];
+      g[c] = vg[c];
+      d[c] = vd[c];
+    }
+    if (first + gridDim.x * RPB < a.rows) load(first + gridDim.x * RPB);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
       float fx[8], fg[8];
-      unpack8<T>(vx[c], fx);
-      unpack8<T>(vg[c], fg);
+      unpack8<T>(x[c], fx);
+      unpack8<T>(g[c], fg);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float h = fx[e] * rstd;
+        const float h = fx[e] * r;
         m = __builtin_fmaf(fg[e] * w[c][e], h, m);
         dw[c][e] += live ? fg[e] * h : 0.0f;
       }
@@ -248,13 +263,13 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_grad_kernel(const 
       const int col = 8 * (l + TPR * c);
       if (!live || col >= a.n) continue;
       float fx[8], fg[8], fd[8], o[8];
-      unpack8<T>(vx[c], fx);
-      unpack8<T>(vg[c], fg);
-      unpack8<T>(vd[c], fd);
+      unpack8<T>(x[c], fx);
+      unpack8<T>(g[c], fg);
+      unpack8<T>(d[c], fd);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        o[e] = rstd * (fg[e] * w[c][e] - fx[e] * rstd * m);
-        if (ds) o[e] += fd[e];
+        o[e] = r * (fg[e] * w[c][e] - fx[e] * r * m);
+        if (a.dsum) o[e] += fd[e];
       }
       *(u32x4*)((T*)a.dx + (int64_t)row * a.n + col) = pack8<T>(o);
     }
@@ -285,27 +300,40 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_grad_kernel(const 
   }
 }
 
-// dw: the blocks' shares added, 32 columns a block, in 32 runs and those in order.
+// dw: the blocks' shares added, 32 columns a block, in 128 runs and those four by four in order.
 template <typename W>
-__global__ void __launch_bounds__(256) norm_dw_kernel(const float* part, int blocks, int n, W* dw) {
-  __shared__ f32x4 lds[256];
+__global__ void __launch_bounds__(1024) norm_dw_kernel(const float* part, int blocks, int n, W* dw) {
+  __shared__ f32x4 lds[1024];
   const int q = threadIdx.x & 7, run = threadIdx.x >> 3;
   const int col = blockIdx.x * 32 + 4 * q;
   f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (col < n)
-    for (int b = run; b < blocks; b += 32) s += *(const f32x4*)(part + (int64_t)b * n + col);
-  lds[threadIdx.x] = s;
+  if (col < n) {
+#pragma unroll 4
+    for (int b = run; b < blocks; b += 128) s += *(const f32x4*)(part + (int64_t)b * n + col);
+  }
+#pragma unroll
+  for (int left = 128; left > 2; left /= 4) {
+    if (run < left) lds[threadIdx.x] = s;
+    __syncthreads();
+    if (run < left / 4) {
+#pragma unroll
+      for (int i = 1; i < 4; ++i) s += lds[threadIdx.x + 8 * i * (left / 4)];
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x < 16) lds[threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.x < 8 && col < n) {
-#pragma unroll
-    for (int i = 1; i < 32; ++i) s += lds[8 * i + q];
+    s += lds[threadIdx.x + 8];
 #pragma unroll
     for (int e = 0; e < 4; ++e) dw[col + e] = (W)s[e];
   }
 }
 
-// Calls f(TPR, C) for rows of n values: a group of lanes up to 512, a wave up to 4096 where there are
-// rows for all, blocks otherwise.
+// Calls f(TPR, C) for rows of n values: a group of lanes for up to 512, a wave for up to 1024, a block of 256
+// threads for up to 8192, of 1024 for more. Also for fewer where there are so few rows that the card
+// holds all their blocks at once: 64 rows of 4096 3.7 us and 4.1 with 256 threads, 16 rows of 6144 to codes
+// 4.1 and 5.4.
 template <typename F>
 hipError_t by_shape(int64_t rows, int64_t n, F&& f) {
 #define SAGE_SHAPE(TPR, C) f(std::integral_constant<int, TPR>(), std::integral_constant<int, C>())
@@ -315,6 +343,7 @@ hipError_t by_shape(int64_t rows, int64_t n, F&& f) {
   if (n <= 512) return SAGE_SHAPE(64, 1);
   if (n <= 1024) return SAGE_SHAPE(64, 2);
   if (n <= 2048) return SAGE_SHAPE(256, 1);
+  if (rows <= 512 && n <= 8192) return SAGE_SHAPE(1024, 1);
   if (n <= 4096) return SAGE_SHAPE(256, 2);
   if (n <= 8192) return SAGE_SHAPE(256, 4);
   if (n <= 16384) return SAGE_SHAPE(1024, 2);
@@ -349,21 +378,24 @@ hipError_t launch_grad(const NormGradArgs& x, const NormGrad& a, hipStream_t s) 
   if (e != hipSuccess) return e;
   const dim3 grid((a.n + 31) / 32);
   if (a.w32)
-    hipLaunchKernelGGL((norm_dw_kernel<float>), grid, dim3(256), 0, s, a.part, blocks, a.n, (float*)x.dw);
+    hipLaunchKernelGGL((norm_dw_kernel<float>), grid, dim3(1024), 0, s, a.part, blocks, a.n, (float*)x.dw);
   else
-    hipLaunchKernelGGL((norm_dw_kernel<T>), grid, dim3(256), 0, s, a.part, blocks, a.n, (T*)x.dw);
+    hipLaunchKernelGGL((norm_dw_kernel<T>), grid, dim3(1024), 0, s, a.part, blocks, a.n, (T*)x.dw);
   return hipGetLastError();
 }
 
 }  // namespace
 
+// Two blocks for each compute unit; four where a block holds several rows and its share of dw is small.
+// Measured with 512, 768, 1024, 2048 blocks: 16384 rows of 4096 107, 114, 127, 124 us (the shares are
+// written and read again), 204000 rows of 128 42.8, 39.8, 38.0, 40.2 us.
 int64_t norm_grad_blocks(int64_t rows, int64_t n) {
   int64_t per = 1;
   (void)by_shape(rows, n, [&](auto tpr, auto) {
     per = tpr.value > 256 ? 1 : 256 / tpr.value;
     return hipSuccess;
   });
-  const int64_t groups = (rows + per - 1) / per, most = n > 8192 ? 512 : 2048;
+  const int64_t groups = (rows + per - 1) / per, most = n > 1024 ? 512 : 1024;
   return groups < most ? groups : most;
 }
 

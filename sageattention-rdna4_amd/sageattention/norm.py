@@ -21,17 +21,19 @@ _NONE = (0, 0, 0)
 def _layout(what, tensors):
     """The row dimensions (d0, d1, d2) that the tensors, all of one shape, have in common, and each one's
     strides in them."""
-    names, tensors = zip(*tensors)
-    shape = tensors[0].shape
-    for name, t in zip(names, tensors):
-        if t.stride(-1) != 1 and shape[-1] > 1:
-            _refuse(what, "stride_last: %s must have contiguous rows" % name)
+    shape = tensors[0][1].shape
+    together = True
+    for name, t in tensors:
         if t.data_ptr() & 15:
             _refuse(what, "ptr_align: %s must be 16-byte aligned" % name)
-    if all(t.is_contiguous() for t in tensors):
-        n = shape[-1]
-        rows = tensors[0].numel() // n
-        return (1, 1, rows), [(0, 0, n)] * len(tensors)
+        if not t.is_contiguous():
+            together = False
+            if t.stride(-1) != 1:
+                _refuse(what, "stride_last: %s must have contiguous rows" % name)
+    n = shape[-1]
+    if together:
+        return (1, 1, tensors[0][1].numel() // n), [(0, 0, n)] * len(tensors)
+    names, tensors = zip(*tensors)
     dims, strides = [], [[] for _ in tensors]
     for i, size in enumerate(shape[:-1]):
         if size == 1:
@@ -60,26 +62,35 @@ def _check(what, x, weight, others):
         _refuse(what, "device: x must be a tensor on the GPU")
     if x.dtype not in _DTYPES:
         _refuse(what, "dtype: x is %s (fp16 and bf16 are served)" % x.dtype)
-    if x.dim() < 1 or x.shape[-1] % 8 or not 8 <= x.shape[-1] <= 32768:
+    shape, dev = x.shape, x.device
+    n = shape[-1] if shape else 0
+    if n % 8 or not 8 <= n <= 32768:
         _refuse(what, "row: x is %s (rows of a multiple of 8 values up to 32768 are served)" % (
-            tuple(x.shape),))
-    if not isinstance(weight, torch.Tensor) or weight.device != x.device:
-        _refuse(what, "device: weight must be a tensor on %s" % x.device)
+            tuple(shape),))
+    if not isinstance(weight, torch.Tensor) or weight.device != dev:
+        _refuse(what, "device: weight must be a tensor on %s" % dev)
     if weight.dtype not in (x.dtype, torch.float32):
         _refuse(what, "dtype: weight is %s (x's %s and float32 are served)" % (weight.dtype, x.dtype))
-    if weight.shape != x.shape[-1:]:
-        _refuse(what, "shape: weight is %s, not %s" % (tuple(weight.shape), tuple(x.shape[-1:])))
+    if weight.shape != shape[-1:]:
+        _refuse(what, "shape: weight is %s, not %s" % (tuple(weight.shape), tuple(shape[-1:])))
     if not weight.is_contiguous():
         _refuse(what, "stride_last: weight must be contiguous")
     if weight.data_ptr() & 15:
         _refuse(what, "ptr_align: weight must be 16-byte aligned")
     for name, t in others:
-        if not isinstance(t, torch.Tensor) or t.device != x.device:
-            _refuse(what, "device: %s must be a tensor on %s" % (name, x.device))
+        if not isinstance(t, torch.Tensor) or t.device != dev:
+            _refuse(what, "device: %s must be a tensor on %s" % (name, dev))
         if t.dtype != x.dtype:
             _refuse(what, "dtype: %s is %s, x %s" % (name, t.dtype, x.dtype))
-        if t.shape != x.shape:
-            _refuse(what, "shape: %s is %s, x %s" % (name, tuple(t.shape), tuple(x.shape)))
+        if t.shape != shape:
+            _refuse(what, "shape: %s is %s, x %s" % (name, tuple(t.shape), tuple(shape)))
+
+
+def _new(x, dtype, whole):
+    """A new contiguous tensor of x's shape, or of a value per row."""
+    if whole and x.is_contiguous() and dtype is x.dtype:
+        return torch.empty_like(x)
+    return torch.empty(x.shape if whole else x.shape[:-1], dtype=dtype, device=x.device)
 
 
 def _norm(what, x, weight, eps, residual, out, keep_rstd):
@@ -89,11 +100,11 @@ def _norm(what, x, weight, eps, residual, out, keep_rstd):
     eps = float(eps)
     if not 0.0 <= eps < math.inf:
         _refuse(what, "eps: must be finite and not negative (got %r)" % (eps,))
-    dev, rows = x.device, x.shape[:-1]
-    y = torch.empty(x.shape, dtype=(x.dtype, torch.int8, torch.float8_e4m3fn)[out], device=dev)
-    scales = torch.empty(rows, dtype=torch.float32, device=dev) if out else None
-    total = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-    rstd = torch.empty(rows, dtype=torch.float32, device=dev) if keep_rstd else None
+    dev, dtype = x.device, x.dtype
+    y = _new(x, (dtype, torch.int8, torch.float8_e4m3fn)[out], True)
+    scales = _new(x, torch.float32, False) if out else None
+    total = None if residual is None else _new(x, dtype, True)
+    rstd = _new(x, torch.float32, False) if keep_rstd else None
     lib = _library(what, dev)
     if x.numel():
         dims, strides = _layout(what, [("x", x)] + others)
@@ -133,8 +144,9 @@ def rms_norm(x, weight, eps=1e-6, residual=None, return_rstd=False):
     residual need a gradient. `return_rstd` appends 1 / sqrt(...) of each row (fp32, x's shape without
     the last dimension), for `rms_norm_backward`; such a call is not recorded.
     """
-    if not return_rstd and torch.is_grad_enabled() and any(
-            isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, residual)):
+    if not return_rstd and torch.is_grad_enabled() and (
+            getattr(x, "requires_grad", False) or getattr(weight, "requires_grad", False)
+            or getattr(residual, "requires_grad", False)):
         return _RmsNorm.apply(x, weight, eps, residual)
     y, _, total, rstd = _norm("rms_norm", x, weight, eps, residual, 0, return_rstd)
     done = (y,) if residual is None else (y, total)
@@ -173,7 +185,7 @@ def rms_norm_backward(dy, x, weight, rstd, dsum=None):
     if rstd.dtype != torch.float32 or rstd.shape != x.shape[:-1] or not rstd.is_contiguous():
         _refuse(what, "rstd: a contiguous float32 tensor of shape %s is needed" % (tuple(x.shape[:-1]),))
     lib = _library(what, dev)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dx = _new(x, x.dtype, True)
     if not x.numel():
         return dx, torch.zeros_like(weight)
     dw = torch.empty_like(weight)

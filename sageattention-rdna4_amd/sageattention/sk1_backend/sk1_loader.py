@@ -422,18 +422,16 @@ class SageLib:
             self._check(-n, "sage_attn_bwd_workspace_bytes")
         return n
 
-    def attn_bwd(self, q, k, v, o, dout, lse, dlse, dq, dk, dv, causal, sm_scale, workspace, stream):
-        """The gradients of `q`, `k`, `v` into `dq`, `dk`, `dv` (see `sage_attn_bwd`)."""
-        B, H, N, D = q.shape
-        _, H_kv, N_kv, _ = k.shape
-        args = []
-        for t in (q, k, v, o, dout):
-            args += (t.data_ptr(),) + t.stride()[:3]
-        args += (lse.data_ptr(), None if dlse is None else dlse.data_ptr())
-        for t in (dq, dk, dv):
-            args += (t.data_ptr(),) + t.stride()[:3]
+    def attn_bwd(self, dtype, causal, read, grads, nhd, lse, dlse, sizes, sm_scale, workspace, stream):
+        """The gradients of q, k, v into `grads` from `read` = (q, k, v, out, dout), (B, H, N, D) tensors
+        or with `nhd` (B, N, H, D) ones; `sizes` = (B, H, N, H_kv, N_kv, D) (see `sage_attn_bwd`)."""
+        views = []
+        for t in read + grads:
+            sb, s1, s2, _ = t.stride()
+            views += (t.data_ptr(), sb, s2, s1) if nhd else (t.data_ptr(), sb, s1, s2)
         rc = self.lib.sage_attn_bwd(
-            _dtype_code(q.dtype), int(bool(causal)), *args, B, H, N, H_kv, N_kv, D, sm_scale,
+            _dtype_code(dtype), int(bool(causal)), *views[:20], lse.data_ptr(),
+            None if dlse is None else dlse.data_ptr(), *views[20:], *sizes, sm_scale,
             workspace.data_ptr(), workspace.numel(), stream)
         if rc:
             self._check(rc, "sage_attn_bwd")

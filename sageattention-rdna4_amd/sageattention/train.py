@@ -9,12 +9,13 @@ forward call's 8-bit codes are not kept), takes two or three launches on the cur
 synchronizes nothing, so that it can be captured into a graph. A call that is not served raises
 `ValueError` with the reason.
 """
-import math
-
 import torch
 
-from .cache import _launch, _library, _refuse, _view
+from .cache import _DTYPES, _HEAD_DIMS, _empty, _launch, _library, _refuse, _view
 from .core import sageattn
+
+#: what the scores' factor may be (a logsumexp is divided by it)
+_LEAST_SCALE = 1e-30
 
 
 def _row_floats(what, name, t, shape, device):
@@ -23,10 +24,24 @@ def _row_floats(what, name, t, shape, device):
         _refuse(what, "device: %s must be a tensor on %s" % (name, device))
     if t.dtype != torch.float32:
         _refuse(what, "dtype: %s must be float32 (got %s)" % (name, t.dtype))
-    if tuple(t.shape) != tuple(shape):
-        _refuse(what, "shape: %s is %s, not %s" % (name, tuple(t.shape), tuple(shape)))
+    if t.shape != shape:
+        _refuse(what, "shape: %s is %s, not %s" % (name, tuple(t.shape), shape))
     if not t.is_contiguous():
         _refuse(what, "stride_last: %s must be contiguous" % name)
+
+
+def _plain(tensors, tensor_layout):
+    """Whether all are contiguous GPU tensors of a served dtype and head_dim, which need no closer look."""
+    if tensor_layout != "HND" and tensor_layout != "NHD":
+        return False
+    for t in tensors:
+        if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES or not t.is_cuda \
+                or not t.is_contiguous() or t.data_ptr() & 15:
+            return False
+        shape = t.shape
+        if len(shape) != 4 or shape[3] not in _HEAD_DIMS or not t.numel():
+            return False
+    return True
 
 
 def sageattn_backward(dout, q, k, v, out, lse, tensor_layout="HND", is_causal=False, sm_scale=None,
@@ -44,24 +59,27 @@ def sageattn_backward(dout, q, k, v, out, lse, tensor_layout="HND", is_causal=Fa
     those of a padded batch's unused rows too: 0 times a NaN or an infinity is NaN.
     """
     what = "sageattn_backward"
-    views = [_view(what, tensor_layout, name, t) for name, t in
-             (("q", q), ("k", k), ("v", v), ("out", out), ("dout", dout))]
-    qq, kk, vv, oo, gg = views
-    dev, dtype = q.device, q.dtype
+    read = (q, k, v, out, dout)
+    if not _plain(read, tensor_layout):
+        for name, t in zip(("q", "k", "v", "out", "dout"), read):
+            _view(what, tensor_layout, name, t)
+    dev, dtype, shape = q.device, q.dtype, q.shape
     for name, t in (("k", k), ("v", v), ("out", out), ("dout", dout)):
         if t.device != dev:
             _refuse(what, "device: %s is on %s, q on %s" % (name, t.device, dev))
         if t.dtype != dtype:
             _refuse(what, "dtype: %s is %s, q %s" % (name, t.dtype, dtype))
-    B, H, N, D = qq.shape
-    H_kv, N_kv = kk.shape[1], kk.shape[2]
-    if kk.shape != vv.shape:
+    if k.shape != v.shape:
         _refuse(what, "shape: k is %s, v %s" % (tuple(k.shape), tuple(v.shape)))
     for name, t in (("out", out), ("dout", dout)):
-        if t.shape != q.shape:
-            _refuse(what, "shape: %s is %s, q %s" % (name, tuple(t.shape), tuple(q.shape)))
-    if kk.shape[0] != B or kk.shape[3] != D:
-        _refuse(what, "shape: k is %s, q %s" % (tuple(k.shape), tuple(q.shape)))
+        if t.shape != shape:
+            _refuse(what, "shape: %s is %s, q %s" % (name, tuple(t.shape), tuple(shape)))
+    if tensor_layout == "HND":
+        (B, H, N, D), (B_kv, H_kv, N_kv, D_kv) = shape, k.shape
+    else:
+        (B, N, H, D), (B_kv, N_kv, H_kv, D_kv) = shape, k.shape
+    if B_kv != B or D_kv != D:
+        _refuse(what, "shape: k is %s, q %s" % (tuple(k.shape), tuple(shape)))
     if H % H_kv:
         _refuse(what, "heads: %d query heads on %d K/V heads" % (H, H_kv))
     if is_causal and N != N_kv:
@@ -70,15 +88,15 @@ def sageattn_backward(dout, q, k, v, out, lse, tensor_layout="HND", is_causal=Fa
     if dlse is not None:
         _row_floats(what, "dlse", dlse, (B, H, N), dev)
     sm = D ** -0.5 if sm_scale is None else float(sm_scale)
-    if not 0.0 < sm < math.inf:
-        _refuse(what, "sm_scale: must be positive and finite (got %r)" % (sm_scale,))
+    if not _LEAST_SCALE <= sm <= 1 / _LEAST_SCALE:
+        _refuse(what, "sm_scale: must lie between 1e-30 and 1e30 (got %r)" % (sm_scale,))
     lib = _library(what, dev)
-    grads = [t.new_empty(t.shape) for t in (q, k, v)]
-    into = grads if tensor_layout == "HND" else [t.transpose(1, 2) for t in grads]
+    grads = tuple([_empty(t) for t in (q, k, v)])
     work = torch.empty(lib.attn_bwd_workspace_bytes(dtype, bool(is_causal), B, H, N, H_kv, N_kv, D),
                        dtype=torch.uint8, device=dev)
-    _launch(dev, lib.attn_bwd, qq, kk, vv, oo, gg, lse, dlse, *into, is_causal, sm, work)
-    return tuple(grads)
+    _launch(dev, lib.attn_bwd, dtype, is_causal, read, grads, tensor_layout == "NHD", lse, dlse,
+            (B, H, N, H_kv, N_kv, D), sm, work)
+    return grads
 
 
 class _Attention(torch.autograd.Function):
