@@ -380,7 +380,7 @@ int64_t sage_attn_bwd_workspace_bytes(int dtype, int causal, int64_t B, int64_t 
  * In fp32: t = x + residual, r = 1 / sqrt(mean t^2 + eps), y = t r w, rounded once.
  *   x, residual  rows of `dtype`, 16-byte aligned, strides (outermost first) multiples of 8 elements; residual
  *                optional
- *   n            a multiple of 8 up to 32768
+ *   n            a multiple of 8 up to 16384
  *   w            (n) of `dtype`, or fp32 with w_fp32; 16-byte aligned
  *   out          0: y in `dtype`; codes with a scale per row by the prologue's scheme (scale =
  *                max(max|y| / 127 or 448, 1e-12), y / scale rounded half to even): 1 int8, 2 e4m3. A row that

@@ -62,8 +62,8 @@ __device__ __forceinline__ bf16x4 read_tr(const bf16* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)p);
 }
 
-constexpr int BC = 128;                // columns (keys, or queries) that a block owns: 32 a wave
-constexpr int BT = 64;                 // rows of the other side in an LDS tile
+constexpr int BC = ATTN_BWD_COLUMNS;   // columns (keys, or queries) that a block owns: 32 a wave
+constexpr int BT = ATTN_BWD_ROWS;      // rows of the other side in an LDS tile
 // Halves of a tile in the loop's code.
 template <int D>
 constexpr int U = D == 64 ? 2 : 1;
@@ -105,7 +105,7 @@ struct Args {
   const float* dlse;
   int H, H_kv, G, N, N_kv, NP;         // NP: N rounded up to tiles
   int planes_q, planes_kv, nb_q, nb_kv; // planes; tiles of 64 rows in each
-  int k_tiles, q_tiles, k_split, q_split, k_blocks;
+  AttnBwdCut keys, queries;
   float sm_scale, c;
   // workspace
   float* nl;        // (planes_q, NP): (P_SHIFT - lse log2 e) / c
@@ -113,9 +113,9 @@ struct Args {
   float* max_do;    // fp16: (planes_q, nb_q): a tile's largest |dout|^2, |d|, and (planes_kv, nb_kv) |v|^2
   float* max_d;
   float* max_v;
-  float* part_k;    // (k_split, planes_kv, k_tiles BC, D) sums of dK, of dV, where k_split > 1
+  float* part_k;    // (keys.cut_blocks, BC, D): sums of dK, of dV, by blocks that hold a part of their tile
   float* part_v;
-  float* part_q;    // (q_split, planes_q, q_tiles BC, D)
+  float* part_q;    // (queries.cut_blocks, BC, D)
 };
 
 template <typename T>
@@ -243,27 +243,24 @@ struct Staging {
   static constexpr int CPR = D / 8, RPI = 64 / CPR, IT = 16 / RPI;
   int lane, w;
   __device__ __forceinline__ Staging(int lane, int w) : lane(lane), w(w) {}
-  // Rows from r0 on (`x`: row 0) to LDS address `lds`. Rows from n on are row n - 1 again: what they would
-  // add is multiplied by P = 0.
-  __device__ __forceinline__ void operator()(const T* x, int64_t sr, int r0, int n, uint32_t lds) const {
+  // The tile from `x` on, of which `left` rows or more are the plane's, to LDS address `lds`. Rows behind the
+  // last one are that one again: what they would add is multiplied by P = 0.
+  __device__ __forceinline__ void operator()(const T* x, int64_t sr, int left, uint32_t lds) const {
     const int l = D == 128 ? lane_anew() : lane;
     const int step = (int)(2 * sr), own = l / CPR;
     const int chunk = 16 * ((l % CPR) ^ swz<D>(own));
-    const T* base = x + (int64_t)(r0 + 16 * w) * sr;
     lds = __builtin_amdgcn_readfirstlane(lds + 16 * w * D * 2);
     // (At head_dim 128 the branch costs more than the clamps: 7.20 ms for 6.94, 32 heads of 16384.)
-    if (D == 64 && r0 + BT <= n) {
+    if (D == 64 && left >= BT) {
+      const T* base = x + 16 * w * sr;
       const int at = own * step;
 #pragma unroll
       for (int i = 0; i < IT; ++i)
-        dma16(base + (int64_t)(RPI * i) * sr, (uint32_t)(at + (chunk ^ 16 * swz<D>(RPI * i))),
-              lds + RPI * i * D * 2);
+        dma16(base + RPI * i * sr, (uint32_t)(at + (chunk ^ 16 * swz<D>(RPI * i))), lds + RPI * i * D * 2);
     } else {
-      base = x + (int64_t)r0 * sr;
-      const int last = n - 1 - r0;
 #pragma unroll
       for (int i = 0; i < IT; ++i)
-        dma16(base, (uint32_t)(min(16 * w + RPI * i + own, last) * step + (chunk ^ 16 * swz<D>(RPI * i))),
+        dma16(x, (uint32_t)(min(16 * w + RPI * i + own, left - 1) * step + (chunk ^ 16 * swz<D>(RPI * i))),
               lds + RPI * i * D * 2);
     }
   }
@@ -317,17 +314,18 @@ __device__ __forceinline__ void load_columns(const T* x, int64_t sr, int r0, int
   for (int s = 0; s < D / 16; ++s) f[s] = *(const typename Vec<T>::x8*)(p + 16 * s);
 }
 
-// A wave's sums, 32 columns of D values each, times f, into rows from r0 on of a 16-bit view or of fp32
-// parts.
+// A wave's sums, 32 columns of D values each, times f, into rows of a 16-bit view from r0 + 32 w on (up to
+// n), or of the block's fp32 part.
 template <typename T, int D>
 __device__ __forceinline__ void store_columns(const f32x16 (&acc)[D / 32], float f, const Out& o, int b,
-                                              int h, float* part, int r0, int n) {
+                                              int h, float* part, int r0, int w, int n) {
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) keep_live(acc[dt]);
-  const int lane = lane_anew(), r = r0 + (lane & 31), col = 4 * (lane >> 5);
+  mfma_result_fence32();
+  const int lane = lane_anew(), own = 32 * w + (lane & 31), r = r0 + own, col = 4 * (lane >> 5);
   if (r >= n) return;
   if (part) {
-    float* p = part + (int64_t)r * D + col;
+    float* p = part + own * D + col;
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -390,14 +388,13 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
   typedef typename Vec<T>::x8 x8;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 5;
-  const int pl = block % a.planes_kv, ts = block / a.planes_kv;
-  const int tile = ts / a.k_split, sp = ts - tile * a.k_split;
-  const int b = pl / a.H_kv, hk = pl - b * a.H_kv;
-  const int k0 = tile * BC, kw = k0 + 32 * w;
+  const AttnBwdPlace at = attn_bwd_place(a.keys, block, a.planes_kv);
+  const int pl = at.plane, b = pl / a.H_kv, hk = pl - b * a.H_kv;
+  const int k0 = at.u * BC, kw = k0 + 32 * w;
   // tiles of queries, head after head of the group
   const int first = CAUSAL ? k0 / BT : 0, per = a.nb_q - first;
   const int n = per * a.G;
-  const int it0 = (int)((int64_t)n * sp / a.k_split), it1 = (int)((int64_t)n * (sp + 1) / a.k_split);
+  const int it0 = at.first(n), it1 = at.end(n);
 
   float scale = 1.0f;
   if (F16) {
@@ -414,18 +411,28 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
   const float* lds_rows = (const float*)(smem + 4 * TILE);
   const uint32_t lds0 = lds_addr(smem);
   const Staging<T, D> stage(lane, w);
-  int gi = it0 / per, ti = first + it0 - gi * per;   // of the next tile to be requested
+  // the next tile to be requested, ti of its head, and where it lies
+  int ti = it0 / per;
+  const int h0 = hk * a.G + ti;
+  ti = first + it0 - ti * per;
+  const T* pq = plane<T>(a.q, b, h0) + (int64_t)ti * BT * a.q.sr;
+  const T* po = plane<T>(a.dout, b, h0) + (int64_t)ti * BT * a.dout.sr;
+  const float* pr = (w & 1 ? a.nd : a.nl) + (int64_t)(b * a.H + h0) * a.NP + ti * BT;
+  const int64_t head_q = a.q.sh - (int64_t)per * BT * a.q.sr;
+  const int64_t head_o = a.dout.sh - (int64_t)per * BT * a.dout.sr;
   auto request = [&](int buf) {
-    const int h = hk * a.G + gi, q0 = ti * BT;
-    stage(plane<T>(a.q, b, h), a.q.sr, q0, a.N, lds0 + buf * TILE);
-    stage(plane<T>(a.dout, b, h), a.dout.sr, q0, a.N, lds0 + (2 + buf) * TILE);
-    const int64_t row = (int64_t)(b * a.H + h) * a.NP + q0;
-    if (w < 2)
-      dma4((w ? a.nd : a.nl) + row, 4 * lane_anew(),
-           lds0 + 4 * TILE + (2 * buf + w) * BT * 4);
-    if (++ti == a.nb_q) {
+    const int left = a.N - ti * BT;
+    stage(pq, a.q.sr, left, lds0 + buf * TILE);
+    stage(po, a.dout.sr, left, lds0 + (2 + buf) * TILE);
+    if (w < 2) dma4(pr, 4 * lane_anew(), lds0 + 4 * TILE + (2 * buf + w) * BT * 4);
+    pq += BT * a.q.sr;
+    po += BT * a.dout.sr;
+    pr += BT;
+    if (++ti == a.nb_q) {                            // on to the group's next head
       ti = first;
-      ++gi;
+      pq += head_q;
+      po += head_o;
+      pr += first * BT;
     }
   };
 
@@ -455,12 +462,17 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
     fence<D, CAUSAL>();
     dp = row_constants(rows + BT);
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) dp = mfma16(row_operand<T>(smem, of.row, at_do, i), vf[i], dp);
+    for (int i = 0; i < D / 16; ++i) {
+      dp = mfma16(row_operand<T>(smem, of.row, at_do, i), vf[i], dp);
+      // P, between dP's products: the matrix unit and the others work at once
+#pragma unroll
+      for (int r = 256 / D * i; r < 256 / D * (i + 1); ++r) s[r] = __builtin_amdgcn_exp2f(s[r] * a.c);
+    }
     fence<D, CAUSAL>();
     x8 pf[2], df[2];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      float p = __builtin_amdgcn_exp2f(s[r] * a.c);
+      float p = s[r];
       pf[r / 8][r % 8] = (T)p;
       if (F16) p *= fs;
       df[r / 8][r % 8] = (T)(p * dp[r]);
@@ -496,11 +508,11 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
   } else {
     for (int it = it0; it < it1; ++it) tile_of(it, (it - it0) & 1);
   }
-  const int64_t part = ((int64_t)sp * a.planes_kv + pl) * a.k_tiles * BC * D;
-  store_columns<T, D>(dk, a.sm_scale / scale, a.dk, b, hk, a.k_split > 1 ? a.part_k + part : nullptr, kw,
-                      a.N_kv);
+  const bool whole = at.parts == 1;
+  const int64_t part = (int64_t)block * BC * D;
+  store_columns<T, D>(dk, a.sm_scale / scale, a.dk, b, hk, whole ? nullptr : a.part_k + part, k0, w, a.N_kv);
   store_columns<T, D>(dv, __builtin_ldexpf(1.0f, -(int)P_SHIFT<T>), a.dv, b, hk,
-                      a.k_split > 1 ? a.part_v + part : nullptr, kw, a.N_kv);
+                      whole ? nullptr : a.part_v + part, k0, w, a.N_kv);
 }
 
 // A block that owns 128 queries of a head.
@@ -510,13 +522,12 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
   constexpr bool F16 = std::is_same_v<T, f16>;
   typedef typename Vec<T>::x8 x8;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int pl = block % a.planes_q, ts = block / a.planes_q;
-  // the longest tiles, the last of a causal plane, begin first
-  const int tile = a.q_tiles - 1 - ts / a.q_split, sp = ts % a.q_split;
-  const int b = pl / a.H, h = pl - b * a.H, hk = h / a.G;
-  const int q0 = tile * BC, qw = q0 + 32 * w;
+  const AttnBwdPlace at = attn_bwd_place(a.queries, block, a.planes_q);
+  const int pl = at.plane, b = pl / a.H, h = pl - b * a.H, hk = h / a.G;
+  // the last tile of a causal plane is its longest
+  const int q0 = (a.queries.tiles - 1 - at.u) * BC, qw = q0 + 32 * w;
   const int n = CAUSAL ? min((q0 + BC) / BT, a.nb_kv) : a.nb_kv;
-  const int it0 = (int)((int64_t)n * sp / a.q_split), it1 = (int)((int64_t)n * (sp + 1) / a.q_split);
+  const int it0 = at.first(n), it1 = at.end(n);
 
   float mv = 0.0f;
   if (F16) {
@@ -525,12 +536,15 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
   }
   // LDS: two tiles of K, two of V
   const uint32_t lds0 = lds_addr(smem);
-  const T* pk = plane<T>(a.k, b, hk);
-  const T* pv = plane<T>(a.v, b, hk);
+  const T* pk = plane<T>(a.k, b, hk) + (int64_t)it0 * BT * a.k.sr;
+  const T* pv = plane<T>(a.v, b, hk) + (int64_t)it0 * BT * a.v.sr;
   const Staging<T, D> stage(lane, w);
   auto request = [&](int it, int buf) {
-    stage(pk, a.k.sr, it * BT, a.N_kv, lds0 + buf * TILE);
-    stage(pv, a.v.sr, it * BT, a.N_kv, lds0 + (2 + buf) * TILE);
+    const int left = a.N_kv - it * BT;
+    stage(pk, a.k.sr, left, lds0 + buf * TILE);
+    stage(pv, a.v.sr, left, lds0 + (2 + buf) * TILE);
+    pk += BT * a.k.sr;
+    pv += BT * a.v.sr;
   };
 
   const Offsets<D> offsets(lane);
@@ -578,13 +592,16 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
     }
     fence<D, CAUSAL>();
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i)
+    for (int i = 0; i < D / 16; ++i) {
       dp = mfma16(row_operand<T>(smem, of.row, at + 2 * TILE, i), gf[i], dp);
+#pragma unroll
+      for (int r = 256 / D * i; r < 256 / D * (i + 1); ++r) s[r] = __builtin_amdgcn_exp2f(s[r] * a.c);
+    }
     fence<D, CAUSAL>();
     x8 df[2];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      float p = __builtin_amdgcn_exp2f(s[r] * a.c);
+      float p = s[r];
       if (F16) p *= fs;
       df[r / 8][r % 8] = (T)(p * dp[r]);
     }
@@ -613,52 +630,60 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
   } else {
     for (int it = it0; it < it1; ++it) tile_of(it, (it - it0) & 1);
   }
-  const int64_t part = ((int64_t)sp * a.planes_q + pl) * a.q_tiles * BC * D;
-  store_columns<T, D>(dq, a.sm_scale / scale, a.dq, b, h, a.q_split > 1 ? a.part_q + part : nullptr, qw, a.N);
+  store_columns<T, D>(dq, a.sm_scale / scale, a.dq, b, h,
+                      at.parts == 1 ? nullptr : a.part_q + (int64_t)block * BC * D, q0, w, a.N);
 }
 
 template <typename T, int D, bool CAUSAL>
 __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) main_kernel(const Args a) {
   __shared__ __align__(1024) u8 smem[LDS_BYTES<D>];
-  if ((int)blockIdx.x < a.k_blocks)
+  if ((int)blockIdx.x < a.keys.blocks)
     keys_block<T, D, CAUSAL>(a, smem, blockIdx.x);
   else
-    queries_block<T, D, CAUSAL>(a, smem, blockIdx.x - a.k_blocks);
+    queries_block<T, D, CAUSAL>(a, smem, blockIdx.x - a.keys.blocks);
 }
 
 // ------------------------------------------------------------------------------------- join
-// The parts' sums added in order, eight values a thread: dK and dV where K's loops are cut, then dQ.
+// The parts of a tile added in order: dK and dV (of = 0, 1) of the keys' cut tiles, then dQ of the queries',
+// 256 chunks of 8 values a block.
 struct JoinArgs {
+  AttnBwdCut cut[2];
   const float* part[3];
   Out out[3];
-  int heads[3], planes[3], rows[3], padded[3], split[3];
-  int64_t begin[4];                    // threads ahead of each tensor's
+  int heads[2], planes[2], rows[2], blocks_k;
 };
 template <typename T, int D>
 __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (id >= a.begin[3]) return;
-  const int x = id >= a.begin[2] ? 2 : id >= a.begin[1] ? 1 : 0;
-  const int64_t row = (id - a.begin[x]) / (D / 8);
-  const int col = (int)((id - a.begin[x]) % (D / 8)) * 8;
-  const int pl = (int)(row / a.rows[x]), r = (int)(row % a.rows[x]);
-  const int64_t step = (int64_t)a.planes[x] * a.padded[x] * D;
-  const float* p = a.part[x] + ((int64_t)pl * a.padded[x] + r) * D + col;
-  f32x4 lo = *(const f32x4*)p, hi = *(const f32x4*)(p + 4);
-  for (int s = 1; s < a.split[x]; ++s) {
-    p += step;
-    lo += *(const f32x4*)p;
-    hi += *(const f32x4*)(p + 4);
+  constexpr int SUB = BC * D / 8 / 256;                     // blocks to a tile
+  int id = blockIdx.x;
+  const bool q = id >= 2 * a.blocks_k;
+  if (q) id -= 2 * a.blocks_k;
+  const int of = q ? 2 : id >= a.blocks_k;
+  if (of == 1) id -= a.blocks_k;
+  const AttnBwdCut& c = a.cut[q];
+  const int sub = id % SUB, planes = a.planes[q], pl = id / SUB % planes, u = id / SUB / planes;
+  int p;
+  const int first = attn_bwd_first_part(c, u, planes, p) + pl;       // its block, the other parts' `planes` apart
+  const int at = sub * 256 + threadIdx.x, row = at / (D / 8), col = at % (D / 8) * 8;
+  const int r = (q ? c.tiles - 1 - u : u) * BC + row;
+  if (r >= a.rows[q]) return;
+  const float* x = a.part[of] + ((int64_t)first * BC + row) * D + col;
+  const int64_t step = (int64_t)planes * BC * D;
+  f32x4 s0 = *(const f32x4*)x, s1 = *(const f32x4*)(x + 4);
+#pragma unroll 4
+  for (int k = 1; k < p; ++k) {
+    s0 += *(const f32x4*)(x + k * step);
+    s1 += *(const f32x4*)(x + k * step + 4);
   }
   typename Vec<T>::x8 y;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    y[e] = (T)lo[e];
-    y[4 + e] = (T)hi[e];
+    y[e] = (T)s0[e];
+    y[4 + e] = (T)s1[e];
   }
-  const int b = pl / a.heads[x], h = pl % a.heads[x];
-  *(typename Vec<T>::x8*)((T*)a.out[x].p + (int64_t)b * a.out[x].sb + (int64_t)h * a.out[x].sh +
-                          (int64_t)r * a.out[x].sr + col) = y;
+  const int b = pl / a.heads[q], h = pl % a.heads[q];
+  *(typename Vec<T>::x8*)((T*)a.out[of].p + (int64_t)b * a.out[of].sb + (int64_t)h * a.out[of].sh +
+                          (int64_t)r * a.out[of].sr + col) = y;
 }
 
 template <typename T, int D>
@@ -675,33 +700,30 @@ hipError_t launch(const AttnBwdArgs& x, const AttnBwdPlan& p, const Args& a, hip
   hipLaunchKernelGGL((rows_kernel<T, D>), dim3(rows), dim3(256), 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  launch_main<T, D>(a, x.causal, (int)(p.k_blocks + p.q_blocks), s);
+  launch_main<T, D>(a, x.causal, a.keys.blocks + a.queries.blocks, s);
   if ((e = hipGetLastError()) != hipSuccess) return e;
+  constexpr int SUB = BC * D / 8 / 256;
   JoinArgs j = {};
+  j.cut[0] = a.keys;
+  j.cut[1] = a.queries;
   j.part[0] = a.part_k;
   j.part[1] = a.part_v;
   j.part[2] = a.part_q;
   j.out[0] = a.dk;
   j.out[1] = a.dv;
   j.out[2] = a.dq;
-  int64_t at = 0;
-  for (int i = 0; i < 3; ++i) {
-    const bool q = i == 2;
-    j.heads[i] = q ? a.H : a.H_kv;
-    j.planes[i] = q ? a.planes_q : a.planes_kv;
-    j.rows[i] = q ? a.N : a.N_kv;
-    j.padded[i] = (int)(q ? p.q_tiles * p.q_rows : p.k_tiles * p.k_rows);
-    j.split[i] = (int)(q ? p.q_split : p.k_split);
-    j.begin[i] = at;
-    if (j.split[i] > 1) at += (int64_t)j.planes[i] * j.rows[i] * (D / 8);
-  }
-  j.begin[3] = at;
-  if (at == 0) return hipSuccess;
-  hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)((at + 255) / 256)), dim3(256), 0, s, j);
+  j.heads[0] = a.H_kv;
+  j.heads[1] = a.H;
+  j.planes[0] = a.planes_kv;
+  j.planes[1] = a.planes_q;
+  j.rows[0] = a.N_kv;
+  j.rows[1] = a.N;
+  j.blocks_k = a.keys.cut * a.planes_kv * SUB;
+  const int blocks = 2 * j.blocks_k + a.queries.cut * a.planes_q * SUB;
+  if (blocks == 0) return hipSuccess;
+  hipLaunchKernelGGL((join_kernel<T, D>), dim3(blocks), dim3(256), 0, s, j);
   return hipGetLastError();
 }
-
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // The workspace's parts, each from a multiple of 256 bytes on.
 struct Offsets64 {
@@ -721,40 +743,14 @@ Offsets64 offsets(const AttnBwdPlan& p, int dtype, int64_t planes_q, int64_t pla
   o.max_do = take(f16 ? planes_q * p.nb_q : 0);
   o.max_d = take(f16 ? planes_q * p.nb_q : 0);
   o.max_v = take(f16 ? planes_kv * p.nb_kv : 0);
-  const int64_t k = p.k_split > 1 ? p.k_split * planes_kv * p.k_tiles * p.k_rows * D : 0;
-  o.part_k = take(k);
-  o.part_v = take(k);
-  o.part_q = take(p.q_split > 1 ? p.q_split * planes_q * p.q_tiles * p.q_rows * D : 0);
+  o.part_k = take((int64_t)p.keys.cut_blocks * BC * D);
+  o.part_v = take((int64_t)p.keys.cut_blocks * BC * D);
+  o.part_q = take((int64_t)p.queries.cut_blocks * BC * D);
   o.end = at;
   return o;
 }
 
 }  // namespace
-
-AttnBwdPlan attn_bwd_plan(int64_t B, int64_t H, int64_t H_kv, int64_t N, int64_t N_kv, int64_t D,
-                          bool causal) {
-  AttnBwdPlan p;
-  p.nb_q = ceil_div(N, BT);
-  p.nb_kv = ceil_div(N_kv, BT);
-  p.k_rows = p.q_rows = BC;
-  p.k_tiles = ceil_div(N_kv, p.k_rows);
-  p.q_tiles = ceil_div(N, p.q_rows);
-  // As many parts as bring each block's steps (four products over a tile for keys, three for queries)
-  // down to its share of what the card runs at once, of 4 tiles or more.
-  const int64_t steps_k = p.nb_q * (H / H_kv), steps_q = p.nb_kv;
-  const int64_t work = B * H_kv * p.k_tiles * steps_k * 4 + B * H * p.q_tiles * steps_q * 3;
-  const int64_t share = ceil_div(work, causal ? 1024 : 512);
-  auto parts = [&](int64_t steps, int64_t cost) {
-    int64_t n = steps * cost / (share < 1 ? 1 : share);
-    if (n > steps / 4) n = steps / 4;
-    return n < 1 ? 1 : n > 64 ? 64 : n;
-  };
-  p.k_split = parts(steps_k, 4);
-  p.q_split = parts(steps_q, 3);
-  p.k_blocks = B * H_kv * p.k_tiles * p.k_split;
-  p.q_blocks = B * H * p.q_tiles * p.q_split;
-  return p;
-}
 
 int64_t attn_bwd_workspace_bytes(const AttnBwdPlan& p, int dtype, int64_t planes_q, int64_t planes_kv,
                                  int64_t D) {
@@ -786,11 +782,8 @@ hipError_t launch_attn_bwd(const AttnBwdArgs& x, hipStream_t s) {
   a.NP = (int)p.nb_q * BT;
   a.planes_q = (int)(x.B * x.H);
   a.planes_kv = (int)(x.B * x.H_kv);
-  a.k_tiles = (int)p.k_tiles;
-  a.q_tiles = (int)p.q_tiles;
-  a.k_split = (int)p.k_split;
-  a.q_split = (int)p.q_split;
-  a.k_blocks = (int)p.k_blocks;
+  a.keys = p.keys;
+  a.queries = p.queries;
   a.sm_scale = x.sm_scale;
   a.c = x.sm_scale * LOG2E_F;
   const Offsets64 o = offsets(p, x.dtype, a.planes_q, a.planes_kv, x.D);

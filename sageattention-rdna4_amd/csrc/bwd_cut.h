@@ -1,0 +1,130 @@
+// How a backward call is cut into blocks (host and device; no HIP dependency, so that a host program can
+// check that every step of every tile is taken once).
+//
+// A tile is 128 columns (keys, or queries) of a plane; its block goes over the other side in steps of 64 rows.
+// Where tiles are few, or some far longer than a resident block's share, they are cut into parts of
+// so many steps, each a block of its own, and a further launch adds the parts' sums in order.
+#pragma once
+#include <stdint.h>
+
+#if defined(__HIPCC__)
+#define SAGE_HD __host__ __device__ __forceinline__
+#else
+#define SAGE_HD inline
+#endif
+
+namespace sage {
+
+constexpr int ATTN_BWD_COLUMNS = 128, ATTN_BWD_ROWS = 64, ATTN_BWD_SEGMENTS = 32;
+
+// One kind of block's tiles, the longest first. Those of `parts` parts come first, end[0] of them, then
+// those of one part less, up to tile end[1], and so on; from tile `cut` on they are whole. Blocks are numbered
+// tile by tile, part by part, plane by plane: cut_blocks of them hold parts.
+struct AttnBwdCut {
+  int tiles, parts, cut, cut_blocks, blocks;
+  int end[ATTN_BWD_SEGMENTS];
+};
+struct AttnBwdPlan {
+  int64_t nb_q, nb_kv;        // steps in a plane of queries, of keys
+  AttnBwdCut keys, queries;
+};
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Tiles u = 0 .. of min(top, base - drop u) steps each in `planes` planes, no part of more than `most`.
+inline AttnBwdCut cut_tiles(int64_t tiles, int64_t base, int64_t drop, int64_t top, int64_t most,
+                            int64_t planes) {
+  const int64_t longest = base < top ? base : top;
+  int64_t parts = ceil_div(longest, most);
+  if (drop && parts > ATTN_BWD_SEGMENTS) {
+    most = ceil_div(longest, ATTN_BWD_SEGMENTS);
+    parts = ceil_div(longest, most);
+  }
+  AttnBwdCut c = {};
+  int64_t lo = 0, blocks = 0;
+  int i = 0;
+  for (int64_t p = parts;; --p, ++i) {
+    int64_t hi = tiles;                       // the end of the tiles of more than (p - 1) most steps
+    const int64_t over = (p - 1) * most;
+    if (p > 1 && drop) hi = over >= longest ? 0 : ceil_div(base - over, drop);
+    hi = hi > tiles ? tiles : hi < lo ? lo : hi;
+    c.end[i] = (int)hi;
+    blocks += (hi - lo) * p * planes;
+    if (p > 1) {
+      c.cut = (int)hi;
+      c.cut_blocks = (int)blocks;
+    }
+    lo = hi;
+    if (p == 1 || hi == tiles) break;
+  }
+  c.tiles = (int)tiles;
+  c.parts = (int)parts;
+  c.blocks = (int)blocks;
+  return c;
+}
+
+inline AttnBwdPlan attn_bwd_plan(int64_t B, int64_t H, int64_t H_kv, int64_t N, int64_t N_kv, int64_t D,
+                                 bool causal) {
+  AttnBwdPlan p;
+  p.nb_q = ceil_div(N, ATTN_BWD_ROWS);
+  p.nb_kv = ceil_div(N_kv, ATTN_BWD_ROWS);
+  const int64_t G = H / H_kv, k_tiles = ceil_div(N_kv, ATTN_BWD_COLUMNS), q_tiles = ceil_div(N, ATTN_BWD_COLUMNS);
+  const int64_t k_planes = B * H_kv, q_planes = B * H;
+  // The steps of the longest tiles, and of all of them, at four products for keys and three for queries;
+  // `share` is each resident block's part of it all.
+  const int64_t k_long = G * p.nb_q, q_long = p.nb_kv;
+  const int64_t k_all = k_planes * (causal ? G * (p.nb_q * k_tiles - k_tiles * (k_tiles - 1)) : k_long * k_tiles);
+  const int64_t q_all = q_planes * (causal ? q_tiles * (q_tiles + 1) : q_long * q_tiles);
+  const int64_t resident = (D == 64 ? 3 : 2) * 256;
+  const int64_t share = (4 * k_all + 3 * q_all) / resident;
+  // A part may take a little more than that: parts are written in fp32 and read again, and tiles that are all
+  // alike fit the card in one go with a fifth more. A tile is cut only where that saves more than the
+  // joining launch costs; no part is under 4 steps. Measured, all tiles in as many parts as the longest one
+  // and so: 2 x 8 heads on 2 of 6449 causal rows of 64 values 358 and 292 us, one head of 16384 rows 550 and
+  // 408, 6 heads on 1 of 1541 rows 101 and 93, 4096 causal rows, 32 heads on 8, 472 and 479.
+  const int64_t may = share + share / (causal ? 20 : 5);
+  auto most = [&](int64_t longest, int64_t cost) {
+    if (longest * cost <= may + 28) return longest;
+    const int64_t steps = ceil_div(may, cost);
+    return steps < 4 ? (int64_t)4 : steps;
+  };
+  p.keys = cut_tiles(k_tiles, k_long, causal ? 2 * G : 0, k_long, most(k_long, 4), k_planes);
+  p.queries = causal ? cut_tiles(q_tiles, 2 * q_tiles, 2, q_long, most(q_long, 3), q_planes)
+                     : cut_tiles(q_tiles, q_long, 0, q_long, most(q_long, 3), q_planes);
+  return p;
+}
+
+// A block's place in a cut: its tile, its plane, and which of its tile's parts it holds.
+struct AttnBwdPlace {
+  int u, plane, part, parts;
+  // the part's share of n steps
+  SAGE_HD int first(int n) const {
+    const int left = n % parts;
+    return n / parts * part + (part < left ? part : left);
+  }
+  SAGE_HD int end(int n) const { return first(n) + n / parts + (part < n % parts ? 1 : 0); }
+};
+SAGE_HD AttnBwdPlace attn_bwd_place(const AttnBwdCut& c, int block, int planes) {
+  int lo = 0, p = c.parts;
+  for (int i = 0;; ++i, --p) {
+    const int hi = c.end[i], here = (hi - lo) * p * planes;
+    if (p == 1 || block < here) break;
+    block -= here;
+    lo = hi;
+  }
+  const int x = block / planes, t = x / p;
+  return {lo + t, block - x * planes, x - t * p, p};
+}
+// The block that holds the first part of cut tile u in plane 0 (those of the other planes follow it, the next
+// part's are `planes` further on), and the tile's parts.
+SAGE_HD int attn_bwd_first_part(const AttnBwdCut& c, int u, int planes, int& parts) {
+  int lo = 0, p = c.parts, first = 0;
+  for (int i = 0; u >= c.end[i]; ++i, --p) {
+    first += (c.end[i] - lo) * p * planes;
+    lo = c.end[i];
+  }
+  parts = p;
+  return first + (u - lo) * p * planes;
+}
+
+}  // namespace sage

@@ -108,15 +108,15 @@ int check_attn_bwd(int dtype, int causal, int64_t B, int64_t H, int64_t N, int64
   if (causal && N != N_kv)
     return fail(SAGE_ERR_INVALID, "seq_len: causal attention needs N == N_kv (N=%lld N_kv=%lld)",
                 (long long)N, (long long)N_kv);
-  // the rows launch, a block per 64 rows of each tensor; the main launch has fewer blocks, or few
+  // the rows launch, a block per 64 rows of each tensor; the others have fewer blocks, or few
   const int64_t tiles = B * H * ((N + 63) / 64), tiles_kv = B * H_kv * ((N_kv + 63) / 64);
   if ((rc = check_grid("the backward pass", tiles + tiles_kv, 256))) return rc;
   const sage::AttnBwdPlan p = sage::attn_bwd_plan(B, H, H_kv, N, N_kv, D, causal != 0);
-  return check_grid("the backward pass", p.k_blocks + p.q_blocks, 256);
+  return check_grid("the backward pass", (int64_t)p.keys.blocks + p.queries.blocks, 256);
 }
 
 // The rows of a norm: in three dimensions, with 32-bit row numbers.
-constexpr int64_t kMaxNorm = 32768, kMaxNormRows = 1 << 30;
+constexpr int64_t kMaxNorm = 16384, kMaxNormRows = 1 << 30;
 int check_norm(int dtype, int64_t d0, int64_t d1, int64_t d2, int64_t n) {
   if (dtype != SAGE_F16 && dtype != SAGE_BF16)
     return fail(SAGE_ERR_INVALID, "dtype: unsupported dtype code %d", dtype);

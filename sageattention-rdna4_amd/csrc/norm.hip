@@ -201,15 +201,21 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_grad_kernel(const 
   __shared__ float lds[2][THREADS / 64];
   __shared__ float cols[RPB > 1 ? THREADS * 8 * C : 1];
   const int l = threadIdx.x % TPR, sub = threadIdx.x / TPR;
-  float w[C][8], dw[C][8];
+  // The weights stay in registers, and the next rows are requested ahead of the sum over the ones at hand,
+  // but where a block of 1024 threads has 128 registers a thread.
+  constexpr bool ROOM = THREADS < 1024;
+  float w[ROOM ? C : 1][8], dw[C][8];
+  auto weights = [&](int c) -> const float(&)[8] {
+    if (!ROOM) load_weights(a.w, a.w32, min(8 * (l + TPR * c), a.n - 8), w[0], T());
+    return w[ROOM ? c : 0];
+  };
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int col = 8 * (l + TPR * c);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) dw[c][e] = w[c][e] = 0.0f;
-    if (col < a.n) load_weights(a.w, a.w32, col, w[c], T());
+    for (int e = 0; e < 8; ++e) dw[c][e] = 0.0f;
+    if (ROOM) load_weights(a.w, a.w32, min(col, a.n - 8), w[c], T());
   }
-  // the next rows are requested ahead of the sum over the ones at hand
   u32x4 vx[C], vg[C], vd[C];
   float rstd;
   auto load = [&](int first) {
@@ -230,11 +236,12 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_grad_kernel(const 
     }
   };
   int turn = 0;
-  load(blockIdx.x * RPB);
+  if (ROOM) load(blockIdx.x * RPB);
   for (int first = blockIdx.x * RPB; first < a.rows; first += gridDim.x * RPB, turn ^= 1) {
     const int row = first + sub;
     const bool live = row < a.rows;
     u32x4 x[C], g[C], d[C];
+    if (!ROOM) load(first);
     const float r = rstd;
     float m = 0.0f;
 #pragma unroll
@@ -243,16 +250,17 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_grad_kernel(const 
       g[c] = vg[c];
       d[c] = vd[c];
     }
-    if (first + gridDim.x * RPB < a.rows) load(first + gridDim.x * RPB);
+    if (ROOM && first + gridDim.x * RPB < a.rows) load(first + gridDim.x * RPB);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       float fx[8], fg[8];
       unpack8<T>(x[c], fx);
       unpack8<T>(g[c], fg);
+      const auto& wc = weights(c);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float h = fx[e] * r;
-        m = __builtin_fmaf(fg[e] * w[c][e], h, m);
+        m = __builtin_fmaf(fg[e] * wc[e], h, m);
         dw[c][e] += live ? fg[e] * h : 0.0f;
       }
     }
@@ -266,9 +274,10 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_grad_kernel(const 
       unpack8<T>(x[c], fx);
       unpack8<T>(g[c], fg);
       unpack8<T>(d[c], fd);
+      const auto& wc = weights(c);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        o[e] = r * (fg[e] * w[c][e] - fx[e] * r * m);
+        o[e] = r * (fg[e] * wc[e] - fx[e] * r * m);
         if (a.dsum) o[e] += fd[e];
       }
       *(u32x4*)((T*)a.dx + (int64_t)row * a.n + col) = pack8<T>(o);
@@ -346,8 +355,7 @@ hipError_t by_shape(int64_t rows, int64_t n, F&& f) {
   if (rows <= 512 && n <= 8192) return SAGE_SHAPE(1024, 1);
   if (n <= 4096) return SAGE_SHAPE(256, 2);
   if (n <= 8192) return SAGE_SHAPE(256, 4);
-  if (n <= 16384) return SAGE_SHAPE(1024, 2);
-  return SAGE_SHAPE(1024, 4);
+  return SAGE_SHAPE(1024, 2);
 #undef SAGE_SHAPE
 }
 

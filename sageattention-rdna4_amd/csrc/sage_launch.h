@@ -4,6 +4,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "bwd_cut.h"
+
 namespace sage {
 
 // Geometry of the two-launch prologue for BH planes of N rows, padded to N_pad (a multiple of 64,
@@ -197,14 +199,7 @@ struct AttnBwdArgs {
   float sm_scale;
   void* workspace;
 };
-// How a call is cut up: tiles of 64 rows in a plane, blocks of k_rows keys and of q_rows queries,
-// each one's loop in k_split or q_split parts. Sizes alone decide it, so a captured call and its
-// workspace agree.
-struct AttnBwdPlan {
-  int64_t nb_q, nb_kv, k_rows, q_rows, k_tiles, q_tiles, k_split, q_split, k_blocks, q_blocks;
-};
-AttnBwdPlan attn_bwd_plan(int64_t B, int64_t H, int64_t H_kv, int64_t N, int64_t N_kv, int64_t D,
-                          bool causal);
+// A plan follows from the sizes alone, so a captured call and its workspace agree.
 int64_t attn_bwd_workspace_bytes(const AttnBwdPlan& p, int dtype, int64_t planes_q, int64_t planes_kv,
                                  int64_t D);
 hipError_t launch_attn_bwd(const AttnBwdArgs& a, hipStream_t stream);

@@ -64,8 +64,8 @@ def _check(what, x, weight, others):
         _refuse(what, "dtype: x is %s (fp16 and bf16 are served)" % x.dtype)
     shape, dev = x.shape, x.device
     n = shape[-1] if shape else 0
-    if n % 8 or not 8 <= n <= 32768:
-        _refuse(what, "row: x is %s (rows of a multiple of 8 values up to 32768 are served)" % (
+    if n % 8 or not 8 <= n <= 16384:
+        _refuse(what, "row: x is %s (rows of a multiple of 8 values up to 16384 are served)" % (
             tuple(shape),))
     if not isinstance(weight, torch.Tensor) or weight.device != dev:
         _refuse(what, "device: weight must be a tensor on %s" % dev)
@@ -137,7 +137,7 @@ def rms_norm(x, weight, eps=1e-6, residual=None, return_rstd=False):
     """x / sqrt(mean(x^2) + eps) * weight over the last dimension; with `residual`, of x + residual, and
     `(y, x + residual)` is returned.
 
-    x: fp16 or bf16, any number of dimensions, rows of a multiple of 8 values up to 32768; rows may lie
+    x: fp16 or bf16, any number of dimensions, rows of a multiple of 8 values up to 16384; rows may lie
     apart (a view of a fused projection), in three dimensions at most. residual: x's shape and dtype.
     weight: (n,) of x's dtype or fp32. The sum is added, normed and scaled in fp32; y and the sum (new,
     contiguous, of x's shape and dtype) are each rounded once. Autograd records the call where x, weight or
