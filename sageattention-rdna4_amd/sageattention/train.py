@@ -30,6 +30,14 @@ def _row_floats(what, name, t, shape, device):
         _refuse(what, "stride_last: %s must be contiguous" % name)
 
 
+def _scale(what, sm_scale, D):
+    """The scores' factor."""
+    sm = D ** -0.5 if sm_scale is None else float(sm_scale)
+    if not _LEAST_SCALE <= sm <= 1 / _LEAST_SCALE:
+        _refuse(what, "sm_scale: must lie between 1e-30 and 1e30 (got %r)" % (sm_scale,))
+    return sm
+
+
 def _plain(tensors, tensor_layout):
     """Whether all are contiguous GPU tensors of a served dtype and head_dim, which need no closer look."""
     if tensor_layout != "HND" and tensor_layout != "NHD":
@@ -50,8 +58,8 @@ def sageattn_backward(dout, q, k, v, out, lse, tensor_layout="HND", is_causal=Fa
 
     q, k, v, tensor_layout, is_causal, sm_scale: as the forward call had them. out, lse: what it returned
     with `return_lse=True`. dlse (B, H, N) fp32: the gradient of lse, where the caller used it. out and
-    dout have q's shape and dtype (any strides that `sageattn` takes), the gradients are contiguous, of
-    q's, k's and v's shapes and dtype.
+    dout have q's shape and dtype (any strides that `sageattn` takes, rows less than 2^24 elements
+    apart), the gradients are contiguous, of q's, k's and v's shapes and dtype.
 
     Keys that are one part of those a query sees (attention over parts, merged by their logsumexp)
     have their gradients from calls with the merged out and lse, a call for each part; dq is the calls'
@@ -87,9 +95,7 @@ def sageattn_backward(dout, q, k, v, out, lse, tensor_layout="HND", is_causal=Fa
     _row_floats(what, "lse", lse, (B, H, N), dev)
     if dlse is not None:
         _row_floats(what, "dlse", dlse, (B, H, N), dev)
-    sm = D ** -0.5 if sm_scale is None else float(sm_scale)
-    if not _LEAST_SCALE <= sm <= 1 / _LEAST_SCALE:
-        _refuse(what, "sm_scale: must lie between 1e-30 and 1e30 (got %r)" % (sm_scale,))
+    sm = _scale(what, sm_scale, D)
     lib = _library(what, dev)
     grads = tuple([_empty(t) for t in (q, k, v)])
     work = torch.empty(lib.attn_bwd_workspace_bytes(dtype, bool(is_causal), B, H, N, H_kv, N_kv, D),
@@ -125,7 +131,10 @@ def sageattn_train(q, k, v, tensor_layout="HND", is_causal=False, sm_scale=None,
     to q, k and v (from the logsumexp's gradient too, with `return_lse`).
 
     The gradients are those of attention itself: the forward call's rounding to 8 bits counts as the
-    identity. Gradients of gradients are not served.
+    identity. Gradients of gradients are not served. To capture a training step into a graph, capture
+    `sageattn(..., return_lse=True)` and `sageattn_backward`, or a forward pass with `torch.autograd.grad`:
+    gradients that autograd adds up in leaves (`backward()`) belong to the stream that first used the leaf.
     """
+    _scale("sageattn_train", sm_scale, 1)
     out, lse = _Attention.apply(q, k, v, tensor_layout, is_causal, sm_scale, kwargs)
     return (out, lse) if return_lse else out

@@ -41,9 +41,11 @@ def forward(q, k, v, causal, sm):
     return torch.exp(s - lse[..., None]) @ v, lse
 
 
-def gradients(dout, q, k, v, out, lse, dlse, causal, sm):
-    """{"dq": (value, tolerance), ..} for 16-bit (B, H, N, D) tensors, head by head of K/V."""
-    u, f16 = U[q.dtype], q.dtype == torch.float16
+def gradients(dout, q, k, v, out, lse, dlse, causal, sm, dtype=None):
+    """{"dq": (value, tolerance), ..} for (B, H, N, D) tensors of 16 bits, or of 64 where `dtype` says what the
+    tolerances count, head by head."""
+    dtype = dtype or q.dtype                       # of the roundings
+    u, f16 = U[dtype], dtype == torch.float16
     B, H, N, D = q.shape
     H_kv, N_kv = k.shape[1:3]
     G = H // H_kv
@@ -77,7 +79,7 @@ def gradients(dout, q, k, v, out, lse, dlse, causal, sm):
             want["dq"][1][b, h] = sm * ((err + N_kv * E * ds.abs()) @ kk.abs())
             want["dk"][0][b, hk] += sm * (ds.t().contiguous() @ qq)
             want["dk"][1][b, hk] += sm * ((err + N * G * E * ds.abs()).t().contiguous() @ qq.abs())
-    least = torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps
+    least = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
     return {n: (x, t + u * x.abs() + least) for n, (x, t) in want.items()}
 
 
