@@ -209,16 +209,28 @@ __global__ void __launch_bounds__(256) rows_kernel(const Args a) {
 }
 
 // ------------------------------------------------------------------------------------- main
-// The largest of n values, by a block of 256 threads; NaNs are passed over.
-__device__ __forceinline__ float block_max(const float* p, int n, float* lds) {
-  float m = 0.0f;
-  for (int i = threadIdx.x; i < n; i += 256) m = fmaxf(m, p[i]);
+// The largest of each list of values, by a block of 256 threads, through K * 4 floats of LDS; NaNs are
+// passed over.
+template <int K>
+__device__ __forceinline__ void block_max(const float* const (&p)[K], const int (&n)[K], float* lds,
+                                          float (&m)[K]) {
 #pragma unroll
-  for (int s = 1; s < 64; s <<= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+  for (int k = 0; k < K; ++k) {
+    m[k] = 0.0f;
+    for (int i = threadIdx.x; i < n[k]; i += 256) m[k] = fmaxf(m[k], p[k][i]);
+  }
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) m[k] = fmaxf(m[k], __shfl_xor(m[k], s, 64));
+  if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) lds[4 * k + (threadIdx.x >> 6)] = m[k];
+  }
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
-  __syncthreads();
-  return fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    m[k] = fmaxf(fmaxf(lds[4 * k], lds[4 * k + 1]), fmaxf(lds[4 * k + 2], lds[4 * k + 3]));
 }
 
 // The power of two that brings `bound` into [2^13, 2^14) (an infinite or vanishing one: as far as
@@ -396,17 +408,6 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
   const int n = per * a.G;
   const int it0 = at.first(n), it1 = at.end(n);
 
-  float scale = 1.0f;
-  if (F16) {
-    const int hq = b * a.H + hk * a.G;
-    const float mo = block_max(a.max_do + (int64_t)hq * a.nb_q, a.G * a.nb_q, (float*)smem);
-    const float md = block_max(a.max_d + (int64_t)hq * a.nb_q, a.G * a.nb_q, (float*)smem);
-    const float mv = block_max(a.max_v + (int64_t)pl * a.nb_kv, a.nb_kv, (float*)smem);
-    scale = scale_for(sqrtf(mo) * sqrtf(mv) + md);
-    __syncthreads();
-  }
-  const float fs = scale * __builtin_ldexpf(1.0f, -(int)P_SHIFT<T>);
-
   // LDS: two tiles of Q, two of dout, and of the rows' two constants
   const float* lds_rows = (const float*)(smem + 4 * TILE);
   const uint32_t lds0 = lds_addr(smem);
@@ -436,10 +437,22 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
     }
   };
 
+  int tc = ti;                                       // the tile at hand
+  if (it0 < it1) request(0);
   const Offsets<D> offsets(lane);
   x8 kf[D / 16], vf[D / 16];
   load_columns<T, D>(plane<T>(a.k, b, hk), a.k.sr, kw, a.N_kv, lane, kf);
   load_columns<T, D>(plane<T>(a.v, b, hk), a.v.sr, kw, a.N_kv, lane, vf);
+  float scale = 1.0f;
+  if (F16) {
+    const int64_t hq = (int64_t)(b * a.H + hk * a.G) * a.nb_q;
+    const int nq = a.G * a.nb_q;
+    float m[3];                                      // by way of the second tile's constants
+    block_max<3>({a.max_do + hq, a.max_d + hq, a.max_v + (int64_t)pl * a.nb_kv}, {nq, nq, a.nb_kv},
+                 (float*)(smem + 4 * TILE) + 2 * BT, m);
+    scale = scale_for(sqrtf(m[0]) * sqrtf(m[2]) + m[1]);
+  }
+  const float fs = scale * __builtin_ldexpf(1.0f, -(int)P_SHIFT<T>);
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) {
@@ -486,10 +499,8 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
         dk[dt] = mfma16(transposed<T>(smem, of.lo, of.hi, at + 32 * t * D, dt), df[t], dk[dt]);
       }
   };
-  int tc = ti;                                       // the tile at hand
   // what was loaded so far is here: in the loop the compiler has nothing of its own to wait for
   __builtin_amdgcn_s_waitcnt(0);
-  if (it0 < it1) request(0);
   auto tile_of = [&](int it, int buf) {
     next_tile();
     const int q0 = tc * BT;
@@ -529,11 +540,6 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
   const int n = CAUSAL ? min((q0 + BC) / BT, a.nb_kv) : a.nb_kv;
   const int it0 = at.first(n), it1 = at.end(n);
 
-  float mv = 0.0f;
-  if (F16) {
-    mv = sqrtf(block_max(a.max_v + (int64_t)(b * a.H_kv + hk) * a.nb_kv, a.nb_kv, (float*)smem));
-    __syncthreads();
-  }
   // LDS: two tiles of K, two of V
   const uint32_t lds0 = lds_addr(smem);
   const T* pk = plane<T>(a.k, b, hk) + (int64_t)it0 * BT * a.k.sr;
@@ -547,15 +553,17 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
     pv += BT * a.v.sr;
   };
 
+  if (it0 < it1) request(it0, 0);
   const Offsets<D> offsets(lane);
   x8 qf[D / 16], gf[D / 16];
   load_columns<T, D>(plane<T>(a.q, b, h), a.q.sr, qw, a.N, lane, qf);
   load_columns<T, D>(plane<T>(a.dout, b, h), a.dout.sr, qw, a.N, lane, gf);
   const int64_t row = (int64_t)pl * a.NP + min(qw + (lane & 31), a.NP - 1);
-  const float nl1 = a.nl[row], nd1 = a.nd[row];
-  float scale = 1.0f;
+  float nl1 = a.nl[row], scale = 1.0f;
+  const float nd1 = a.nd[row];
   if (F16) {
-    float sq = 0.0f;
+    float sq = 0.0f, mv[1];
+    block_max<1>({a.max_v + (int64_t)(b * a.H_kv + hk) * a.nb_kv}, {a.nb_kv}, (float*)(smem + 4 * TILE), mv);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
 #pragma unroll
@@ -564,9 +572,10 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
         sq = __builtin_fmaf(x, x, sq);
       }
     sq += __shfl_xor(sq, 32, 64);
-    scale = scale_for(sqrtf(sq) * mv + fabsf(nd1));
+    scale = scale_for(sqrtf(sq) * sqrtf(mv[0]) + fabsf(nd1));
+    // P meets dS alone here: its power of two is part of the exponent
+    nl1 += (log2f(scale) - P_SHIFT<T>) / a.c;
   }
-  const float fs = scale * __builtin_ldexpf(1.0f, -(int)P_SHIFT<T>);
   f32x16 dq[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) clear(dq[dt]);
@@ -600,11 +609,7 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
     fence<D, CAUSAL>();
     x8 df[2];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float p = s[r];
-      if (F16) p *= fs;
-      df[r / 8][r % 8] = (T)(p * dp[r]);
-    }
+    for (int r = 0; r < 16; ++r) df[r / 8][r % 8] = (T)(s[r] * dp[r]);
     fence<D, CAUSAL>();
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -613,7 +618,6 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
         dq[dt] = mfma16(transposed<T>(smem, of.lo, of.hi, at + 32 * t * D, dt), df[t], dq[dt]);
   };
   __builtin_amdgcn_s_waitcnt(0);                     // as in keys_block
-  if (it0 < it1) request(it0, 0);
   const int end = CAUSAL ? min(qw + 32, a.N_kv) : a.N_kv;
   auto tile_of = [&](int it, int buf) {
     next_tile();

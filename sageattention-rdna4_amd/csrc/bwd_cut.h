@@ -106,9 +106,9 @@ struct AttnBwdPlace {
 };
 SAGE_HD AttnBwdPlace attn_bwd_place(const AttnBwdCut& c, int block, int planes) {
   int lo = 0, p = c.parts;
-  for (int i = 0;; ++i, --p) {
+  for (int i = 0; p > 1; ++i, --p) {
     const int hi = c.end[i], here = (hi - lo) * p * planes;
-    if (p == 1 || block < here) break;
+    if (block < here) break;
     block -= here;
     lo = hi;
   }
