@@ -62,7 +62,6 @@ __device__ __forceinline__ bf16x4 read_tr(const bf16* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)p);
 }
 
-constexpr int BC = ATTN_BWD_COLUMNS;   // columns (keys, or queries) that a block owns: 32 a wave
 constexpr int BT = ATTN_BWD_ROWS;      // rows of the other side in an LDS tile
 // Halves of a tile in the loop's code.
 template <int D>
@@ -113,9 +112,9 @@ struct Args {
   float* max_do;    // fp16: (planes_q, nb_q): a tile's largest |dout|^2, |d|, and (planes_kv, nb_kv) |v|^2
   float* max_d;
   float* max_v;
-  float* part_k;    // (keys.cut_blocks, BC, D): sums of dK, of dV, by blocks that hold a part of their tile
+  float* part_k;    // (keys.cut_blocks, columns, D): sums of dK, of dV, by blocks that hold a part of their tile
   float* part_v;
-  float* part_q;    // (queries.cut_blocks, BC, D)
+  float* part_q;    // (queries.cut_blocks, columns, D)
 };
 
 template <typename T>
@@ -392,17 +391,54 @@ __device__ __forceinline__ f32x16 row_constants(const float* rows) {
   return x;
 }
 
-// A block that owns 128 keys of a K/V head.
-template <typename T, int D, bool CAUSAL>
+// Blocks of two pairs of waves (CW = 2): the second pair's sums, over the second halves of the steps' rows, are
+// added to the first's, by way of the tiles' LDS. True for the waves that hold them.
+template <int D, typename... X>
+__device__ __forceinline__ bool merge_pairs(u8* smem, int w, X&... x) {
+  float* at = (float*)smem + (w & 1) * (sizeof...(X) * 32 * D) + 4 * lane_anew();
+  (
+      [&](auto& acc) {
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) keep_live(acc[dt]);
+      }(x),
+      ...);
+  mfma_result_fence32();
+  __syncthreads();
+  auto each = [&](auto&& f) {
+    float* p = at;
+    auto of = [&](auto& acc) {
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i, p += 256) f(acc[dt], i, (f32x4*)p);
+    };
+    (of(x), ...);
+  };
+  if (w >= 2)
+    each([](const f32x16& v, int i, f32x4* p) {
+      *p = (f32x4){v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+    });
+  __syncthreads();
+  if (w < 2)
+    each([](f32x16& v, int i, const f32x4* p) {
+      const f32x4 y = *p;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * i + e] += y[e];
+    });
+  return w < 2;
+}
+
+// A block that owns 32 CW keys of a K/V head.
+template <typename T, int D, bool CAUSAL, int CW>
 __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
-  constexpr int TILE = BT * D * 2;
+  constexpr int TILE = BT * D * 2, BC = 32 * CW;
   constexpr bool F16 = std::is_same_v<T, f16>;
   typedef typename Vec<T>::x8 x8;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 5;
   const AttnBwdPlace at = attn_bwd_place(a.keys, block, a.planes_kv);
   const int pl = at.plane, b = pl / a.H_kv, hk = pl - b * a.H_kv;
-  const int k0 = at.u * BC, kw = k0 + 32 * w;
+  const int k0 = at.u * BC, kw = k0 + 32 * (w % CW);
   // tiles of queries, head after head of the group
   const int first = CAUSAL ? k0 / BT : 0, per = a.nb_q - first;
   const int n = per * a.G;
@@ -508,8 +544,10 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
     if (it + 1 < it1) request(buf ^ 1);
     const float* rows = lds_rows + 2 * buf * BT + 4 * g;
 #pragma unroll U<D>
-    for (int u = 0; u < 2; ++u)
+    for (int x = 0; x < CW / 2; ++x) {
+      const int u = CW == 4 ? x : w >> 1;
       if (!CAUSAL || q0 + 32 * u + 31 >= kw) step(q0 + 32 * u, (buf * BT + 32 * u) * D * 2, rows + 32 * u);
+    }
   };
   if (D == 64) {
     for (int it = it0; it < it1; it += 2) {
@@ -519,6 +557,7 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
   } else {
     for (int it = it0; it < it1; ++it) tile_of(it, (it - it0) & 1);
   }
+  if (CW == 2 && !merge_pairs<D>(smem, w, dk, dv)) return;
   const bool whole = at.parts == 1;
   const int64_t part = (int64_t)block * BC * D;
   store_columns<T, D>(dk, a.sm_scale / scale, a.dk, b, hk, whole ? nullptr : a.part_k + part, k0, w, a.N_kv);
@@ -526,17 +565,17 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
                       whole ? nullptr : a.part_v + part, k0, w, a.N_kv);
 }
 
-// A block that owns 128 queries of a head.
-template <typename T, int D, bool CAUSAL>
+// A block that owns 32 CW queries of a head.
+template <typename T, int D, bool CAUSAL, int CW>
 __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block) {
-  constexpr int TILE = BT * D * 2;
+  constexpr int TILE = BT * D * 2, BC = 32 * CW;
   constexpr bool F16 = std::is_same_v<T, f16>;
   typedef typename Vec<T>::x8 x8;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const AttnBwdPlace at = attn_bwd_place(a.queries, block, a.planes_q);
   const int pl = at.plane, b = pl / a.H, h = pl - b * a.H, hk = h / a.G;
   // the last tile of a causal plane is its longest
-  const int q0 = (a.queries.tiles - 1 - at.u) * BC, qw = q0 + 32 * w;
+  const int q0 = (a.queries.tiles - 1 - at.u) * BC, qw = q0 + 32 * (w % CW);
   const int n = CAUSAL ? min((q0 + BC) / BT, a.nb_kv) : a.nb_kv;
   const int it0 = at.first(n), it1 = at.end(n);
 
@@ -623,8 +662,10 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
     next_tile();
     if (it + 1 < it1) request(it + 1, buf ^ 1);
 #pragma unroll U<D>
-    for (int u = 0; u < 2; ++u)
+    for (int x = 0; x < CW / 2; ++x) {
+      const int u = CW == 4 ? x : w >> 1;
       if (it * BT + 32 * u < end) step(it * BT + 32 * u, (buf * BT + 32 * u) * D * 2);
+    }
   };
   if (D == 64) {
     for (int it = it0; it < it1; it += 2) {
@@ -634,17 +675,18 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
   } else {
     for (int it = it0; it < it1; ++it) tile_of(it, (it - it0) & 1);
   }
+  if (CW == 2 && !merge_pairs<D>(smem, w, dq)) return;
   store_columns<T, D>(dq, a.sm_scale / scale, a.dq, b, h,
                       at.parts == 1 ? nullptr : a.part_q + (int64_t)block * BC * D, q0, w, a.N);
 }
 
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, bool CAUSAL, int CW>
 __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) main_kernel(const Args a) {
   __shared__ __align__(1024) u8 smem[LDS_BYTES<D>];
   if ((int)blockIdx.x < a.keys.blocks)
-    keys_block<T, D, CAUSAL>(a, smem, blockIdx.x);
+    keys_block<T, D, CAUSAL, CW>(a, smem, blockIdx.x);
   else
-    queries_block<T, D, CAUSAL>(a, smem, blockIdx.x - a.keys.blocks);
+    queries_block<T, D, CAUSAL, CW>(a, smem, blockIdx.x - a.keys.blocks);
 }
 
 // ------------------------------------------------------------------------------------- join
@@ -656,7 +698,7 @@ struct JoinArgs {
   Out out[3];
   int heads[2], planes[2], rows[2], blocks_k;
 };
-template <typename T, int D>
+template <typename T, int D, int BC>
 __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
   constexpr int SUB = BC * D / 8 / 256;                     // blocks to a tile
   int id = blockIdx.x;
@@ -690,22 +732,16 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
                           (int64_t)r * a.out[of].sr + col) = y;
 }
 
-template <typename T, int D>
-void launch_main(const Args& a, bool causal, int blocks, hipStream_t s) {
+template <typename T, int D, int CW>
+void launch_main(const Args& a, bool causal, hipStream_t s) {
+  const dim3 grid(a.keys.blocks + a.queries.blocks);
   if (causal)
-    hipLaunchKernelGGL((main_kernel<T, D, true>), dim3(blocks), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((main_kernel<T, D, true, CW>), grid, dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((main_kernel<T, D, false>), dim3(blocks), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((main_kernel<T, D, false, CW>), grid, dim3(256), 0, s, a);
 }
-
-template <typename T, int D>
-hipError_t launch(const AttnBwdArgs& x, const AttnBwdPlan& p, const Args& a, hipStream_t s) {
-  const int rows = a.planes_q * a.nb_q + (x.dtype == 0 ? a.planes_kv * a.nb_kv : 0);
-  hipLaunchKernelGGL((rows_kernel<T, D>), dim3(rows), dim3(256), 0, s, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  launch_main<T, D>(a, x.causal, a.keys.blocks + a.queries.blocks, s);
-  if ((e = hipGetLastError()) != hipSuccess) return e;
+template <typename T, int D, int BC>
+hipError_t launch_join(const Args& a, hipStream_t s) {
   constexpr int SUB = BC * D / 8 / 256;
   JoinArgs j = {};
   j.cut[0] = a.keys;
@@ -725,8 +761,22 @@ hipError_t launch(const AttnBwdArgs& x, const AttnBwdPlan& p, const Args& a, hip
   j.blocks_k = a.keys.cut * a.planes_kv * SUB;
   const int blocks = 2 * j.blocks_k + a.queries.cut * a.planes_q * SUB;
   if (blocks == 0) return hipSuccess;
-  hipLaunchKernelGGL((join_kernel<T, D>), dim3(blocks), dim3(256), 0, s, j);
+  hipLaunchKernelGGL((join_kernel<T, D, BC>), dim3(blocks), dim3(256), 0, s, j);
   return hipGetLastError();
+}
+
+template <typename T, int D>
+hipError_t launch(const AttnBwdArgs& x, const AttnBwdPlan& p, const Args& a, hipStream_t s) {
+  const int rows = a.planes_q * a.nb_q + (x.dtype == 0 ? a.planes_kv * a.nb_kv : 0);
+  hipLaunchKernelGGL((rows_kernel<T, D>), dim3(rows), dim3(256), 0, s, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  if (p.columns == 128)
+    launch_main<T, D, 4>(a, x.causal, s);
+  else
+    launch_main<T, D, 2>(a, x.causal, s);
+  if ((e = hipGetLastError()) != hipSuccess) return e;
+  return p.columns == 128 ? launch_join<T, D, 128>(a, s) : launch_join<T, D, 64>(a, s);
 }
 
 // The workspace's parts, each from a multiple of 256 bytes on.
@@ -747,9 +797,9 @@ Offsets64 offsets(const AttnBwdPlan& p, int dtype, int64_t planes_q, int64_t pla
   o.max_do = take(f16 ? planes_q * p.nb_q : 0);
   o.max_d = take(f16 ? planes_q * p.nb_q : 0);
   o.max_v = take(f16 ? planes_kv * p.nb_kv : 0);
-  o.part_k = take((int64_t)p.keys.cut_blocks * BC * D);
-  o.part_v = take((int64_t)p.keys.cut_blocks * BC * D);
-  o.part_q = take((int64_t)p.queries.cut_blocks * BC * D);
+  o.part_k = take((int64_t)p.keys.cut_blocks * p.columns * D);
+  o.part_v = take((int64_t)p.keys.cut_blocks * p.columns * D);
+  o.part_q = take((int64_t)p.queries.cut_blocks * p.columns * D);
   o.end = at;
   return o;
 }

@@ -1,7 +1,8 @@
 // How a backward call is cut into blocks (host and device; no HIP dependency, so that a host program can
 // check that every step of every tile is taken once).
 //
-// A tile is 128 columns (keys, or queries) of a plane; its block goes over the other side in steps of 64 rows.
+// A tile is 128 columns (keys, or queries) of a plane, 64 in small calls; its block goes over the other side
+// in steps of 64 rows.
 // Where tiles are few, or some far longer than a resident block's share, they are cut into parts of
 // so many steps, each a block of its own, and a further launch adds the parts' sums in order.
 #pragma once
@@ -15,7 +16,7 @@
 
 namespace sage {
 
-constexpr int ATTN_BWD_COLUMNS = 128, ATTN_BWD_ROWS = 64, ATTN_BWD_SEGMENTS = 32;
+constexpr int ATTN_BWD_ROWS = 64, ATTN_BWD_SEGMENTS = 32;
 
 // One kind of block's tiles, the longest first. Those of `parts` parts come first, end[0] of them, then
 // those of one part less, up to tile end[1], and so on; from tile `cut` on they are whole. Blocks are numbered
@@ -25,6 +26,7 @@ struct AttnBwdCut {
   int end[ATTN_BWD_SEGMENTS];
 };
 struct AttnBwdPlan {
+  int64_t columns;            // of a tile
   int64_t nb_q, nb_kv;        // steps in a plane of queries, of keys
   AttnBwdCut keys, queries;
 };
@@ -68,15 +70,23 @@ inline AttnBwdPlan attn_bwd_plan(int64_t B, int64_t H, int64_t H_kv, int64_t N, 
   AttnBwdPlan p;
   p.nb_q = ceil_div(N, ATTN_BWD_ROWS);
   p.nb_kv = ceil_div(N_kv, ATTN_BWD_ROWS);
-  const int64_t G = H / H_kv, k_tiles = ceil_div(N_kv, ATTN_BWD_COLUMNS), q_tiles = ceil_div(N, ATTN_BWD_COLUMNS);
-  const int64_t k_planes = B * H_kv, q_planes = B * H;
-  // The steps of the longest tiles, and of all of them, at four products for keys and three for queries;
-  // `share` is each resident block's part of it all.
+  const int64_t G = H / H_kv, k_planes = B * H_kv, q_planes = B * H;
+  // Blocks of four waves own 128 columns, 32 a wave. Where there is less than one for each compute unit and
+  // their loops are short, they own 64: two pairs of waves, each of which takes half of a step's rows, so
+  // that a step takes half as long. (Long loops are better cut, below.) 128 and 64 columns (us): 8 heads of 257
+  // causal rows 28 and 23, of 1024 42 and 36, 12 of 900 48 and 38, 10 of 1024 rows of 64 values 39 and 29; 4
+  // of 2048, in parts, 59 and 64.
   const int64_t k_long = G * p.nb_q, q_long = p.nb_kv;
-  const int64_t k_all = k_planes * (causal ? G * (p.nb_q * k_tiles - k_tiles * (k_tiles - 1)) : k_long * k_tiles);
-  const int64_t q_all = q_planes * (causal ? q_tiles * (q_tiles + 1) : q_long * q_tiles);
+  const bool few = k_planes * ceil_div(N_kv, 128) + q_planes * ceil_div(N, 128) <= 256;
+  p.columns = few && k_long <= 24 && q_long <= 24 ? 64 : 128;
+  const int64_t wide = p.columns / ATTN_BWD_ROWS, k_tiles = ceil_div(N_kv, p.columns), q_tiles = ceil_div(N, p.columns);
+  // The steps of the longest tiles, and of all of them, at two products' time for keys and one and a half
+  // for queries, twice that for 128 columns; `share` is each resident block's part of it all.
+  const int64_t k_all = k_planes * (causal ? G * (p.nb_q * k_tiles - wide * k_tiles * (k_tiles - 1) / 2) : k_long * k_tiles);
+  const int64_t q_all = q_planes * (causal ? wide * q_tiles * (q_tiles + 1) / 2 : q_long * q_tiles);
   const int64_t resident = (D == 64 ? 3 : 2) * 256;
-  const int64_t share = (4 * k_all + 3 * q_all) / resident;
+  const int64_t k_cost = 4 * wide, q_cost = 3 * wide;
+  const int64_t share = (k_cost * k_all + q_cost * q_all) / resident;
   // A part may take a little more than that: parts are written in fp32 and read again, and tiles that are all
   // alike fit the card in one go with a fifth more. A tile is cut only where that saves more than the
   // joining launch costs; no part is under 4 steps. Measured, all tiles in as many parts as the longest one
@@ -84,13 +94,14 @@ inline AttnBwdPlan attn_bwd_plan(int64_t B, int64_t H, int64_t H_kv, int64_t N, 
   // 408, 6 heads on 1 of 1541 rows 101 and 93, 4096 causal rows, 32 heads on 8, 472 and 479.
   const int64_t may = share + share / (causal ? 20 : 5);
   auto most = [&](int64_t longest, int64_t cost) {
-    if (longest * cost <= may + 28) return longest;
+    if (longest * cost <= may + 56) return longest;
     const int64_t steps = ceil_div(may, cost);
     return steps < 4 ? (int64_t)4 : steps;
   };
-  p.keys = cut_tiles(k_tiles, k_long, causal ? 2 * G : 0, k_long, most(k_long, 4), k_planes);
-  p.queries = causal ? cut_tiles(q_tiles, 2 * q_tiles, 2, q_long, most(q_long, 3), q_planes)
-                     : cut_tiles(q_tiles, q_long, 0, q_long, most(q_long, 3), q_planes);
+  const int64_t most_k = most(k_long, k_cost), most_q = most(q_long, q_cost);
+  p.keys = cut_tiles(k_tiles, k_long, causal ? wide * G : 0, k_long, most_k, k_planes);
+  p.queries = causal ? cut_tiles(q_tiles, wide * q_tiles, wide, q_long, most_q, q_planes)
+                     : cut_tiles(q_tiles, q_long, 0, q_long, most_q, q_planes);
   return p;
 }
 

@@ -49,24 +49,26 @@ int check(const AttnBwdCut& c, int planes, F steps) {
   return 0;
 }
 int main() {
-  long plans = 0, cut = 0;
+  long plans = 0, cut = 0, narrow = 0;
   const int lengths[] = {1, 2, 63, 64, 65, 128, 129, 257, 500, 777, 1024, 1541, 1777, 2048, 4097, 6449, 11000, 16384, 47520};
   for (int B : {1, 2, 3, 9}) for (int H_kv : {1, 2, 8, 10}) for (int G : {1, 3, 4, 6, 32}) for (int D : {64, 128})
     for (int N : lengths) for (int N_kv : lengths) for (int causal = 0; causal < 2; ++causal) {
       if (causal && N != N_kv) continue;
       if ((long)B * H_kv * G * N > 2000000) continue;
       const AttnBwdPlan p = attn_bwd_plan(B, (long)H_kv * G, H_kv, N, N_kv, D, causal);
-      const int nb = (int)p.nb_q, nk = (int)p.nb_kv, tq = p.queries.tiles;
-      if (p.keys.tiles != (N_kv + 127) / 128 || tq != (N + 127) / 128) return bad("tiles", N, N_kv, tq);
-      if (check(p.keys, B * H_kv, [&](int u) { return G * (nb - (causal ? 2 * u : 0)); })) return 1;
+      const int nb = (int)p.nb_q, nk = (int)p.nb_kv, tq = p.queries.tiles, c = (int)p.columns, wide = c / 64;
+      if (c != 64 && c != 128) return bad("columns", c, 0, 0);
+      if (p.keys.tiles != (N_kv + c - 1) / c || tq != (N + c - 1) / c) return bad("tiles", N, N_kv, tq);
+      if (check(p.keys, B * H_kv, [&](int u) { return G * (nb - (causal ? wide * u : 0)); })) return 1;
       if (check(p.queries, B * H_kv * G, [&](int u) {
-            const int end = 2 * (tq - u);
+            const int end = wide * (tq - u);
             return causal ? (end < nk ? end : nk) : nk;
           })) return 1;
       ++plans;
       cut += p.keys.cut > 0;
+      narrow += wide == 1;
     }
-  std::printf("plans %%ld %%ld\n", plans, cut);
+  std::printf("plans %%ld %%ld %%ld\n", plans, cut, narrow);
   return 0;
 }
 """
@@ -84,8 +86,8 @@ def _run(tmp_path, header):
 def test_every_step_once(tmp_path):
     res = _run(tmp_path, SRC)
     assert res.returncode == 0, res.stdout
-    plans, cut = (int(x) for x in res.stdout.split()[1:])
-    assert plans > 10000 and cut > 2000
+    plans, cut, narrow = (int(x) for x in res.stdout.split()[1:])
+    assert plans > 10000 and cut > 2000 and 500 < narrow < plans - 500
 
 
 def test_a_lost_step_is_found(tmp_path):

@@ -75,6 +75,15 @@ def test_cut_loops_and_full_grids(dtype, D, B, H, H_kv, N, N_kv, causal):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("N,N_kv,causal", [
+    (1, 1, True), (33, 33, True), (64, 64, True), (129, 129, True), (65, 31, False), (31, 130, False)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_planes(dtype, N, N_kv, causal, D):
+    """Short sequences by blocks of 128 columns (few planes take blocks of 64)."""
+    verify(case(20, 16, 8, N, N_kv, D, dtype, causal, "NHD", dlse=not causal, seed=N))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
 def test_strides(dtype):
     """Views of fused projections, head slices, a gradient whose rows lie apart."""
     gen = torch.Generator(device="cuda").manual_seed(3)
