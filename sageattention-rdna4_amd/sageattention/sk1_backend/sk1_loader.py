@@ -422,17 +422,19 @@ class SageLib:
             self._check(-n, "sage_attn_bwd_workspace_bytes")
         return n
 
-    def attn_bwd(self, dtype, causal, read, grads, nhd, lse, dlse, sizes, sm_scale, workspace, stream):
-        """The gradients of q, k, v into `grads` from `read` = (q, k, v, out, dout), (B, H, N, D) tensors
-        or with `nhd` (B, N, H, D) ones; `sizes` = (B, H, N, H_kv, N_kv, D) (see `sage_attn_bwd`)."""
-        views = []
-        for t in read + grads:
-            sb, s1, s2, _ = t.stride()
-            views += (t.data_ptr(), sb, s2, s1) if nhd else (t.data_ptr(), sb, s1, s2)
+    def attn_bwd(self, dtype, causal, read, strides, grads, grad_strides, lse, dlse, sizes, sm_scale,
+                 workspace, stream):
+        """The gradients of q, k, v into `grads` from `read` = (q, k, v, out, dout), each with its (batch,
+        head, row) strides; `sizes` = (B, H, N, H_kv, N_kv, D) (see `sage_attn_bwd`)."""
+        q, k, v, o, g = read
+        qs, ks, vs, os_, gs = strides
+        dq, dk, dv = grads
+        dqs, dks, dvs = grad_strides
         rc = self.lib.sage_attn_bwd(
-            _dtype_code(dtype), int(bool(causal)), *views[:20], lse.data_ptr(),
-            None if dlse is None else dlse.data_ptr(), *views[20:], *sizes, sm_scale,
-            workspace.data_ptr(), workspace.numel(), stream)
+            _dtype_code(dtype), int(bool(causal)), q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs,
+            o.data_ptr(), *os_, g.data_ptr(), *gs, lse.data_ptr(),
+            None if dlse is None else dlse.data_ptr(), dq.data_ptr(), *dqs, dk.data_ptr(), *dks,
+            dv.data_ptr(), *dvs, *sizes, sm_scale, workspace.data_ptr(), workspace.numel(), stream)
         if rc:
             self._check(rc, "sage_attn_bwd")
 

@@ -39,17 +39,27 @@ def _scale(what, sm_scale, D):
 
 
 def _plain(tensors, tensor_layout):
-    """Whether all are contiguous GPU tensors of a served dtype and head_dim, which need no closer look."""
+    """Whether all are contiguous GPU tensors of one served dtype, of one device, of a served head_dim, which
+    need no closer look."""
     if tensor_layout != "HND" and tensor_layout != "NHD":
         return False
+    first = tensors[0]
+    if not isinstance(first, torch.Tensor) or first.dtype not in _DTYPES or not first.is_cuda:
+        return False
+    dtype, device = first.dtype, first.device
     for t in tensors:
-        if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES or not t.is_cuda \
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device \
                 or not t.is_contiguous() or t.data_ptr() & 15:
             return False
         shape = t.shape
-        if len(shape) != 4 or shape[3] not in _HEAD_DIMS or not t.numel():
+        if len(shape) != 4 or shape[3] not in _HEAD_DIMS or 0 in shape:
             return False
     return True
+
+
+def _strides(t, nhd):
+    sb, s1, s2, _ = t.stride()
+    return (sb, s2, s1) if nhd else (sb, s1, s2)
 
 
 def sageattn_backward(dout, q, k, v, out, lse, tensor_layout="HND", is_causal=False, sm_scale=None,
@@ -68,15 +78,16 @@ def sageattn_backward(dout, q, k, v, out, lse, tensor_layout="HND", is_causal=Fa
     """
     what = "sageattn_backward"
     read = (q, k, v, out, dout)
-    if not _plain(read, tensor_layout):
+    plain = _plain(read, tensor_layout)
+    if not plain:
         for name, t in zip(("q", "k", "v", "out", "dout"), read):
             _view(what, tensor_layout, name, t)
+        for name, t in (("k", k), ("v", v), ("out", out), ("dout", dout)):
+            if t.device != q.device:
+                _refuse(what, "device: %s is on %s, q on %s" % (name, t.device, q.device))
+            if t.dtype != q.dtype:
+                _refuse(what, "dtype: %s is %s, q %s" % (name, t.dtype, q.dtype))
     dev, dtype, shape = q.device, q.dtype, q.shape
-    for name, t in (("k", k), ("v", v), ("out", out), ("dout", dout)):
-        if t.device != dev:
-            _refuse(what, "device: %s is on %s, q on %s" % (name, t.device, dev))
-        if t.dtype != dtype:
-            _refuse(what, "dtype: %s is %s, q %s" % (name, t.dtype, dtype))
     if k.shape != v.shape:
         _refuse(what, "shape: k is %s, v %s" % (tuple(k.shape), tuple(v.shape)))
     for name, t in (("out", out), ("dout", dout)):
@@ -97,10 +108,16 @@ def sageattn_backward(dout, q, k, v, out, lse, tensor_layout="HND", is_causal=Fa
         _row_floats(what, "dlse", dlse, (B, H, N), dev)
     sm = _scale(what, sm_scale, D)
     lib = _library(what, dev)
-    grads = tuple([_empty(t) for t in (q, k, v)])
+    grads = (_empty(q), _empty(k), _empty(v))
     work = torch.empty(lib.attn_bwd_workspace_bytes(dtype, bool(is_causal), B, H, N, H_kv, N_kv, D),
                        dtype=torch.uint8, device=dev)
-    _launch(dev, lib.attn_bwd, dtype, is_causal, read, grads, tensor_layout == "NHD", lse, dlse,
+    nhd = tensor_layout == "NHD"
+    # (batch, head, row) strides: of contiguous tensors by their sizes
+    rows, rows_kv = ((N * H * D, D, H * D), (N_kv * H_kv * D, D, H_kv * D)) if nhd else \
+        ((H * N * D, N * D, D), (H_kv * N_kv * D, N_kv * D, D))
+    whole = (rows, rows_kv, rows_kv, rows, rows)
+    strides = whole if plain else [_strides(t, nhd) for t in read]
+    _launch(dev, lib.attn_bwd, dtype, is_causal, read, strides, grads, whole[:3], lse, dlse,
             (B, H, N, H_kv, N_kv, D), sm, work)
     return grads
 
