@@ -341,7 +341,7 @@ int64_t sage_cache_attn_workspace_bytes(int64_t B, int64_t H, int64_t H_kv, int6
                                         int64_t max_pages, int64_t D);
 
 /*
- * Attention's backward pass: the gradients of q, k and v from that of the output, in two or three
+ * Attention's backward pass: the gradients of q, k and v from that of the output, in one to three
  * launches. No counterpart in the reference, whose kernels have no gradients. With
  * P_ij = exp(sm_scale q_i.k_j - lse_i) (0 for j > i when causal) and d_i = dout_i.o_i - dlse_i:
  *   dv_j = sum_i P_ij dout_i,  dS_ij = P_ij (dout_i.v_j - d_i),
@@ -353,7 +353,7 @@ int64_t sage_cache_attn_workspace_bytes(int64_t B, int64_t H, int64_t H_kv, int6
  *                    part of (o and dout are then those of the whole); -infinity: the row saw nothing
  *   dlse             optional (B, H, N) fp32: the gradient of lse
  *   sm_scale         from 1e-30 to 1e30
- *   workspace        sage_attn_bwd_workspace_bytes bytes, 256-byte aligned
+ *   workspace        sage_attn_bwd_workspace_bytes bytes, 256-byte aligned; NULL where that is 0
  * P and dS are rounded to `dtype` ahead of their products (fp16: scaled by powers of two that keep
  * them in range), every sum is fp32, and the results are rounded once. They are the same from call to
  * call. Where P is 0 its other factor has to be finite: 0 times a NaN or an infinity is NaN.
@@ -371,7 +371,7 @@ int sage_attn_bwd(int dtype, int causal,
                   int64_t B, int64_t H, int64_t N, int64_t H_kv, int64_t N_kv, int64_t D,
                   float sm_scale, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Bytes of workspace of a sage_attn_bwd call of these sizes, or -SAGE_ERR_INVALID. */
+/* Bytes of workspace of a sage_attn_bwd call of these sizes (0: none), or -SAGE_ERR_INVALID. */
 int64_t sage_attn_bwd_workspace_bytes(int dtype, int causal, int64_t B, int64_t H, int64_t N,
                                       int64_t H_kv, int64_t N_kv, int64_t D);
 

@@ -7,7 +7,7 @@
 //                                               dK_j = sm_scale sum_i dS_ij q_i.
 // A row whose logsumexp is -infinity saw nothing: its P are zeros.
 //
-// Three launches at most. `rows` works out what S and dP of each row begin with, -lse / sm_scale and -d (a
+// Three launches at most, one in small calls. `rows` works out what S and dP of each row begin with, -lse / sm_scale and -d (a
 // product's first summand, so that neither costs an operation). `main` holds blocks of two kinds: one owns keys and goes over the queries that see them (S, dP, dV, dK), the other owns queries
 // and goes over their keys (S, dP, dQ). Seven products, where one kind of block that adds its dQ
 // to memory would take five: but added atomically, in an order that changes from call to call, and
@@ -110,6 +110,7 @@ struct Args {
   int H, H_kv, G, N, N_kv, NP;         // NP: N rounded up to tiles
   int planes_q, planes_kv, nb_q, nb_kv; // planes; tiles of 64 rows in each
   AttnBwdCut keys, queries;
+  int alone;                            // AttnBwdPlan::alone
   float sm_scale, c;
   // workspace
   float* nl;        // (planes_q, NP): (P_SHIFT - lse log2 e) / c
@@ -125,6 +126,12 @@ struct Args {
 template <typename T>
 __device__ __forceinline__ const T* plane(const Rows& x, int b, int h) {
   return (const T*)x.p + (int64_t)b * x.sb + (int64_t)h * x.sh;
+}
+
+// What a row's S begins with: (P_SHIFT - lse log2 e) / c, nothing seen for a logsumexp of -infinity.
+template <typename T>
+__device__ __forceinline__ float row_start(float lse, float c) {
+  return lse == NEG_INF ? NEG_INF : __builtin_fmaf(-LOG2E_F, lse, P_SHIFT<T>) / c;
 }
 
 // ------------------------------------------------------------------------------------- rows
@@ -176,8 +183,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const Args a) {
       float nl = NEG_INF, nd = 0.0f;
       if (r < n_rows) {
         const int64_t row = (int64_t)p * a.N + r;
-        const float l = a.lse[row];
-        nl = l == NEG_INF ? NEG_INF : __builtin_fmaf(-LOG2E_F, l, P_SHIFT<T>) / a.c;
+        nl = row_start<T>(a.lse[row], a.c);
         nd = (a.dlse ? a.dlse[row] : 0.0f) - dot;
       }
       if (cg == 0) {
@@ -213,16 +219,9 @@ __global__ void __launch_bounds__(256) rows_kernel(const Args a) {
 }
 
 // ------------------------------------------------------------------------------------- main
-// The largest of each list of values, by a block of 256 threads, through K * 4 floats of LDS; NaNs are
-// passed over.
+// Each of the threads' values' largest over a block of 256, through K * 4 floats of LDS; NaNs are passed over.
 template <int K>
-__device__ __forceinline__ void block_max(const float* const (&p)[K], const int (&n)[K], float* lds,
-                                          float (&m)[K]) {
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    m[k] = 0.0f;
-    for (int i = threadIdx.x; i < n[k]; i += 256) m[k] = fmaxf(m[k], p[k][i]);
-  }
+__device__ __forceinline__ void block_max(float* lds, float (&m)[K]) {
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1)
 #pragma unroll
@@ -236,6 +235,12 @@ __device__ __forceinline__ void block_max(const float* const (&p)[K], const int 
   for (int k = 0; k < K; ++k)
     m[k] = fmaxf(fmaxf(lds[4 * k], lds[4 * k + 1]), fmaxf(lds[4 * k + 2], lds[4 * k + 3]));
 }
+// The largest of n values, as far as this thread has seen them.
+__device__ __forceinline__ float largest(const float* p, int n) {
+  float m = 0.0f;
+  for (int i = threadIdx.x; i < n; i += 256) m = fmaxf(m, p[i]);
+  return m;
+}
 
 // The power of two that brings `bound` into [2^13, 2^14) (an infinite or vanishing one: as far as
 // exponents of 100 go).
@@ -248,9 +253,10 @@ __device__ __forceinline__ float scale_for(float bound) {
   return ldexpf(1.0f, min(max(e, -100), 100));
 }
 
-// LDS of a block: two tiles of each of two tensors, and of the rows' two constants.
-template <int D>
-constexpr int LDS_BYTES = 4 * BT * D * 2 + 2 * 2 * BT * 4;
+// LDS of a block: two tiles of each of two tensors, and of the rows' two constants (CW = 2: of all tiles',
+// where the block works them out).
+template <int D, int CW>
+constexpr int LDS_BYTES = 4 * BT * D * 2 + 2 * 2 * BT * 4 + (CW == 2 ? ATTN_BWD_ALONE * 2 * BT * 4 : 0);
 
 // A tile of BT rows of a plane on its way into LDS, a quarter by each wave, 1 KB a request: 64 lanes of
 // 16 bytes, RPI rows.
@@ -433,6 +439,84 @@ __device__ __forceinline__ bool merge_pairs(u8* smem, int w, X&... x) {
   return w < 2;
 }
 
+// A wave works out the constants of a tile's 64 rows (from `g` and `o` on, `left` of them or more): what S and
+// dP begin with, to `to` and to + BT. top: the largest |dout|^2 and |d| so far.
+template <typename T, int D>
+__device__ __forceinline__ void tile_rows(const T* g, int64_t g_sr, const T* o, int64_t o_sr, const float* lse,
+                                          const float* dlse, int left, float c, float* to, int lane,
+                                          float (&top)[2]) {
+  constexpr int CG = D / 8, R = 64 / CG, IT = 8;      // 64 or 32 rows at a time
+  const int cg = lane % CG, rg = lane / CG;
+#pragma unroll 1
+  for (int r0 = rg; r0 < 64; r0 += IT * R) {
+    u32x4 x[IT], y[IT];
+    float l[IT], dl[IT];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int r = min(r0 + i * R, left - 1);
+      x[i] = *(const u32x4*)(g + (int64_t)r * g_sr + 8 * cg);
+      y[i] = *(const u32x4*)(o + (int64_t)r * o_sr + 8 * cg);
+      l[i] = lse[r];
+      dl[i] = dlse ? dlse[r] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      float fx[8], fy[8], dot = 0.0f, sq = 0.0f;
+      unpack8<T>(x[i], fx);
+      unpack8<T>(y[i], fy);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        dot = __builtin_fmaf(fx[e], fy[e], dot);
+        sq = __builtin_fmaf(fx[e], fx[e], sq);
+      }
+#pragma unroll
+      for (int m = 1; m < CG; m <<= 1) {
+        dot += __shfl_xor(dot, m, 64);
+        if (std::is_same_v<T, f16>) sq += __shfl_xor(sq, m, 64);
+      }
+      const int r = r0 + i * R;
+      const bool live = r < left;
+      const float nd = live ? dl[i] - dot : 0.0f;
+      top[0] = fmaxf(top[0], sq);
+      top[1] = fmaxf(top[1], fabsf(nd));
+      if (cg == 0) {
+        to[r] = live ? row_start<T>(l[i], c) : NEG_INF;
+        to[BT + r] = nd;
+      }
+    }
+  }
+}
+
+// The largest |x|^2 of n rows, as far as this thread has seen them.
+template <typename T, int D>
+__device__ __forceinline__ float largest_row(const T* x, int64_t sr, int n) {
+  constexpr int CG = D / 8;
+  const int cg = threadIdx.x % CG;
+  float m = 0.0f;
+  for (int r = threadIdx.x / CG; r < (n + 256 / CG - 1) / (256 / CG) * (256 / CG); r += 256 / CG) {
+    float f[8], sq = 0.0f;
+    unpack8<T>(*(const u32x4*)(x + (int64_t)min(r, n - 1) * sr + 8 * cg), f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sq = __builtin_fmaf(f[e], f[e], sq);
+#pragma unroll
+    for (int s = 1; s < CG; s <<= 1) sq += __shfl_xor(sq, s, 64);
+    m = fmaxf(m, sq);
+  }
+  return m;
+}
+
+// |x|^2 of a lane's column, and x . y of two.
+template <typename T, int D>
+__device__ __forceinline__ float column_dot(const typename Vec<T>::x8 (&x)[D / 16],
+                                            const typename Vec<T>::x8 (&y)[D / 16]) {
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = __builtin_fmaf((float)x[i][e], (float)y[i][e], s);
+  return s + __shfl_xor(s, 32, 64);
+}
+
 // A block that owns 32 CW keys of a K/V head.
 template <typename T, int D, bool CAUSAL, int CW>
 __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
@@ -459,22 +543,24 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
   ti = first + it0 - ti * per;
   const T* pq = plane<T>(a.q, b, h0) + (int64_t)ti * BT * a.q.sr;
   const T* po = plane<T>(a.dout, b, h0) + (int64_t)ti * BT * a.dout.sr;
-  const float* pr = (w & 1 ? a.nd : a.nl) + (int64_t)(b * a.H + h0) * a.NP + ti * BT;
+  const bool alone = CW == 2 && a.alone;
+  float* own_rows = (float*)(smem + 4 * TILE) + 4 * BT;   // alone: constants of all the block's tiles
+  const float* pr = alone ? nullptr : (w & 1 ? a.nd : a.nl) + (int64_t)(b * a.H + h0) * a.NP + ti * BT;
   const int64_t head_q = a.q.sh - (int64_t)per * BT * a.q.sr;
   const int64_t head_o = a.dout.sh - (int64_t)per * BT * a.dout.sr;
   auto request = [&](int buf) {
     const int left = a.N - ti * BT;
     stage(pq, a.q.sr, left, lds0 + buf * TILE);
     stage(po, a.dout.sr, left, lds0 + (2 + buf) * TILE);
-    if (w < 2) dma4(pr, 4 * lane_anew(), lds0 + 4 * TILE + (2 * buf + w) * BT * 4);
+    if (w < 2 && !alone) dma4(pr, 4 * lane_anew(), lds0 + 4 * TILE + (2 * buf + w) * BT * 4);
     pq += BT * a.q.sr;
     po += BT * a.dout.sr;
-    pr += BT;
+    if (!alone) pr += BT;
     if (++ti == a.nb_q) {                            // on to the group's next head
       ti = first;
       pq += head_q;
       po += head_o;
-      pr += first * BT;
+      if (!alone) pr += first * BT;
     }
   };
 
@@ -484,13 +570,28 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
   x8 kf[D / 16], vf[D / 16];
   load_columns<T, D>(plane<T>(a.k, b, hk), a.k.sr, kw, a.N_kv, lane, kf);
   load_columns<T, D>(plane<T>(a.v, b, hk), a.v.sr, kw, a.N_kv, lane, vf);
-  float scale = 1.0f;
-  if (F16) {
+  // the largest |dout|^2, |d| and |v|^2
+  float scale = 1.0f, m[3] = {0.0f, 0.0f, 0.0f};
+  if (alone) {
+    float top[2] = {0.0f, 0.0f};
+    for (int i = w; i < it1 - it0; i += 4) {
+      const int gi = (it0 + i) / per, t = first + it0 + i - gi * per, h = hk * a.G + gi;
+      const int64_t row = (int64_t)(b * a.H + h) * a.N + t * BT;
+      tile_rows<T, D>(plane<T>(a.dout, b, h) + (int64_t)t * BT * a.dout.sr, a.dout.sr,
+                      plane<T>(a.o, b, h) + (int64_t)t * BT * a.o.sr, a.o.sr, a.lse + row,
+                      a.dlse ? a.dlse + row : nullptr, a.N - t * BT, a.c, own_rows + 2 * BT * i, lane, top);
+    }
+    m[0] = top[0];
+    m[1] = top[1];
+    if (F16) m[2] = column_dot<T, D>(vf, vf);
+  } else if (F16) {
     const int64_t hq = (int64_t)(b * a.H + hk * a.G) * a.nb_q;
-    const int nq = a.G * a.nb_q;
-    float m[3];                                      // by way of the second tile's constants
-    block_max<3>({a.max_do + hq, a.max_d + hq, a.max_v + (int64_t)pl * a.nb_kv}, {nq, nq, a.nb_kv},
-                 (float*)(smem + 4 * TILE) + 2 * BT, m);
+    m[0] = largest(a.max_do + hq, a.G * a.nb_q);
+    m[1] = largest(a.max_d + hq, a.G * a.nb_q);
+    m[2] = largest(a.max_v + (int64_t)pl * a.nb_kv, a.nb_kv);
+  }
+  if (F16) {
+    block_max<3>((float*)(smem + 4 * TILE) + 2 * BT, m);   // by way of the second tile's constants
     scale = scale_for(sqrtf(m[0]) * sqrtf(m[2]) + m[1]);
   }
   const float fs = scale * __builtin_ldexpf(1.0f, -(int)P_SHIFT<T>);
@@ -547,7 +648,7 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
     const int q0 = tc * BT;
     tc = ti;
     if (it + 1 < it1) request(buf ^ 1);
-    const float* rows = lds_rows + 2 * buf * BT + 4 * g;
+    const float* rows = (alone ? own_rows + 2 * BT * (it - it0) : lds_rows + 2 * buf * BT) + 4 * g;
 #pragma unroll U<D>
     for (int x = 0; x < CW / 2; ++x) {
       const int u = CW == 4 ? x : w >> 1;
@@ -602,21 +703,24 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
   x8 qf[D / 16], gf[D / 16];
   load_columns<T, D>(plane<T>(a.q, b, h), a.q.sr, qw, a.N, lane, qf);
   load_columns<T, D>(plane<T>(a.dout, b, h), a.dout.sr, qw, a.N, lane, gf);
-  const int64_t row = (int64_t)pl * a.NP + min(qw + (lane & 31), a.NP - 1);
-  float nl1 = a.nl[row], scale = 1.0f;
-  const float nd1 = a.nd[row];
+  float nl1, nd1, scale = 1.0f;
+  if (CW == 2 && a.alone) {
+    x8 of[D / 16];
+    load_columns<T, D>(plane<T>(a.o, b, h), a.o.sr, qw, a.N, lane, of);
+    const int64_t row = (int64_t)pl * a.N + min(qw + (lane & 31), a.N - 1);
+    nl1 = row_start<T>(a.lse[row], a.c);
+    nd1 = (a.dlse ? a.dlse[row] : 0.0f) - column_dot<T, D>(gf, of);
+  } else {
+    const int64_t row = (int64_t)pl * a.NP + min(qw + (lane & 31), a.NP - 1);
+    nl1 = a.nl[row];
+    nd1 = a.nd[row];
+  }
   if (F16) {
-    float sq = 0.0f, mv[1];
-    block_max<1>({a.max_v + (int64_t)(b * a.H_kv + hk) * a.nb_kv}, {a.nb_kv}, (float*)(smem + 4 * TILE), mv);
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = (float)gf[i][e];
-        sq = __builtin_fmaf(x, x, sq);
-      }
-    sq += __shfl_xor(sq, 32, 64);
-    scale = scale_for(sqrtf(sq) * sqrtf(mv[0]) + fabsf(nd1));
+    const int plane_kv = b * a.H_kv + hk;
+    float mv[1] = {CW == 2 && a.alone ? largest_row<T, D>(plane<T>(a.v, b, hk), a.v.sr, a.N_kv)
+                                      : largest(a.max_v + (int64_t)plane_kv * a.nb_kv, a.nb_kv)};
+    block_max<1>((float*)(smem + 4 * TILE), mv);
+    scale = scale_for(sqrtf(column_dot<T, D>(gf, gf)) * sqrtf(mv[0]) + fabsf(nd1));
     // P meets dS alone here: its power of two is part of the exponent
     nl1 += (log2f(scale) - P_SHIFT<T>) / a.c;
   }
@@ -687,7 +791,7 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
 
 template <typename T, int D, bool CAUSAL, int CW>
 __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) main_kernel(const Args a) {
-  __shared__ __align__(1024) u8 smem[LDS_BYTES<D>];
+  __shared__ __align__(1024) u8 smem[LDS_BYTES<D, CW>];
   if ((int)blockIdx.x < a.keys.blocks)
     keys_block<T, D, CAUSAL, CW>(a, smem, blockIdx.x);
   else
@@ -772,10 +876,12 @@ hipError_t launch_join(const Args& a, hipStream_t s) {
 
 template <typename T, int D>
 hipError_t launch(const AttnBwdArgs& x, const AttnBwdPlan& p, const Args& a, hipStream_t s) {
-  const int rows = a.planes_q * a.nb_q + (x.dtype == 0 ? a.planes_kv * a.nb_kv : 0);
-  hipLaunchKernelGGL((rows_kernel<T, D>), dim3(rows), dim3(256), 0, s, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  hipError_t e = hipSuccess;
+  if (!p.alone) {
+    const int rows = a.planes_q * a.nb_q + (x.dtype == 0 ? a.planes_kv * a.nb_kv : 0);
+    hipLaunchKernelGGL((rows_kernel<T, D>), dim3(rows), dim3(256), 0, s, a);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
   if (p.columns == 128)
     launch_main<T, D, 4>(a, x.causal, s);
   else
@@ -796,9 +902,9 @@ Offsets64 offsets(const AttnBwdPlan& p, int dtype, int64_t planes_q, int64_t pla
     at += (floats * 4 + 255) / 256 * 256;
     return was;
   };
-  const bool f16 = dtype == 0;
-  o.nl = take(planes_q * p.nb_q * BT);
-  o.nd = take(planes_q * p.nb_q * BT);
+  const bool f16 = dtype == 0 && !p.alone;
+  o.nl = take(p.alone ? 0 : planes_q * p.nb_q * BT);
+  o.nd = take(p.alone ? 0 : planes_q * p.nb_q * BT);
   o.max_do = take(f16 ? planes_q * p.nb_q : 0);
   o.max_d = take(f16 ? planes_q * p.nb_q : 0);
   o.max_v = take(f16 ? planes_kv * p.nb_kv : 0);
@@ -843,6 +949,7 @@ hipError_t launch_attn_bwd(const AttnBwdArgs& x, hipStream_t s) {
   a.planes_kv = (int)(x.B * x.H_kv);
   a.keys = p.keys;
   a.queries = p.queries;
+  a.alone = p.alone;
   a.sm_scale = x.sm_scale;
   a.c = x.sm_scale * LOG2E_F;
   const Offsets64 o = offsets(p, x.dtype, a.planes_q, a.planes_kv, x.D);

@@ -16,7 +16,7 @@
 
 namespace sage {
 
-constexpr int ATTN_BWD_ROWS = 64, ATTN_BWD_SEGMENTS = 32;
+constexpr int ATTN_BWD_ROWS = 64, ATTN_BWD_SEGMENTS = 32, ATTN_BWD_ALONE = 6;
 
 // One kind of block's tiles, the longest first. Those of `parts` parts come first, end[0] of them, then
 // those of one part less, up to tile end[1], and so on; from tile `cut` on they are whole. Blocks are numbered
@@ -27,6 +27,7 @@ struct AttnBwdCut {
 };
 struct AttnBwdPlan {
   int64_t columns;            // of a tile
+  bool alone;                 // no launch ahead: blocks work out their rows' constants by themselves
   int64_t nb_q, nb_kv;        // steps in a plane of queries, of keys
   AttnBwdCut keys, queries;
 };
@@ -79,6 +80,12 @@ inline AttnBwdPlan attn_bwd_plan(int64_t B, int64_t H, int64_t H_kv, int64_t N, 
   const int64_t k_long = G * p.nb_q, q_long = p.nb_kv;
   const bool few = k_planes * ceil_div(N_kv, 128) + q_planes * ceil_div(N, 128) <= 256;
   p.columns = few && k_long <= 24 && q_long <= 24 ? 64 : 128;
+  // With loops this short a block also works out its rows' constants, a tile a wave, which takes about as long
+  // as a launch ahead but spares the host one (8 heads, in a graph, so and with a launch: 128 rows of 64
+  // values 8.6 and 9.7 us, 257 12.8 and 11.8, 512 15.5 and 13.8, 128 rows of 128 values 14.6 and 13.7, 257
+  // 22.5 and 17.4; a call takes the host 13.0 and 16.4 us).
+  const int64_t steps = ATTN_BWD_ALONE * 64 / D;
+  p.alone = p.columns == 64 && k_long <= steps && q_long <= steps;
   const int64_t wide = p.columns / ATTN_BWD_ROWS, k_tiles = ceil_div(N_kv, p.columns), q_tiles = ceil_div(N, p.columns);
   // The steps of the longest tiles, and of all of them, at two products' time for keys and one and a half
   // for queries, twice that for 128 columns; `share` is each resident block's part of it all.

@@ -865,7 +865,7 @@ int sage_attn_bwd(int dtype, int causal, const void* q, int64_t q_sb, int64_t q_
     return fail(SAGE_ERR_INVALID, "sm_scale: must lie between 1e-30 and 1e30 (got %g)", (double)sm_scale);
   const int64_t need = sage::attn_bwd_workspace_bytes(
       sage::attn_bwd_plan(B, H, H_kv, N, N_kv, D, causal != 0), dtype, B * H, B * H_kv, D);
-  if (workspace == nullptr || workspace_bytes < (size_t)need || ((uintptr_t)workspace & 255u))
+  if (need && (workspace == nullptr || workspace_bytes < (size_t)need || ((uintptr_t)workspace & 255u)))
     return fail(SAGE_ERR_INVALID, "workspace: need %lld bytes, 256-byte aligned (got %zu)",
                 (long long)need, workspace_bytes);
   a.dtype = dtype;

@@ -423,7 +423,7 @@ class SageLib:
         return n
 
     def attn_bwd(self, dtype, causal, read, strides, grads, grad_strides, lse, dlse, sizes, sm_scale,
-                 workspace, stream):
+                 workspace, workspace_bytes, stream):
         """The gradients of q, k, v into `grads` from `read` = (q, k, v, out, dout), each with its (batch,
         head, row) strides; `sizes` = (B, H, N, H_kv, N_kv, D) (see `sage_attn_bwd`)."""
         q, k, v, o, g = read
@@ -434,7 +434,8 @@ class SageLib:
             _dtype_code(dtype), int(bool(causal)), q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs,
             o.data_ptr(), *os_, g.data_ptr(), *gs, lse.data_ptr(),
             None if dlse is None else dlse.data_ptr(), dq.data_ptr(), *dqs, dk.data_ptr(), *dks,
-            dv.data_ptr(), *dvs, *sizes, sm_scale, workspace.data_ptr(), workspace.numel(), stream)
+            dv.data_ptr(), *dvs, *sizes, sm_scale, None if workspace is None else workspace.data_ptr(),
+            workspace_bytes, stream)
         if rc:
             self._check(rc, "sage_attn_bwd")
 

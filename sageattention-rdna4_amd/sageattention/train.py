@@ -5,7 +5,7 @@
 
 `sageattn_backward` is the pass itself, for a program that keeps the forward call's output and
 logsumexp on its own. It recomputes the probabilities from Q, K and the logsumexp in 16 bits (the
-forward call's 8-bit codes are not kept), takes two or three launches on the current stream and
+forward call's 8-bit codes are not kept), takes one to three launches on the current stream and
 synchronizes nothing, so that it can be captured into a graph. A call that is not served raises
 `ValueError` with the reason.
 """
@@ -109,8 +109,8 @@ def sageattn_backward(dout, q, k, v, out, lse, tensor_layout="HND", is_causal=Fa
     sm = _scale(what, sm_scale, D)
     lib = _library(what, dev)
     grads = (_empty(q), _empty(k), _empty(v))
-    work = torch.empty(lib.attn_bwd_workspace_bytes(dtype, bool(is_causal), B, H, N, H_kv, N_kv, D),
-                       dtype=torch.uint8, device=dev)
+    size = lib.attn_bwd_workspace_bytes(dtype, bool(is_causal), B, H, N, H_kv, N_kv, D)
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     nhd = tensor_layout == "NHD"
     # (batch, head, row) strides: of contiguous tensors by their sizes
     rows, rows_kv = ((N * H * D, D, H * D), (N_kv * H_kv * D, D, H_kv * D)) if nhd else \
@@ -118,7 +118,7 @@ def sageattn_backward(dout, q, k, v, out, lse, tensor_layout="HND", is_causal=Fa
     whole = (rows, rows_kv, rows_kv, rows, rows)
     strides = whole if plain else [_strides(t, nhd) for t in read]
     _launch(dev, lib.attn_bwd, dtype, is_causal, read, strides, grads, whole[:3], lse, dlse,
-            (B, H, N, H_kv, N_kv, D), sm, work)
+            (B, H, N, H_kv, N_kv, D), sm, work, size)
     return grads
 
 

@@ -171,6 +171,48 @@ def test_scales_of_the_scores(dtype, sm):
     verify(case(1, 2, 2, 129, 129, 64, dtype, True, sm=sm))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D,H,H_kv,N,N_kv,causal", [
+    (64, 6, 2, 100, 100, True), (64, 4, 2, 130, 384, False), (64, 3, 1, 1, 33, False), (128, 4, 4, 192, 192, True),
+    (128, 6, 2, 60, 150, False), (64, 2, 2, 384, 384, True)])
+def test_small_calls_in_one_launch(dtype, D, H, H_kv, N, N_kv, causal):
+    """Blocks that work out their rows' constants by themselves: shared heads, ragged ends, rows that saw nothing,
+    rows that lie apart."""
+    from sageattention.sk1_backend.sk1_loader import SageLib
+    assert SageLib.get().attn_bwd_workspace_bytes(dtype, causal, 1, H, N, H_kv, N_kv, D) == 0
+    c = case(1, H, H_kv, N, N_kv, D, dtype, causal, "NHD", dlse=True, seed=D)
+    empty = torch.rand(1, H, N, device="cuda") < 0.2
+    c["lse"] = c["lse"].masked_fill(empty, -torch.inf)
+    for n in ("dout", "out", "q"):
+        wide = torch.zeros(1, N, H, D + 8, dtype=dtype, device="cuda")
+        wide[..., :D] = c[n]
+        c[n] = wide[..., :D]
+    got = verify(c)
+    assert (got[0].transpose(1, 2)[empty] == 0).all()
+    assert all(torch.equal(a, b) for a, b in zip(got, verify(c)))
+
+
+@pytest.mark.parametrize("dtype,N_kv", [(F16, 131073), (BF16, 100000)])
+def test_long_keys_and_long_queries(dtype, N_kv):
+    """A few queries on many keys, and many queries on a few keys."""
+    verify(case(1, 2, 1, 3, N_kv, 128, dtype, False))
+    verify(case(1, 2, 1, N_kv, 5, 64, dtype, False))
+
+
+def test_keys_past_32_bits():
+    """K and V whose rows lie past 2^31 elements: heads of a long cache in 16 bits."""
+    N_kv, heads = 300000, 60
+    store = torch.zeros(1, N_kv, heads, 128, dtype=BF16, device="cuda")
+    assert store.numel() > 1 << 31
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for h in (3, 59):
+        store[:, :, h] = torch.randn(1, N_kv, 128, generator=gen, device="cuda").to(BF16)
+    c = case(1, 1, 1, 40, 64, 128, BF16, False, "NHD")
+    k, v = store[:, :, 59:], store[:, :, 3:4]
+    o, lse = forward(*(t.transpose(1, 2) for t in (c["q"], k, v)), False, 128 ** -0.5)
+    verify(dict(c, k=k, v=v, out=o.to(BF16).transpose(1, 2), lse=lse.float()))
+
+
 def test_zero_gradient_is_zero():
     from sageattention import sageattn_backward
     for dtype in (F16, BF16):

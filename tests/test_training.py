@@ -64,11 +64,13 @@ def test_backward_checks(lib):
     _refused(lib, call(dlse=ctypes.c_void_p(2)), b"4-byte")
     for scale in (0.0, -1.0, float("nan"), float("inf"), 1e-31, 1e31):
         _refused(lib, call(scale=scale), b"sm_scale")
-    _refused(lib, call(work=None), b"workspace")
-    _refused(lib, call(work=ctypes.c_void_p(64)), b"workspace")
-    need = lib.sage_attn_bwd_workspace_bytes(1, 0, 1, 4, 100, 2, 80, 64)
-    assert need >= 2 * 4 * 128 * 4
-    _refused(lib, call(size=need - 1), b"need %d bytes" % need)
+    large = dict(N=1000, N_kv=800)
+    _refused(lib, call(work=None, **large), b"workspace")
+    _refused(lib, call(work=ctypes.c_void_p(64), **large), b"workspace")
+    need = lib.sage_attn_bwd_workspace_bytes(1, 0, 1, 4, 1000, 2, 800, 64)
+    assert need >= 2 * 4 * 1024 * 4
+    _refused(lib, call(size=need - 1, **large), b"need %d bytes" % need)
+    assert lib.sage_attn_bwd_workspace_bytes(0, 0, 1, 4, 100, 2, 80, 64) == 0      # small calls need none
     _refused(lib, call(B=1 << 14, H=1 << 10), b"grid")
 
 
