@@ -7,8 +7,9 @@
 //                                               dK_j = sm_scale sum_i dS_ij q_i.
 // A row whose logsumexp is -infinity saw nothing: its P are zeros.
 //
-// Three launches at most, one in small calls. `rows` works out what S and dP of each row begin with, -lse / sm_scale and -d (a
-// product's first summand, so that neither costs an operation). `main` holds blocks of two kinds: one owns keys and goes over the queries that see them (S, dP, dV, dK), the other owns queries
+// Three launches at most, one in small calls. `rows` works out what S and dP of each row begin with,
+// -lse / sm_scale and -d (a product's first summand, so that neither costs an operation). `main` holds blocks
+// of two kinds: one owns keys and goes over the queries that see them (S, dP, dV, dK), the other owns queries
 // and goes over their keys (S, dP, dQ). Seven products, where one kind of block that adds its dQ
 // to memory would take five: but added atomically, in an order that changes from call to call, and
 // with 4 bytes read and written per pair of query and key in fp32. Where there are too few blocks for
