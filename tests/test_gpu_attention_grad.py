@@ -181,7 +181,7 @@ def test_small_calls_in_one_launch(dtype, D, H, H_kv, N, N_kv, causal):
     from sageattention.sk1_backend.sk1_loader import SageLib
     assert SageLib.get().attn_bwd_workspace_bytes(dtype, causal, 1, H, N, H_kv, N_kv, D) == 0
     c = case(1, H, H_kv, N, N_kv, D, dtype, causal, "NHD", dlse=True, seed=D)
-    empty = torch.rand(1, H, N, device="cuda") < 0.2
+    empty = torch.rand(1, H, N, generator=torch.Generator("cuda").manual_seed(1), device="cuda") < 0.2
     c["lse"] = c["lse"].masked_fill(empty, -torch.inf)
     for n in ("dout", "out", "q"):
         wide = torch.zeros(1, N, H, D + 8, dtype=dtype, device="cuda")
@@ -190,6 +190,34 @@ def test_small_calls_in_one_launch(dtype, D, H, H_kv, N, N_kv, causal):
     got = verify(c)
     assert (got[0].transpose(1, 2)[empty] == 0).all()
     assert all(torch.equal(a, b) for a, b in zip(got, verify(c)))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("B,H,H_kv,N,N_kv,layout", [
+    (1, 2, 2, 1600, 77, "NHD"), (2, 3, 1, 1541, 128, "HND"), (1, 4, 2, 1000, 64, "NHD"), (1, 2, 1, 1777, 65, "HND"),
+    (1, 4, 4, 1537, 1, "HND"), (1, 1, 1, 1999, 33, "NHD"), (40, 10, 10, 63, 96, "HND"), (3, 48, 12, 257, 97, "NHD"),
+    (2, 40, 40, 1300, 17, "HND")])
+def test_few_keys(dtype, B, H, H_kv, N, N_kv, layout):
+    """Many queries on keys that one block holds: key counts around its tiles and its waves, ragged queries, shared
+    heads, rows that saw nothing, one part and many."""
+    c = case(B, H, H_kv, N, N_kv, 64, dtype, False, layout, dlse=True, seed=N_kv)
+    empty = torch.rand(B, H, N, generator=torch.Generator("cuda").manual_seed(2), device="cuda") < 0.1
+    c["lse"] = c["lse"].masked_fill(empty, -torch.inf)
+    got = verify(c)
+    dq = got[0] if layout == "HND" else got[0].transpose(1, 2)
+    assert (dq[empty] == 0).all()
+    assert all(torch.equal(a, b) for a, b in zip(got, verify(c)))
+
+
+def test_few_keys_of_rows_of_unlike_size():
+    """Each query's dS has a power of two of its own for dQ: gradients 2^-8 times their neighbours' lose nothing."""
+    c = case(1, 2, 2, 1600, 77, 64, F16, False)
+    small = torch.arange(1600, device="cuda") % 2 == 1
+    c["dout"] = torch.where(small[:, None], c["dout"] * 2.0 ** -8, c["dout"])
+    whole = verify(c)[0]
+    c["dout"] = torch.where(small[:, None], c["dout"], torch.zeros_like(c["dout"]))
+    alone = verify(c)[0]
+    assert torch.equal(whole[:, :, small], alone[:, :, small])
 
 
 @pytest.mark.parametrize("dtype,N_kv", [(F16, 131073), (BF16, 100000)])
