@@ -341,7 +341,7 @@ int64_t sage_cache_attn_workspace_bytes(int64_t B, int64_t H, int64_t H_kv, int6
                                         int64_t max_pages, int64_t D);
 
 /*
- * Attention's backward pass: the gradients of q, k and v from that of the output, in one to three
+ * Attention's backward pass: the gradients of q, k and v from that of the output, in one to four
  * launches. No counterpart in the reference, whose kernels have no gradients. With
  * P_ij = exp(sm_scale q_i.k_j - lse_i) (0 for j > i when causal) and d_i = dout_i.o_i - dlse_i:
  *   dv_j = sum_i P_ij dout_i,  dS_ij = P_ij (dout_i.v_j - d_i),
@@ -349,11 +349,14 @@ int64_t sage_cache_attn_workspace_bytes(int64_t B, int64_t H, int64_t H_kv, int6
  * k's and v's summed over the query heads of their group.
  *   q, o, dout, dq   logical (B, H, N, D) views, D = 64 or 128; k, v, dk, dv (B, H_kv, N_kv, D); rows
  *                    less than 2^24 elements apart; the outputs overlap nothing else
- *   lse              (B, H, N) fp32: the forward call's, or that of a larger set of keys that these are
- *                    part of (o and dout are then those of the whole); -infinity: the row saw nothing
+ *   o, lse           both NULL: worked out anew, as those of attention on q, k and v (sage_attn_fwd_ex's are
+ *                    those of 8-bit scores, which P is not formed from). Or lse (B, H, N) fp32, the logsumexp
+ *                    of the 16-bit scores, or that of a larger set of keys that these are part of (o and dout
+ *                    are then those of the whole); -infinity: the row saw nothing
  *   dlse             optional (B, H, N) fp32: the gradient of lse
  *   sm_scale         from 1e-30 to 1e30
- *   workspace        sage_attn_bwd_workspace_bytes bytes, 256-byte aligned; NULL where that is 0
+ *   workspace        sage_attn_bwd_workspace_bytes bytes (without o and lse
+ *                    sage_attn_bwd_anew_workspace_bytes), 256-byte aligned; NULL where that is 0
  * P and dS are rounded to `dtype` ahead of their products (fp16: scaled by powers of two that keep
  * them in range), every sum is fp32, and the results are rounded once. They are the same from call to
  * call. Where P is 0 its other factor has to be finite: 0 times a NaN or an infinity is NaN.
@@ -371,9 +374,12 @@ int sage_attn_bwd(int dtype, int causal,
                   int64_t B, int64_t H, int64_t N, int64_t H_kv, int64_t N_kv, int64_t D,
                   float sm_scale, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Bytes of workspace of a sage_attn_bwd call of these sizes (0: none), or -SAGE_ERR_INVALID. */
+/* Bytes of workspace of a sage_attn_bwd call of these sizes (0: none), or -SAGE_ERR_INVALID; `anew`: of a
+ * call without o and lse. */
 int64_t sage_attn_bwd_workspace_bytes(int dtype, int causal, int64_t B, int64_t H, int64_t N,
                                       int64_t H_kv, int64_t N_kv, int64_t D);
+int64_t sage_attn_bwd_anew_workspace_bytes(int dtype, int causal, int64_t B, int64_t H, int64_t N,
+                                           int64_t H_kv, int64_t N_kv, int64_t D);
 
 /*
  * Root-mean-square norm of d0 x d1 x d2 rows of n values, in one launch. No counterpart in the reference.

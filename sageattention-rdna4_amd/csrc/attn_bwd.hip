@@ -7,7 +7,12 @@
 //                                               dK_j = sm_scale sum_i dS_ij q_i.
 // A row whose logsumexp is -infinity saw nothing: its P are zeros.
 //
-// Three launches at most, one in small calls. `rows` works out what S and dP of each row begin with,
+// A call without output and logsumexp (that of a forward pass by 8-bit scores, whose logsumexp is not that of
+// the scores formed here) works out both anew: `stats` goes over a query's keys once with a running maximum, for
+//     lse_i = log sum_j exp(sm_scale q_i.k_j),      d_i = sum_j P_ij dout_i.v_j - dlse_i,
+// so that a row's P sum to 1 and its dS to dlse_i, however far the scores spread and whatever K's mean.
+//
+// Four launches at most, one in small calls. `rows` works out what S and dP of each row begin with,
 // -lse / sm_scale and -d (a product's first summand, so that neither costs an operation). `main` holds blocks
 // of two kinds: one owns keys and goes over the queries that see them (S, dP, dV, dK), the other owns queries
 // and goes over their keys (S, dP, dQ). Seven products, where one kind of block that adds its dQ
@@ -112,6 +117,7 @@ struct Args {
   int planes_q, planes_kv, nb_q, nb_kv; // planes; tiles of 64 rows in each
   AttnBwdCut keys, queries;
   int alone;                            // AttnBwdPlan::alone
+  int columns;                          // of a tile
   float sm_scale, c;
   // workspace
   float* nl;        // (planes_q, NP): (P_SHIFT - lse log2 e) / c
@@ -119,6 +125,7 @@ struct Args {
   float* max_do;    // fp16: (planes_q, nb_q): a tile's largest |dout|^2, |d|, and (planes_kv, nb_kv) |v|^2
   float* max_d;
   float* max_v;
+  float* stats;     // without lse: (3, queries.blocks, 128): a part's largest score, sum of weights, of weights times dP
   float* part_k;    // (keys.cut_blocks, columns, D): sums of dK, of dV, by blocks that hold a part of their tile
   float* part_v;
   float* part_q;    // (queries.cut_blocks, columns, D)
@@ -135,9 +142,22 @@ __device__ __forceinline__ float row_start(float lse, float c) {
   return lse == NEG_INF ? NEG_INF : __builtin_fmaf(-LOG2E_F, lse, P_SHIFT<T>) / c;
 }
 
+// A row's largest score m, and over its keys the sums l of the weights exp2(c (score - m)) and t of weights times dP;
+// nothing seen yet.
+struct Stats {
+  float m = -3e38f, l = 0.0f, t = 0.0f;
+  __device__ __forceinline__ void add(const Stats& x, float c) {
+    const float top = fmaxf(m, x.m);
+    const float f = __builtin_amdgcn_exp2f((m - top) * c), g = __builtin_amdgcn_exp2f((x.m - top) * c);
+    l = l * f + x.l * g;
+    t = t * f + x.t * g;
+    m = top;
+  }
+};
+
 // ------------------------------------------------------------------------------------- rows
-// 64 rows of a plane per block, D / 8 lanes to a row.
-template <typename T, int D>
+// 64 rows of a plane per block, D / 8 lanes to a row. ANEW: the constants come from what `stats` left.
+template <typename T, int D, bool ANEW>
 __global__ void __launch_bounds__(256) rows_kernel(const Args a) {
   constexpr int CG = D / 8, R = 64 / CG, IT = 16 / R;
   constexpr bool F16 = std::is_same_v<T, f16>;
@@ -162,7 +182,15 @@ __global__ void __launch_bounds__(256) rows_kernel(const Args a) {
     const int r = min(r0 + i * R + rg, n_rows - 1);
     x[i] = *(const u32x4*)(px + (int64_t)r * first.sr);
     y[i] = x[i];
-    if (!of_v) y[i] = *(const u32x4*)(py + (int64_t)r * a.o.sr);
+    if (!ANEW && !of_v) y[i] = *(const u32x4*)(py + (int64_t)r * a.o.sr);
+  }
+  // ANEW: where the parts of the block's rows lie (all in one tile)
+  const float* stats = a.stats;
+  int parts = 0;
+  if (ANEW && !of_v) {
+    const int tile = (at - p * nb) * 64 / a.columns;
+    const int block = attn_bwd_first_part(a.queries, a.queries.tiles - 1 - tile, a.planes_q, parts) + p;
+    stats += (int64_t)block * 128 - tile * a.columns;
   }
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
@@ -182,10 +210,36 @@ __global__ void __launch_bounds__(256) rows_kernel(const Args a) {
     }
     if (!of_v) {
       float nl = NEG_INF, nd = 0.0f;
+      if (ANEW) {
+        // each of the row's lanes takes some parts (and, of blocks of two pairs of waves, both pairs' sums)
+        const int64_t all = (int64_t)a.queries.blocks * 128, step = (int64_t)a.planes_q * 128;
+        const int pairs = 128 / a.columns;
+        Stats sum;
+        for (int k = cg; k < parts * pairs; k += CG) {
+          const float* f = stats + k / pairs * step + k % pairs * a.columns + min(r, n_rows - 1);
+          Stats x;
+          x.m = f[0];
+          x.l = f[all];
+          x.t = f[2 * all];
+          sum.add(x, a.c);
+        }
+#pragma unroll
+        for (int m = 1; m < CG; m <<= 1) {
+          Stats x;
+          x.m = __shfl_xor(sum.m, m, 64);
+          x.l = __shfl_xor(sum.l, m, 64);
+          x.t = __shfl_xor(sum.t, m, 64);
+          sum.add(x, a.c);
+        }
+        nl = (P_SHIFT<T> - log2f(sum.l)) / a.c - sum.m;
+        dot = sum.t / sum.l;
+      }
       if (r < n_rows) {
         const int64_t row = (int64_t)p * a.N + r;
-        nl = row_start<T>(a.lse[row], a.c);
+        if (!ANEW) nl = row_start<T>(a.lse[row], a.c);
         nd = (a.dlse ? a.dlse[row] : 0.0f) - dot;
+      } else {
+        nl = NEG_INF;
       }
       if (cg == 0) {
         a.nl[(int64_t)p * a.NP + r] = nl;
@@ -790,6 +844,95 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
                       at.parts == 1 ? nullptr : a.part_q + (int64_t)block * BC * D, q0, w, a.N);
 }
 
+// ------------------------------------------------------------------------------------- stats
+// The queries' blocks of the main launch, cut in the same way: S and dP alone, and their sums. Each half of a
+// wave has every other four keys of its 32 queries, each pair of waves (CW = 2) half of a step's.
+template <typename T, int D, bool CAUSAL, int CW>
+__global__ void __launch_bounds__(256, D == 64 ? 4 : 2) stats_kernel(const Args a) {
+  constexpr int TILE = BT * D * 2, BC = 32 * CW;
+  typedef typename Vec<T>::x8 x8;
+  __shared__ __align__(1024) u8 smem[4 * TILE];        // two tiles of K, two of V
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const AttnBwdPlace at = attn_bwd_place(a.queries, blockIdx.x, a.planes_q);
+  const int pl = at.plane, b = pl / a.H, h = pl - b * a.H, hk = h / a.G;
+  const int q0 = (a.queries.tiles - 1 - at.u) * BC, qw = q0 + 32 * (w % CW);
+  const int n = CAUSAL ? min((q0 + BC) / BT, a.nb_kv) : a.nb_kv;
+  const int it0 = at.first(n), it1 = at.end(n);
+  const uint32_t lds0 = lds_addr(smem);
+  const T* pk = plane<T>(a.k, b, hk) + (int64_t)it0 * BT * a.k.sr;
+  const T* pv = plane<T>(a.v, b, hk) + (int64_t)it0 * BT * a.v.sr;
+  const Staging<T, D> stage(lane, w);
+  auto request = [&](int it, int buf) {
+    const int left = a.N_kv - it * BT;
+    stage(pk, a.k.sr, left, lds0 + buf * TILE);
+    stage(pv, a.v.sr, left, lds0 + (2 + buf) * TILE);
+    pk += BT * a.k.sr;
+    pv += BT * a.v.sr;
+  };
+  if (it0 < it1) request(it0, 0);
+  const Offsets<D> offsets(lane);
+  x8 qf[D / 16], gf[D / 16];
+  load_columns<T, D>(plane<T>(a.q, b, h), a.q.sr, qw, a.N, lane, qf);
+  load_columns<T, D>(plane<T>(a.dout, b, h), a.dout.sr, qw, a.N, lane, gf);
+  Stats sum;
+  // 32 keys from ku on, which lie at `at`
+  auto step = [&](int ku, int at) {
+    const Offsets<D> of = offsets.rows(at);
+    f32x16 s, dp;
+    clear(s);
+    clear(dp);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) s = mfma16(row_operand<T>(smem, of.row, at, i), qf[i], s);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) dp = mfma16(row_operand<T>(smem, of.row, at + 2 * TILE, i), gf[i], dp);
+    if (ku + 31 >= (CAUSAL ? qw + 1 : a.N_kv)) {
+      const int l = lane_anew(), query = qw + (l & 31);
+      const int left = (CAUSAL ? min(query + 1, a.N_kv) : a.N_kv) - ku - 4 * (l >> 5);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (8 * (r / 4) + r % 4 >= left) s[r] = NEG_INF;
+    }
+    float top = sum.m;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+    const float f = __builtin_amdgcn_exp2f((sum.m - top) * a.c);
+    sum.m = top;
+    float l = 0.0f, t = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float p = __builtin_amdgcn_exp2f((s[r] - top) * a.c);
+      l += p;
+      t = __builtin_fmaf(p, dp[r], t);
+    }
+    sum.l = __builtin_fmaf(sum.l, f, l);
+    sum.t = __builtin_fmaf(sum.t, f, t);
+  };
+  __builtin_amdgcn_s_waitcnt(0);                       // as in keys_block
+  const int end = CAUSAL ? min(qw + 32, a.N_kv) : a.N_kv;
+  for (int it = it0; it < it1; ++it) {
+    const int buf = (it - it0) & 1;
+    next_tile();
+    if (it + 1 < it1) request(it + 1, buf ^ 1);
+#pragma unroll 1
+    for (int x = 0; x < CW / 2; ++x) {
+      const int u = CW == 4 ? x : w >> 1;
+      if (it * BT + 32 * u < end) step(it * BT + 32 * u, (buf * BT + 32 * u) * D * 2);
+    }
+  }
+  Stats x;
+  x.m = __shfl_xor(sum.m, 32, 64);
+  x.l = __shfl_xor(sum.l, 32, 64);
+  x.t = __shfl_xor(sum.t, 32, 64);
+  sum.add(x, a.c);
+  if (lane < 32) {
+    const int64_t all = (int64_t)a.queries.blocks * 128;
+    float* to = a.stats + (int64_t)blockIdx.x * 128 + 32 * w + lane;
+    to[0] = sum.m;
+    to[all] = sum.l;
+    to[2 * all] = sum.t;
+  }
+}
+
 template <typename T, int D, bool CAUSAL, int CW>
 __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) main_kernel(const Args a) {
   __shared__ __align__(1024) u8 smem[LDS_BYTES<D, CW>];
@@ -875,14 +1018,29 @@ hipError_t launch_join(const Args& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+template <typename T, int D, int CW>
+void launch_stats(const Args& a, bool causal, hipStream_t s) {
+  if (causal)
+    hipLaunchKernelGGL((stats_kernel<T, D, true, CW>), dim3(a.queries.blocks), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((stats_kernel<T, D, false, CW>), dim3(a.queries.blocks), dim3(256), 0, s, a);
+}
+
 template <typename T, int D>
 hipError_t launch(const AttnBwdArgs& x, const AttnBwdPlan& p, const Args& a, hipStream_t s) {
   hipError_t e = hipSuccess;
-  if (!p.alone) {
-    const int rows = a.planes_q * a.nb_q + (x.dtype == 0 ? a.planes_kv * a.nb_kv : 0);
-    hipLaunchKernelGGL((rows_kernel<T, D>), dim3(rows), dim3(256), 0, s, a);
+  const int rows = a.planes_q * a.nb_q + (x.dtype == 0 ? a.planes_kv * a.nb_kv : 0);
+  if (!x.lse) {
+    if (p.columns == 128)
+      launch_stats<T, D, 4>(a, x.causal, s);
+    else
+      launch_stats<T, D, 2>(a, x.causal, s);
     if ((e = hipGetLastError()) != hipSuccess) return e;
+    hipLaunchKernelGGL((rows_kernel<T, D, true>), dim3(rows), dim3(256), 0, s, a);
+  } else if (!p.alone) {
+    hipLaunchKernelGGL((rows_kernel<T, D, false>), dim3(rows), dim3(256), 0, s, a);
   }
+  if ((e = hipGetLastError()) != hipSuccess) return e;
   if (p.columns == 128)
     launch_main<T, D, 4>(a, x.causal, s);
   else
@@ -893,9 +1051,9 @@ hipError_t launch(const AttnBwdArgs& x, const AttnBwdPlan& p, const Args& a, hip
 
 // The workspace's parts, each from a multiple of 256 bytes on.
 struct Offsets64 {
-  int64_t nl, nd, max_do, max_d, max_v, part_k, part_v, part_q, end;
+  int64_t nl, nd, max_do, max_d, max_v, stats, part_k, part_v, part_q, end;
 };
-Offsets64 offsets(const AttnBwdPlan& p, int dtype, int64_t planes_q, int64_t planes_kv, int64_t D) {
+Offsets64 offsets(const AttnBwdPlan& p, int dtype, bool anew, int64_t planes_q, int64_t planes_kv, int64_t D) {
   Offsets64 o;
   int64_t at = 0;
   auto take = [&](int64_t floats) {
@@ -909,6 +1067,7 @@ Offsets64 offsets(const AttnBwdPlan& p, int dtype, int64_t planes_q, int64_t pla
   o.max_do = take(f16 ? planes_q * p.nb_q : 0);
   o.max_d = take(f16 ? planes_q * p.nb_q : 0);
   o.max_v = take(f16 ? planes_kv * p.nb_kv : 0);
+  o.stats = take(anew ? 3 * (int64_t)p.queries.blocks * 128 : 0);
   o.part_k = take((int64_t)p.keys.cut_blocks * p.columns * D);
   o.part_v = take((int64_t)p.keys.cut_blocks * p.columns * D);
   o.part_q = take((int64_t)p.queries.cut_blocks * p.columns * D);
@@ -918,13 +1077,13 @@ Offsets64 offsets(const AttnBwdPlan& p, int dtype, int64_t planes_q, int64_t pla
 
 }  // namespace
 
-int64_t attn_bwd_workspace_bytes(const AttnBwdPlan& p, int dtype, int64_t planes_q, int64_t planes_kv,
-                                 int64_t D) {
-  return offsets(p, dtype, planes_q, planes_kv, D).end;
+int64_t attn_bwd_workspace_bytes(int dtype, bool causal, bool anew, int64_t B, int64_t H, int64_t H_kv, int64_t N,
+                                 int64_t N_kv, int64_t D) {
+  return offsets(attn_bwd_plan(B, H, H_kv, N, N_kv, D, causal, anew), dtype, anew, B * H, B * H_kv, D).end;
 }
 
 hipError_t launch_attn_bwd(const AttnBwdArgs& x, hipStream_t s) {
-  const AttnBwdPlan p = attn_bwd_plan(x.B, x.H, x.H_kv, x.N, x.N_kv, x.D, x.causal != 0);
+  const AttnBwdPlan p = attn_bwd_plan(x.B, x.H, x.H_kv, x.N, x.N_kv, x.D, x.causal != 0, !x.lse);
   Args a;
   auto rows = [](const View& v) { return Rows{v.p, v.sb, v.sh, v.sr}; };
   auto out = [](const View& v) { return Out{const_cast<void*>(v.p), v.sb, v.sh, v.sr}; };
@@ -951,15 +1110,17 @@ hipError_t launch_attn_bwd(const AttnBwdArgs& x, hipStream_t s) {
   a.keys = p.keys;
   a.queries = p.queries;
   a.alone = p.alone;
+  a.columns = (int)p.columns;
   a.sm_scale = x.sm_scale;
   a.c = x.sm_scale * LOG2E_F;
-  const Offsets64 o = offsets(p, x.dtype, a.planes_q, a.planes_kv, x.D);
+  const Offsets64 o = offsets(p, x.dtype, !x.lse, a.planes_q, a.planes_kv, x.D);
   u8* ws = (u8*)x.workspace;
   a.nl = (float*)(ws + o.nl);
   a.nd = (float*)(ws + o.nd);
   a.max_do = (float*)(ws + o.max_do);
   a.max_d = (float*)(ws + o.max_d);
   a.max_v = (float*)(ws + o.max_v);
+  a.stats = (float*)(ws + o.stats);
   a.part_k = (float*)(ws + o.part_k);
   a.part_v = (float*)(ws + o.part_v);
   a.part_q = (float*)(ws + o.part_q);

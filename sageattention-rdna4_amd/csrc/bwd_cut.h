@@ -66,8 +66,9 @@ inline AttnBwdCut cut_tiles(int64_t tiles, int64_t base, int64_t drop, int64_t t
   return c;
 }
 
+// anew: the call works out its logsumexp by itself, in launches ahead.
 inline AttnBwdPlan attn_bwd_plan(int64_t B, int64_t H, int64_t H_kv, int64_t N, int64_t N_kv, int64_t D,
-                                 bool causal) {
+                                 bool causal, bool anew = false) {
   AttnBwdPlan p;
   p.nb_q = ceil_div(N, ATTN_BWD_ROWS);
   p.nb_kv = ceil_div(N_kv, ATTN_BWD_ROWS);
@@ -85,7 +86,7 @@ inline AttnBwdPlan attn_bwd_plan(int64_t B, int64_t H, int64_t H_kv, int64_t N, 
   // values 8.6 and 9.7 us, 257 12.8 and 11.8, 512 15.5 and 13.8, 128 rows of 128 values 14.6 and 13.7, 257
   // 22.5 and 17.4; a call takes the host 13.0 and 16.4 us).
   const int64_t steps = ATTN_BWD_ALONE * 64 / D;
-  p.alone = p.columns == 64 && k_long <= steps && q_long <= steps;
+  p.alone = !anew && p.columns == 64 && k_long <= steps && q_long <= steps;
   const int64_t wide = p.columns / ATTN_BWD_ROWS, k_tiles = ceil_div(N_kv, p.columns), q_tiles = ceil_div(N, p.columns);
   // The steps of the longest tiles, and of all of them, at two products' time for keys and one and a half
   // for queries, twice that for 128 columns; `share` is each resident block's part of it all.
@@ -133,7 +134,7 @@ SAGE_HD AttnBwdPlace attn_bwd_place(const AttnBwdCut& c, int block, int planes) 
   const int x = block / planes, t = x / p;
   return {lo + t, block - x * planes, x - t * p, p};
 }
-// The block that holds the first part of cut tile u in plane 0 (those of the other planes follow it, the next
+// The block that holds the first part of tile u in plane 0 (those of the other planes follow it, the next
 // part's are `planes` further on), and the tile's parts.
 SAGE_HD int attn_bwd_first_part(const AttnBwdCut& c, int u, int planes, int& parts) {
   int lo = 0, p = c.parts, first = 0;

@@ -822,8 +822,15 @@ int64_t sage_attn_bwd_workspace_bytes(int dtype, int causal, int64_t B, int64_t 
   const int rc = check_attn_bwd(dtype, causal, B, H, N, H_kv, N_kv, D);
   if (rc) return -rc;
   g_err.clear();
-  return sage::attn_bwd_workspace_bytes(sage::attn_bwd_plan(B, H, H_kv, N, N_kv, D, causal != 0),
-                                        dtype, B * H, B * H_kv, D);
+  return sage::attn_bwd_workspace_bytes(dtype, causal != 0, false, B, H, H_kv, N, N_kv, D);
+}
+
+int64_t sage_attn_bwd_anew_workspace_bytes(int dtype, int causal, int64_t B, int64_t H, int64_t N,
+                                           int64_t H_kv, int64_t N_kv, int64_t D) {
+  const int rc = check_attn_bwd(dtype, causal, B, H, N, H_kv, N_kv, D);
+  if (rc) return -rc;
+  g_err.clear();
+  return sage::attn_bwd_workspace_bytes(dtype, causal != 0, true, B, H, H_kv, N, N_kv, D);
 }
 
 int sage_attn_bwd(int dtype, int causal, const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sr,
@@ -851,20 +858,21 @@ int sage_attn_bwd(int dtype, int causal, const void* q, int64_t q_sb, int64_t q_
     const sage::View* view;
   } views[] = {{"q", &a.q}, {"k", &a.k}, {"v", &a.v}, {"o", &a.o}, {"dout", &a.dout},
                {"dq", &a.dq}, {"dk", &a.dk}, {"dv", &a.dv}};
+  const bool anew = !o && !lse;
   for (const auto& x : views) {
+    if (anew && x.view == &a.o) continue;
     if ((rc = check_view(x.name, x.view->p, x.view->sb, x.view->sh, x.view->sr))) return rc;
     // the 64 rows of a tile are reached by 32-bit offsets from its first
     if (x.view->sr > kMaxRowStride)
       return fail(SAGE_ERR_INVALID, "%s: stride_int32 (rows %lld elements apart, at most %lld are served)",
                   x.name, (long long)x.view->sr, (long long)kMaxRowStride);
   }
-  if (!lse) return fail(SAGE_ERR_INVALID, "lse is NULL");
+  if (!lse && !anew) return fail(SAGE_ERR_INVALID, "lse is NULL");
   if (((uintptr_t)lse & 3u) || ((uintptr_t)dlse & 3u))
     return fail(SAGE_ERR_INVALID, "ptr_align: lse and dlse must be 4-byte aligned");
   if (!(sm_scale >= 1e-30f) || !(sm_scale <= 1e30f))   // the logsumexp is divided by it
     return fail(SAGE_ERR_INVALID, "sm_scale: must lie between 1e-30 and 1e30 (got %g)", (double)sm_scale);
-  const int64_t need = sage::attn_bwd_workspace_bytes(
-      sage::attn_bwd_plan(B, H, H_kv, N, N_kv, D, causal != 0), dtype, B * H, B * H_kv, D);
+  const int64_t need = sage::attn_bwd_workspace_bytes(dtype, causal != 0, anew, B, H, H_kv, N, N_kv, D);
   if (need && (workspace == nullptr || workspace_bytes < (size_t)need || ((uintptr_t)workspace & 255u)))
     return fail(SAGE_ERR_INVALID, "workspace: need %lld bytes, 256-byte aligned (got %zu)",
                 (long long)need, workspace_bytes);

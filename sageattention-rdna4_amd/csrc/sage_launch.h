@@ -191,17 +191,17 @@ struct View {
 };
 struct AttnBwdArgs {
   int dtype, causal;
-  View q, k, v, o, dout;      // read
+  View q, k, v, o, dout;      // read; o.p and lse NULL: worked out anew
   View dq, dk, dv;            // written
-  const float* lse;           // (B, H, N)
+  const float* lse;           // (B, H, N) or NULL
   const float* dlse;          // optional (B, H, N)
   int64_t B, H, H_kv, N, N_kv, D;
   float sm_scale;
   void* workspace;
 };
-// A plan follows from the sizes alone, so a captured call and its workspace agree.
-int64_t attn_bwd_workspace_bytes(const AttnBwdPlan& p, int dtype, int64_t planes_q, int64_t planes_kv,
-                                 int64_t D);
+// A plan follows from the sizes alone (and whether lse is NULL), so a captured call and its workspace agree.
+int64_t attn_bwd_workspace_bytes(int dtype, bool causal, bool anew, int64_t B, int64_t H, int64_t H_kv, int64_t N,
+                                 int64_t N_kv, int64_t D);
 hipError_t launch_attn_bwd(const AttnBwdArgs& a, hipStream_t stream);
 
 // Rows of n contiguous values in up to three dimensions, the last of d2 rows, the middle one of d1.

@@ -183,8 +183,9 @@ class SageLib:
         L.sage_attn_bwd.restype = i32
         L.sage_attn_bwd.argtypes = ([i32] * 2 + view * 5 + [vp, vp] + view * 3 + [i64] * 6
                                     + [f32, vp, ctypes.c_size_t, vp])
-        L.sage_attn_bwd_workspace_bytes.restype = i64
-        L.sage_attn_bwd_workspace_bytes.argtypes = [i32] * 2 + [i64] * 6
+        for size in (L.sage_attn_bwd_workspace_bytes, L.sage_attn_bwd_anew_workspace_bytes):
+            size.restype = i64
+            size.argtypes = [i32] * 2 + [i64] * 6
         rows = [vp, i64, i64, i64]
         L.sage_rms_norm.restype = i32
         L.sage_rms_norm.argtypes = [i32] * 3 + rows * 2 + [vp] + [i64] * 4 + [f32] + [vp] * 5
@@ -414,10 +415,10 @@ class SageLib:
             self._check(rc, "sage_cache_attn")
 
     @functools.lru_cache(maxsize=4096)
-    def attn_bwd_workspace_bytes(self, dtype, causal, B, H, N, H_kv, N_kv, D):
-        """Bytes of `sage_attn_bwd`'s workspace, a function of the sizes alone."""
-        n = self.lib.sage_attn_bwd_workspace_bytes(_dtype_code(dtype), int(bool(causal)), B, H, N,
-                                                   H_kv, N_kv, D)
+    def attn_bwd_workspace_bytes(self, dtype, causal, B, H, N, H_kv, N_kv, D, anew=False):
+        """Bytes of `sage_attn_bwd`'s workspace, a function of the sizes alone; `anew`: without out and lse."""
+        size = self.lib.sage_attn_bwd_anew_workspace_bytes if anew else self.lib.sage_attn_bwd_workspace_bytes
+        n = size(_dtype_code(dtype), int(bool(causal)), B, H, N, H_kv, N_kv, D)
         if n < 0:
             self._check(-n, "sage_attn_bwd_workspace_bytes")
         return n
@@ -425,14 +426,14 @@ class SageLib:
     def attn_bwd(self, dtype, causal, read, strides, grads, grad_strides, lse, dlse, sizes, sm_scale,
                  workspace, workspace_bytes, stream):
         """The gradients of q, k, v into `grads` from `read` = (q, k, v, out, dout), each with its (batch,
-        head, row) strides; `sizes` = (B, H, N, H_kv, N_kv, D) (see `sage_attn_bwd`)."""
+        head, row) strides, out and lse None together; `sizes` = (B, H, N, H_kv, N_kv, D) (see `sage_attn_bwd`)."""
         q, k, v, o, g = read
         qs, ks, vs, os_, gs = strides
         dq, dk, dv = grads
         dqs, dks, dvs = grad_strides
         rc = self.lib.sage_attn_bwd(
             _dtype_code(dtype), int(bool(causal)), q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs,
-            o.data_ptr(), *os_, g.data_ptr(), *gs, lse.data_ptr(),
+            None if o is None else o.data_ptr(), *os_, g.data_ptr(), *gs, None if lse is None else lse.data_ptr(),
             None if dlse is None else dlse.data_ptr(), dq.data_ptr(), *dqs, dk.data_ptr(), *dks,
             dv.data_ptr(), *dvs, *sizes, sm_scale, None if workspace is None else workspace.data_ptr(),
             workspace_bytes, stream)
