@@ -358,7 +358,7 @@ int64_t sage_cache_attn_workspace_bytes(int64_t B, int64_t H, int64_t H_kv, int6
  *   workspace        sage_attn_bwd_workspace_bytes bytes (without o and lse
  *                    sage_attn_bwd_anew_workspace_bytes), 256-byte aligned; NULL where that is 0
  * P and dS are rounded to `dtype` ahead of their products (fp16: scaled by powers of two that keep
- * them in range), every sum is fp32, and the results are rounded once. They are the same from call to
+ * them in range, P no larger than 2^1.99), every sum is fp32, and the results are rounded once. They are the same from call to
  * call. Where P is 0 its other factor has to be finite: 0 times a NaN or an infinity is NaN.
  */
 int sage_attn_bwd(int dtype, int causal,

@@ -78,11 +78,15 @@ constexpr int BT = ATTN_BWD_ROWS;      // rows of the other side in an LDS tile
 template <int D>
 constexpr int U = D == 64 ? 2 : 1;
 constexpr float NEG_INF = -__builtin_inff();
-// fp16 operands: P is held times 2^12, so that it is a normal number from 2^-26 up and may pass 1 by a
-// factor of 15 (a logsumexp of quantized scores is off by some hundredths), dS times a power of two
-// that brings its bound into [2^13, 2^14).
+// fp16 operands: P is held times 2^12, so that it is a normal number from 2^-26 up, dS times a power of two
+// that brings its bound (for P of 1 and less) into [2^13, 2^14).
 template <typename T>
 constexpr float P_SHIFT = std::is_same_v<T, f16> ? 12.0f : 0.0f;
+// P passes 1 where a given logsumexp lies under its scores, by some units if it is that of quantized ones (spread
+// 100, int8: P of 54). fp16's ends at 2^1.99, so that neither P nor dS passes 65504; a NaN stays one. (One operation a
+// score, 313 us for 302 with 20 heads of 4096 rows of 64 values. The mode bit for saturating conversions costs
+// nothing, but makes a NaN a number; a tile's largest exponent, and a branch where it is over, 321 us.)
+constexpr float P_MOST = 1.99f;
 
 // The 16-byte chunk of a tile's row r that lies at position c ^ swz(r). A row read takes 16 rows'
 // (or 8 rows' two) chunks in a pass, a transposed read 4 rows' 64 bytes: both touch each bank once.
@@ -435,6 +439,12 @@ __device__ __forceinline__ void fence() {
   if (D == 64 || !CAUSAL) __builtin_amdgcn_sched_barrier(0);
 }
 
+// 2^x; fp16: 2^most at most.
+template <typename T>
+__device__ __forceinline__ float weight(float x, float most) {
+  return __builtin_amdgcn_exp2f(std::is_same_v<T, f16> ? __builtin_elementwise_minimum(x, most) : x);
+}
+
 __device__ __forceinline__ void clear(f32x16& x) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) x[r] = 0.0f;
@@ -676,7 +686,7 @@ __device__ __forceinline__ void keys_block(const Args& a, u8* smem, int block) {
       dp = mfma16(row_operand<T>(smem, of.row, at_do, i), vf[i], dp);
       // P, between dP's products: the matrix unit and the others work at once
 #pragma unroll
-      for (int r = 256 / D * i; r < 256 / D * (i + 1); ++r) s[r] = __builtin_amdgcn_exp2f(s[r] * a.c);
+      for (int r = 256 / D * i; r < 256 / D * (i + 1); ++r) s[r] = weight<T>(s[r] * a.c, P_SHIFT<T> + P_MOST);
     }
     fence<D, CAUSAL>();
     x8 pf[2], df[2];
@@ -758,7 +768,7 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
   x8 qf[D / 16], gf[D / 16];
   load_columns<T, D>(plane<T>(a.q, b, h), a.q.sr, qw, a.N, lane, qf);
   load_columns<T, D>(plane<T>(a.dout, b, h), a.dout.sr, qw, a.N, lane, gf);
-  float nl1, nd1, scale = 1.0f;
+  float nl1, nd1, scale = 1.0f, most = 0.0f;           // most: the largest exponent
   if (CW == 2 && a.alone) {
     x8 of[D / 16];
     load_columns<T, D>(plane<T>(a.o, b, h), a.o.sr, qw, a.N, lane, of);
@@ -777,7 +787,9 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
     block_max<1>((float*)(smem + 4 * TILE), mv);
     scale = scale_for(sqrtf(column_dot<T, D>(gf, gf)) * sqrtf(mv[0]) + fabsf(nd1));
     // P meets dS alone here: its power of two is part of the exponent
-    nl1 += (log2f(scale) - P_SHIFT<T>) / a.c;
+    const float shift = log2f(scale);
+    nl1 += (shift - P_SHIFT<T>) / a.c;
+    most = shift + P_MOST;
   }
   f32x16 dq[D / 32];
 #pragma unroll
@@ -807,7 +819,7 @@ __device__ __forceinline__ void queries_block(const Args& a, u8* smem, int block
     for (int i = 0; i < D / 16; ++i) {
       dp = mfma16(row_operand<T>(smem, of.row, at + 2 * TILE, i), gf[i], dp);
 #pragma unroll
-      for (int r = 256 / D * i; r < 256 / D * (i + 1); ++r) s[r] = __builtin_amdgcn_exp2f(s[r] * a.c);
+      for (int r = 256 / D * i; r < 256 / D * (i + 1); ++r) s[r] = weight<T>(s[r] * a.c, most);
     }
     fence<D, CAUSAL>();
     x8 df[2];

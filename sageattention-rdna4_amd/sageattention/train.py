@@ -73,7 +73,8 @@ def sageattn_backward(dout, q, k, v, out=None, lse=None, tensor_layout="HND", is
 
     out, lse: left out after `sageattn`, whose output and logsumexp are those of 8-bit scores; the pass
     works out those of the 16-bit scores that it forms, two products more to its seven. Given together they
-    are attention's in 16 bits or more. Keys that are one part of those a query sees (attention over parts,
+    are attention's in 16 bits or more (a logsumexp under its scores leaves results finite: weights end at
+    4 in fp16). Keys that are one part of those a query sees (attention over parts,
     merged by their logsumexp) have their gradients from calls with the merged out and lse, a call for each
     part; dq is the calls' sum. A row with a logsumexp of -infinity saw nothing and counts for nothing. Values have to be finite,
     those of a padded batch's unused rows too: 0 times a NaN or an infinity is NaN.

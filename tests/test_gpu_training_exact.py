@@ -337,3 +337,39 @@ def test_block_of_a_transformer():
         # gradients see scores that the roundings of q and k, at 2^-11 of |score| = 8 or less, have moved
         assert rel <= 30 * 2.0 ** -11, (name, rel)
         print(name, "%.2g" % rel)
+
+
+@pytest.mark.parametrize("D,N,causal", [(64, 200, False), (64, 700, True), (128, 150, True), (128, 2048, True)])
+def test_a_logsumexp_under_its_scores(D, N, causal):
+    """A given logsumexp that is some units under that of the scores, as one of scores of fewer bits may be: fp16's weights
+    end at 2^1.99 in place of infinity, those under it are the formula's, and results stay finite."""
+    from sageattention import sageattn_backward
+    q, k, v, dout, _ = inputs(1, 2, 2, N, N, D, F16, spread=4.0)
+    out, lse = forward(q, k, v, causal, D ** -0.5)
+    for less in (2.0, 5.0, 40.0):
+        got = sageattn_backward(dout, q, k, v, out.half(), (lse - less).float(), is_causal=causal)
+        assert all(torch.isfinite(t).all() for t in got), less
+        s = (mm(q[0].double(), k[0].double()) * D ** -0.5).masked_fill(~seen_of(N, N, causal, "cuda"), -torch.inf)
+        p = torch.exp(s - (lse - less).float()[0, ..., None])
+        held = p.clamp(max=2.0 ** 1.99)
+        e = (D + 8) * E * D ** -0.5 * mm(q[0].double().abs(), k[0].double().abs()) + (D / 16 + 8) * E * (lse[0, ..., None].abs() + less + 1)
+        want = held.transpose(1, 2).contiguous() @ dout[0].double()
+        tol = (held * (U[F16] + e + N * E) + 2.0 ** -37).transpose(1, 2).contiguous() @ dout[0].double().abs() + U[F16] * want.abs()
+        assert ((got[2][0].double() - want).abs() <= tol + 2.0 ** -24).all(), less
+
+
+def test_the_forward_calls_own_results_stay_finite():
+    from sageattention import sageattn, sageattn_backward
+    q, k, v, dout, _ = inputs(1, 4, 4, 2048, 2048, 128, F16, spread=100.0)
+    out, lse = sageattn(q, k, v, is_causal=True, return_lse=True)
+    assert all(torch.isfinite(t).all() for t in sageattn_backward(dout, q, k, v, out, lse, is_causal=True))
+
+
+def test_results_past_fp16_are_infinite():
+    """A gradient over 65504 comes out as infinity, which a loss scale is lowered by, not as the largest number."""
+    from sageattention import sageattn_backward
+    for N in (70, 3000):
+        q, k, v, _, _ = inputs(1, 2, 2, N, N, 64, F16)
+        dout = torch.full_like(q, 60000.0)
+        dv = sageattn_backward(dout, q, k, v, is_causal=True)[2]
+        assert torch.isposinf(dv[0, :, 0]).all()        # key 0: the sum of all rows' weights on it is over 1.1
