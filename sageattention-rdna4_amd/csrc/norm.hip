@@ -140,20 +140,23 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_kernel(const Norm 
     for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(t[c][e], t[c][e], ss);
   }
   ss = combine<TPR>(ss, lds[0], add);
-  float rstd = rsqrtf(__fadd_rn(__fdiv_rn(ss, (float)a.n), a.eps));
-  // bf16 rows of 1e19 and over: the squares' sum ends at 3e38, that of values 2^80 times smaller does not
-  // (eps is nothing beside it). The row's threads all have the same sum, so all go this way.
-  if (!std::is_same_v<T, f16> && !(ss < __builtin_inff())) {
+  const float mean = __fadd_rn(__fdiv_rn(ss, (float)a.n), a.eps);
+  float rstd = rsqrtf(mean);
+  // bf16 rows of 1e19 and over: the squares' sum ends at 3e38, that of values 2^80 times smaller does not. Rows under
+  // 2^-45 with an eps under 2^-90: squares vanish (under 2^-126), those of values 2^80 times larger do not.
+  // The row's threads all have the same sum, so all go this way.
+  if (!std::is_same_v<T, f16> && !(ss < __builtin_inff() && mean >= 0x1p-90f)) {
+    const float f = mean < 0x1p-90f ? 0x1p80f : 0x1p-80f;
     ss = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float s = t[c][e] * 0x1p-80f;
+        const float s = t[c][e] * f;
         ss = __builtin_fmaf(s, s, ss);
       }
     ss = combine<TPR>(ss, lds[1], add);
-    rstd = rsqrtf(__fdiv_rn(ss, (float)a.n)) * 0x1p-80f;
+    rstd = rsqrtf(__fadd_rn(__fdiv_rn(ss, (float)a.n), a.eps * f * f)) * f;
   }
   const int64_t base = (int64_t)row * a.n;
   const bool live = row < a.rows;
