@@ -12,6 +12,7 @@ the reason.
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from .cache import _DTYPES, _launch, _library, _refuse
 
@@ -142,11 +143,13 @@ def rms_norm(x, weight, eps=1e-6, residual=None, return_rstd=False):
     weight: (n,) of x's dtype or fp32. The sum is added, normed and scaled in fp32; y and the sum (new,
     contiguous, of x's shape and dtype) are each rounded once. Autograd records the call where x, weight or
     residual need a gradient. `return_rstd` appends 1 / sqrt(...) of each row (fp32, x's shape without
-    the last dimension), for `rms_norm_backward`; such a call is not recorded.
+    the last dimension), for `rms_norm_backward`; such a call is not recorded. Forward-mode tangents are
+    refused (`NotImplementedError`).
     """
-    if not return_rstd and torch.is_grad_enabled() and (
+    # (a forward-mode tangent, which needs no gradient, is refused there)
+    if not return_rstd and (forward_ad._current_level >= 0 or torch.is_grad_enabled() and (
             getattr(x, "requires_grad", False) or getattr(weight, "requires_grad", False)
-            or getattr(residual, "requires_grad", False)):
+            or getattr(residual, "requires_grad", False))):
         return _RmsNorm.apply(x, weight, eps, residual)
     y, _, total, rstd = _norm("rms_norm", x, weight, eps, residual, 0, return_rstd)
     done = (y,) if residual is None else (y, total)

@@ -51,3 +51,22 @@ def test_a_row_of_zeros():
     from sageattention import rms_norm
     x, w = torch.zeros(2, 64, dtype=BF16, device="cuda"), torch.ones(64, dtype=BF16, device="cuda")
     assert (rms_norm(x, w) == 0).all() and (rms_norm(x, w, 1e-38) == 0).all() and torch.isnan(rms_norm(x, w, 0.0)).all()
+
+
+def test_forward_mode_tangents_are_refused():
+    """A tangent is not dropped without a word: the call raises, with gradients enabled or not; other tensors pass."""
+    import torch.autograd.forward_ad as forward_ad
+    from sageattention import rms_norm, sageattn_train
+    x, w = torch.randn(3, 64, device="cuda").half(), torch.ones(64, device="cuda").half()
+    want = rms_norm(x, w)
+    q = torch.randn(1, 2, 40, 64, device="cuda").half()
+    with forward_ad.dual_level():
+        dual = [forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, w, q)]
+        for enabled in (True, False):
+            with torch.set_grad_enabled(enabled):
+                for call in (lambda: rms_norm(dual[0], w), lambda: rms_norm(x, dual[1]),
+                             lambda: rms_norm(x, w, residual=dual[0]), lambda: sageattn_train(dual[2], q, q)):
+                    with pytest.raises(NotImplementedError):
+                        call()
+                assert torch.equal(rms_norm(x, w), want)
+    assert torch.equal(rms_norm(x, w), want)
