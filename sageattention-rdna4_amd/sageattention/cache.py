@@ -86,6 +86,14 @@ def _empty(like):
     return torch.empty_like(like) if like.is_contiguous() else like.new_empty(like.shape)
 
 
+def _gradient(t):
+    """A gradient as the kernels take it, whatever autograd hands over: contiguous, from a multiple of 16 bytes on."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() & 15 else t
+
+
 def _ints(what, name, t, device, rows, columns=None):
     """Checks an int32 tensor (rows,), or (rows, columns) with contiguous rows (columns -1: any);
     returns the elements between two rows, 0 where there is one."""

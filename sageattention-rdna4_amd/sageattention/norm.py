@@ -14,7 +14,7 @@ import math
 import torch
 from torch.autograd import forward_ad
 
-from .cache import _DTYPES, _launch, _library, _refuse
+from .cache import _DTYPES, _gradient, _launch, _library, _refuse
 
 _NONE = (0, 0, 0)
 
@@ -129,8 +129,7 @@ class _RmsNorm(torch.autograd.Function):
         t, weight, rstd = ctx.saved_tensors
         if dy is None:                     # only the sum was used
             return dsum, None, None, dsum
-        dx, dw = rms_norm_backward(dy.contiguous(), t, weight, rstd,
-                                   None if dsum is None else dsum.contiguous())
+        dx, dw = rms_norm_backward(_gradient(dy), t, weight, rstd, _gradient(dsum))
         return dx, dw, None, dx if ctx.residual else None
 
 

@@ -11,7 +11,7 @@ synchronizes nothing, so that it can be captured into a graph. A call that is no
 """
 import torch
 
-from .cache import _DTYPES, _HEAD_DIMS, _empty, _launch, _library, _refuse, _view
+from .cache import _DTYPES, _HEAD_DIMS, _empty, _gradient, _launch, _library, _refuse, _view
 from .core import sageattn
 
 #: what the scores' factor may be (a logsumexp is divided by it)
@@ -147,9 +147,8 @@ class _Attention(torch.autograd.Function):
         q, k, v = ctx.saved_tensors
         if dout is None and dlse is None:
             return (None,) * 7
-        dout = q.new_zeros(q.shape) if dout is None else dout.contiguous()
-        dlse = None if dlse is None else dlse.contiguous()
-        return sageattn_backward(dout, q, k, v, None, None, *ctx.call, dlse=dlse) + (None,) * 4
+        dout = q.new_zeros(q.shape) if dout is None else _gradient(dout)
+        return sageattn_backward(dout, q, k, v, None, None, *ctx.call, dlse=_gradient(dlse)) + (None,) * 4
 
 
 def sageattn_train(q, k, v, tensor_layout="HND", is_causal=False, sm_scale=None, return_lse=False,

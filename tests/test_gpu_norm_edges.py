@@ -70,3 +70,21 @@ def test_forward_mode_tangents_are_refused():
                         call()
                 assert torch.equal(rms_norm(x, w), want)
     assert torch.equal(rms_norm(x, w), want)
+
+
+def test_gradients_that_begin_off_16_bytes():
+    """Results joined behind an odd number of values, as a flat buffer of parameters and activations: the gradients come
+    back as contiguous views 2 bytes off, and are taken."""
+    from sageattention import rms_norm, sageattn_train
+    x, w = torch.randn(5, 64, device="cuda").half().requires_grad_(), torch.ones(64, device="cuda").half().requires_grad_()
+    q = torch.randn(1, 2, 40, 64, device="cuda").half().requires_grad_()
+    odd = torch.zeros(1, device="cuda").half()
+    for make, leaves in ((lambda: rms_norm(x, w), (x, w)), (lambda: rms_norm(x, w, residual=x), (x, w)),
+                         (lambda: sageattn_train(q, q, q), (q,)),
+                         (lambda: sageattn_train(q, q, q, return_lse=True), (q,))):
+        results = make()
+        results = results if isinstance(results, tuple) else (results,)
+        want = torch.autograd.grad(results, leaves, [t.detach() for t in results], retain_graph=True)
+        flat = [torch.cat([odd.to(t.dtype), t.flatten()]) for t in results]
+        got = torch.autograd.grad(flat, leaves, [torch.cat([odd.to(t.dtype), t.detach().flatten()]) for t in results])
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
