@@ -23,8 +23,9 @@
 //
 // What bounds it. 32 heads on 8 of 16384 causal rows, bf16, head_dim 128: 6.5 to 6.7 ms by the card, the seven
 // products at 1160 to 1200 TFLOP/s, where a large library product reaches 1227: the power cap, at a clock
-// of 1.7 GHz with the matrix units busy for 65 % of the cycles. 20 heads of 4096 rows of 64 values, fp16, 306 to
-// 330 us: the same clock, matrix units 53 %, vector instructions (five to a score) 48 %.
+// of 1.7 GHz with the matrix units busy for 66 % of the cycles. 20 heads of 4096 rows of 64 values, fp16, 313 to
+// 342 us: the same clock, matrix units 51 %, vector instructions (six to a score) 54 %. `stats` takes 2.56 ms and 142 us
+// of these: six vector instructions a score on two products, matrix units 45 and 27 %.
 //
 // Layout. A wave owns 32 columns (keys, or queries) of 16-bit operands in registers and multiplies
 // them with 32 rows of the other side at a time by 32x32x16 MFMAs. The result has a column per lane,

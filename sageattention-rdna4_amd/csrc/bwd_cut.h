@@ -97,7 +97,8 @@ inline AttnBwdPlan attn_bwd_plan(int64_t B, int64_t H, int64_t H_kv, int64_t N, 
   const int64_t share = (k_cost * k_all + q_cost * q_all) / resident;
   // A part may take a little more than that: parts are written in fp32 and read again, and tiles that are all
   // alike fit the card in one go with a fifth more. A tile is cut only where that saves more than the
-  // joining launch costs; no part is under 4 steps. Measured, all tiles in as many parts as the longest one
+  // joining launch costs (for each kind by itself, also where the other one's parts need that launch anyway); no part is
+  // under 4 steps. Measured, all tiles in as many parts as the longest one
   // and so: 2 x 8 heads on 2 of 6449 causal rows of 64 values 358 and 292 us, one head of 16384 rows 550 and
   // 408, 6 heads on 1 of 1541 rows 101 and 93, 4096 causal rows, 32 heads on 8, 472 and 479.
   const int64_t may = share + share / (causal ? 20 : 5);

@@ -77,7 +77,9 @@ def sageattn_backward(dout, q, k, v, out=None, lse=None, tensor_layout="HND", is
     4 in fp16). Keys that are one part of those a query sees (attention over parts,
     merged by their logsumexp) have their gradients from calls with the merged out and lse, a call for each
     part; dq is the calls' sum. A row with a logsumexp of -infinity saw nothing and counts for nothing. Values have to be finite,
-    those of a padded batch's unused rows too: 0 times a NaN or an infinity is NaN.
+    those of a padded batch's unused rows too: 0 times a NaN or an infinity is NaN. fp16 needs a loss scale only
+    where dout or the gradients themselves leave its range; dK loses bits of rows whose gradient is some 2^15 under the
+    largest row's of the heads that share a key.
     """
     what = "sageattn_backward"
     anew = out is None and lse is None
