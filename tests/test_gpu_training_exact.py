@@ -373,3 +373,45 @@ def test_results_past_fp16_are_infinite():
         dout = torch.full_like(q, 60000.0)
         dv = sageattn_backward(dout, q, k, v, is_causal=True)[2]
         assert torch.isposinf(dv[0, :, 0]).all()        # key 0: the sum of all rows' weights on it is over 1.1
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_a_nan_stays_with_its_queries(dtype):
+    """A query's or a gradient's NaN: that row's dq, and its head's dk and dv; the other rows' dq are as they were."""
+    from sageattention import sageattn_backward
+    q, k, v, dout, _ = inputs(1, 2, 2, 200, 200, 64, dtype)
+    before = sageattn_backward(dout, q, k, v)
+    others = torch.ones(1, 2, 200, dtype=torch.bool, device="cuda")
+    others[0, 1, 77] = False
+    for t in (q, dout):
+        was = t[0, 1, 77, 5].item()
+        t[0, 1, 77, 5] = torch.nan
+        dq, dk, dv = sageattn_backward(dout, q, k, v)
+        t[0, 1, 77, 5] = was
+        assert torch.isnan(dq[0, 1, 77]).all() and torch.equal(dq[others], before[0][others])
+        assert torch.isnan(dk[0, 1]).all() and torch.isnan(dv[0, 1, :, 5]).all()
+        assert torch.equal(dk[0, 0], before[1][0, 0]) and torch.equal(dv[0, 0], before[2][0, 0])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_rows_without_a_gradient_count_for_nothing(dtype):
+    """A padded batch's unused rows, whose gradient is zero: their dq is 0, and dk and dv are those of the others."""
+    from sageattention import sageattn_backward
+    q, k, v, dout, _ = inputs(2, 4, 2, 300, 140, 64, dtype, spread=4.0)
+    dout[:, :, 130:] = 0
+    got = sageattn_backward(dout, q, k, v)
+    assert (got[0][:, :, 130:] == 0).all()
+    verify(got, q, k, v, dout, None, "HND", False)
+    assert all((g == 0).all() for g in sageattn_backward(torch.zeros_like(dout), q, k, v))
+
+
+def test_keys_past_32_bits_and_long_keys():
+    from sageattention import sageattn_backward
+    store = torch.zeros(1, 300000, 60, 128, dtype=BF16, device="cuda")
+    assert store.numel() > 1 << 31
+    q, k, v, dout, dlse = inputs(1, 1, 1, 40, 300000, 128, BF16, "NHD", spread=2.0)
+    store[:, :, 59:], store[:, :, 3:4] = k, v
+    got = sageattn_backward(dout, q, store[:, :, 59:], store[:, :, 3:4], tensor_layout="NHD", dlse=dlse)
+    verify(got, q, k, v, dout, dlse, "NHD", False)
+    q, k, v, dout, dlse = inputs(1, 2, 1, 1, 131073, 64, F16, spread=2.0)
+    verify(sageattn_backward(dout, q, k, v, dlse=dlse), q, k, v, dout, dlse, "HND", False)
